@@ -4,4 +4,4 @@ selection, int8 Q/K quantiser and block-sparse flash attention behind a C ABI
 
 __version__ = "0.1.0"
 
-__all__ = ["ops", "pipeline", "kernel", "workloads", "layout", "budget", "selector"]
+__all__ = ["ops", "pipeline", "kernel", "workloads", "layout", "budget", "selector", "rotary"]

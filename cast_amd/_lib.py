@@ -19,6 +19,7 @@ TORCH_OPS_PATH = Path(__file__).resolve().parent / "_lib" / "librcsa_torch.so"
 RCSA_OK = 0
 RCSA_BF16 = 0
 RCSA_F32 = 1
+RCSA_F16 = 2
 RCSA_ORDER_INDEX = 0
 RCSA_ORDER_RANK = 1
 RCSA_ORDER_RANK_LOCAL = 2
@@ -74,6 +75,15 @@ SIGNATURES: dict[str, list] = {
     "rcsa_order_lists_max_blocks": [],
     "rcsa_order_lists": [_P, _P] + [_I] * 6 + [_P] + [_I] * 6 + [_P, _P, _P, _I, _P, _P],
     "rcsa_order_split_lists": [_P, _P] + [_I] * 6 + [_P] + [_I] * 7 + [_P, _P, _P, _I, _P, _P],
+    "rcsa_rope": [_P, _P, c_int, _I, _I, _I, _I, _P, _P, c_int, _P, _I, _P, _P, _I, c_int,
+                  c_float, _P],
+    "rcsa_norm_rope": [_P] * 6 + [c_int, _P, _P, _P, _P, c_int, _I, _I, c_float, c_int, _P, c_int,
+                                  _P, _I, _P, _P, _I, c_int, c_float, _P, _I, _I, _I, _I, _P, _P,
+                                  _P],
+    "rcsa_window_attn_plan": [_P, _I, ctypes.POINTER(c_int64)],
+    "rcsa_window_attn_workspace_bytes": [_P, _I],
+    "rcsa_window_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _P] + [_I] * 7 + [c_float, _I, _P, _I,
+                                                                             _P],
     "rcsa_pack_tokens": [_P, c_int, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P],
     "rcsa_unpack_tokens": [_P, _I, _I, _I, _I, _P, _I, _P, _P],
     "rcsa_status_string": [c_int],
@@ -104,7 +114,8 @@ def load() -> ctypes.CDLL:
         fn.restype = (ctypes.c_char_p if name == "rcsa_status_string"
                       else c_int64 if name in ("rcsa_attn_workspace_bytes",
                                                "rcsa_attn_noalloc_scratch_bytes",
-                                               "rcsa_order_lists_max_blocks")
+                                               "rcsa_order_lists_max_blocks",
+                                               "rcsa_window_attn_workspace_bytes")
                       else c_int)
     _lib = lib
     return lib

@@ -9,8 +9,8 @@
 // bad layout.  Every tensor is checked to span the elements the call's dims
 // and strides reach, so no argument combination makes a kernel read or write
 // past the tensors it was given.  Nothing here synchronises, and nothing but
-// layer_call, order_lists and valid_bits, which allocate their outputs, allocates device
-// memory.
+// layer_call, order_lists, valid_bits, rope, norm_rope and window_attention, which
+// allocate their outputs (and the last its workspace), allocates device memory.
 //
 // The C ABI is bound at load time (rcsa::bind_library) from the library the
 // Python side loaded, so one librcsa.so serves both the ctypes binding and
@@ -48,6 +48,11 @@ struct Api {
   decltype(&rcsa_quantize_key) quantize_key = nullptr;
   decltype(&rcsa_attn_split_plan) attn_split_plan = nullptr;
   decltype(&rcsa_attn_workspace_bytes) attn_workspace_bytes = nullptr;
+  decltype(&rcsa_rope) rope = nullptr;
+  decltype(&rcsa_norm_rope) norm_rope = nullptr;
+  decltype(&rcsa_window_attn_plan) window_attn_plan = nullptr;
+  decltype(&rcsa_window_attn_workspace_bytes) window_attn_workspace_bytes = nullptr;
+  decltype(&rcsa_window_attn) window_attn = nullptr;
 };
 
 std::mutex g_mu;
@@ -80,6 +85,11 @@ void bind_library(const std::string& path) {
   bind_one(h, "rcsa_quantize_key", api.quantize_key);
   bind_one(h, "rcsa_attn_split_plan", api.attn_split_plan);
   bind_one(h, "rcsa_attn_workspace_bytes", api.attn_workspace_bytes);
+  bind_one(h, "rcsa_rope", api.rope);
+  bind_one(h, "rcsa_norm_rope", api.norm_rope);
+  bind_one(h, "rcsa_window_attn_plan", api.window_attn_plan);
+  bind_one(h, "rcsa_window_attn_workspace_bytes", api.window_attn_workspace_bytes);
+  bind_one(h, "rcsa_window_attn", api.window_attn);
   g_api = api;
   g_bound = true;
 }
@@ -800,6 +810,295 @@ std::vector<at::Tensor> layer_call(
   return res;
 }
 
+// ---- Rotary positions and windowed attention (cast_amd/ops.py: rope, norm_rope,
+// window_attention, paged_attention) ----
+
+int float_code(const char* op, const at::Tensor& t, const char* name) {
+  const at::ScalarType dt = t.scalar_type();
+  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, op, ": ", name,
+              " must be bfloat16, float16 or float32");
+  return dt == at::kBFloat16 ? RCSA_BF16 : dt == at::kHalf ? RCSA_F16 : RCSA_F32;
+}
+
+// A tensor [., ., ., D] whose rows the kernels reach by its own strides.
+void want_rows(const char* op, const at::Tensor& t, at::ScalarType dt, const char* name) {
+  want(op, t, dt, name);
+  TORCH_CHECK(t.dim() == 4 && (t.stride(3) == 1 || t.size(3) <= 1), op, ": ", name,
+              " must be 4-D with a contiguous last dim");
+}
+
+// An output: no two of its elements share memory through a stride of 0.
+void want_own(const char* op, const at::Tensor& t, const char* name) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    TORCH_CHECK(t.stride(i) > 0 || t.size(i) <= 1, op, ": ", name, " must not be expanded");
+}
+
+// (the stride of a dimension of one element says nothing)
+void put_strides(const at::Tensor& t, int64_t* s) {
+  for (int64_t i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+struct Turns {
+  int64_t n_axes, n_pairs, pos_strides[3];
+  int pos_i64;
+};
+
+// positions [L], [B, L] (one axis), [L, A] or [B, L, A]; turns fp64 and axis int32 of the
+// pairs.
+Turns want_turns(const char* op, const at::Tensor& positions, const at::Tensor& turns,
+                 const c10::optional<at::Tensor>& axis, int64_t n_axes, int64_t B, int64_t L,
+                 int64_t D) {
+  const at::ScalarType dt = positions.scalar_type();
+  TORCH_CHECK(dt == at::kInt || dt == at::kLong, op, ": positions must be int32 or int64");
+  TORCH_CHECK(n_axes >= 1, op, ": the plan has no position axis");
+  const int64_t tok = positions.dim() - (n_axes > 1 ? 1 : 0);
+  TORCH_CHECK((tok == 1 || tok == 2) && positions.size(tok - 1) == L &&
+                  (tok == 1 || positions.size(0) == B || positions.size(0) == 1) &&
+                  (n_axes == 1 || positions.size(tok) == n_axes), op,
+              ": positions must be [L] or [B, L], with ", n_axes, " axes last when more than one");
+  want(op, turns, at::kDouble, "turns");
+  want(op, axis, at::kInt, "axis");
+  TORCH_CHECK(turns.dim() == 1 && turns.is_contiguous() && 2 * turns.numel() <= D &&
+                  (!axis.has_value() || (axis->is_contiguous() && axis->numel() == turns.numel())),
+              op, ": the plan turns ", 2 * turns.numel(), " channels of a head of ", D);
+  Turns r;
+  r.n_axes = n_axes;
+  r.n_pairs = turns.numel();
+  r.pos_i64 = dt == at::kLong;
+  r.pos_strides[0] = tok == 2 && positions.size(0) == B ? positions.stride(0) : 0;
+  r.pos_strides[1] = positions.stride(tok - 1);
+  r.pos_strides[2] = n_axes > 1 ? positions.stride(tok) : 0;
+  return r;
+}
+
+at::Tensor rope(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns,
+                const c10::optional<at::Tensor>& axis, int64_t n_axes, bool interleaved,
+                double scale, const c10::optional<at::Tensor>& out_) {
+  const char* op = "rope";
+  const Api& a = api(op);
+  int dev = -1;
+  on_device(op, dev, x, "x");
+  on_device(op, dev, positions, "positions");
+  on_device(op, dev, turns, "the plan");
+  on_device(op, dev, axis, "the plan");
+  on_device(op, dev, out_, "out");
+  const int code = float_code(op, x, "x");
+  want_rows(op, x, x.scalar_type(), "x");
+  const int64_t B = x.size(0), L = x.size(1), H = x.size(2), D = x.size(3);
+  const Turns t = want_turns(op, positions, turns, axis, n_axes, B, L, D);
+  const Launch l(device_of(op, dev));
+  const at::Tensor out = out_.has_value() ? *out_ : at::empty({B, L, H, D}, x.options());
+  want_rows(op, out, x.scalar_type(), "out");
+  want_own(op, out, "out");
+  TORCH_CHECK(out.sizes() == x.sizes(), op, ": out must have x's shape");
+  if (x.numel() == 0) return out;
+  int64_t s[6];
+  put_strides(x, s);
+  put_strides(out, s + 3);
+  check_status(a, op, a.rope(x.data_ptr(), out.data_ptr(), code, B, L, H, D, s,
+                             positions.data_ptr(), t.pos_i64, t.pos_strides, t.n_axes,
+                             ptr<const double>(turns), ptr<const int32_t>(axis), t.n_pairs,
+                             interleaved, static_cast<float>(scale), l.stream));
+  return out;
+}
+
+// A cache's table and the int32 [B] vectors of its requests.
+void want_table(const char* op, const at::Tensor& table, int64_t B) {
+  want(op, table, at::kInt, "the block table");
+  TORCH_CHECK(table.dim() == 2 && table.size(0) == B && table.size(1) > 0 &&
+                  (table.stride(1) == 1 || table.size(1) == 1), op,
+              ": the block table must be int32 [B, pages] with contiguous rows");
+}
+void want_vector(const char* op, const c10::optional<at::Tensor>& t, int64_t B, const char* name) {
+  want(op, t, at::kInt, name);
+  TORCH_CHECK(!t.has_value() || (t->dim() == 1 && t->size(0) == B && t->is_contiguous()), op, ": ",
+              name, " must be int32 [B]");
+}
+
+// (q_out, k_out); with pages k_out is empty, keys and values are in the pages.
+std::vector<at::Tensor> norm_rope(
+    const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& v,
+    const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
+    double eps, bool across_heads, const at::Tensor& positions, const at::Tensor& turns,
+    const c10::optional<at::Tensor>& axis, int64_t n_axes, bool interleaved, double scale,
+    const c10::optional<at::Tensor>& k_pages, const c10::optional<at::Tensor>& v_pages,
+    const c10::optional<at::Tensor>& table, const c10::optional<at::Tensor>& starts,
+    const c10::optional<at::Tensor>& lengths, const c10::optional<at::Tensor>& q_out_,
+    const c10::optional<at::Tensor>& k_out_) {
+  const char* op = "norm_rope";
+  const Api& a = api(op);
+  int dev = -1;
+  on_device(op, dev, q, "q");
+  on_device(op, dev, k, "k");
+  on_device(op, dev, positions, "positions");
+  on_device(op, dev, turns, "the plan");
+  for (const auto* t : {&v, &q_weight, &k_weight, &axis, &k_pages, &v_pages, &table, &starts,
+                        &lengths, &q_out_, &k_out_})
+    on_device(op, dev, *t, "an operand");
+  const int code = float_code(op, q, "q");
+  const at::ScalarType dt = q.scalar_type();
+  want_rows(op, q, dt, "q");
+  want_rows(op, k, dt, "k");
+  const int64_t B = q.size(0), L = q.size(1), Hq = q.size(2), Hk = k.size(2), D = q.size(3);
+  TORCH_CHECK(k.size(0) == B && k.size(1) == L && k.size(3) == D, op,
+              ": q and k differ in batch, tokens or channels");
+  const bool paged = table.has_value();
+  TORCH_CHECK(paged == v.has_value() && paged == k_pages.has_value() &&
+                  paged == v_pages.has_value() && !(paged && k_out_.has_value()) &&
+                  (paged || !starts.has_value()), op,
+              ": v, the pages and starts go with a block table, k_out without one");
+  const Turns t = want_turns(op, positions, turns, axis, n_axes, B, L, D);
+  int w_code = RCSA_F32;
+  int64_t ws[2] = {0, 0}, i = 0;
+  at::ScalarType w_dt = at::kFloat;
+  bool any = false;
+  for (const auto* w : {&q_weight, &k_weight}) {
+    if (w->has_value()) {
+      const int64_t H = i == 0 ? Hq : Hk;
+      w_code = float_code(op, **w, "a weight");
+      TORCH_CHECK(!any || (*w)->scalar_type() == w_dt, op, ": the weights must share a dtype");
+      any = true;
+      w_dt = (*w)->scalar_type();
+      TORCH_CHECK((*w)->is_contiguous() && (*w)->numel() % D == 0 &&
+                      ((*w)->numel() == D || (*w)->numel() == H * D), op,
+                  ": a weight must be contiguous [D] or [H, D]");
+      ws[i] = (*w)->numel() == D ? 0 : D;
+    }
+    ++i;
+  }
+  want_vector(op, starts, B, "starts");
+  want_vector(op, lengths, B, "lengths");
+  const Launch l(device_of(op, dev));
+  const at::Tensor q_out = q_out_.has_value() ? *q_out_ : at::empty({B, L, Hq, D}, q.options());
+  want_rows(op, q_out, dt, "q_out");
+  want_own(op, q_out, "q_out");
+  TORCH_CHECK(q_out.sizes() == q.sizes(), op, ": q_out must have q's shape");
+  int64_t s[18] = {};
+  put_strides(q, s);
+  put_strides(k, s + 3);
+  put_strides(q_out, s + 9);
+  at::Tensor k_out;
+  int64_t max_pages = 0, n_pages = 0, page = 0, table_stride = 0;
+  void* kp = nullptr;
+  if (paged) {
+    want_table(op, *table, B);
+    want_rows(op, *v, dt, "v");
+    want_rows(op, *k_pages, dt, "the key pages");
+    want_rows(op, *v_pages, dt, "the value pages");
+    want_own(op, *k_pages, "the key pages");
+    want_own(op, *v_pages, "the value pages");
+    TORCH_CHECK(v->sizes() == k.sizes(), op, ": v must have k's shape");
+    TORCH_CHECK(k_pages->sizes() == v_pages->sizes() && k_pages->size(2) == Hk &&
+                    k_pages->size(3) == D && k_pages->size(0) > 0 && k_pages->size(1) > 0, op,
+                ": the pages must be [pages, slots, ", Hk, ", ", D, "]");
+    put_strides(*v, s + 6);
+    put_strides(*k_pages, s + 12);
+    put_strides(*v_pages, s + 15);
+    max_pages = table->size(1);
+    table_stride = table->stride(0);
+    n_pages = k_pages->size(0);
+    page = k_pages->size(1);
+    kp = k_pages->data_ptr();
+    k_out = at::empty({0}, q.options());
+  } else {
+    k_out = k_out_.has_value() ? *k_out_ : at::empty({B, L, Hk, D}, k.options());
+    want_rows(op, k_out, dt, "k_out");
+    want_own(op, k_out, "k_out");
+    TORCH_CHECK(k_out.sizes() == k.sizes(), op, ": k_out must have k's shape");
+    put_strides(k_out, s + 12);
+    kp = k_out.data_ptr();
+  }
+  if (q.numel() == 0 || k.numel() == 0) {
+    TORCH_CHECK(B * L * D == 0, op, ": no heads");
+    return {q_out, k_out};
+  }
+  const int64_t dims[5] = {B, L, Hq, Hk, D};
+  check_status(a, op, a.norm_rope(
+      q.data_ptr(), k.data_ptr(), ptr<const void>(v), q_out.data_ptr(), kp,
+      paged ? v_pages->data_ptr() : nullptr, code, dims, s, ptr<const void>(q_weight),
+      ptr<const void>(k_weight), w_code, ws[0], ws[1], static_cast<float>(eps), across_heads,
+      positions.data_ptr(), t.pos_i64, t.pos_strides, t.n_axes, ptr<const double>(turns),
+      ptr<const int32_t>(axis), t.n_pairs, interleaved, static_cast<float>(scale),
+      ptr<const int32_t>(table), table_stride, max_pages, n_pages, page,
+      ptr<const int32_t>(starts), ptr<const int32_t>(lengths), l.stream));
+  return {q_out, k_out};
+}
+
+// Dense (k, v [B, Lk, Hk, D]) or, with a table, paged (k, v [pages, slots, Hk, D])
+// attention over a window and the first keys; n_split 0: planned.  (out) or (out, lse).
+std::vector<at::Tensor> window_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+    const c10::optional<at::Tensor>& table, const c10::optional<at::Tensor>& q_lengths,
+    const c10::optional<at::Tensor>& k_lengths, int64_t window, int64_t sinks, int64_t block,
+    double sm_scale, bool return_lse, const c10::optional<at::Tensor>& out_, int64_t n_split,
+    int64_t max_keys) {
+  const bool paged = table.has_value();
+  const char* op = paged ? "paged_attention" : "window_attention";
+  const Api& a = api(op);
+  int dev = -1;
+  on_device(op, dev, q, "q");
+  on_device(op, dev, k, "k");
+  on_device(op, dev, v, "v");
+  for (const auto* t : {&table, &q_lengths, &k_lengths, &out_}) on_device(op, dev, *t, "an operand");
+  const at::ScalarType dt = q.scalar_type();
+  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf, op, ": q must be bfloat16 or float16");
+  want_rows(op, q, dt, "q");
+  want_rows(op, k, dt, "k");
+  want_rows(op, v, dt, "v");
+  const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k.size(2);
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(3) == D && (paged || k.size(0) == B), op,
+              ": k and v must have one shape, and q's batch and channels");
+  want_vector(op, q_lengths, B, "q_lengths");
+  want_vector(op, k_lengths, B, "k_lengths");
+  int64_t max_pages = 0, n_pages = 0, page = 0, table_stride = 0, Lk = k.size(1);
+  if (paged) {
+    want_table(op, *table, B);
+    TORCH_CHECK(k_lengths.has_value() && k.size(0) > 0 && k.size(1) > 0, op,
+                ": needs lengths and pages");
+    max_pages = table->size(1);
+    table_stride = table->stride(0);
+    n_pages = k.size(0);
+    page = k.size(1);
+    Lk = max_pages * page;
+  }
+  const Launch l(device_of(op, dev));
+  const at::Tensor out = out_.has_value() ? *out_ : at::empty({B, Lq, Hq, D}, q.options());
+  want_rows(op, out, dt, "out");
+  want_own(op, out, "out");
+  TORCH_CHECK(out.sizes() == q.sizes(), op, ": out must have q's shape");
+  std::vector<at::Tensor> res{out};
+  if (return_lse) res.push_back(at::empty({B, Hq, Lq}, q.options().dtype(at::kFloat)));
+  if (q.numel() == 0) return res;
+  const int64_t dims[6] = {B, Lq, Lk, Hq, Hk, D};
+  int64_t s[12];
+  put_strides(q, s);
+  put_strides(k, s + 3);
+  put_strides(v, s + 6);
+  put_strides(out, s + 9);
+  int64_t ns = n_split;
+  if (ns < 1) {
+    int64_t most = max_keys >= 0 ? std::min(max_keys, Lk) : Lk;
+    if (window > 0) most = std::min(most, window + sinks + Lq);
+    check_status(a, op, a.window_attn_plan(dims, most, &ns));
+  }
+  at::Tensor ws;
+  int64_t ws_bytes = 0;
+  if (ns > 1) {
+    ws_bytes = a.window_attn_workspace_bytes(dims, ns);
+    TORCH_CHECK(ws_bytes >= 0, op, ": no workspace for ", ns, " shares");
+    ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+  }
+  const bool none = !paged && Lk == 0;  // no keys: no key memory either
+  check_status(a, op, a.window_attn(
+      q.data_ptr(), none ? q.data_ptr() : k.data_ptr(), none ? q.data_ptr() : v.data_ptr(),
+      out.data_ptr(), return_lse ? ptr<float>(res[1]) : nullptr,
+      dt == at::kBFloat16 ? RCSA_BF16 : RCSA_F16, dims, s, ptr<const int32_t>(q_lengths),
+      ptr<const int32_t>(k_lengths), ptr<const int32_t>(table), table_stride, max_pages, n_pages,
+      page, window, sinks, block, static_cast<float>(sm_scale), ns,
+      ns > 1 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
+  return res;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(rcsa, m) {
@@ -852,4 +1151,19 @@ TORCH_LIBRARY(rcsa, m) {
       "Tensor? allowed, int mask_stride_bh, bool int8, float sm_scale, bool return_lse, "
       "int n_split, Tensor? q_slot, Tensor? k_slot) -> Tensor[]",
       &layer_call);
+  m.def(
+      "rope(Tensor x, Tensor positions, Tensor turns, Tensor? axis, int n_axes, "
+      "bool interleaved, float scale, Tensor(a!)? out) -> Tensor",
+      &rope);
+  m.def(
+      "norm_rope(Tensor q, Tensor k, Tensor? v, Tensor? q_weight, Tensor? k_weight, float eps, "
+      "bool across_heads, Tensor positions, Tensor turns, Tensor? axis, int n_axes, "
+      "bool interleaved, float scale, Tensor(a!)? k_pages, Tensor(b!)? v_pages, Tensor? table, "
+      "Tensor? starts, Tensor? lengths, Tensor(c!)? q_out, Tensor(d!)? k_out) -> Tensor[]",
+      &norm_rope);
+  m.def(
+      "window_attention(Tensor q, Tensor k, Tensor v, Tensor? table, Tensor? q_lengths, "
+      "Tensor? k_lengths, int window, int sinks, int block, float sm_scale, bool return_lse, "
+      "Tensor(a!)? out, int n_split, int max_keys) -> Tensor[]",
+      &window_attention);
 }

@@ -1,0 +1,568 @@
+// Windowed attention, tiles of 128 rows: one pass over the visible keys with the
+// running maximum and sum of the softmax.
+//
+// Work: a workgroup takes 128 rows of one key head (32 a wavefront, 4
+// wavefronts) and streams the 32-key tiles that any of them sees: the tiles of
+// the first keys, then those of the window.  Three workgroups share a compute
+// unit, so that one's exponentials run beside another's matrix products.
+// A tile's K and V go global -> LDS without registers into a ring of three
+// slots; rows past the keys, and pages that are not there, land as zeros.
+// S^T = K Q^T puts one query row in a lane (its 16 + 16 keys in the two lane
+// halves), so a row's maximum and sum need one lane swap, and P^T is the second
+// operand of O^T = V^T P^T as it stands.  Only the tiles at the window's edges
+// are masked; a wavefront none of whose rows sees a tile only copies it.
+#include "window_attn.h"
+
+namespace rcsa {
+
+template <typename T, int D>
+struct WindowCfg {
+  static constexpr int BM = 128, NW = 4, STAGES = 3;
+  static constexpr int KROW = D * 2, CPR = KROW / 16;   // bytes and 16-byte chunks of a row
+  static constexpr int QSTEPS = D / 16, NDT = D / 32;
+  static constexpr int TILE = kTileKeys * KROW;         // bytes of a K (or V) tile
+  static constexpr int RPU = 1024 / KROW;               // rows of a 1 KiB copy
+  static constexpr int UPW = TILE / 1024 / NW;          // copies of a wavefront, K and V each
+  static constexpr int OPS = 2 * UPW;
+};
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3)))
+window_tile_kernel(WindowArgs a) {
+  using C = WindowCfg<T, D>;
+  using O = Half<T>;
+  typedef typename O::op8 op8;
+  __shared__ __attribute__((aligned(1024))) char s_0[2 * C::TILE];
+  __shared__ __attribute__((aligned(1024))) char s_1[2 * C::TILE];
+  __shared__ __attribute__((aligned(1024))) char s_2[2 * C::TILE];
+
+  // XCD x (workgroups go round-robin) runs a contiguous run of items: neighbours
+  // share most of their window in its L2.
+  const uint32_t ns = static_cast<uint32_t>(a.n_split);
+  const uint32_t items = static_cast<uint32_t>(a.n_items);
+  const uint32_t per = (items * ns + kNumXcd - 1) / kNumXcd;
+  const uint32_t at = (blockIdx.x % kNumXcd) * per + blockIdx.x / kNumXcd;
+  if (blockIdx.x / kNumXcd >= per || at >= items * ns) return;
+  const uint32_t item = at / ns, share = at - item * ns;
+  const uint32_t nrb = static_cast<uint32_t>(a.n_rblocks);
+  const int rb = static_cast<int>(item % nrb);
+  const int bh = static_cast<int>(item / nrb);
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hf = lane >> 5, lr = lane & 31;
+
+  const int cap = PAGED ? a.max_pages * a.page : a.Lk;
+  int k_len = a.k_len == nullptr ? cap : ld_const(a.k_len + b);
+  k_len = k_len < 0 ? 0 : (k_len > cap ? cap : k_len);
+  int q_len = a.q_len == nullptr ? a.Lq : ld_const(a.q_len + b);
+  q_len = q_len < 0 ? 0 : (q_len > a.Lq ? a.Lq : q_len);
+  const int n_rows = q_len * a.G;
+  const int row0 = rb * C::BM;
+  if (row0 >= n_rows) return;
+  const int shift = k_len - q_len;  // position of query 0
+
+  // this lane's row; rows past the last stand at the last one's place, unwritten
+  const int row = row0 + wave * 32 + lr;
+  const bool live = row < n_rows;
+  const int rrow = live ? row : n_rows - 1;
+  const int qi = rrow / a.G, head = hk * a.G + rrow - qi * a.G;
+  const KeyRange kr = key_range(a, qi + shift, k_len);
+  const int sink = a.sinks < kr.hi ? a.sinks : kr.hi;
+
+  // uniform ranges: of the item, and of this wavefront's first and last rows
+  auto range_of = [&](int r) __attribute__((always_inline)) -> KeyRange {
+    r = r < n_rows ? r : n_rows - 1;
+    return key_range(a, r / a.G + shift, k_len);
+  };
+  const KeyRange i_first = range_of(row0), i_last = range_of(row0 + C::BM - 1);
+  const KeyRange w_first = range_of(row0 + wave * 32), w_last = range_of(row0 + wave * 32 + 31);
+  const int sinks_hi = a.sinks < i_last.hi ? a.sinks : i_last.hi;
+  const int win_t0 = i_first.lo / kTileKeys;
+  const int win_n = (i_last.hi + kTileKeys - 1) / kTileKeys - win_t0;
+  int sink_n = (sinks_hi + kTileKeys - 1) / kTileKeys;
+  sink_n = sink_n < win_t0 ? sink_n : win_t0;
+  const int all = sink_n + (win_n > 0 ? win_n : 0);
+  const int s_begin = static_cast<int>(static_cast<int64_t>(all) * share / ns);
+  const int steps = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / ns) - s_begin;
+
+  const T* const qp = static_cast<const T*>(a.q) + b * a.sq[0] + static_cast<int64_t>(qi) * a.sq[1] +
+                      head * a.sq[2];
+  op8 q_op[C::QSTEPS];
+#pragma unroll
+  for (int st = 0; st < C::QSTEPS; ++st)
+    q_op[st] = *reinterpret_cast<const op8*>(qp + (hf * C::QSTEPS + st) * 8);
+
+  v16f o_acc[C::NDT];
+#pragma unroll
+  for (int dt = 0; dt < C::NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  const char* const kbase = static_cast<const char*>(a.k) +
+                            ((PAGED ? 0 : b * a.sk[0]) + hk * a.sk[2]) * 2;
+  const char* const vbase = static_cast<const char*>(a.v) +
+                            ((PAGED ? 0 : b * a.sv[0]) + hk * a.sv[2]) * 2;
+  const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
+  const int32_t* const table = PAGED ? a.table + b * a.table_stride : nullptr;
+
+  // Copies: wavefront w moves rows 8w .. 8w + 7 of the tile (of its half w / 2 of
+  // 16 rows, which lies in one page), RPU rows a copy, chunks swizzled by row.
+  uint32_t k_lo[C::UPW], v_lo[C::UPW];
+#pragma unroll
+  for (int i = 0; i < C::UPW; ++i) {
+    const int r = (wave * C::UPW + i) * C::RPU + lane / C::CPR;  // row of the tile
+    const uint32_t in_half = static_cast<uint32_t>(r & 15);
+    k_lo[i] = in_half * krb + (((lane % C::CPR) ^ (swz_k<C::KROW>(r) & (C::CPR - 1))) * 16);
+    v_lo[i] = in_half * vrb + (((lane % C::CPR) ^ (swz_v(r) & (C::CPR - 1))) * 16);
+  }
+  // A step: its first key and, paged, the pages of its two halves.
+  struct Step {
+    int key;        // -1: past the list
+    int page0, page1;
+    int slot0, slot1;
+  };
+  auto key_of = [&](int s) __attribute__((always_inline)) -> int {
+    const int t = s_begin + s;
+    return s >= steps ? -1 : (t < sink_n ? t : win_t0 + t - sink_n) * kTileKeys;
+  };
+  auto step_of = [&](int s) __attribute__((always_inline)) -> Step {
+    Step r{key_of(s), 0, 0, 0, 0};
+    if constexpr (PAGED) {
+      const uint32_t key = r.key < 0 ? 0u : static_cast<uint32_t>(r.key);
+      const uint32_t page = static_cast<uint32_t>(a.page);
+      uint32_t col0 = key / page;
+      r.slot0 = static_cast<int>(key - col0 * page);
+      r.slot1 = r.slot0 + 16;
+      uint32_t col1 = col0;
+      if (r.slot1 >= a.page) {
+        r.slot1 -= a.page;
+        ++col1;
+      }
+      const uint32_t last = static_cast<uint32_t>(a.max_pages) - 1u;
+      col1 = col1 < last ? col1 : last;
+      r.page0 = ld_const(table + col0);
+      r.page1 = ld_const(table + col1);
+    }
+    return r;
+  };
+  auto page_ok = [&](int p) __attribute__((always_inline)) -> bool {
+    return !PAGED || static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
+  };
+  auto stage = [&](const Step& s, char* dst) __attribute__((always_inline)) {
+    const int half = wave >> 1;
+    const int key = (s.key < 0 ? 0 : s.key) + 16 * half;
+    int64_t krow, vrow;
+    bool there = s.key >= 0;
+    if constexpr (PAGED) {
+      const int page = half ? s.page1 : s.page0;
+      const int64_t slot = half ? s.slot1 : s.slot0;
+      there = there && page_ok(page);
+      const int64_t pg = there ? page : 0;
+      krow = (pg * a.sk[0] + slot * a.sk[1]) * 2;
+      vrow = (pg * a.sv[0] + slot * a.sv[1]) * 2;
+    } else {
+      krow = static_cast<uint64_t>(static_cast<uint32_t>(key)) * krb;
+      vrow = static_cast<uint64_t>(static_cast<uint32_t>(key)) * vrb;
+    }
+    const int left = k_len - key;
+    const int rows = !there || left <= 0 ? 0 : (left < 16 ? left : 16);
+    char* const ks = const_cast<char*>(kbase) + (rows ? krow : 0);
+    char* const vs = const_cast<char*>(vbase) + (rows ? vrow : 0);
+    const int kn = rows ? (rows - 1) * static_cast<int>(krb) + C::KROW : 0;
+    const int vn = rows ? (rows - 1) * static_cast<int>(vrb) + C::KROW : 0;
+#pragma unroll
+    for (int i = 0; i < C::UPW; ++i) {
+      buffer_copy16(ks, kn, k_lo[i], dst + (wave * C::UPW + i) * 1024);
+      buffer_copy16(vs, vn, v_lo[i], dst + C::TILE + (wave * C::UPW + i) * 1024);
+    }
+  };
+
+  // LDS read offsets (tile and step offsets are immediates)
+  int k_off[C::QSTEPS];
+  {
+    const int r = key_perm(lr);
+    const int sw = swz_k<C::KROW>(r) & (C::CPR - 1);
+#pragma unroll
+    for (int st = 0; st < C::QSTEPS; ++st)
+      k_off[st] = r * C::KROW + (((hf * C::QSTEPS + st) ^ sw) * 16);
+  }
+  int v_off[C::NDT];
+  {
+    const int grp = lane >> 4, gi = lane & 15;
+    const int r = 16 * (grp >> 1) + (gi >> 2);
+    const int sw = swz_v(r) & (C::CPR - 1);
+#pragma unroll
+    for (int dt = 0; dt < C::NDT; ++dt) {
+      const int d = 32 * dt + 16 * (grp & 1) + 4 * (gi & 3);
+      v_off[dt] = C::TILE + r * C::KROW + (((d >> 3) ^ sw) * 16) + (d & 7) * 2;
+    }
+  }
+  v16f zero;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) zero[r] = 0.0f;
+
+  auto below = [&](int x) __attribute__((always_inline)) -> uint32_t {  // bits of keys < x
+    const int n = x < 0 ? 0 : (x > 16 ? 16 : x);
+    return (1u << n) - 1u;
+  };
+  auto compute = [&](const char* tile, const Step& s) __attribute__((always_inline)) {
+    const bool pages = page_ok(s.page0) && page_ok(s.page1);
+    // every row of the wavefront sees the whole tile
+    const bool inside = pages && s.key + kTileKeys <= w_first.hi &&
+                        (s.key >= w_last.lo || s.key + kTileKeys <= a.sinks);
+    v4i kraw[C::QSTEPS];
+#pragma unroll
+    for (int st = 0; st < C::QSTEPS; ++st)
+      kraw[st] = *reinterpret_cast<const v4i*>(tile + k_off[st]);
+    v16f s_acc = zero;
+#pragma unroll
+    for (int st = 0; st < C::QSTEPS; ++st)
+      s_acc = O::mfma(__builtin_bit_cast(op8, kraw[st]), q_op[st], s_acc);
+    float rv[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
+    if (!inside) {
+      const int k0 = s.key + 16 * hf;
+      uint32_t bits = below(kr.hi - k0) & (~below(kr.lo - k0) | below(sink - k0));
+      if (PAGED && !page_ok(hf ? s.page1 : s.page0)) bits = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rv[r] = ((bits >> r) & 1u) ? rv[r] : -INFINITY;
+    }
+    const float c = a.scale_log2;
+    op8 p_op[2];
+    auto exps = [&]() __attribute__((always_inline)) -> float {
+      const float bias = m_run == -INFINITY ? 0.0f : -m_run;
+      float lsum[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(rv[8 * u + jj], c, bias));
+          p_op[u][jj] = static_cast<T>(e);
+          if (u == 0 && jj < 4) lsum[jj] = e;
+          else lsum[jj & 3] += e;
+        }
+      return (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
+    };
+    // the running maximum moves only when a term passes 2^kTau (a lane's partial
+    // sum bounds its terms)
+    float part = exps();
+    if (__ballot(m_run == -INFINITY || !(part <= kTauPow)) != 0) {
+      float rmax = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
+      rmax = pair_max(rmax);
+      const float m_blk = rmax == -INFINITY ? -INFINITY : rmax * c;
+      if (__ballot(m_blk > m_run + kTau) != 0) {
+        const float m_new = fmaxf(m_run, m_blk);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < C::NDT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+        m_run = m_new;
+        part = exps();
+      }
+    }
+    l_run += part;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int dt = 0; dt < C::NDT; ++dt) {
+        const char* p0 = tile + v_off[dt] + 8 * u * C::KROW;
+        const auto lo = O::read_tr(p0);
+        const auto hi = O::read_tr(p0 + 4 * C::KROW);
+        o_acc[dt] = O::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), p_op[u],
+                            o_acc[dt]);
+      }
+  };
+
+  // ring: step j in slot j % 3, two steps in flight; every step copies (past the
+  // list through empty ranges), so every wait counts the same operations
+  Step st[C::STAGES];
+  st[0] = step_of(0);
+  st[1] = step_of(1);
+  stage(st[0], s_0);
+  __builtin_amdgcn_sched_barrier(0);
+  stage(st[1], s_1);
+  __builtin_amdgcn_sched_barrier(0);
+  Step next = step_of(2);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * C::OPS));  // Q has landed
+  auto iteration = [&](auto slot_c, int j) __attribute__((always_inline)) {
+    constexpr int J = decltype(slot_c)::value;
+    constexpr int F = (J + C::STAGES - 1) % C::STAGES;
+    char* const tile = J == 0 ? s_0 : J == 1 ? s_1 : s_2;
+    char* const fill = F == 0 ? s_0 : F == 1 ? s_1 : s_2;
+    wait_vm_barrier<C::OPS>();
+    st[F] = next;
+    stage(st[F], fill);
+    __builtin_amdgcn_sched_barrier(0);
+    next = step_of(j + C::STAGES);
+    const Step& s = st[J];
+    const bool seen = s.key >= 0 && s.key < w_last.hi &&
+                      (s.key + kTileKeys > w_first.lo || s.key < a.sinks);
+    if (seen) compute(tile, s);
+  };
+  const int rounds = (steps + C::STAGES - 1) / C::STAGES;
+  for (int rd = 0; rd < rounds; ++rd) {
+    const int j = rd * C::STAGES;
+    iteration(std::integral_constant<int, 0>{}, j);
+    iteration(std::integral_constant<int, 1>{}, j + 1);
+    iteration(std::integral_constant<int, 2>{}, j + 2);
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
+
+  const float l = pair_sum(l_run), m = m_run;
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (a NaN sum stays one)
+  bool bad = false;  // a product that is no number in a row whose sum is one
+#pragma unroll
+  for (int dt = 0; dt < C::NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      o_acc[dt][r] *= inv;
+      bad = bad || !(fabsf(o_acc[dt][r]) < INFINITY);
+    }
+  const int64_t wrow = (static_cast<int64_t>(share) * a.n_items + item) * C::BM + row - row0;
+  T* const op = static_cast<T*>(a.out) + b * a.so[0] + static_cast<int64_t>(qi) * a.so[1] +
+                head * a.so[2];
+  if (live) {
+#pragma unroll
+    for (int dt = 0; dt < C::NDT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d0 = 32 * dt + 8 * g + 4 * hf;
+        if (ns > 1) {
+          *reinterpret_cast<v4f*>(a.ws_o + wrow * D + d0) =
+              v4f{o_acc[dt][4 * g], o_acc[dt][4 * g + 1], o_acc[dt][4 * g + 2],
+                  o_acc[dt][4 * g + 3]};
+        } else {
+          typename O::op4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(o_acc[dt][4 * g + e]);
+          *reinterpret_cast<typename O::op4*>(op + d0) = w;
+        }
+      }
+    if (hf == 0) {
+      if (ns > 1)
+        a.ws_ml[wrow] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
+      else if (a.lse)
+        a.lse[(static_cast<int64_t>(b) * a.Hq + head) * a.Lq + qi] =
+            l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+    }
+  }
+  // A row whose products met a value that it does not see (0 * inf or 0 * NaN of a
+  // masked key): its sum is taken again over its own keys, one row at a time.
+  uint64_t again = __ballot(bad && live && l > 0.0f && l < INFINITY);
+  again |= again >> 32;
+  if (static_cast<uint32_t>(again) == 0) return;
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the stores above come first)
+  for (uint32_t rows = static_cast<uint32_t>(again); rows != 0; rows &= rows - 1) {
+    constexpr int N = D / 64;
+    const int i = __builtin_ctz(rows);
+    const int r = row0 + wave * 32 + i;
+    const int ri = r / a.G, rh = hk * a.G + r - ri * a.G;
+    const KeyRange rk = key_range(a, ri + shift, k_len);
+    const int rsink = a.sinks < rk.hi ? a.sinks : rk.hi;
+    const T* const rq = static_cast<const T*>(a.q) + b * a.sq[0] +
+                        static_cast<int64_t>(ri) * a.sq[1] + rh * a.sq[2];
+    const float rm = __shfl(m, i, kWave), rinv = __shfl(inv, i, kWave);
+    float acc[N], qv[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      acc[c] = 0.0f;
+      qv[c] = static_cast<float>(rq[lane + 64 * c]);
+    }
+    for (int s = 0; s < steps; ++s)
+      for (int j = key_of(s), end = j + kTileKeys; j < end; ++j) {
+        if (!(j < rk.hi && (j >= rk.lo || j < rsink))) continue;
+        int64_t ko = j * a.sk[1], vo = j * a.sv[1];
+        if constexpr (PAGED) {
+          const int page = table[j / a.page];
+          if (!page_ok(page)) continue;
+          const int64_t slot = j % a.page;
+          ko = page * a.sk[0] + slot * a.sk[1];
+          vo = page * a.sv[0] + slot * a.sv[1];
+        }
+        const T* const kp = reinterpret_cast<const T*>(kbase) + ko;
+        const T* const vp = reinterpret_cast<const T*>(vbase) + vo;
+        float x = 0.0f;
+#pragma unroll
+        for (int c = 0; c < N; ++c) x = fmaf(qv[c], static_cast<float>(kp[lane + 64 * c]), x);
+        const float p = __builtin_amdgcn_exp2f(fmaf(wave_sum(x), a.scale_log2, -rm));
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+          acc[c] = fmaf(p, static_cast<float>(vp[lane + 64 * c]), acc[c]);
+      }
+    const int64_t wr = (static_cast<int64_t>(share) * a.n_items + item) * C::BM + r - row0;
+    T* const dst = static_cast<T*>(a.out) + b * a.so[0] + static_cast<int64_t>(ri) * a.so[1] +
+                   rh * a.so[2];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (ns > 1) a.ws_o[wr * D + lane + 64 * c] = acc[c] * rinv;
+      else dst[lane + 64 * c] = static_cast<T>(acc[c] * rinv);
+    }
+  }
+}
+
+// The shares of every row joined: w_s = l_s 2^(m_s - M), out = sum w_s O_s / sum w_s.
+// One thread per row and 8 channels; the shares are added in their order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_merge_kernel(WindowArgs a, int rows_per_item) {
+  constexpr int CPR = D / 8;
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t all_rows = a.n_items * rows_per_item;
+  const int64_t wrow = v / CPR;
+  if (wrow >= all_rows) return;
+  const int c = static_cast<int>(v % CPR);
+  const int64_t item = wrow / rows_per_item;
+  const int64_t bh = item / a.n_rblocks;
+  const int b = static_cast<int>(bh / a.Hk), hk = static_cast<int>(bh % a.Hk);
+  int q_len = a.q_len == nullptr ? a.Lq : a.q_len[b];
+  q_len = q_len < 0 ? 0 : (q_len > a.Lq ? a.Lq : q_len);
+  const int64_t row = (item % a.n_rblocks) * rows_per_item + wrow % rows_per_item;
+  if (row >= static_cast<int64_t>(q_len) * a.G) return;
+  const int qi = static_cast<int>(row / a.G);
+  const int head = hk * a.G + static_cast<int>(row % a.G);
+  float mx = -INFINITY;
+  for (int s = 0; s < a.n_split; ++s) mx = fmaxf(mx, a.ws_ml[s * all_rows + wrow].x);
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float sum = 0.0f;
+  for (int s = 0; s < a.n_split; ++s) {
+    const float2 ml = a.ws_ml[s * all_rows + wrow];
+    if (ml.x == -INFINITY) continue;
+    const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+    sum += w;
+    float o[8];
+    Vec8<float>::load(a.ws_o + (s * all_rows + wrow) * D + c * 8, o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, o[j], acc[j]);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  typename Half<T>::op8 r;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = static_cast<T>(acc[j] * inv);
+  T* const op = static_cast<T*>(a.out) + b * a.so[0] + qi * a.so[1] + head * a.so[2] + c * 8;
+  *reinterpret_cast<typename Half<T>::op8*>(op) = r;
+  if (a.lse && c == 0)
+    a.lse[(static_cast<int64_t>(b) * a.Hq + head) * a.Lq + qi] =
+        sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
+}
+
+template <typename T, int D>
+static int launch_window(WindowArgs& a, hipStream_t s) {
+  const int64_t wgs = (a.n_items * a.n_split + kNumXcd - 1) / kNumXcd * kNumXcd;
+  if (wgs >= (1ll << 31)) return RCSA_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>(wgs));
+  if (a.table) window_tile_kernel<T, D, true><<<grid, dim3(256), 0, s>>>(a);
+  else window_tile_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
+  if (a.n_split > 1) {
+    const int64_t n = (a.n_items * 128 * (D / 8) + 255) / 256;
+    if (n >= (1ll << 31)) return RCSA_ERR_SHAPE;
+    window_merge_kernel<T, D><<<dim3(static_cast<unsigned>(n)), dim3(256), 0, s>>>(a, 128);
+  }
+  return launch_status();
+}
+
+// Blocks of rows of a key head.
+static int64_t row_blocks(int64_t Lq, int64_t G) { return (Lq * G + 127) / 128; }
+
+static bool window_dims(const int64_t* d) {
+  for (int i = 0; i < 6; ++i)
+    if (d[i] <= 0 && !(i == 2 && d[i] == 0)) return false;
+  return d[4] <= d[3] && d[3] % d[4] == 0 && d[0] < (1 << 20) && d[1] < (1 << 24) &&
+         d[3] < (1 << 16) && d[1] * (d[3] / d[4]) < (1 << 30) && (d[5] == 64 || d[5] == 128) &&
+         d[0] * d[4] * row_blocks(d[1], d[3] / d[4]) < (1ll << 26);
+}
+
+}  // namespace rcsa
+
+using namespace rcsa;
+
+// Shares of every item.  Workgroups run three to a compute unit; an item costs
+// its steps plus a fixed part of about kFixed steps (Q, first tile, epilogue).
+extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
+  if (!dims || !n_split) return RCSA_ERR_NULL;
+  if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
+  *n_split = 1;
+  return RCSA_OK;
+}
+
+extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
+  if (!dims || !window_dims(dims) || n_split < 1 || n_split > 64) return -1;
+  if (n_split == 1) return 0;
+  const int64_t rows = dims[0] * dims[4] * row_blocks(dims[1], dims[3] / dims[4]) * 128;
+  return n_split * rows * (dims[5] * 4 + 8);
+}
+
+extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
+                                int dtype, const int64_t* dims, const int64_t* strides,
+                                const int32_t* q_lengths, const int32_t* k_lengths,
+                                const int32_t* block_table, int64_t table_stride,
+                                int64_t max_pages, int64_t n_pages, int64_t page_size,
+                                int64_t window, int64_t sinks, int64_t block, float sm_scale,
+                                int64_t n_split, void* workspace, int64_t workspace_bytes,
+                                hipStream_t stream) {
+  if (!q || !k || !v || !out || !dims || !strides) return RCSA_ERR_NULL;
+  if (dtype != RCSA_BF16 && dtype != RCSA_F16) return RCSA_ERR_DTYPE;
+  if (!window_dims(dims)) return RCSA_ERR_SHAPE;
+  const int64_t most = 1ll << 30;  // positions, windows and blocks stay far from 2^31
+  if (dims[2] >= most || window < 0 || sinks < 0 || block < 0) return RCSA_ERR_SHAPE;
+  if (block == 0 && (window != 0 || sinks != 0)) return RCSA_ERR_SHAPE;
+  if (block_table && (max_pages <= 0 || n_pages <= 0 || page_size <= 0 || page_size % 16 ||
+                      n_pages >= most || page_size >= most || max_pages >= most / page_size))
+    return RCSA_ERR_SHAPE;
+  if (n_split < 1 || n_split > 64) return RCSA_ERR_SHAPE;
+  for (int i = 0; i < 12; ++i)
+    if (strides[i] < 0 || strides[i] % (i < 9 ? 8 : 4)) return RCSA_ERR_STRIDE;
+  if (strides[4] >= (1 << 25) || strides[7] >= (1 << 25)) return RCSA_ERR_STRIDE;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(workspace) ||
+      (reinterpret_cast<uintptr_t>(out) & 7u))
+    return RCSA_ERR_ALIGN;
+  if (n_split > 1 && (!workspace ||
+                      workspace_bytes < rcsa_window_attn_workspace_bytes(dims, n_split)))
+    return RCSA_ERR_SHAPE;
+  WindowArgs a{};
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.lse = lse;
+  for (int i = 0; i < 3; ++i) {
+    a.sq[i] = strides[i];
+    a.sk[i] = strides[3 + i];
+    a.sv[i] = strides[6 + i];
+    a.so[i] = strides[9 + i];
+  }
+  a.B = static_cast<int>(dims[0]);
+  a.Lq = static_cast<int>(dims[1]);
+  a.Lk = static_cast<int>(dims[2]);
+  a.Hq = static_cast<int>(dims[3]);
+  a.Hk = static_cast<int>(dims[4]);
+  a.G = a.Hq / a.Hk;
+  a.q_len = q_lengths;
+  a.k_len = k_lengths;
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.max_pages = static_cast<int>(max_pages);
+  a.n_pages = static_cast<int>(n_pages);
+  a.page = static_cast<int>(page_size);
+  a.window = static_cast<int>(window < most ? window : 0);
+  a.sinks = static_cast<int>(sinks < most ? sinks : most);
+  a.block = static_cast<int>(block < most ? block : most);
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.n_rblocks = static_cast<int>(row_blocks(a.Lq, a.G));
+  a.n_items = static_cast<int64_t>(a.B) * a.Hk * a.n_rblocks;
+  a.n_split = static_cast<int>(n_split);
+  a.ws_o = static_cast<float*>(workspace);
+  a.ws_ml = n_split > 1 ? reinterpret_cast<float2*>(a.ws_o + n_split * a.n_items * 128 * dims[5])
+                        : nullptr;
+  if (dtype == RCSA_BF16)
+    return dims[5] == 128 ? launch_window<__bf16, 128>(a, stream)
+                          : launch_window<__bf16, 64>(a, stream);
+  return dims[5] == 128 ? launch_window<_Float16, 128>(a, stream)
+                        : launch_window<_Float16, 64>(a, stream);
+}

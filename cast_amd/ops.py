@@ -20,7 +20,8 @@ from ._lib import (RCSA_BF16, RCSA_F32, RCSA_ORDER_INDEX, RCSA_ORDER_RANK,
 __all__ = [
     "pool_query", "pool_key", "block_scores", "select_topk", "quantize_key",
     "sparse_attn_bf16", "sparse_attn_int8", "pack_tokens", "unpack_tokens", "row_budgets",
-    "quantize_key_select", "order_lists",
+    "quantize_key_select", "order_lists", "rope", "norm_rope", "PagedCache",
+    "window_attention", "paged_attention",
 ]
 
 
@@ -1171,3 +1172,187 @@ def int8_linear_group(x_i8: torch.Tensor, x_scale: torch.Tensor, projections, *,
     _lib.torch_ops().int8_linear_group(x_i8, xs, [p[0] for p in ready], [p[1] for p in ready],
                                        [p[2] for p in ready], outs)
     return outs
+
+
+def _no_grad(fn: str, *tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{fn}: no gradient is computed; call it under torch.no_grad()")
+
+
+def _heads(x: torch.Tensor, name: str, fn: str) -> None:
+    if x.ndim != 4 or (x.stride(3) != 1 and x.shape[3] > 1):
+        raise ValueError(f"{fn}: {name} must be [B, L, H, D] with a contiguous last dim, "
+                         f"got {tuple(x.shape)}")
+
+
+def _plan_fits(plan, D: int, fn: str) -> None:
+    if plan.rotary_dim > D:
+        raise ValueError(f"{fn}: the plan turns {plan.rotary_dim} channels of a head of {D}")
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, plan, *,
+         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x [B, L, H, D]`` (bf16, fp16 or fp32, any strides) with its first channels turned by
+    position (``rcsa_rope``).
+
+    ``plan``: a :class:`cast_amd.rotary.RotaryPlan`.  ``positions``: int32 or int64 ``[L]`` or
+    ``[B, L]``, with the plan's axes last when it has more than one; any sign (negated
+    positions undo a rotation of scale 1), as far as 64-bit angles reach.  fp32 between, one
+    rounding at the end.  ``out`` (x's shape and dtype, any strides) may be ``x`` itself and
+    must not overlap it otherwise."""
+    fn = "rope"
+    _require_cuda(fn, x, positions, plan.turns)
+    _no_grad(fn, x)
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"{fn}: expected bfloat16, float16 or float32, got {x.dtype}")
+    _heads(x, "x", fn)
+    _plan_fits(plan, x.shape[3], fn)
+    return _lib.torch_ops().rope(x, positions, plan.turns, plan.axis, plan.n_axes,
+                                 plan.interleaved, plan.scale, out)
+
+
+class PagedCache(NamedTuple):
+    """Keys and values in pages, and the pages of every request: key j of request b is row
+    ``j % slots`` of page ``table[b, j // slots]``; an entry outside the pages hides its
+    keys."""
+    k: torch.Tensor      # [pages, slots, Hk, D]
+    v: torch.Tensor      # [pages, slots, Hk, D]
+    table: torch.Tensor  # int32 [B, pages of a request]
+
+
+def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan, *,
+              q_weight: Optional[torch.Tensor] = None,
+              k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              across_heads: bool = False, v: Optional[torch.Tensor] = None,
+              cache: Optional[PagedCache] = None, starts: Optional[torch.Tensor] = None,
+              lengths: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
+              k_out: Optional[torch.Tensor] = None):
+    """RMS norms of ``q [B, L, Hq, D]`` and ``k [B, L, Hk, D]`` and the rotation of
+    :func:`rope`, in one pass (``rcsa_norm_rope``).
+
+    ``x * rsqrt(mean(x^2) + eps) * weight``, the mean over a head or, with
+    ``across_heads``, over all heads of a token (the reference normalises the whole
+    projection, P/matrix_curvature_phase_frame_weave.py:5391-5393); a weight is ``[D]`` or
+    ``[H, D]`` (None: 1).  Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be q / k.
+
+    With ``cache`` the keys, and ``v [B, L, Hk, D]`` as it is, go to the cache instead: token
+    t of request b to index ``starts[b] + t`` (int32 ``[B]``; None: t), dropped where the
+    table has no page for it; ``k_out`` is then None.  No two tokens may go to one row.
+    ``lengths`` (int32 ``[B]``) leaves the rows of tokens ``t >= lengths[b]`` as they were."""
+    fn = "norm_rope"
+    _require_cuda(fn, q, k, positions, plan.turns)
+    _no_grad(fn, q, k, v, q_weight, k_weight)
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"{fn}: expected bfloat16, float16 or float32, got {q.dtype}")
+    if k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+        raise TypeError(f"{fn}: q, k and v must share a dtype")
+    _heads(q, "q", fn)
+    _heads(k, "k", fn)
+    _plan_fits(plan, q.shape[3], fn)
+    if (cache is None) != (v is None):
+        raise ValueError(f"{fn}: give v and cache together")
+    if cache is None and starts is not None:
+        raise ValueError(f"{fn}: starts goes with a cache")
+    if cache is not None and k_out is not None:
+        raise ValueError(f"{fn}: k_out goes without a cache")
+    kp, vp, table = cache if cache is not None else (None, None, None)
+    qo, ko = _lib.torch_ops().norm_rope(
+        q, k, v, q_weight, k_weight, float(eps), bool(across_heads), positions, plan.turns,
+        plan.axis, plan.n_axes, plan.interleaved, plan.scale, kp, vp, table, starts, lengths,
+        q_out, k_out)
+    return qo, (ko if cache is None else None)
+
+
+def _window(window, sinks, block, causal, fn: str) -> tuple[int, int, int]:
+    """(window, sinks, block) as the kernel reads them (0: no window, no order)."""
+    if window is not None and window <= 0:
+        raise ValueError(f"{fn}: window must be positive (None: no window), got {window}")
+    if sinks < 0 or block <= 0:
+        raise ValueError(f"{fn}: sinks must not be negative and block must be positive")
+    if not causal:
+        if window is not None or sinks or block != 1:
+            raise ValueError(f"{fn}: window, sinks and block go with causal rows")
+        return 0, 0, 0
+    return (0, 0, int(block)) if window is None else (int(window), int(sinks), int(block))
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
+                     window: Optional[int] = None, sinks: int = 0, block: int = 1,
+                     causal: bool = True, q_lengths: Optional[torch.Tensor] = None,
+                     k_lengths: Optional[torch.Tensor] = None,
+                     sm_scale: Optional[float] = None, return_lse: bool = False,
+                     out: Optional[torch.Tensor] = None, n_split: Optional[int] = None):
+    """Attention of ``q [B, Lq, Hq, D]`` over a sliding window of ``k, v [B, Lk, Hk, D]``
+    and their first ``sinks`` keys (``rcsa_window_attn``); bf16 or fp16, Hq a multiple of
+    Hk, D 64 or 128, any 16-byte aligned strides.
+
+    The queries are the last positions: query i is at ``p = i + Lk - Lq`` and sees the keys
+    below ``e = (p // block + 1) * block`` that are at or past ``e - window`` or among the
+    first ``sinks``.  ``block`` 1 is causal by token; a frame's tokens as ``block`` see
+    their whole frame.  ``window=None`` sees every key below e, ``causal=False`` every key.
+    ``q_lengths`` / ``k_lengths`` (int32 ``[B]``) are the own lengths of a padded batch:
+    rows past a request's queries stay as they were (give ``out``), keys past its keys are
+    not read.  A row that sees no key gives 0 (LSE -inf); a key or value that a row does not
+    see does not reach it, whatever it holds.
+
+    fp32 softmax, rounded once; returns ``out [B, Lq, Hq, D]`` and, with ``return_lse``, the
+    natural log-sum-exp ``[B, Hq, Lq]``.  ``n_split`` (None: planned) shares the keys of
+    a block of rows among that many workgroups."""
+    fn = "window_attention"
+    _require_cuda(fn, q, k, v)
+    _no_grad(fn, q, k, v)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{fn}: q, k and v must share bfloat16 or float16")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _heads(t, name, fn)
+    B, _, Hq, D = q.shape
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hq % max(k.shape[2], 1):
+        raise ValueError(f"{fn}: q {tuple(q.shape)} needs k and v [{B}, Lk, a divisor of {Hq}, "
+                         f"{D}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    w, s, b = _window(window, sinks, block, causal, fn)
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    res = _lib.torch_ops().window_attention(q, k, v, None, q_lengths, k_lengths, w, s, b, scale,
+                                            return_lse, out, _shares(n_split, fn), -1)
+    return tuple(res) if return_lse else res[0]
+
+
+def _shares(n_split: Optional[int], fn: str) -> int:
+    if n_split is not None and n_split < 1:
+        raise ValueError(f"{fn}: n_split must be positive, got {n_split}")
+    return 0 if n_split is None else int(n_split)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *,
+                    q_lengths: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                    sinks: int = 0, block: int = 1, causal: bool = True,
+                    sm_scale: Optional[float] = None, return_lse: bool = False,
+                    out: Optional[torch.Tensor] = None, max_length: Optional[int] = None,
+                    n_split: Optional[int] = None):
+    """:func:`window_attention` of ``q [B, T, Hq, D]``, the last T positions of every request
+    (one new token, or a chunk), over a :class:`PagedCache`: ``lengths`` (int32 ``[B]``) keys
+    of each request, the new ones among them.  Pages hold a multiple of 16 keys.
+
+    Pages that no row sees are not read, so their table entries may be anything; an entry
+    outside the pages hides its keys.  ``max_length`` bounds the lengths (what the table
+    holds, if None): it only plans how the keys are shared among workgroups, a longer
+    request is still read to its end."""
+    fn = "paged_attention"
+    _require_cuda(fn, q, cache.k, cache.v, cache.table, lengths)
+    _no_grad(fn, q, cache.k, cache.v)
+    if q.dtype not in (torch.bfloat16, torch.float16) or cache.k.dtype != q.dtype \
+            or cache.v.dtype != q.dtype:
+        raise TypeError(f"{fn}: q and the pages must share bfloat16 or float16")
+    _heads(q, "q", fn)
+    B, _, Hq, D = q.shape
+    kp = cache.k
+    if kp.ndim != 4 or kp.shape != cache.v.shape or kp.shape[3] != D \
+            or Hq % max(kp.shape[2], 1) or kp.shape[1] % 16:
+        raise ValueError(f"{fn}: q {tuple(q.shape)} needs pages [pages, slots (a multiple of 16), "
+                         f"a divisor of {Hq}, {D}], got {tuple(kp.shape)} and "
+                         f"{tuple(cache.v.shape)}")
+    w, s, b = _window(window, sinks, block, causal, fn)
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    res = _lib.torch_ops().window_attention(
+        q, kp, cache.v, cache.table, q_lengths, lengths, w, s, b, scale, return_lse, out,
+        _shares(n_split, fn), -1 if max_length is None else int(max_length))
+    return tuple(res) if return_lse else res[0]

@@ -39,8 +39,9 @@ enum {
   RCSA_ERR_SCRATCH = 7   /* the request exceeds the library's static scratch */
 };
 
-/* Element type codes for inputs that may be bf16 or fp32. */
-enum { RCSA_BF16 = 0, RCSA_F32 = 1 };
+/* Element type codes for inputs that may be bf16 or fp32 (the rotary and the windowed
+ * entry points also take fp16). */
+enum { RCSA_BF16 = 0, RCSA_F32 = 1, RCSA_F16 = 2 };
 
 /* Selection output order. */
 enum {
@@ -681,6 +682,86 @@ int rcsa_int8_linear_group(const int8_t* x, const float* x_scale, int64_t n_line
                            const void* const* bias, const int64_t* N, void* const* out,
                            const int64_t* ldo, int out_f32, int64_t M, int64_t K,
                            hipStream_t stream);
+
+/*
+ * Rotary positions, with the norms of queries and keys.  No reference kernel: the
+ * reference applies its norms and its (frame, row, column) rotation in torch ahead of
+ * the layer (P/matrix_curvature_phase_frame_weave.py:5391-5403).
+ *
+ * rcsa_rope: x [B][L][H][D] (bf16, fp16 or fp32; strides: host array, batch, token and
+ * head stride of x, then of out) -> out, which may be x itself (same strides) and must
+ * not overlap it otherwise.  Pair i < n_pairs of every head, channels (i, n_pairs + i) or
+ * (interleaved) (2i, 2i + 1), turns by position[axis[i]] * turns[i] whole turns:
+ *   a' = scale (a cos - b sin), b' = scale (a sin + b cos);
+ * channels from 2 n_pairs on pass through.  positions: int32, or int64 when
+ * positions_i64, addressed with pos_strides (host array: batch, token, axis); turns fp64
+ * [n_pairs]; axis int32 [n_pairs] in [0, n_axes), NULL: all 0.  The product is taken and
+ * reduced in 64 bits, so far positions lose nothing.  D <= 512, H <= 4096.  Rows of
+ * 16-byte aligned tensors with D a multiple of 16 (up to 256) and n_pairs of 8 move as
+ * vectors; any other shape runs element by element.
+ *
+ * rcsa_norm_rope: q [B][L][Hq][D] and k [B][L][Hk][D], dims = {B, L, Hq, Hk, D},
+ *   y = x * rsqrt(mean(x^2) + eps) * weight, then the rotation of rcsa_rope,
+ * with the mean over a head or (across_heads) over all heads of the token; weights (NULL:
+ * 1) of type weight_dtype, one [D] for all heads (stride 0) or [H][D] (stride D), 16-byte
+ * aligned for the vector form.  strides: host array of 18, batch/token/head of q, k, v,
+ * q_out, k_out, v_out.  Without block_table k_out is [B][L][Hk][D] and v, v_out are NULL.
+ * With it k_out and v_out are the pages of a cache (their strides: page, slot, head), v
+ * [B][L][Hk][D] is copied beside the keys, and token t of request b goes to index
+ * at = starts[b] + t (starts NULL: t), row at % page_size of page
+ * block_table[b * table_stride + at / page_size]; a row whose page is not in
+ * [0, n_pages), or past max_pages, is dropped.  No row may appear twice.  lengths
+ * (nullable, int32 [B]): tokens t >= lengths[b] are neither read nor written.
+ */
+int rcsa_rope(const void* x, void* out, int dtype, int64_t batch, int64_t len, int64_t heads,
+              int64_t head_dim, const int64_t* strides, const void* positions, int positions_i64,
+              const int64_t* pos_strides, int64_t n_axes, const double* turns,
+              const int32_t* axis, int64_t n_pairs, int interleaved, float scale,
+              hipStream_t stream);
+int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                   void* v_out, int dtype, const int64_t* dims, const int64_t* strides,
+                   const void* q_weight, const void* k_weight, int weight_dtype,
+                   int64_t q_weight_stride, int64_t k_weight_stride, float eps, int across_heads,
+                   const void* positions, int positions_i64, const int64_t* pos_strides,
+                   int64_t n_axes, const double* turns, const int32_t* axis, int64_t n_pairs,
+                   int interleaved, float scale, const int32_t* block_table,
+                   int64_t table_stride, int64_t max_pages, int64_t n_pages, int64_t page_size,
+                   const int32_t* starts, const int32_t* lengths, hipStream_t stream);
+
+/*
+ * Attention over a sliding window and the first keys, dense or paged.  No reference
+ * kernel: the reference's dense layers call an external attention
+ * (P/matrix_curvature_phase_frame_weave.py:5446-5455).
+ *
+ * dims = {B, Lq, Lk, Hq, Hk, D}: q [B][Lq][Hq][D], out alike, bf16 or fp16, Hq a multiple
+ * of Hk, D 64 or 128; k, v [B][Lk][Hk][D], or with block_table pages [n_pages][page_size]
+ * [Hk][D] (page_size a multiple of 16; Lk unused), key j of request b in row
+ * j % page_size of page block_table[b * table_stride + j / page_size].  strides: host
+ * array of 12, batch (page), token (slot) and head stride of q, k, v, out.  q_lengths,
+ * k_lengths (nullable, int32 [B], clamped to the storage) give the requests' own lengths.
+ * Query i of a request is at position p = i + k_len - q_len and sees key j when
+ *   j < min(e, k_len) and (j >= e - window or j < sinks), e = (floor(p / block) + 1) block;
+ * window 0: no window; block 1: by token, n: by blocks of n positions (frames), 0: every
+ * key (window and sinks 0).  A page that is not in [0, n_pages) hides its keys.
+ *   out = softmax(sm_scale q k) v in fp32, rounded once; lse (nullable) [B][Hq][Lq] the
+ * natural log of the row's sum; a row that sees nothing gives 0 and -inf.  What a row
+ * does not see does not reach it, NaN and infinities included.  Rows i >= q_len are left
+ * as they were.  q, k, v rows 16-byte, out rows 8-byte aligned.
+ *
+ * n_split (1 to 64) shares the keys of every block of rows among as many workgroups; more
+ * than 1 needs a workspace of rcsa_window_attn_workspace_bytes (16-byte aligned, used by
+ * this call alone until it ends).  rcsa_window_attn_plan picks n_split; max_keys bounds
+ * the keys that a row sees.
+ */
+int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split);
+int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split);
+int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
+                     int dtype, const int64_t* dims, const int64_t* strides,
+                     const int32_t* q_lengths, const int32_t* k_lengths,
+                     const int32_t* block_table, int64_t table_stride, int64_t max_pages,
+                     int64_t n_pages, int64_t page_size, int64_t window, int64_t sinks,
+                     int64_t block, float sm_scale, int64_t n_split, void* workspace,
+                     int64_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }
