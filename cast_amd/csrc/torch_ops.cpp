@@ -1025,7 +1025,7 @@ std::vector<at::Tensor> norm_rope(
 }
 
 // Dense (k, v [B, Lk, Hk, D]) or, with a table, paged (k, v [pages, slots, Hk, D])
-// attention over a window and the first keys; n_split 0: planned.  (out) or (out, lse).
+// attention over a window and the first keys; n_split -1: planned.  (out) or (out, lse).
 std::vector<at::Tensor> window_attention(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const c10::optional<at::Tensor>& table, const c10::optional<at::Tensor>& q_lengths,
@@ -1076,18 +1076,17 @@ std::vector<at::Tensor> window_attention(
   put_strides(v, s + 6);
   put_strides(out, s + 9);
   int64_t ns = n_split;
-  if (ns < 1) {
+  if (ns < 0) {
     int64_t most = max_keys >= 0 ? std::min(max_keys, Lk) : Lk;
     if (window > 0) most = std::min(most, window + sinks + Lq);
     check_status(a, op, a.window_attn_plan(dims, most, &ns));
   }
   at::Tensor ws;
   int64_t ws_bytes = 0;
-  if (ns > 1) {
-    ws_bytes = a.window_attn_workspace_bytes(dims, ns);
-    TORCH_CHECK(ws_bytes >= 0, op, ": no workspace for ", ns, " shares");
-    ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
-  }
+  ws_bytes = a.window_attn_workspace_bytes(dims, ns);
+  TORCH_CHECK(ws_bytes >= 0, op, ": no launch of ", ns, " shares for q ", q.sizes(), ", k ",
+              k.sizes());
+  if (ws_bytes > 0) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
   const bool none = !paged && Lk == 0;  // no keys: no key memory either
   check_status(a, op, a.window_attn(
       q.data_ptr(), none ? q.data_ptr() : k.data_ptr(), none ? q.data_ptr() : v.data_ptr(),
@@ -1095,7 +1094,7 @@ std::vector<at::Tensor> window_attention(
       dt == at::kBFloat16 ? RCSA_BF16 : RCSA_F16, dims, s, ptr<const int32_t>(q_lengths),
       ptr<const int32_t>(k_lengths), ptr<const int32_t>(table), table_stride, max_pages, n_pages,
       page, window, sinks, block, static_cast<float>(sm_scale), ns,
-      ns > 1 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
+      ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
   return res;
 }
 

@@ -37,7 +37,12 @@ struct WindowArgs {
   int n_split;
   float* ws_o;                      // [n_split][n_items][rows][D] normalised partial outputs
   float2* ws_ml;                    // [n_split][n_items][rows] their (max, sum)
+  // few rows (one wavefront a unit): units wanted in all, 0: one a key head
+  int units;
 };
+
+constexpr int kFewRows = 32;        // rows of a key head that one wavefront takes
+constexpr int kMaxPlanned = 512;    // requests whose lengths every wavefront reads
 
 // The keys of a position: [0, sink) and [lo, hi).
 struct KeyRange {
@@ -50,6 +55,99 @@ __device__ __forceinline__ KeyRange key_range(const WindowArgs& a, int p, int k_
   const int hi = e < k_len ? e : k_len;
   const int lo = a.window == 0 || e <= a.window ? 0 : e - a.window;
   return {lo < hi ? lo : hi, hi};
+}
+
+// A request's lengths, clamped to the storage.
+struct Request {
+  int k_len, q_len;
+};
+__device__ __forceinline__ Request request_of(const WindowArgs& a, int b) {
+  const int cap = a.table != nullptr ? a.max_pages * a.page : a.Lk;
+  int k = a.k_len == nullptr ? cap : a.k_len[b];
+  int q = a.q_len == nullptr ? a.Lq : a.q_len[b];
+  k = k < 0 ? 0 : (k > cap ? cap : k);
+  q = q < 0 ? 0 : (q > a.Lq ? a.Lq : q);
+  return {k, q};
+}
+// The tiles that rows of key ranges first .. last see: sink_n of the first keys, then win_n
+// from tile win_t0 on.
+struct Tiles {
+  int sink_n, win_t0, win_n;
+  __device__ __forceinline__ int all() const { return sink_n + win_n; }
+};
+__device__ __forceinline__ Tiles tiles_of(const WindowArgs& a, KeyRange first, KeyRange last) {
+  const int sinks = a.sinks < last.hi ? a.sinks : last.hi;
+  Tiles t;
+  t.win_t0 = first.lo / kTileKeys;
+  t.win_n = (last.hi + kTileKeys - 1) / kTileKeys - t.win_t0;
+  t.win_n = t.win_n < 0 ? 0 : t.win_n;
+  t.sink_n = (sinks + kTileKeys - 1) / kTileKeys;
+  t.sink_n = t.sink_n < t.win_t0 ? t.sink_n : t.win_t0;
+  return t;
+}
+
+// Few rows: the visible tiles of all requests are dealt to about a.units wavefronts in
+// units of `chunk` tiles of one key head, however uneven the lengths.  A wavefront
+// reads the lengths (one lane a request) and finds its unit; u = (units of the
+// requests before) * Hk + share * Hk + hk.
+constexpr int kLeastTiles = 2;
+__device__ __forceinline__ int request_tiles(const WindowArgs& a, int b) {
+  const Request r = request_of(a, b);
+  if (r.q_len == 0) return -1;
+  const int p = r.k_len - r.q_len;
+  return tiles_of(a, key_range(a, p, r.k_len), key_range(a, p + r.q_len - 1, r.k_len)).all();
+}
+// Tiles of a unit: all lanes of the wavefront call it.
+__device__ __forceinline__ int unit_chunk(const WindowArgs& a, int lane) {
+  if (a.units == 0) return 1 << 30;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const int n = b0 + lane < a.B ? request_tiles(a, b0 + lane) : 0;
+    int s = n > 0 ? n : 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
+    total += s;
+  }
+  const int64_t c = (total * a.Hk + a.units - 1) / a.units;
+  return c < kLeastTiles ? kLeastTiles : static_cast<int>(c);
+}
+__device__ __forceinline__ int units_of(int tiles, int chunk) {
+  return tiles < 0 ? 0 : (tiles <= chunk ? 1 : (tiles + chunk - 1) / chunk);
+}
+// Units of the requests before b (all lanes call it).
+__device__ __forceinline__ int units_before(const WindowArgs& a, int b, int chunk, int lane) {
+  if (a.units == 0) return b;
+  int s = 0;
+  for (int b0 = 0; b0 < b; b0 += kWave)
+    if (b0 + lane < b) s += units_of(request_tiles(a, b0 + lane), chunk);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
+  return s;
+}
+// The request, share and number of shares of unit index w (of one key head), b -1 past
+// the last (all lanes call it).
+struct Unit {
+  int b, share, shares;
+};
+__device__ __forceinline__ Unit unit_at(const WindowArgs& a, int w, int chunk, int lane) {
+  if (a.units == 0) return {w < a.B ? w : -1, 0, 1};
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const int n = b0 + lane < a.B ? units_of(request_tiles(a, b0 + lane), chunk) : 0;
+    int sum = n;  // inclusive prefix over the lanes
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+      const int up = __shfl_up(sum, o, kWave);
+      if (lane >= o) sum += up;
+    }
+    const uint64_t past = __ballot(before + sum > w);
+    if (past != 0) {
+      const int l = __builtin_ctzll(past);
+      return {b0 + l, w - before - __shfl(sum - n, l, kWave), __shfl(n, l, kWave)};
+    }
+    before += __shfl(sum, kWave - 1, kWave);
+  }
+  return {-1, 0, 0};
 }
 
 template <typename T>

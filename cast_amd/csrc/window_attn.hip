@@ -15,9 +15,9 @@
 
 namespace rcsa {
 
-template <typename T, int D>
+template <typename T, int D, int NW_>
 struct WindowCfg {
-  static constexpr int BM = 128, NW = 4, STAGES = 3;
+  static constexpr int NW = NW_, BM = 32 * NW, STAGES = 3;
   static constexpr int KROW = D * 2, CPR = KROW / 16;   // bytes and 16-byte chunks of a row
   static constexpr int QSTEPS = D / 16, NDT = D / 32;
   static constexpr int TILE = kTileKeys * KROW;         // bytes of a K (or V) tile
@@ -26,40 +26,58 @@ struct WindowCfg {
   static constexpr int OPS = 2 * UPW;
 };
 
-template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3)))
-window_tile_kernel(WindowArgs a) {
-  using C = WindowCfg<T, D>;
+template <typename T, int D, bool PAGED, int NW>
+__global__ void __launch_bounds__(64 * NW)
+__attribute__((amdgpu_waves_per_eu(NW == 1 ? 1 : 3, 3)))
+window_kernel(WindowArgs a) {
+  using C = WindowCfg<T, D, NW>;
   using O = Half<T>;
   typedef typename O::op8 op8;
   __shared__ __attribute__((aligned(1024))) char s_0[2 * C::TILE];
   __shared__ __attribute__((aligned(1024))) char s_1[2 * C::TILE];
   __shared__ __attribute__((aligned(1024))) char s_2[2 * C::TILE];
 
-  // XCD x (workgroups go round-robin) runs a contiguous run of items: neighbours
-  // share most of their window in its L2.
-  const uint32_t ns = static_cast<uint32_t>(a.n_split);
-  const uint32_t items = static_cast<uint32_t>(a.n_items);
-  const uint32_t per = (items * ns + kNumXcd - 1) / kNumXcd;
-  const uint32_t at = (blockIdx.x % kNumXcd) * per + blockIdx.x / kNumXcd;
-  if (blockIdx.x / kNumXcd >= per || at >= items * ns) return;
-  const uint32_t item = at / ns, share = at - item * ns;
-  const uint32_t nrb = static_cast<uint32_t>(a.n_rblocks);
-  const int rb = static_cast<int>(item % nrb);
-  const int bh = static_cast<int>(item / nrb);
-  const int b = bh / a.Hk, hk = bh - b * a.Hk;
-
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, lr = lane & 31;
 
-  const int cap = PAGED ? a.max_pages * a.page : a.Lk;
-  int k_len = a.k_len == nullptr ? cap : ld_const(a.k_len + b);
-  k_len = k_len < 0 ? 0 : (k_len > cap ? cap : k_len);
-  int q_len = a.q_len == nullptr ? a.Lq : ld_const(a.q_len + b);
-  q_len = q_len < 0 ? 0 : (q_len > a.Lq ? a.Lq : q_len);
+  // The work of this workgroup: rows row0 .. of key head hk of request b, share `share` of
+  // the `ns` shares of their tiles; its rows of the workspace start at ws_row.
+  int b, hk, row0, share;
+  uint32_t ns;
+  int64_t ws_row;
+  if constexpr (NW > 1) {
+    // XCD x (workgroups go round-robin) runs a contiguous run of items: neighbours
+    // share most of their window in its L2.
+    ns = static_cast<uint32_t>(a.n_split);
+    const uint32_t items = static_cast<uint32_t>(a.n_items);
+    const uint32_t per = (items * ns + kNumXcd - 1) / kNumXcd;
+    const uint32_t at = (blockIdx.x % kNumXcd) * per + blockIdx.x / kNumXcd;
+    if (at >= items * ns) return;
+    const uint32_t item = at / ns;
+    share = static_cast<int>(at - item * ns);
+    const uint32_t nrb = static_cast<uint32_t>(a.n_rblocks);
+    row0 = static_cast<int>(item % nrb) * C::BM;
+    const int bh = static_cast<int>(item / nrb);
+    b = bh / a.Hk;
+    hk = bh - b * a.Hk;
+    ws_row = (static_cast<int64_t>(share) * a.n_items + item) * C::BM;
+  } else {
+    const int chunk = unit_chunk(a, lane);
+    const int w = static_cast<int>(blockIdx.x) / a.Hk;
+    const Unit u = unit_at(a, w, chunk, lane);
+    if (u.b < 0) return;
+    b = __builtin_amdgcn_readfirstlane(u.b);
+    share = __builtin_amdgcn_readfirstlane(u.share);
+    ns = __builtin_amdgcn_readfirstlane(u.shares);
+    hk = static_cast<int>(blockIdx.x) - w * a.Hk;
+    row0 = 0;
+    ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
+  }
+  const Request rq = request_of(a, b);
+  const int k_len = __builtin_amdgcn_readfirstlane(rq.k_len);
+  const int q_len = __builtin_amdgcn_readfirstlane(rq.q_len);
   const int n_rows = q_len * a.G;
-  const int row0 = rb * C::BM;
   if (row0 >= n_rows) return;
   const int shift = k_len - q_len;  // position of query 0
 
@@ -78,12 +96,8 @@ window_tile_kernel(WindowArgs a) {
   };
   const KeyRange i_first = range_of(row0), i_last = range_of(row0 + C::BM - 1);
   const KeyRange w_first = range_of(row0 + wave * 32), w_last = range_of(row0 + wave * 32 + 31);
-  const int sinks_hi = a.sinks < i_last.hi ? a.sinks : i_last.hi;
-  const int win_t0 = i_first.lo / kTileKeys;
-  const int win_n = (i_last.hi + kTileKeys - 1) / kTileKeys - win_t0;
-  int sink_n = (sinks_hi + kTileKeys - 1) / kTileKeys;
-  sink_n = sink_n < win_t0 ? sink_n : win_t0;
-  const int all = sink_n + (win_n > 0 ? win_n : 0);
+  const Tiles tl = tiles_of(a, i_first, i_last);
+  const int sink_n = tl.sink_n, win_t0 = tl.win_t0, all = tl.all();
   const int s_begin = static_cast<int>(static_cast<int64_t>(all) * share / ns);
   const int steps = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / ns) - s_begin;
 
@@ -108,8 +122,9 @@ window_tile_kernel(WindowArgs a) {
   const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
   const int32_t* const table = PAGED ? a.table + b * a.table_stride : nullptr;
 
-  // Copies: wavefront w moves rows 8w .. 8w + 7 of the tile (of its half w / 2 of
-  // 16 rows, which lies in one page), RPU rows a copy, chunks swizzled by row.
+  // Copies: of four wavefronts, w moves rows 8w .. 8w + 7 of the tile (of its half w / 2 of
+  // 16 rows, which lies in one page), RPU rows a copy, chunks swizzled by row; a
+  // single one moves both halves.
   uint32_t k_lo[C::UPW], v_lo[C::UPW];
 #pragma unroll
   for (int i = 0; i < C::UPW; ++i) {
@@ -151,8 +166,9 @@ window_tile_kernel(WindowArgs a) {
   auto page_ok = [&](int p) __attribute__((always_inline)) -> bool {
     return !PAGED || static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
   };
-  auto stage = [&](const Step& s, char* dst) __attribute__((always_inline)) {
-    const int half = wave >> 1;
+  // copies [i0, i0 + n) of a step, all in half `half` of its tile
+  auto stage_half = [&](const Step& s, char* dst, int half, int i0, auto n_c)
+      __attribute__((always_inline)) {
     const int key = (s.key < 0 ? 0 : s.key) + 16 * half;
     int64_t krow, vrow;
     bool there = s.key >= 0;
@@ -174,9 +190,17 @@ window_tile_kernel(WindowArgs a) {
     const int kn = rows ? (rows - 1) * static_cast<int>(krb) + C::KROW : 0;
     const int vn = rows ? (rows - 1) * static_cast<int>(vrb) + C::KROW : 0;
 #pragma unroll
-    for (int i = 0; i < C::UPW; ++i) {
-      buffer_copy16(ks, kn, k_lo[i], dst + (wave * C::UPW + i) * 1024);
-      buffer_copy16(vs, vn, v_lo[i], dst + C::TILE + (wave * C::UPW + i) * 1024);
+    for (int i = 0; i < decltype(n_c)::value; ++i) {
+      buffer_copy16(ks, kn, k_lo[i0 + i], dst + (wave * C::UPW + i0 + i) * 1024);
+      buffer_copy16(vs, vn, v_lo[i0 + i], dst + C::TILE + (wave * C::UPW + i0 + i) * 1024);
+    }
+  };
+  auto stage = [&](const Step& s, char* dst) __attribute__((always_inline)) {
+    if constexpr (NW == 1) {
+      stage_half(s, dst, 0, 0, std::integral_constant<int, C::UPW / 2>{});
+      stage_half(s, dst, 1, C::UPW / 2, std::integral_constant<int, C::UPW / 2>{});
+    } else {
+      stage_half(s, dst, wave >> 1, 0, std::integral_constant<int, C::UPW>{});
     }
   };
 
@@ -326,7 +350,7 @@ window_tile_kernel(WindowArgs a) {
       o_acc[dt][r] *= inv;
       bad = bad || !(fabsf(o_acc[dt][r]) < INFINITY);
     }
-  const int64_t wrow = (static_cast<int64_t>(share) * a.n_items + item) * C::BM + row - row0;
+  const int64_t wrow = ws_row + row - row0;
   T* const op = static_cast<T*>(a.out) + b * a.so[0] + static_cast<int64_t>(qi) * a.so[1] +
                 head * a.so[2];
   if (live) {
@@ -397,7 +421,7 @@ window_tile_kernel(WindowArgs a) {
         for (int c = 0; c < N; ++c)
           acc[c] = fmaf(p, static_cast<float>(vp[lane + 64 * c]), acc[c]);
       }
-    const int64_t wr = (static_cast<int64_t>(share) * a.n_items + item) * C::BM + r - row0;
+    const int64_t wr = ws_row + r - row0;
     T* const dst = static_cast<T*>(a.out) + b * a.so[0] + static_cast<int64_t>(ri) * a.so[1] +
                    rh * a.so[2];
 #pragma unroll
@@ -452,13 +476,82 @@ __global__ void __launch_bounds__(256) window_merge_kernel(WindowArgs a, int row
         sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
 }
 
+// The same for units of few rows: a workgroup takes one row, its threads (share,
+// 8 channels); the shares are added in a fixed order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
+  constexpr int CPR = D / 8, GROUPS = 256 / CPR;
+  __shared__ float s_acc[GROUPS][D], s_sum[GROUPS], s_max[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int R = a.Lq * a.G;
+  const int row = static_cast<int>(blockIdx.x) % R;
+  const int bh = static_cast<int>(blockIdx.x) / R;
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const Request rq = request_of(a, b);
+  if (row >= rq.q_len * a.G) return;
+  const int chunk = unit_chunk(a, lane);
+  const int shares = units_of(request_tiles(a, b), chunk);
+  if (shares <= 1) return;  // written by its only unit
+  const int64_t first = static_cast<int64_t>(units_before(a, b, chunk, lane)) * a.Hk + hk;
+  auto at = [&](int s) __attribute__((always_inline)) -> int64_t {
+    return (first + static_cast<int64_t>(s) * a.Hk) * R + row;
+  };
+  float mx = -INFINITY;
+  for (int s = tid; s < shares; s += 256) mx = fmaxf(mx, a.ws_ml[at(s)].x);
+  mx = wave_max(mx);
+  if (lane == 0) s_max[tid >> 6] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  const int c = tid % CPR, g = tid / CPR;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float sum = 0.0f;
+  for (int s = g; s < shares; s += GROUPS) {
+    const float2 ml = a.ws_ml[at(s)];
+    if (ml.x == -INFINITY) continue;
+    const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+    sum += w;
+    float o[8];
+    Vec8<float>::load(a.ws_o + at(s) * D + c * 8, o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, o[j], acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s_acc[g][c * 8 + j] = acc[j];
+  if (c == 0) s_sum[g] = sum;
+  __syncthreads();
+  if (tid >= D) return;
+  float total = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    total += s_sum[i];
+    o += s_acc[i][tid];
+  }
+  const int qi = row / a.G, head = hk * a.G + row - qi * a.G;
+  static_cast<T*>(a.out)[b * a.so[0] + qi * a.so[1] + head * a.so[2] + tid] =
+      static_cast<T>(total == 0.0f ? 0.0f : o / total);
+  if (a.lse && tid == 0)
+    a.lse[(static_cast<int64_t>(b) * a.Hq + head) * a.Lq + qi] =
+        total == 0.0f ? -INFINITY : (mx + __log2f(total)) * 0.69314718055994531f;
+}
+
 template <typename T, int D>
 static int launch_window(WindowArgs& a, hipStream_t s) {
+  if (a.n_split == 0) {
+    const int64_t n = a.units + static_cast<int64_t>(a.B) * a.Hk;
+    const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * a.Lq * a.G;
+    if (n >= (1ll << 31) || rows >= (1ll << 31)) return RCSA_ERR_SHAPE;
+    const dim3 grid(static_cast<unsigned>(n));
+    if (a.table) window_kernel<T, D, true, 1><<<grid, dim3(64), 0, s>>>(a);
+    else window_kernel<T, D, false, 1><<<grid, dim3(64), 0, s>>>(a);
+    if (a.units)
+      window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
+    return launch_status();
+  }
   const int64_t wgs = (a.n_items * a.n_split + kNumXcd - 1) / kNumXcd * kNumXcd;
   if (wgs >= (1ll << 31)) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs));
-  if (a.table) window_tile_kernel<T, D, true><<<grid, dim3(256), 0, s>>>(a);
-  else window_tile_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
+  if (a.table) window_kernel<T, D, true, 4><<<grid, dim3(256), 0, s>>>(a);
+  else window_kernel<T, D, false, 4><<<grid, dim3(256), 0, s>>>(a);
   if (a.n_split > 1) {
     const int64_t n = (a.n_items * 128 * (D / 8) + 255) / 256;
     if (n >= (1ll << 31)) return RCSA_ERR_SHAPE;
@@ -469,6 +562,13 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
 
 // Blocks of rows of a key head.
 static int64_t row_blocks(int64_t Lq, int64_t G) { return (Lq * G + 127) / 128; }
+
+// Units of few rows wanted in all: kUnits, as four rounds of the three wavefronts that
+// share a compute unit's LDS.  Every wavefront reads all lengths to find its unit, so
+// past kMaxPlanned requests each key head is one unit.
+constexpr int64_t kUnits = 3072;
+static bool few_rows(const int64_t* d) { return d[1] * (d[3] / d[4]) <= kFewRows; }
+static int64_t wanted_units(const int64_t* d) { return d[0] > kMaxPlanned ? 0 : kUnits; }
 
 static bool window_dims(const int64_t* d) {
   for (int i = 0; i < 6; ++i)
@@ -482,20 +582,24 @@ static bool window_dims(const int64_t* d) {
 
 using namespace rcsa;
 
-// Shares of every item.  Workgroups run three to a compute unit; an item costs
-// its steps plus a fixed part of about kFixed steps (Q, first tile, epilogue).
+// Few rows of a key head go to units of one wavefront (n_split 0), more to tiles of 128
+// rows in n_split shares.
 extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
-  *n_split = 1;
+  *n_split = few_rows(dims) ? 0 : 1;
   return RCSA_OK;
 }
 
 extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
-  if (!dims || !window_dims(dims) || n_split < 1 || n_split > 64) return -1;
+  if (!dims || !window_dims(dims) || n_split < 0 || n_split > 64) return -1;
+  const int64_t G = dims[3] / dims[4], row = dims[5] * 4 + 8;
+  if (n_split == 0)
+    return !few_rows(dims) ? -1
+           : wanted_units(dims) == 0
+               ? 0 : (wanted_units(dims) + dims[0] * dims[4]) * dims[1] * G * row;
   if (n_split == 1) return 0;
-  const int64_t rows = dims[0] * dims[4] * row_blocks(dims[1], dims[3] / dims[4]) * 128;
-  return n_split * rows * (dims[5] * 4 + 8);
+  return n_split * dims[0] * dims[4] * row_blocks(dims[1], G) * 128 * row;
 }
 
 extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
@@ -515,16 +619,15 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   if (block_table && (max_pages <= 0 || n_pages <= 0 || page_size <= 0 || page_size % 16 ||
                       n_pages >= most || page_size >= most || max_pages >= most / page_size))
     return RCSA_ERR_SHAPE;
-  if (n_split < 1 || n_split > 64) return RCSA_ERR_SHAPE;
+  if (n_split < 0 || n_split > 64 || (n_split == 0 && !few_rows(dims))) return RCSA_ERR_SHAPE;
   for (int i = 0; i < 12; ++i)
     if (strides[i] < 0 || strides[i] % (i < 9 ? 8 : 4)) return RCSA_ERR_STRIDE;
   if (strides[4] >= (1 << 25) || strides[7] >= (1 << 25)) return RCSA_ERR_STRIDE;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(workspace) ||
       (reinterpret_cast<uintptr_t>(out) & 7u))
     return RCSA_ERR_ALIGN;
-  if (n_split > 1 && (!workspace ||
-                      workspace_bytes < rcsa_window_attn_workspace_bytes(dims, n_split)))
-    return RCSA_ERR_SHAPE;
+  const int64_t need = rcsa_window_attn_workspace_bytes(dims, n_split);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return RCSA_ERR_SHAPE;
   WindowArgs a{};
   a.q = q;
   a.k = k;
@@ -557,9 +660,10 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   a.n_rblocks = static_cast<int>(row_blocks(a.Lq, a.G));
   a.n_items = static_cast<int64_t>(a.B) * a.Hk * a.n_rblocks;
   a.n_split = static_cast<int>(n_split);
+  a.units = n_split == 0 ? static_cast<int>(wanted_units(dims)) : 0;
+  const int64_t ws_rows = need / (dims[5] * 4 + 8);
   a.ws_o = static_cast<float*>(workspace);
-  a.ws_ml = n_split > 1 ? reinterpret_cast<float2*>(a.ws_o + n_split * a.n_items * 128 * dims[5])
-                        : nullptr;
+  a.ws_ml = need ? reinterpret_cast<float2*>(a.ws_o + ws_rows * dims[5]) : nullptr;
   if (dtype == RCSA_BF16)
     return dims[5] == 128 ? launch_window<__bf16, 128>(a, stream)
                           : launch_window<__bf16, 64>(a, stream);

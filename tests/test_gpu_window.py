@@ -138,6 +138,22 @@ def test_lengths_past_the_storage_and_negative(dev):
     _check(out, None, q, k, v, [4, 4, 0], [50, 20, 50], 0, 0, 1, True, 1 / 8, fill=9.0)
 
 
+def test_many_requests(dev):
+    """More requests than a wavefront has lanes, and more than it plans for: every length,
+    none too, one new token."""
+    from cast_amd import ops
+    for B in (70, 600):
+        q, k, v = _inputs(B, B, 1, 97, 4, 2, 64, BF)
+        k_len = [(37 * b) % 98 for b in range(B)]
+        q_len = [int(b % 11 != 3) for b in range(B)]
+        out = torch.full(q.shape, 9.0, dtype=BF, device=dev)
+        got, lse = ops.window_attention(
+            q.to(dev), k.to(dev), v.to(dev), out=out, return_lse=True,
+            q_lengths=torch.tensor(q_len, dtype=torch.int32, device=dev),
+            k_lengths=torch.tensor(k_len, dtype=torch.int32, device=dev))
+        _check(out, lse, q, k, v, q_len, k_len, 0, 0, 1, True, 1 / 8, fill=9.0)
+
+
 def test_no_keys(dev):
     from cast_amd import ops
     q, k, v = (t.to(dev) for t in _inputs(1, 2, 5, 0, 2, 2, 64, BF))

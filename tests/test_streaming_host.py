@@ -112,7 +112,10 @@ def test_window_abi_refusals(lib, kw, status):
 def test_window_plan_and_workspace(lib):
     n = ctypes.c_int64(-1)
     assert lib.rcsa_window_attn_plan(_arr(1, 1, 4096, 8, 8, 128), 4096, ctypes.byref(n)) == 0
+    assert n.value == 0  # few rows: units of one wavefront
+    assert lib.rcsa_window_attn_plan(_arr(1, 64, 4096, 8, 8, 128), 4096, ctypes.byref(n)) == 0
     assert 1 <= n.value <= 64
+    assert lib.rcsa_window_attn_workspace_bytes(_arr(1, 64, 64, 8, 8, 128), 0) == -1
     assert lib.rcsa_window_attn_plan(_arr(1, 1, 4096, 8, 3, 128), 4096, ctypes.byref(n)) == SHAPE
     assert lib.rcsa_window_attn_workspace_bytes(_arr(1, 1, 64, 8, 8, 128), 1) == 0
     assert lib.rcsa_window_attn_workspace_bytes(_arr(1, 1, 64, 8, 8, 128), 65) == -1
