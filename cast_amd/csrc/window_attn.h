@@ -30,6 +30,8 @@ struct WindowArgs {
   const int32_t* table;             // [B][max_pages], nullable: dense k, v
   int64_t table_stride;
   int max_pages, n_pages, page;     // page: keys of a page, a multiple of 16
+  uint32_t page_mul;                // division of half tiles by the halves of a page
+  int page_sh1, page_sh2;
   int window, sinks, block;         // block 0: no order among positions
   float scale_log2;                 // sm_scale * log2(e)
   int n_rblocks;                    // blocks of rows of a key head

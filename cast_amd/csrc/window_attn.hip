@@ -38,7 +38,7 @@ window_kernel(WindowArgs a) {
   __shared__ __attribute__((aligned(1024))) char s_2[2 * C::TILE];
 
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hf = lane >> 5, lr = lane & 31;
 
   // The work of this workgroup: rows row0 .. of key head hk of request b, share `share` of
@@ -81,13 +81,23 @@ window_kernel(WindowArgs a) {
   if (row0 >= n_rows) return;
   const int shift = k_len - q_len;  // position of query 0
 
-  // this lane's row; rows past the last stand at the last one's place, unwritten
-  const int row = row0 + wave * 32 + lr;
-  const bool live = row < n_rows;
-  const int rrow = live ? row : n_rows - 1;
-  const int qi = rrow / a.G, head = hk * a.G + rrow - qi * a.G;
-  const KeyRange kr = key_range(a, qi + shift, k_len);
-  const int sink = a.sinks < kr.hi ? a.sinks : kr.hi;
+  // This lane's row; rows past the last stand at the last one's place, unwritten.  (Its
+  // place and keys are found again where they are needed: registers are short.)
+  struct Row {
+    int row, qi, head;
+    bool live;
+  };
+  auto my_row = [&]() __attribute__((always_inline)) -> Row {
+    int row = row0 + wave * 32 + lr;
+    asm volatile("" : "+v"(row));
+    Row r;
+    r.row = row;
+    r.live = row < n_rows;
+    const int at = r.live ? row : n_rows - 1;
+    r.qi = at / a.G;
+    r.head = hk * a.G + at - r.qi * a.G;
+    return r;
+  };
 
   // uniform ranges: of the item, and of this wavefront's first and last rows
   auto range_of = [&](int r) __attribute__((always_inline)) -> KeyRange {
@@ -101,12 +111,15 @@ window_kernel(WindowArgs a) {
   const int s_begin = static_cast<int>(static_cast<int64_t>(all) * share / ns);
   const int steps = static_cast<int>(static_cast<int64_t>(all) * (share + 1) / ns) - s_begin;
 
-  const T* const qp = static_cast<const T*>(a.q) + b * a.sq[0] + static_cast<int64_t>(qi) * a.sq[1] +
-                      head * a.sq[2];
   op8 q_op[C::QSTEPS];
+  {
+    const Row r = my_row();
+    const T* const qp = static_cast<const T*>(a.q) + b * a.sq[0] +
+                        static_cast<int64_t>(r.qi) * a.sq[1] + r.head * a.sq[2];
 #pragma unroll
-  for (int st = 0; st < C::QSTEPS; ++st)
-    q_op[st] = *reinterpret_cast<const op8*>(qp + (hf * C::QSTEPS + st) * 8);
+    for (int st = 0; st < C::QSTEPS; ++st)
+      q_op[st] = *reinterpret_cast<const op8*>(qp + (hf * C::QSTEPS + st) * 8);
+  }
 
   v16f o_acc[C::NDT];
 #pragma unroll
@@ -133,75 +146,84 @@ window_kernel(WindowArgs a) {
     k_lo[i] = in_half * krb + (((lane % C::CPR) ^ (swz_k<C::KROW>(r) & (C::CPR - 1))) * 16);
     v_lo[i] = in_half * vrb + (((lane % C::CPR) ^ (swz_v(r) & (C::CPR - 1))) * 16);
   }
-  // A step: its first key and, paged, the pages of its two halves.
+  // A step: its first key (-1: past the list) and, paged, the pages of its two halves
+  // until they are staged, then whether they are there (bits 0 and 1).
   struct Step {
-    int key;        // -1: past the list
-    int page0, page1;
-    int slot0, slot1;
+    int key, page0, page1;
+  };
+  struct Staged {
+    int key, there;
   };
   auto key_of = [&](int s) __attribute__((always_inline)) -> int {
     const int t = s_begin + s;
     return s >= steps ? -1 : (t < sink_n ? t : win_t0 + t - sink_n) * kTileKeys;
   };
+  auto page_ok = [&](int p) __attribute__((always_inline)) -> bool {
+    return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
+  };
+  // column of half tile h = key / 16 (scalar arithmetic: the unsigned division by an
+  // invariant, two shifts and a high product)
+  const uint32_t page = PAGED ? static_cast<uint32_t>(a.page) : 16u;
+  auto col_of = [&](uint32_t h) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t t = __umulhi(a.page_mul, h);
+    return (t + ((h - t) >> a.page_sh1)) >> a.page_sh2;
+  };
   auto step_of = [&](int s) __attribute__((always_inline)) -> Step {
-    Step r{key_of(s), 0, 0, 0, 0};
-    if constexpr (PAGED) {
+    Step r{key_of(s), 0, 0};
+    if constexpr (PAGED) {  // (a half lies in one page: pages hold whole halves)
       const uint32_t key = r.key < 0 ? 0u : static_cast<uint32_t>(r.key);
-      const uint32_t page = static_cast<uint32_t>(a.page);
-      uint32_t col0 = key / page;
-      r.slot0 = static_cast<int>(key - col0 * page);
-      r.slot1 = r.slot0 + 16;
-      uint32_t col1 = col0;
-      if (r.slot1 >= a.page) {
-        r.slot1 -= a.page;
-        ++col1;
-      }
       const uint32_t last = static_cast<uint32_t>(a.max_pages) - 1u;
+      const uint32_t col0 = col_of(key >> 4);
+      uint32_t col1 = col_of((key >> 4) + 1u);
       col1 = col1 < last ? col1 : last;
       r.page0 = ld_const(table + col0);
       r.page1 = ld_const(table + col1);
     }
     return r;
   };
-  auto page_ok = [&](int p) __attribute__((always_inline)) -> bool {
-    return !PAGED || static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
+  auto uniform = [&](int64_t x) __attribute__((always_inline)) -> int64_t {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
+    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
   };
   // copies [i0, i0 + n) of a step, all in half `half` of its tile
   auto stage_half = [&](const Step& s, char* dst, int half, int i0, auto n_c)
       __attribute__((always_inline)) {
-    const int key = (s.key < 0 ? 0 : s.key) + 16 * half;
+    const uint32_t key = static_cast<uint32_t>(s.key < 0 ? 0 : s.key) + 16u * half;
     int64_t krow, vrow;
     bool there = s.key >= 0;
     if constexpr (PAGED) {
-      const int page = half ? s.page1 : s.page0;
-      const int64_t slot = half ? s.slot1 : s.slot0;
-      there = there && page_ok(page);
-      const int64_t pg = there ? page : 0;
-      krow = (pg * a.sk[0] + slot * a.sk[1]) * 2;
-      vrow = (pg * a.sv[0] + slot * a.sv[1]) * 2;
+      const int pg = half ? s.page1 : s.page0;
+      there = there && page_ok(pg);
+      const uint32_t slot = key - col_of(key >> 4) * page;
+      const int64_t at = there ? pg : 0;
+      krow = uniform((at * a.sk[0] + static_cast<int64_t>(slot) * a.sk[1]) * 2);
+      vrow = uniform((at * a.sv[0] + static_cast<int64_t>(slot) * a.sv[1]) * 2);
     } else {
-      krow = static_cast<uint64_t>(static_cast<uint32_t>(key)) * krb;
-      vrow = static_cast<uint64_t>(static_cast<uint32_t>(key)) * vrb;
+      krow = static_cast<uint64_t>(key) * krb;
+      vrow = static_cast<uint64_t>(key) * vrb;
     }
-    const int left = k_len - key;
-    const int rows = !there || left <= 0 ? 0 : (left < 16 ? left : 16);
-    char* const ks = const_cast<char*>(kbase) + (rows ? krow : 0);
-    char* const vs = const_cast<char*>(vbase) + (rows ? vrow : 0);
-    const int kn = rows ? (rows - 1) * static_cast<int>(krb) + C::KROW : 0;
-    const int vn = rows ? (rows - 1) * static_cast<int>(vrb) + C::KROW : 0;
+    const int left = k_len - static_cast<int>(key);
+    const int rows = __builtin_amdgcn_readfirstlane(
+        !there || left <= 0 ? 0 : (left < 16 ? left : 16));
+    char* const ks = const_cast<char*>(kbase) + krow;
+    char* const vs = const_cast<char*>(vbase) + vrow;
+    // (row strides are at least a row: a lane of row r < rows stays below)
+    const int kn = rows * static_cast<int>(krb), vn = rows * static_cast<int>(vrb);
 #pragma unroll
     for (int i = 0; i < decltype(n_c)::value; ++i) {
       buffer_copy16(ks, kn, k_lo[i0 + i], dst + (wave * C::UPW + i0 + i) * 1024);
       buffer_copy16(vs, vn, v_lo[i0 + i], dst + C::TILE + (wave * C::UPW + i0 + i) * 1024);
     }
   };
-  auto stage = [&](const Step& s, char* dst) __attribute__((always_inline)) {
+  auto stage = [&](const Step& s, char* dst) __attribute__((always_inline)) -> Staged {
     if constexpr (NW == 1) {
       stage_half(s, dst, 0, 0, std::integral_constant<int, C::UPW / 2>{});
       stage_half(s, dst, 1, C::UPW / 2, std::integral_constant<int, C::UPW / 2>{});
     } else {
       stage_half(s, dst, wave >> 1, 0, std::integral_constant<int, C::UPW>{});
     }
+    return {s.key, PAGED ? (page_ok(s.page0) ? 1 : 0) + (page_ok(s.page1) ? 2 : 0) : 3};
   };
 
   // LDS read offsets (tile and step offsets are immediates)
@@ -232,8 +254,11 @@ window_kernel(WindowArgs a) {
     const int n = x < 0 ? 0 : (x > 16 ? 16 : x);
     return (1u << n) - 1u;
   };
-  auto compute = [&](const char* tile, const Step& s) __attribute__((always_inline)) {
-    const bool pages = page_ok(s.page0) && page_ok(s.page1);
+  // The scalar loads of a later step go out behind the first products (they return out of
+  // order, so a wait for LDS behind them would wait for them too).
+  auto compute = [&](const char* tile, const Staged& s, auto&& prefetch)
+      __attribute__((always_inline)) {
+    const bool pages = !PAGED || s.there == 3;
     // every row of the wavefront sees the whole tile
     const bool inside = pages && s.key + kTileKeys <= w_first.hi &&
                         (s.key >= w_last.lo || s.key + kTileKeys <= a.sinks);
@@ -245,13 +270,19 @@ window_kernel(WindowArgs a) {
 #pragma unroll
     for (int st = 0; st < C::QSTEPS; ++st)
       s_acc = O::mfma(__builtin_bit_cast(op8, kraw[st]), q_op[st], s_acc);
+    __builtin_amdgcn_sched_group_barrier(0x100, C::QSTEPS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, C::QSTEPS, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    prefetch();
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
     if (!inside) {
+      const KeyRange kr = key_range(a, my_row().qi + shift, k_len);
+      const int sink = a.sinks < kr.hi ? a.sinks : kr.hi;
       const int k0 = s.key + 16 * hf;
       uint32_t bits = below(kr.hi - k0) & (~below(kr.lo - k0) | below(sink - k0));
-      if (PAGED && !page_ok(hf ? s.page1 : s.page0)) bits = 0;
+      if (PAGED && !((s.there >> hf) & 1)) bits = 0;
 #pragma unroll
       for (int r = 0; r < 16; ++r) rv[r] = ((bits >> r) & 1u) ? rv[r] : -INFINITY;
     }
@@ -293,26 +324,39 @@ window_kernel(WindowArgs a) {
       }
     }
     l_run += part;
+    // (the reads of the second half of the keys are in flight beside the first half's
+    // products)
+    auto v_group = [&](int u, op8 (&op)[C::NDT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int dt = 0; dt < C::NDT; ++dt) {
+        const char* const p0 = tile + v_off[dt] + 8 * u * C::KROW;
+        const auto lo = O::read_tr(p0);
+        const auto hi = O::read_tr(p0 + 4 * C::KROW);
+        op[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    };
+    op8 vop[2][C::NDT];
+    v_group(0, vop[0]);
+    v_group(1, vop[1]);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int dt = 0; dt < C::NDT; ++dt) {
-        const char* p0 = tile + v_off[dt] + 8 * u * C::KROW;
-        const auto lo = O::read_tr(p0);
-        const auto hi = O::read_tr(p0 + 4 * C::KROW);
-        o_acc[dt] = O::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), p_op[u],
-                            o_acc[dt]);
-      }
+      for (int dt = 0; dt < C::NDT; ++dt) o_acc[dt] = O::mfma(vop[u][dt], p_op[u], o_acc[dt]);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * C::NDT, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * C::NDT; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i < C::NDT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
   };
 
   // ring: step j in slot j % 3, two steps in flight; every step copies (past the
   // list through empty ranges), so every wait counts the same operations
-  Step st[C::STAGES];
-  st[0] = step_of(0);
-  st[1] = step_of(1);
-  stage(st[0], s_0);
+  Staged st[C::STAGES];
+  const Step first = step_of(0), second = step_of(1);
+  st[0] = stage(first, s_0);
   __builtin_amdgcn_sched_barrier(0);
-  stage(st[1], s_1);
+  st[1] = stage(second, s_1);
   __builtin_amdgcn_sched_barrier(0);
   Step next = step_of(2);
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * C::OPS));  // Q has landed
@@ -322,14 +366,14 @@ window_kernel(WindowArgs a) {
     char* const tile = J == 0 ? s_0 : J == 1 ? s_1 : s_2;
     char* const fill = F == 0 ? s_0 : F == 1 ? s_1 : s_2;
     wait_vm_barrier<C::OPS>();
-    st[F] = next;
-    stage(st[F], fill);
+    st[F] = stage(next, fill);
     __builtin_amdgcn_sched_barrier(0);
-    next = step_of(j + C::STAGES);
-    const Step& s = st[J];
+    const Staged s = st[J];
     const bool seen = s.key >= 0 && s.key < w_last.hi &&
                       (s.key + kTileKeys > w_first.lo || s.key < a.sinks);
-    if (seen) compute(tile, s);
+    auto prefetch = [&]() __attribute__((always_inline)) { next = step_of(j + C::STAGES); };
+    if (seen) compute(tile, s, prefetch);
+    else prefetch();
   };
   const int rounds = (steps + C::STAGES - 1) / C::STAGES;
   for (int rd = 0; rd < rounds; ++rd) {
@@ -350,10 +394,11 @@ window_kernel(WindowArgs a) {
       o_acc[dt][r] *= inv;
       bad = bad || !(fabsf(o_acc[dt][r]) < INFINITY);
     }
-  const int64_t wrow = ws_row + row - row0;
-  T* const op = static_cast<T*>(a.out) + b * a.so[0] + static_cast<int64_t>(qi) * a.so[1] +
-                head * a.so[2];
-  if (live) {
+  const Row my = my_row();
+  const int64_t wrow = ws_row + my.row - row0;
+  T* const op = static_cast<T*>(a.out) + b * a.so[0] + static_cast<int64_t>(my.qi) * a.so[1] +
+                my.head * a.so[2];
+  if (my.live) {
 #pragma unroll
     for (int dt = 0; dt < C::NDT; ++dt)
 #pragma unroll
@@ -374,13 +419,13 @@ window_kernel(WindowArgs a) {
       if (ns > 1)
         a.ws_ml[wrow] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
       else if (a.lse)
-        a.lse[(static_cast<int64_t>(b) * a.Hq + head) * a.Lq + qi] =
+        a.lse[(static_cast<int64_t>(b) * a.Hq + my.head) * a.Lq + my.qi] =
             l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
     }
   }
   // A row whose products met a value that it does not see (0 * inf or 0 * NaN of a
   // masked key): its sum is taken again over its own keys, one row at a time.
-  uint64_t again = __ballot(bad && live && l > 0.0f && l < INFINITY);
+  uint64_t again = __ballot(bad && my.live && l > 0.0f && l < INFINITY);
   again |= again >> 32;
   if (static_cast<uint32_t>(again) == 0) return;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the stores above come first)
@@ -405,11 +450,11 @@ window_kernel(WindowArgs a) {
         if (!(j < rk.hi && (j >= rk.lo || j < rsink))) continue;
         int64_t ko = j * a.sk[1], vo = j * a.sv[1];
         if constexpr (PAGED) {
-          const int page = table[j / a.page];
-          if (!page_ok(page)) continue;
+          const int pg = table[j / a.page];
+          if (!page_ok(pg)) continue;
           const int64_t slot = j % a.page;
-          ko = page * a.sk[0] + slot * a.sk[1];
-          vo = page * a.sv[0] + slot * a.sv[1];
+          ko = pg * a.sk[0] + slot * a.sk[1];
+          vo = pg * a.sv[0] + slot * a.sv[1];
         }
         const T* const kp = reinterpret_cast<const T*>(kbase) + ko;
         const T* const vp = reinterpret_cast<const T*>(vbase) + vo;
@@ -622,7 +667,10 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   if (n_split < 0 || n_split > 64 || (n_split == 0 && !few_rows(dims))) return RCSA_ERR_SHAPE;
   for (int i = 0; i < 12; ++i)
     if (strides[i] < 0 || strides[i] % (i < 9 ? 8 : 4)) return RCSA_ERR_STRIDE;
-  if (strides[4] >= (1 << 25) || strides[7] >= (1 << 25)) return RCSA_ERR_STRIDE;
+  // (rows of keys do not overlap; the stride of a single one says nothing)
+  const bool one = !block_table && dims[2] <= 1;
+  for (int i = 4; i < 8; i += 3)
+    if (strides[i] >= (1 << 25) || (!one && strides[i] < dims[5])) return RCSA_ERR_STRIDE;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(workspace) ||
       (reinterpret_cast<uintptr_t>(out) & 7u))
     return RCSA_ERR_ALIGN;
@@ -640,6 +688,7 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
     a.sv[i] = strides[6 + i];
     a.so[i] = strides[9 + i];
   }
+  if (one) a.sk[1] = a.sv[1] = dims[5];
   a.B = static_cast<int>(dims[0]);
   a.Lq = static_cast<int>(dims[1]);
   a.Lk = static_cast<int>(dims[2]);
@@ -653,6 +702,14 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   a.max_pages = static_cast<int>(max_pages);
   a.n_pages = static_cast<int>(n_pages);
   a.page = static_cast<int>(page_size);
+  if (block_table) {
+    const uint64_t d = static_cast<uint64_t>(page_size) / 16;
+    int l = 0;
+    while ((1ull << l) < d) ++l;
+    a.page_mul = static_cast<uint32_t>((1ull << 32) * ((1ull << l) - d) / d + 1);
+    a.page_sh1 = l < 1 ? l : 1;
+    a.page_sh2 = l < 1 ? 0 : l - 1;
+  }
   a.window = static_cast<int>(window < most ? window : 0);
   a.sinks = static_cast<int>(sinks < most ? sinks : most);
   a.block = static_cast<int>(block < most ? block : most);

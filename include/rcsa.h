@@ -746,7 +746,8 @@ int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, voi
  *   out = softmax(sm_scale q k) v in fp32, rounded once; lse (nullable) [B][Hq][Lq] the
  * natural log of the row's sum; a row that sees nothing gives 0 and -inf.  What a row
  * does not see does not reach it, NaN and infinities included.  Rows i >= q_len are left
- * as they were.  q, k, v rows 16-byte, out rows 8-byte aligned.
+ * as they were.  q, k, v rows 16-byte, out rows 8-byte aligned; the token (slot) strides of
+ * k and v are at least D and below 2^25 elements.
  *
  * n_split (1 to 64) shares the keys of every block of rows among as many workgroups; more
  * than 1 needs a workspace of rcsa_window_attn_workspace_bytes (16-byte aligned, used by

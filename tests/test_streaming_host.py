@@ -102,6 +102,8 @@ def _window(lib, q=4096, k=4096, out=4096, dtype=0, dims=(1, 4, 8, 2, 1, 64),
     (dict(n_split=0), SHAPE), (dict(n_split=65), SHAPE), (dict(n_split=2), SHAPE),
     (dict(n_split=2, ws=4096, ws_bytes=64), SHAPE),
     (dict(strides=(512, 128, 63) + (512, 64, 64) * 3), STRIDE),
+    (dict(strides=(512, 128, 64, 512, 0, 64, 512, 64, 64, 512, 128, 64)), STRIDE),
+    (dict(strides=(512, 128, 64, 512, 64, 64, 512, 56, 64, 512, 128, 64)), STRIDE),
     (dict(strides=(512, 128, 64, 512, 1 << 25, 64, 512, 64, 64, 512, 128, 64)), STRIDE),
     (dict(strides=(512, 128, 64, -512, 64, 64, 512, 64, 64, 512, 128, 64)), STRIDE),
     (dict(q=4098), ALIGN), (dict(k=4104), ALIGN), (dict(out=4100), ALIGN)])
