@@ -37,10 +37,14 @@ struct WindowArgs {
   int n_rblocks;                    // blocks of rows of a key head
   int64_t n_items;                  // B * Hk * n_rblocks
   int n_split;
-  float* ws_o;                      // [n_split][n_items][rows][D] normalised partial outputs
-  float2* ws_ml;                    // [n_split][n_items][rows] their (max, sum)
-  // few rows (one wavefront a unit): units wanted in all, 0: one a key head
-  int units;
+  float* ws_o;                      // [share][row][D] normalised partial outputs
+  float2* ws_ml;                    // [share][row] their (max, sum)
+  // Row blocks in XCD runs of xcd_items, of which the first xcd_whole run whole and the
+  // others in n_split shares; descending: the longest (last) row blocks first, dealt
+  // round-robin.
+  int xcd_items, xcd_whole;
+  int descending;
+  int units;  // few rows: the wavefronts that fit in one round, 0: one unit a key head
 };
 
 constexpr int kFewRows = 32;        // rows of a key head that one wavefront takes
@@ -88,68 +92,102 @@ __device__ __forceinline__ Tiles tiles_of(const WindowArgs& a, KeyRange first, K
   return t;
 }
 
-// Few rows: the visible tiles of all requests are dealt to about a.units wavefronts in
-// units of `chunk` tiles of one key head, however uneven the lengths.  A wavefront
-// reads the lengths (one lane a request) and finds its unit; u = (units of the
-// requests before) * Hk + share * Hk + hk.
-constexpr int kLeastTiles = 2;
-__device__ __forceinline__ int request_tiles(const WindowArgs& a, int b) {
-  const Request r = request_of(a, b);
+// Few rows: the visible tiles of all requests are dealt to units of one wavefront each,
+// `chunk` tiles of one key head at most, however uneven the lengths.  A wavefront reads
+// the lengths, one lane a request, and finds its unit among them; unit index = (units
+// of the requests before) * Hk + share * Hk + hk.
+__device__ __forceinline__ int request_tiles(const WindowArgs& a, Request r) {
   if (r.q_len == 0) return -1;
   const int p = r.k_len - r.q_len;
   return tiles_of(a, key_range(a, p, r.k_len), key_range(a, p + r.q_len - 1, r.k_len)).all();
 }
-// Tiles of a unit: all lanes of the wavefront call it.
-__device__ __forceinline__ int unit_chunk(const WindowArgs& a, int lane) {
-  if (a.units == 0) return 1 << 30;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const int n = b0 + lane < a.B ? request_tiles(a, b0 + lane) : 0;
-    int s = n > 0 ? n : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
-    total += s;
-  }
-  const int64_t c = (total * a.Hk + a.units - 1) / a.units;
-  return c < kLeastTiles ? kLeastTiles : static_cast<int>(c);
-}
 __device__ __forceinline__ int units_of(int tiles, int chunk) {
   return tiles < 0 ? 0 : (tiles <= chunk ? 1 : (tiles + chunk - 1) / chunk);
 }
-// Units of the requests before b (all lanes call it).
-__device__ __forceinline__ int units_before(const WindowArgs& a, int b, int chunk, int lane) {
-  if (a.units == 0) return b;
-  int s = 0;
-  for (int b0 = 0; b0 < b; b0 += kWave)
-    if (b0 + lane < b) s += units_of(request_tiles(a, b0 + lane), chunk);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
-  return s;
+// One round of the wavefronts that fit (a.units) where that leaves units of up to
+// kUnitTiles tiles; beyond, units of that size, or more of them than four rounds.  A unit
+// costs about 5 us before its first tile has landed (a tile streams in 0.4 to 1), and the
+// units of a last, short round leave compute units idle.
+constexpr int kLeastTiles = 2, kUnitTiles = 16;
+__device__ __forceinline__ int chunk_of(const WindowArgs& a, int64_t total) {
+  const int64_t t = total * a.Hk;
+  const int64_t one = (t + a.units - 1) / a.units;
+  int64_t c = (t + 4 * a.units - 1) / (4 * a.units);
+  c = c < kUnitTiles ? kUnitTiles : c;
+  c = c < one ? c : one;
+  return static_cast<int>(c < kLeastTiles ? kLeastTiles : c);
 }
-// The request, share and number of shares of unit index w (of one key head), b -1 past
-// the last (all lanes call it).
 struct Unit {
-  int b, share, shares;
+  int b, share, shares;  // b -1: no such unit
+  int before;            // units (of one key head) of the requests before b
+  Request r;
 };
-__device__ __forceinline__ Unit unit_at(const WindowArgs& a, int w, int chunk, int lane) {
-  if (a.units == 0) return {w < a.B ? w : -1, 0, 1};
+__device__ __forceinline__ int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int lane_sum(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
+  return x;
+}
+__device__ __forceinline__ int lane_prefix(int x, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int up = __shfl_up(x, o, kWave);
+    x += lane >= o ? up : 0;
+  }
+  return x;
+}
+// Unit index `w` of a key head (of_request false), or the units of request w (true).  Every
+// lane of the wavefront calls it; the result is uniform.
+template <bool OF_REQUEST>
+__device__ __forceinline__ Unit find_unit(const WindowArgs& a, int w, int lane) {
+  if (a.units == 0) {  // a unit for every request
+    if (w >= a.B) return {-1, 0, 0, 0, {0, 0}};
+    const Request r = request_of(a, w);
+    return {w, 0, 1, w, {uniform_int(r.k_len), uniform_int(r.q_len)}};
+  }
+  if (a.B <= kWave) {  // one load of the lengths (a single request needs no lanes' sums)
+    Request r{0, 0};
+    if (lane < a.B) r = request_of(a, lane);
+    const int tiles = lane < a.B ? request_tiles(a, r) : -1;
+    const int mine = tiles > 0 ? tiles : 0;
+    const int chunk = chunk_of(a, a.B == 1 ? uniform_int(mine) : uniform_int(lane_sum(mine)));
+    const int n = units_of(tiles, chunk);
+    const int upto = a.B == 1 ? n : lane_prefix(n, lane);
+    int l = w;
+    if (!OF_REQUEST) {
+      const uint64_t past = __ballot(lane < a.B && upto > w);
+      if (past == 0) return {-1, 0, 0, 0, {0, 0}};
+      l = __builtin_ctzll(past);
+    }
+    auto at = [&](int x) __attribute__((always_inline)) { return __builtin_amdgcn_readlane(x, l); };
+    const int shares = at(n), before = at(upto) - shares;
+    return {l, w - before, shares, before, {at(r.k_len), at(r.q_len)}};
+  }
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kWave) {
+    const int t = b0 + lane < a.B ? request_tiles(a, request_of(a, b0 + lane)) : 0;
+    total += lane_sum(t > 0 ? t : 0);
+  }
+  const int chunk = uniform_int(chunk_of(a, total));
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
-    const int n = b0 + lane < a.B ? units_of(request_tiles(a, b0 + lane), chunk) : 0;
-    int sum = n;  // inclusive prefix over the lanes
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int up = __shfl_up(sum, o, kWave);
-      if (lane >= o) sum += up;
-    }
-    const uint64_t past = __ballot(before + sum > w);
+    Request r{0, 0};
+    if (b0 + lane < a.B) r = request_of(a, b0 + lane);
+    const int n = b0 + lane < a.B ? units_of(request_tiles(a, r), chunk) : 0;
+    const int upto = before + lane_prefix(n, lane);
+    const uint64_t past =
+        OF_REQUEST ? (w - b0 < kWave ? 1ull << (w - b0) : 0) : __ballot(upto > w);
     if (past != 0) {
       const int l = __builtin_ctzll(past);
-      return {b0 + l, w - before - __shfl(sum - n, l, kWave), __shfl(n, l, kWave)};
+      auto at = [&](int x) __attribute__((always_inline)) {
+        return __builtin_amdgcn_readlane(x, l);
+      };
+      const int shares = at(n), bef = at(upto) - shares;
+      return {b0 + l, w - bef, shares, bef, {at(r.k_len), at(r.q_len)}};
     }
-    before += __shfl(sum, kWave - 1, kWave);
+    before = __builtin_amdgcn_readlane(upto, kWave - 1);
   }
-  return {-1, 0, 0};
+  return {-1, 0, 0, 0, {0, 0}};
 }
 
 template <typename T>

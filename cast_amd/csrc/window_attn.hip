@@ -28,7 +28,7 @@ struct WindowCfg {
 
 template <typename T, int D, bool PAGED, int NW>
 __global__ void __launch_bounds__(64 * NW)
-__attribute__((amdgpu_waves_per_eu(NW == 1 ? 1 : 3, 3)))
+__attribute__((amdgpu_waves_per_eu(NW == 1 ? 1 : (D == 64 ? 4 : 3), D == 64 ? 4 : 3)))
 window_kernel(WindowArgs a) {
   using C = WindowCfg<T, D, NW>;
   using O = Half<T>;
@@ -46,37 +46,42 @@ window_kernel(WindowArgs a) {
   int b, hk, row0, share;
   uint32_t ns;
   int64_t ws_row;
+  Request rq;
   if constexpr (NW > 1) {
-    // XCD x (workgroups go round-robin) runs a contiguous run of items: neighbours
-    // share most of their window in its L2.
-    ns = static_cast<uint32_t>(a.n_split);
-    const uint32_t items = static_cast<uint32_t>(a.n_items);
-    const uint32_t per = (items * ns + kNumXcd - 1) / kNumXcd;
-    const uint32_t at = (blockIdx.x % kNumXcd) * per + blockIdx.x / kNumXcd;
-    if (at >= items * ns) return;
-    const uint32_t item = at / ns;
-    share = static_cast<int>(at - item * ns);
-    const uint32_t nrb = static_cast<uint32_t>(a.n_rblocks);
-    row0 = static_cast<int>(item % nrb) * C::BM;
-    const int bh = static_cast<int>(item / nrb);
+    // XCD x (workgroups go round-robin) runs a contiguous run of items, so that neighbours
+    // share most of their window in its L2, or every 8th from the longest on.
+    const int xcd = static_cast<int>(blockIdx.x % kNumXcd);
+    const int slot = static_cast<int>(blockIdx.x / kNumXcd);
+    const int tail = slot - a.xcd_whole;
+    ns = tail < 0 ? 1u : static_cast<uint32_t>(a.n_split);
+    const int in_xcd = tail < 0 ? slot : a.xcd_whole + tail / a.n_split;
+    share = tail < 0 ? 0 : tail % a.n_split;
+    if (in_xcd >= a.xcd_items) return;
+    const int64_t item = a.descending ? static_cast<int64_t>(in_xcd) * kNumXcd + xcd
+                                      : static_cast<int64_t>(xcd) * a.xcd_items + in_xcd;
+    if (item >= a.n_items) return;
+    const uint32_t it = static_cast<uint32_t>(item), nrb = static_cast<uint32_t>(a.n_rblocks);
+    const uint32_t heads = static_cast<uint32_t>(a.B * a.Hk);
+    const int bh = static_cast<int>(a.descending ? it % heads : it / nrb);
+    row0 = static_cast<int>(a.descending ? nrb - 1 - it / heads : it % nrb) * C::BM;
     b = bh / a.Hk;
     hk = bh - b * a.Hk;
-    ws_row = (static_cast<int64_t>(share) * a.n_items + item) * C::BM;
+    const int64_t n_tail = static_cast<int64_t>(a.xcd_items - a.xcd_whole) * kNumXcd;
+    ws_row = (share * n_tail + xcd * (a.xcd_items - a.xcd_whole) + in_xcd - a.xcd_whole) * C::BM;
+    rq = request_of(a, b);
   } else {
-    const int chunk = unit_chunk(a, lane);
     const int w = static_cast<int>(blockIdx.x) / a.Hk;
-    const Unit u = unit_at(a, w, chunk, lane);
+    const Unit u = find_unit<false>(a, w, lane);
     if (u.b < 0) return;
-    b = __builtin_amdgcn_readfirstlane(u.b);
-    share = __builtin_amdgcn_readfirstlane(u.share);
-    ns = __builtin_amdgcn_readfirstlane(u.shares);
+    b = u.b;
+    share = u.share;
+    ns = static_cast<uint32_t>(u.shares);
     hk = static_cast<int>(blockIdx.x) - w * a.Hk;
     row0 = 0;
     ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
+    rq = u.r;
   }
-  const Request rq = request_of(a, b);
-  const int k_len = __builtin_amdgcn_readfirstlane(rq.k_len);
-  const int q_len = __builtin_amdgcn_readfirstlane(rq.q_len);
+  const int k_len = uniform_int(rq.k_len), q_len = uniform_int(rq.q_len);
   const int n_rows = q_len * a.G;
   if (row0 >= n_rows) return;
   const int shift = k_len - q_len;  // position of query 0
@@ -133,6 +138,8 @@ window_kernel(WindowArgs a) {
   const char* const vbase = static_cast<const char*>(a.v) +
                             ((PAGED ? 0 : b * a.sv[0]) + hk * a.sv[2]) * 2;
   const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
+  const uint32_t kpage = static_cast<uint32_t>(a.sk[0] * 2);  // (paged)
+  const uint32_t vpage = static_cast<uint32_t>(a.sv[0] * 2);
   const int32_t* const table = PAGED ? a.table + b * a.table_stride : nullptr;
 
   // Copies: of four wavefronts, w moves rows 8w .. 8w + 7 of the tile (of its half w / 2 of
@@ -181,24 +188,20 @@ window_kernel(WindowArgs a) {
     }
     return r;
   };
-  auto uniform = [&](int64_t x) __attribute__((always_inline)) -> int64_t {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(x));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(x >> 32));
-    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-  };
   // copies [i0, i0 + n) of a step, all in half `half` of its tile
   auto stage_half = [&](const Step& s, char* dst, int half, int i0, auto n_c)
       __attribute__((always_inline)) {
     const uint32_t key = static_cast<uint32_t>(s.key < 0 ? 0 : s.key) + 16u * half;
-    int64_t krow, vrow;
+    uint64_t krow, vrow;
     bool there = s.key >= 0;
     if constexpr (PAGED) {
       const int pg = half ? s.page1 : s.page0;
       there = there && page_ok(pg);
       const uint32_t slot = key - col_of(key >> 4) * page;
-      const int64_t at = there ? pg : 0;
-      krow = uniform((at * a.sk[0] + static_cast<int64_t>(slot) * a.sk[1]) * 2);
-      vrow = uniform((at * a.sv[0] + static_cast<int64_t>(slot) * a.sv[1]) * 2);
+      // (32 x 32-bit scalar products: a page spans less than 4 GiB)
+      const uint32_t at = there ? static_cast<uint32_t>(pg) : 0u;
+      krow = static_cast<uint64_t>(at) * kpage + static_cast<uint64_t>(slot) * krb;
+      vrow = static_cast<uint64_t>(at) * vpage + static_cast<uint64_t>(slot) * vrb;
     } else {
       krow = static_cast<uint64_t>(key) * krb;
       vrow = static_cast<uint64_t>(key) * vrb;
@@ -477,25 +480,32 @@ window_kernel(WindowArgs a) {
   }
 }
 
-// The shares of every row joined: w_s = l_s 2^(m_s - M), out = sum w_s O_s / sum w_s.
-// One thread per row and 8 channels; the shares are added in their order.
+// The shares of the split row blocks joined: w_s = l_s 2^(m_s - M),
+// out = sum w_s O_s / sum w_s.  One thread per row and 8 channels; the shares are added in
+// their order.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) window_merge_kernel(WindowArgs a, int rows_per_item) {
-  constexpr int CPR = D / 8;
+__global__ void __launch_bounds__(256) window_merge_kernel(WindowArgs a) {
+  constexpr int CPR = D / 8, BM = 128;
   const int64_t v = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t all_rows = a.n_items * rows_per_item;
+  const int per = a.xcd_items - a.xcd_whole;
+  const int64_t all_rows = static_cast<int64_t>(per) * kNumXcd * BM;
   const int64_t wrow = v / CPR;
   if (wrow >= all_rows) return;
   const int c = static_cast<int>(v % CPR);
-  const int64_t item = wrow / rows_per_item;
-  const int64_t bh = item / a.n_rblocks;
-  const int b = static_cast<int>(bh / a.Hk), hk = static_cast<int>(bh % a.Hk);
-  int q_len = a.q_len == nullptr ? a.Lq : a.q_len[b];
-  q_len = q_len < 0 ? 0 : (q_len > a.Lq ? a.Lq : q_len);
-  const int64_t row = (item % a.n_rblocks) * rows_per_item + wrow % rows_per_item;
-  if (row >= static_cast<int64_t>(q_len) * a.G) return;
-  const int qi = static_cast<int>(row / a.G);
-  const int head = hk * a.G + static_cast<int>(row % a.G);
+  const int t = static_cast<int>(wrow / BM);
+  const int xcd = t / per, in_xcd = a.xcd_whole + t % per;
+  const int64_t item = a.descending ? static_cast<int64_t>(in_xcd) * kNumXcd + xcd
+                                    : static_cast<int64_t>(xcd) * a.xcd_items + in_xcd;
+  if (item >= a.n_items) return;
+  const uint32_t it = static_cast<uint32_t>(item), nrb = static_cast<uint32_t>(a.n_rblocks);
+  const uint32_t heads = static_cast<uint32_t>(a.B * a.Hk);
+  const int bh = static_cast<int>(a.descending ? it % heads : it / nrb);
+  const int b = bh / a.Hk, hk = bh - b * a.Hk;
+  const int q_len = request_of(a, b).q_len;
+  const int row = static_cast<int>(a.descending ? nrb - 1 - it / heads : it % nrb) * BM +
+                  static_cast<int>(wrow % BM);
+  if (row >= q_len * a.G) return;
+  const int qi = row / a.G, head = hk * a.G + row - qi * a.G;
   float mx = -INFINITY;
   for (int s = 0; s < a.n_split; ++s) mx = fmaxf(mx, a.ws_ml[s * all_rows + wrow].x);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -532,12 +542,11 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
   const int row = static_cast<int>(blockIdx.x) % R;
   const int bh = static_cast<int>(blockIdx.x) / R;
   const int b = bh / a.Hk, hk = bh - b * a.Hk;
-  const Request rq = request_of(a, b);
-  if (row >= rq.q_len * a.G) return;
-  const int chunk = unit_chunk(a, lane);
-  const int shares = units_of(request_tiles(a, b), chunk);
+  const Unit u = find_unit<true>(a, b, lane);
+  if (row >= u.r.q_len * a.G) return;
+  const int shares = u.shares;
   if (shares <= 1) return;  // written by its only unit
-  const int64_t first = static_cast<int64_t>(units_before(a, b, chunk, lane)) * a.Hk + hk;
+  const int64_t first = static_cast<int64_t>(u.before) * a.Hk + hk;
   auto at = [&](int s) __attribute__((always_inline)) -> int64_t {
     return (first + static_cast<int64_t>(s) * a.Hk) * R + row;
   };
@@ -582,7 +591,7 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
 template <typename T, int D>
 static int launch_window(WindowArgs& a, hipStream_t s) {
   if (a.n_split == 0) {
-    const int64_t n = a.units + static_cast<int64_t>(a.B) * a.Hk;
+    const int64_t n = 4ll * a.units + static_cast<int64_t>(a.B) * a.Hk;
     const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * a.Lq * a.G;
     if (n >= (1ll << 31) || rows >= (1ll << 31)) return RCSA_ERR_SHAPE;
     const dim3 grid(static_cast<unsigned>(n));
@@ -592,15 +601,15 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
       window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
     return launch_status();
   }
-  const int64_t wgs = (a.n_items * a.n_split + kNumXcd - 1) / kNumXcd * kNumXcd;
+  const int64_t tail = a.xcd_items - a.xcd_whole;
+  const int64_t wgs = (a.xcd_whole + tail * a.n_split) * kNumXcd;
   if (wgs >= (1ll << 31)) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs));
   if (a.table) window_kernel<T, D, true, 4><<<grid, dim3(256), 0, s>>>(a);
   else window_kernel<T, D, false, 4><<<grid, dim3(256), 0, s>>>(a);
-  if (a.n_split > 1) {
-    const int64_t n = (a.n_items * 128 * (D / 8) + 255) / 256;
-    if (n >= (1ll << 31)) return RCSA_ERR_SHAPE;
-    window_merge_kernel<T, D><<<dim3(static_cast<unsigned>(n)), dim3(256), 0, s>>>(a, 128);
+  if (a.n_split > 1 && tail > 0) {
+    const int64_t n = (tail * kNumXcd * 128 * (D / 8) + 255) / 256;
+    window_merge_kernel<T, D><<<dim3(static_cast<unsigned>(n)), dim3(256), 0, s>>>(a);
   }
   return launch_status();
 }
@@ -608,13 +617,13 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
 // Blocks of rows of a key head.
 static int64_t row_blocks(int64_t Lq, int64_t G) { return (Lq * G + 127) / 128; }
 
-// Units of few rows wanted in all: kUnits, as four rounds of the three wavefronts that
-// share a compute unit's LDS.  Every wavefront reads all lengths to find its unit, so
-// past kMaxPlanned requests each key head is one unit.
-constexpr int64_t kUnits = 3072;
 static bool few_rows(const int64_t* d) { return d[1] * (d[3] / d[4]) <= kFewRows; }
-static int64_t wanted_units(const int64_t* d) { return d[0] > kMaxPlanned ? 0 : kUnits; }
-
+// Wavefronts of few rows that fit at once: their rings fill a compute unit's 160 KB of LDS
+// three (D 64: six) times.  Every one reads all lengths to find its unit, so past kMaxPlanned
+// requests each key head is one unit.
+static int64_t units_of_round(const int64_t* d) {
+  return d[0] > kMaxPlanned ? 0 : (d[5] == 128 ? 3 : 6) * 256;
+}
 static bool window_dims(const int64_t* d) {
   for (int i = 0; i < 6; ++i)
     if (d[i] <= 0 && !(i == 2 && d[i] == 0)) return false;
@@ -623,28 +632,59 @@ static bool window_dims(const int64_t* d) {
          d[0] * d[4] * row_blocks(d[1], d[3] / d[4]) < (1ll << 26);
 }
 
+// Row blocks of an XCD, and of these the ones in whole rounds of its compute units.
+static int64_t xcd_items_of(const int64_t* d) {
+  return (d[0] * d[4] * row_blocks(d[1], d[3] / d[4]) + kNumXcd - 1) / kNumXcd;
+}
+static int64_t xcd_cus() {
+  const int64_t n = cus_per_xcd();
+  return n > 0 ? n : 32;
+}
+static int64_t xcd_whole_of(int64_t items, int64_t n_split) {
+  return n_split == 1 ? items : whole_items(items, xcd_cus());
+}
+
 }  // namespace rcsa
 
 using namespace rcsa;
 
-// Few rows of a key head go to units of one wavefront (n_split 0), more to tiles of 128
-// rows in n_split shares.
+// Few rows of a key head go to units of one wavefront (n_split 0), more to blocks of 128
+// rows.  Of these the ones past an XCD's whole rounds (one block to a compute unit; three
+// share it in time) leave compute units idle: their keys go to n_split workgroups, which
+// makes that round ceil(tail n / U) (keys / n + kFixed) tiles long.
 extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
-  *n_split = few_rows(dims) ? 0 : 1;
+  *n_split = 0;
+  if (few_rows(dims)) return RCSA_OK;
+  *n_split = 1;
+  const int64_t cux = xcd_cus(), items = xcd_items_of(dims);
+  const int64_t tail = items % cux;
+  if (tail == 0) return RCSA_OK;
+  constexpr int64_t kFixed = 16;
+  const int64_t tiles = (max_keys + kTileKeys - 1) / kTileKeys;
+  int64_t best = tiles + kFixed;
+  for (int64_t n = 2; n <= 16 && n * 4 <= tiles; ++n) {
+    const int64_t cost = (tail * n + cux - 1) / cux * ((tiles + n - 1) / n + kFixed) +
+                         kFixed;  // (the join)
+    if (cost < best - best / 16) {
+      best = cost;
+      *n_split = n;
+    }
+  }
   return RCSA_OK;
 }
 
 extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
   if (!dims || !window_dims(dims) || n_split < 0 || n_split > 64) return -1;
   const int64_t G = dims[3] / dims[4], row = dims[5] * 4 + 8;
-  if (n_split == 0)
-    return !few_rows(dims) ? -1
-           : wanted_units(dims) == 0
-               ? 0 : (wanted_units(dims) + dims[0] * dims[4]) * dims[1] * G * row;
-  if (n_split == 1) return 0;
-  return n_split * dims[0] * dims[4] * row_blocks(dims[1], G) * 128 * row;
+  if (n_split == 0) {
+    if (!few_rows(dims)) return -1;
+    const int64_t units = units_of_round(dims);
+    return units == 0 ? 0 : (4 * units + dims[0] * dims[4]) * dims[1] * G * row;
+  }
+  const int64_t items = xcd_items_of(dims);
+  return n_split == 1 ? 0 : n_split * (items - xcd_whole_of(items, n_split)) * kNumXcd * 128 * row;
 }
 
 extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
@@ -667,6 +707,8 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   if (n_split < 0 || n_split > 64 || (n_split == 0 && !few_rows(dims))) return RCSA_ERR_SHAPE;
   for (int i = 0; i < 12; ++i)
     if (strides[i] < 0 || strides[i] % (i < 9 ? 8 : 4)) return RCSA_ERR_STRIDE;
+  if (block_table && (strides[3] >= (1ll << 31) || strides[6] >= (1ll << 31)))
+    return RCSA_ERR_STRIDE;
   // (rows of keys do not overlap; the stride of a single one says nothing)
   const bool one = !block_table && dims[2] <= 1;
   for (int i = 4; i < 8; i += 3)
@@ -717,7 +759,13 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   a.n_rblocks = static_cast<int>(row_blocks(a.Lq, a.G));
   a.n_items = static_cast<int64_t>(a.B) * a.Hk * a.n_rblocks;
   a.n_split = static_cast<int>(n_split);
-  a.units = n_split == 0 ? static_cast<int>(wanted_units(dims)) : 0;
+  a.units = n_split == 0 ? static_cast<int>(units_of_round(dims)) : 0;
+  const int64_t xcd_items = xcd_items_of(dims);
+  if (xcd_items >= (1ll << 30)) return RCSA_ERR_SHAPE;
+  a.xcd_items = static_cast<int>(xcd_items);
+  a.xcd_whole = static_cast<int>(xcd_whole_of(xcd_items, n_split));
+  // rows without a window see more keys the later they stand
+  a.descending = a.window == 0 && a.block != 0;
   const int64_t ws_rows = need / (dims[5] * 4 + 8);
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = need ? reinterpret_cast<float2*>(a.ws_o + ws_rows * dims[5]) : nullptr;

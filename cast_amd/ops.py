@@ -1297,7 +1297,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
 
     fp32 softmax, rounded once; returns ``out [B, Lq, Hq, D]`` and, with ``return_lse``, the
     natural log-sum-exp ``[B, Hq, Lq]``.  ``n_split`` (None: planned) shares the keys of
-    a block of rows among that many workgroups."""
+    the blocks of rows that would leave compute units idle among that many workgroups."""
     fn = "window_attention"
     _require_cuda(fn, q, k, v)
     _no_grad(fn, q, k, v)
