@@ -1,5 +1,5 @@
-// Windowed attention over dense or paged keys: arguments and helpers shared by
-// the tile kernel (window_attn.hip).
+// Windowed attention over dense or paged keys: what the kernels of 128-row blocks
+// (window_attn.hip) and of units of few rows (window_units.hip) share.
 //
 // Query i of a request with q_len queries and k_len keys is at position
 // p = i + k_len - q_len; e(p) = (floor(p / block) + 1) * block is the end of its
@@ -20,18 +20,36 @@ typedef _Float16 v4hf __attribute__((ext_vector_type(4)));
 
 constexpr int kTileKeys = 32;
 
+__device__ __forceinline__ int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Division of n < 2^31 by an invariant: a high product and two shifts.
+struct Divisor {
+  uint32_t d, mul;
+  int sh1, sh2;
+};
+inline Divisor divisor(uint32_t d) {
+  int l = 0;
+  while ((1ull << l) < d) ++l;
+  return {d, static_cast<uint32_t>((1ull << 32) * ((1ull << l) - d) / d + 1), l < 1 ? l : 1,
+          l < 1 ? 0 : l - 1};
+}
+__device__ __forceinline__ int divide(int n, const Divisor& v) {
+  const uint32_t u = static_cast<uint32_t>(n), t = __umulhi(v.mul, u);
+  return static_cast<int>((t + ((u - t) >> v.sh1)) >> v.sh2);
+}
+
 struct WindowArgs {
   const void *q, *k, *v;
   void* out;
   float* lse;                       // [B][Hq][Lq], nullable
   int64_t sq[3], sk[3], sv[3], so[3];  // (batch, row, head); paged k, v: (page, slot, head)
   int B, Lq, Lk, Hq, Hk, G;
+  Divisor by_G, by_Hk, by_block, by_rblocks, by_heads;  // by_heads: B * Hk
+  Divisor by_half_page;             // half tiles of a page
   const int32_t *q_len, *k_len;     // [B], nullable: Lq, Lk
   const int32_t* table;             // [B][max_pages], nullable: dense k, v
   int64_t table_stride;
   int max_pages, n_pages, page;     // page: keys of a page, a multiple of 16
-  uint32_t page_mul;                // division of half tiles by the halves of a page
-  int page_sh1, page_sh2;
   int window, sinks, block;         // block 0: no order among positions
   float scale_log2;                 // sm_scale * log2(e)
   int n_rblocks;                    // blocks of rows of a key head
@@ -44,7 +62,8 @@ struct WindowArgs {
   // round-robin.
   int xcd_items, xcd_whole;
   int descending;
-  int units;  // few rows: the wavefronts that fit in one round, 0: one unit a key head
+  int units;  // few rows: wavefronts of one round, 0: one unit a key head
+  float per_unit;  // 1 / units
 };
 
 constexpr int kFewRows = 32;        // rows of a key head that one wavefront takes
@@ -57,7 +76,7 @@ struct KeyRange {
 __device__ __forceinline__ KeyRange key_range(const WindowArgs& a, int p, int k_len) {
   if (a.block == 0) return {0, k_len};
   if (p < 0) return {0, 0};
-  const int e = (a.block == 1 ? p : p / a.block * a.block + a.block - 1) + 1;
+  const int e = a.block == 1 ? p + 1 : divide(p, a.by_block) * a.block + a.block;
   const int hi = e < k_len ? e : k_len;
   const int lo = a.window == 0 || e <= a.window ? 0 : e - a.window;
   return {lo < hi ? lo : hi, hi};
@@ -92,6 +111,24 @@ __device__ __forceinline__ Tiles tiles_of(const WindowArgs& a, KeyRange first, K
   return t;
 }
 
+// Which key head and block of rows is entry in_xcd of XCD xcd's run (bh -1: none): a
+// contiguous run of items, or every 8th from the longest (last) row blocks on.
+struct ItemAt {
+  int bh, rblock;
+};
+__device__ __forceinline__ ItemAt item_at(const WindowArgs& a, int xcd, int in_xcd) {
+  const int64_t item = a.descending ? static_cast<int64_t>(in_xcd) * kNumXcd + xcd
+                                    : static_cast<int64_t>(xcd) * a.xcd_items + in_xcd;
+  if (in_xcd >= a.xcd_items || item >= a.n_items) return {-1, 0};
+  const int i = static_cast<int>(item);
+  if (a.descending) {
+    const int back = divide(i, a.by_heads);
+    return {i - back * static_cast<int>(a.by_heads.d), a.n_rblocks - 1 - back};
+  }
+  const int bh = divide(i, a.by_rblocks);
+  return {bh, i - bh * a.n_rblocks};
+}
+
 // Few rows: the visible tiles of all requests are dealt to units of one wavefront each,
 // `chunk` tiles of one key head at most, however uneven the lengths.  A wavefront reads
 // the lengths, one lane a request, and finds its unit among them; unit index = (units
@@ -108,21 +145,21 @@ __device__ __forceinline__ int units_of(int tiles, int chunk) {
 // kUnitTiles tiles; beyond, units of that size, or more of them than four rounds.  A unit
 // costs about 5 us before its first tile has landed (a tile streams in 0.4 to 1), and the
 // units of a last, short round leave compute units idle.
+// (Products in fp32 that round up: a plan, the same for every wavefront.)
 constexpr int kLeastTiles = 2, kUnitTiles = 16;
 __device__ __forceinline__ int chunk_of(const WindowArgs& a, int64_t total) {
-  const int64_t t = total * a.Hk;
-  const int64_t one = (t + a.units - 1) / a.units;
-  int64_t c = (t + 4 * a.units - 1) / (4 * a.units);
+  const float t = static_cast<float>(total) * a.Hk * 1.000001f;
+  const int one = static_cast<int>(t * a.per_unit) + 1;
+  int c = static_cast<int>(t * (0.25f * a.per_unit)) + 1;
   c = c < kUnitTiles ? kUnitTiles : c;
   c = c < one ? c : one;
-  return static_cast<int>(c < kLeastTiles ? kLeastTiles : c);
+  return c < kLeastTiles ? kLeastTiles : c;
 }
 struct Unit {
   int b, share, shares;  // b -1: no such unit
   int before;            // units (of one key head) of the requests before b
   Request r;
 };
-__device__ __forceinline__ int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int lane_sum(int x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
@@ -214,5 +251,353 @@ struct Half<_Float16> {
     return __builtin_bit_cast(op4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(RCSA_LDS(v4bf, p)));
   }
 };
+
+// Where a wavefront's 32 rows stand: rows row0 .. of key head hk of request b, of n_rows;
+// position of query 0; the tiles [begin, begin + steps) of the rows' tiles are its
+// share's, one of `shares`, which writes rows ws_row .. of the workspace.
+struct Place {
+  int b, hk, row0, n_rows, shift, k_len;
+  int shares, begin, steps;
+  Tiles tiles;
+  int64_t ws_row;
+};
+// First key of step s, -1 past the last.
+__device__ __forceinline__ int key_of(const Place& p, int s) {
+  const int t = p.begin + s;
+  return s >= p.steps ? -1
+                      : (t < p.tiles.sink_n ? t : p.tiles.win_t0 + t - p.tiles.sink_n) * kTileKeys;
+}
+__device__ __forceinline__ KeyRange row_range(const WindowArgs& a, const Place& p, int row) {
+  row = row < p.n_rows ? row : p.n_rows - 1;
+  return key_range(a, divide(row, a.by_G) + p.shift, p.k_len);
+}
+// The lane's row; rows past the last stand at the last one's place, unwritten.  (Found again
+// where it is needed: registers are short.)
+struct Row {
+  int row, qi, head;
+  bool live;
+};
+__device__ __forceinline__ Row row_of(const WindowArgs& a, const Place& p, int row) {
+  asm volatile("" : "+v"(row));
+  const bool live = row < p.n_rows;
+  const int at = live ? row : p.n_rows - 1, qi = divide(at, a.by_G);
+  return {row, qi, p.hk * a.G + at - qi * a.G, live};
+}
+
+// A step: its first key and, paged, the pages of its two halves of 16 keys (a half lies in
+// one page: pages hold whole halves).  Scalar arithmetic and loads throughout.
+struct Step {
+  int key, page0, page1;
+};
+__device__ __forceinline__ bool page_ok(const WindowArgs& a, int p) {
+  return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
+}
+template <bool PAGED>
+__device__ __forceinline__ Step step_of(const WindowArgs& a, const Place& p, const int32_t* table,
+                                        int s) {
+  Step r{key_of(p, s), 0, 0};
+  if constexpr (PAGED) {
+    const int half = (r.key < 0 ? 0 : r.key) >> 4;
+    const int col0 = divide(half, a.by_half_page);
+    int col1 = divide(half + 1, a.by_half_page);
+    col1 = col1 < a.max_pages ? col1 : a.max_pages - 1;
+    r.page0 = ld_const(table + col0);
+    r.page1 = ld_const(table + col1);
+  }
+  return r;
+}
+// This share's part of all tiles (parts differ by at most one tile).
+__device__ __forceinline__ void share_of(Place& p, int share) {
+  const uint32_t n = static_cast<uint32_t>(p.tiles.all()), k = static_cast<uint32_t>(p.shares);
+  const int q = uniform_int(static_cast<int>(k == 1 ? n : n / k));
+  const int rem = static_cast<int>(n) - q * p.shares;
+  p.begin = share * q + (share < rem ? share : rem);
+  p.steps = q + (share < rem ? 1 : 0);
+}
+// Whether the step's halves are there: bits 0 and 1.
+template <bool PAGED>
+__device__ __forceinline__ int halves_there(const WindowArgs& a, const Step& s) {
+  return PAGED ? (page_ok(a, s.page0) ? 1 : 0) + (page_ok(a, s.page1) ? 2 : 0) : 3;
+}
+// The 16 rows of a half of a step: offsets of its first row, rows that are there.  (32 x
+// 32-bit products: a page spans less than 4 GiB.)
+struct HalfRows {
+  uint64_t k, v;
+  int rows;
+};
+template <bool PAGED>
+__device__ __forceinline__ HalfRows half_rows(const WindowArgs& a, const Step& s, int half,
+                                              int k_len, uint32_t krb, uint32_t vrb) {
+  const int key = (s.key < 0 ? 0 : s.key) + 16 * half;
+  HalfRows r;
+  bool there = s.key >= 0;
+  if constexpr (PAGED) {
+    const int pg = half ? s.page1 : s.page0;
+    there = there && page_ok(a, pg);
+    const uint32_t slot = static_cast<uint32_t>(key - divide(key >> 4, a.by_half_page) * a.page);
+    const uint32_t at = there ? static_cast<uint32_t>(pg) : 0u;
+    r.k = static_cast<uint64_t>(at) * static_cast<uint32_t>(a.sk[0] * 2) +
+          static_cast<uint64_t>(slot) * krb;
+    r.v = static_cast<uint64_t>(at) * static_cast<uint32_t>(a.sv[0] * 2) +
+          static_cast<uint64_t>(slot) * vrb;
+  } else {
+    r.k = static_cast<uint64_t>(static_cast<uint32_t>(key)) * krb;
+    r.v = static_cast<uint64_t>(static_cast<uint32_t>(key)) * vrb;
+  }
+  const int left = k_len - key;
+  r.rows = uniform_int(!there || left <= 0 ? 0 : (left < 16 ? left : 16));
+  return r;
+}
+
+// 32 rows against staged tiles of 32 keys: S^T = K Q^T puts a query row in a lane (its
+// 16 + 16 keys in the two lane halves), so a row's maximum and sum need one lane swap,
+// and P^T is the second operand of O^T = V^T P^T as it stands.  The running maximum moves
+// only when a term passes 2^kTau.  P is rounded to the type for its product, the sums
+// keep fp32.
+template <typename T, int D>
+struct RowTile {
+  using O = Half<T>;
+  typedef typename O::op8 op8;
+  static constexpr int KROW = D * 2, CPR = KROW / 16;  // bytes and 16-byte chunks of a row
+  static constexpr int QSTEPS = D / 16, NDT = D / 32;
+  static constexpr int TILE = kTileKeys * KROW;        // bytes of a K (or V) tile
+  op8 q_op[QSTEPS];
+  v16f o_acc[NDT];
+  float m_run, l_run;
+  int k_off[QSTEPS], v_off[NDT];  // LDS read offsets (V behind K)
+
+  __device__ __forceinline__ void init(int lane) {
+    const int hf = lane >> 5, lr = lane & 31;
+    const int kr = key_perm(lr), ks = swz_k<KROW>(kr) & (CPR - 1);
+#pragma unroll
+    for (int st = 0; st < QSTEPS; ++st)
+      k_off[st] = kr * KROW + (((hf * QSTEPS + st) ^ ks) * 16);
+    const int grp = lane >> 4, gi = lane & 15;
+    const int vr = 16 * (grp >> 1) + (gi >> 2), vs = swz_v(vr) & (CPR - 1);
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      const int d = 32 * dt + 16 * (grp & 1) + 4 * (gi & 3);
+      v_off[dt] = TILE + vr * KROW + (((d >> 3) ^ vs) * 16) + (d & 7) * 2;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.0f;
+    m_run = -INFINITY;
+    l_run = 0.0f;
+  }
+  __device__ __forceinline__ void load_q(const T* row, int hf) {
+#pragma unroll
+    for (int st = 0; st < QSTEPS; ++st)
+      q_op[st] = *reinterpret_cast<const op8*>(row + (hf * QSTEPS + st) * 8);
+  }
+
+  // One tile: `inside` when every row sees all of it, else bits() gives the lane's 16 keys.
+  // prefetch() issues scalar loads for later steps: behind the first products (they return
+  // out of order, so a wait for LDS behind them would wait for them too).
+  template <typename Bits, typename Pre>
+  __device__ __forceinline__ void step(const char* tile, float c, bool inside, Bits&& bits,
+                                       Pre&& prefetch) {
+    v4i kraw[QSTEPS];
+#pragma unroll
+    for (int st = 0; st < QSTEPS; ++st)
+      kraw[st] = *reinterpret_cast<const v4i*>(tile + k_off[st]);
+    v16f s_acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < QSTEPS; ++st)
+      s_acc = O::mfma(__builtin_bit_cast(op8, kraw[st]), q_op[st], s_acc);
+    __builtin_amdgcn_sched_group_barrier(0x100, QSTEPS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, QSTEPS, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    prefetch();
+    float rv[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
+    if (!inside) {
+      const uint32_t seen = bits();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rv[r] = ((seen >> r) & 1u) ? rv[r] : -INFINITY;
+    }
+    op8 p_op[2];
+    auto exps = [&]() __attribute__((always_inline)) -> float {
+      const float bias = m_run == -INFINITY ? 0.0f : -m_run;
+      float lsum[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) {
+          const float e = __builtin_amdgcn_exp2f(fmaf(rv[8 * u + jj], c, bias));
+          p_op[u][jj] = static_cast<T>(e);
+          if (u == 0 && jj < 4) lsum[jj] = e;
+          else lsum[jj & 3] += e;
+        }
+      return (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
+    };
+    // (a lane's partial sum bounds its terms)
+    float part = exps();
+    if (__ballot(m_run == -INFINITY || !(part <= kTauPow)) != 0) {
+      float rmax = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
+      rmax = pair_max(rmax);
+      const float m_blk = rmax == -INFINITY ? -INFINITY : rmax * c;
+      if (__ballot(m_blk > m_run + kTau) != 0) {
+        const float m_new = fmaxf(m_run, m_blk);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+        m_run = m_new;
+        part = exps();
+      }
+    }
+    l_run += part;
+    // (the reads of the second half of the keys are in flight beside the first half's
+    // products)
+    auto v_group = [&](int u, op8 (&op)[NDT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        const char* const p0 = tile + v_off[dt] + 8 * u * KROW;
+        const auto lo = O::read_tr(p0);
+        const auto hi = O::read_tr(p0 + 4 * KROW);
+        op[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    };
+    op8 vop[2][NDT];
+    v_group(0, vop[0]);
+    v_group(1, vop[1]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) o_acc[dt] = O::mfma(vop[u][dt], p_op[u], o_acc[dt]);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * NDT, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * NDT; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i < NDT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+  }
+};
+
+// The lane's 16 keys of the tile at `key` that row `row` sees, as bits.
+__device__ __forceinline__ uint32_t seen_bits(const WindowArgs& a, const Place& p, int row, int hf,
+                                              int key, int there) {
+  const KeyRange kr = key_range(a, row_of(a, p, row).qi + p.shift, p.k_len);
+  const int k0 = key + 16 * hf, sink = a.sinks < kr.hi ? a.sinks : kr.hi;
+  auto below = [](int x) -> uint32_t {  // bits of keys < x
+    const int n = x < 0 ? 0 : (x > 16 ? 16 : x);
+    return (1u << n) - 1u;
+  };
+  const uint32_t bits = below(kr.hi - k0) & (~below(kr.lo - k0) | below(sink - k0));
+  return (there >> hf) & 1 ? bits : 0u;
+}
+
+// The end of a wavefront's rows: normalise, write the rows (or the share's partial ones and
+// their (max, sum)) and the LSE.
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void finish_rows(const WindowArgs& a, const Place& p, RowTile<T, D>& t,
+                                            int lane, const char* kbase, const char* vbase,
+                                            const int32_t* table) {
+  typedef typename Half<T>::op4 op4;
+  const int hf = lane >> 5, lr = lane & 31;
+  const float l = pair_sum(t.l_run), m = t.m_run;
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (a NaN sum stays one)
+  bool bad = false;  // a product that is no number in a row whose sum is one
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      t.o_acc[dt][r] *= inv;
+      bad = bad || !(fabsf(t.o_acc[dt][r]) < INFINITY);
+    }
+  const Row my = row_of(a, p, p.row0 + lr);
+  const int64_t wrow = p.ws_row + lr;
+  if (my.live) {
+    if (p.shares > 1) {
+      float* const wp = a.ws_o + wrow * D + 4 * hf;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<v4f*>(wp + 32 * dt + 8 * g) =
+              v4f{t.o_acc[dt][4 * g], t.o_acc[dt][4 * g + 1], t.o_acc[dt][4 * g + 2],
+                  t.o_acc[dt][4 * g + 3]};
+      if (hf == 0)
+        a.ws_ml[wrow] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
+    } else {
+      T* const op = static_cast<T*>(a.out) + p.b * a.so[0] +
+                    static_cast<int64_t>(my.qi) * a.so[1] + my.head * a.so[2] + 4 * hf;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          op4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(t.o_acc[dt][4 * g + e]);
+          *reinterpret_cast<op4*>(op + 32 * dt + 8 * g) = w;
+        }
+      if (hf == 0 && a.lse)
+        a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
+            l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+    }
+  }
+  // A row whose products met a value that it does not see (0 * inf or 0 * NaN of a
+  // masked key): its sum is taken again over its own keys, one row at a time.
+  uint64_t again = __ballot(bad && my.live && l > 0.0f && l < INFINITY);
+  again |= again >> 32;
+  if (static_cast<uint32_t>(again) == 0) return;
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the stores above come first)
+  for (uint32_t rows = static_cast<uint32_t>(again); rows != 0; rows &= rows - 1) {
+    constexpr int N = D / 64;
+    const int i = __builtin_ctz(rows);
+    const Row r = row_of(a, p, p.row0 + i);
+    const KeyRange rk = row_range(a, p, p.row0 + i);
+    const int rsink = a.sinks < rk.hi ? a.sinks : rk.hi;
+    const T* const rq = static_cast<const T*>(a.q) + p.b * a.sq[0] +
+                        static_cast<int64_t>(r.qi) * a.sq[1] + r.head * a.sq[2];
+    const float rm = __shfl(m, i, kWave), rinv = __shfl(inv, i, kWave);
+    float acc[N], qv[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      acc[c] = 0.0f;
+      qv[c] = static_cast<float>(rq[lane + 64 * c]);
+    }
+    for (int s = 0; s < p.steps; ++s)
+      for (int j = key_of(p, s), end = j + kTileKeys; j < end; ++j) {
+        if (!(j < rk.hi && (j >= rk.lo || j < rsink))) continue;
+        int64_t ko = j * a.sk[1], vo = j * a.sv[1];
+        if constexpr (PAGED) {
+          const int col = divide(j >> 4, a.by_half_page), pg = table[col];
+          if (!page_ok(a, pg)) continue;
+          const int64_t slot = j - col * a.page;
+          ko = pg * a.sk[0] + slot * a.sk[1];
+          vo = pg * a.sv[0] + slot * a.sv[1];
+        }
+        const T* const kp = reinterpret_cast<const T*>(kbase) + ko;
+        const T* const vp = reinterpret_cast<const T*>(vbase) + vo;
+        float x = 0.0f;
+#pragma unroll
+        for (int c = 0; c < N; ++c) x = fmaf(qv[c], static_cast<float>(kp[lane + 64 * c]), x);
+        const float pr = __builtin_amdgcn_exp2f(fmaf(wave_sum(x), a.scale_log2, -rm));
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+          acc[c] = fmaf(pr, static_cast<float>(vp[lane + 64 * c]), acc[c]);
+      }
+    T* const dst = static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(r.qi) * a.so[1] +
+                   r.head * a.so[2];
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      if (p.shares > 1) a.ws_o[(p.ws_row + i) * D + lane + 64 * c] = acc[c] * rinv;
+      else dst[lane + 64 * c] = static_cast<T>(acc[c] * rinv);
+    }
+  }
+}
+
+// Units of few rows and their join (window_units.hip); type 0: bf16, 1: fp16.
+int launch_window_units(WindowArgs& a, int type, int64_t D, hipStream_t s);
 
 }  // namespace rcsa

@@ -1,0 +1,181 @@
+// Windowed attention of few rows (one new token of each request, or a few): at most 32
+// rows of a key head, one wavefront a unit of the visible tiles of all requests.
+//
+// The keys and values are read once and bound the time, so what counts is bytes in
+// flight: a wavefront holds the next tile (16 KB at D 128) in registers while it works
+// on the one in its own LDS, eight wavefronts to a compute unit, no barriers.  The loop
+// is one tile long: a unit of a few tiles runs through little code that is not yet in
+// the instruction cache.
+#include "window_attn.h"
+
+namespace rcsa {
+
+template <typename T, int D, bool PAGED>
+__global__ void __launch_bounds__(64)
+__attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
+window_unit_kernel(WindowArgs a) {
+  using R = RowTile<T, D>;
+  constexpr int RPU = 1024 / R::KROW;          // rows of a 1 KiB load
+  constexpr int UPH = 16 * R::KROW / 1024;     // loads of a half tile, K and V each
+  __shared__ __attribute__((aligned(1024))) char tile[2 * R::TILE];
+  const int lane = threadIdx.x, hf = lane >> 5, lr = lane & 31;
+
+  const int w = divide(static_cast<int>(blockIdx.x), a.by_Hk);
+  const Unit u = find_unit<false>(a, w, lane);
+  if (u.b < 0) return;
+  Place p;
+  p.b = u.b;
+  p.hk = static_cast<int>(blockIdx.x) - w * a.Hk;
+  p.row0 = 0;
+  p.n_rows = u.r.q_len * a.G;
+  if (p.n_rows == 0) return;
+  p.k_len = u.r.k_len;
+  p.shift = u.r.k_len - u.r.q_len;
+  p.shares = u.shares;
+  p.ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
+  const KeyRange first = row_range(a, p, 0), last = row_range(a, p, p.n_rows - 1);
+  p.tiles = tiles_of(a, first, last);
+  share_of(p, u.share);
+
+  const char* const kbase = static_cast<const char*>(a.k) +
+                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
+  const char* const vbase = static_cast<const char*>(a.v) +
+                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
+  const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
+  const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
+
+  // load i of a half: rows i RPU + lane / CPR, chunk lane % CPR; rows past the keys and
+  // pages that are not there read zeros through ranges that end before them
+  v4i kst[2 * UPH], vst[2 * UPH];
+  const int lrow = lane / R::CPR, chunk = lane % R::CPR;
+  const uint32_t k_lo = lrow * krb + chunk * 16, v_lo = lrow * vrb + chunk * 16;
+  auto load = [&](const Step& s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const HalfRows hr = half_rows<PAGED>(a, s, h, p.k_len, krb, vrb);
+      const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(kbase) + hr.k, 0, hr.rows * static_cast<int>(krb), kRsrcWord3);
+      const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(vbase) + hr.v, 0, hr.rows * static_cast<int>(vrb), kRsrcWord3);
+#pragma unroll
+      for (int i = 0; i < UPH; ++i) {
+        kst[h * UPH + i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(
+            kr, static_cast<int>(k_lo + i * RPU * krb), 0, 0));
+        vst[h * UPH + i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(
+            vr, static_cast<int>(v_lo + i * RPU * vrb), 0, 0));
+      }
+    }
+  };
+  Step cur = step_of<PAGED>(a, p, table, 0);
+  Step next = step_of<PAGED>(a, p, table, 1);
+  R t;
+  {
+    const Row r = row_of(a, p, lr);
+    t.load_q(static_cast<const T*>(a.q) + p.b * a.sq[0] + static_cast<int64_t>(r.qi) * a.sq[1] +
+                 r.head * a.sq[2], hf);
+  }
+  load(cur);
+  t.init(lane);
+  // Q has landed before the loop (its waits there would drain the loads of the next tile)
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(4 * UPH));
+  // LDS places of the loads: the swizzles are sums of a row's bits modulo 2, and load i adds
+  // bits i RPU to the lane's (none that V's takes)
+  const int k_at = lrow * R::KROW + ((chunk ^ (swz_k<R::KROW>(lrow) & (R::CPR - 1))) * 16);
+  const int v_at = R::TILE + lrow * R::KROW + ((chunk ^ (swz_v(lrow) & (R::CPR - 1))) * 16);
+  for (int s = 0; s < p.steps; ++s) {
+#pragma unroll
+    for (int i = 0; i < 2 * UPH; ++i) {
+      const int kx = (swz_k<R::KROW>(i * RPU) & (R::CPR - 1)) * 16;
+      *reinterpret_cast<v4i*>(tile + (k_at ^ kx) + i * 1024) = kst[i];
+      *reinterpret_cast<v4i*>(tile + v_at + i * 1024) = vst[i];
+    }
+    const Step now = cur;
+    cur = next;
+    if (s + 1 < p.steps) load(cur);
+    const int there = halves_there<PAGED>(a, now);
+    const bool inside = there == 3 && now.key + kTileKeys <= first.hi &&
+                        (now.key >= last.lo || now.key + kTileKeys <= a.sinks);
+    t.step(tile, a.scale_log2, inside, [&]() __attribute__((always_inline)) {
+      return seen_bits(a, p, lr, hf, now.key, there);
+    }, [&]() __attribute__((always_inline)) { next = step_of<PAGED>(a, p, table, s + 2); });
+  }
+  finish_rows<T, D, PAGED>(a, p, t, lane, kbase, vbase, table);
+}
+
+// The units of every row joined: w_s = l_s 2^(m_s - M), out = sum w_s O_s / sum w_s.  A
+// workgroup takes one row, its threads (share, 8 channels); the shares are added in a
+// fixed order.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
+  constexpr int CPR = D / 8, GROUPS = 256 / CPR;
+  __shared__ float s_acc[GROUPS][D], s_sum[GROUPS], s_max[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int R = a.Lq * a.G;
+  const int row = static_cast<int>(blockIdx.x) % R;
+  const int bh = static_cast<int>(blockIdx.x) / R;
+  const int b = divide(bh, a.by_Hk), hk = bh - b * a.Hk;
+  const Unit u = find_unit<true>(a, b, lane);
+  if (row >= u.r.q_len * a.G) return;
+  const int shares = u.shares;
+  if (shares <= 1) return;  // written by its only unit
+  const int64_t first = static_cast<int64_t>(u.before) * a.Hk + hk;
+  auto at = [&](int s) __attribute__((always_inline)) -> int64_t {
+    return (first + static_cast<int64_t>(s) * a.Hk) * R + row;
+  };
+  float mx = -INFINITY;
+  for (int s = tid; s < shares; s += 256) mx = fmaxf(mx, a.ws_ml[at(s)].x);
+  mx = wave_max(mx);
+  if (lane == 0) s_max[tid >> 6] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  const int c = tid % CPR, g = tid / CPR;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float sum = 0.0f;
+  for (int s = g; s < shares; s += GROUPS) {
+    const float2 ml = a.ws_ml[at(s)];
+    if (ml.x == -INFINITY) continue;
+    const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+    sum += w;
+    float o[8];
+    Vec8<float>::load(a.ws_o + at(s) * D + c * 8, o);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, o[j], acc[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s_acc[g][c * 8 + j] = acc[j];
+  if (c == 0) s_sum[g] = sum;
+  __syncthreads();
+  if (tid >= D) return;
+  float total = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) {
+    total += s_sum[i];
+    o += s_acc[i][tid];
+  }
+  const int qi = divide(row, a.by_G), head = hk * a.G + row - qi * a.G;
+  static_cast<T*>(a.out)[b * a.so[0] + qi * a.so[1] + head * a.so[2] + tid] =
+      static_cast<T>(total == 0.0f ? 0.0f : o / total);
+  if (a.lse && tid == 0)
+    a.lse[(static_cast<int64_t>(b) * a.Hq + head) * a.Lq + qi] =
+        total == 0.0f ? -INFINITY : (mx + __log2f(total)) * 0.69314718055994531f;
+}
+
+template <typename T, int D>
+static int launch_units(WindowArgs& a, hipStream_t s) {
+  const int64_t n = 4ll * a.units + static_cast<int64_t>(a.B) * a.Hk;
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * a.Lq * a.G;
+  if (n >= (1ll << 31) || rows >= (1ll << 31)) return RCSA_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>(n));
+  if (a.table) window_unit_kernel<T, D, true><<<grid, dim3(64), 0, s>>>(a);
+  else window_unit_kernel<T, D, false><<<grid, dim3(64), 0, s>>>(a);
+  if (a.units)
+    window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
+  return launch_status();
+}
+
+int launch_window_units(WindowArgs& a, int type, int64_t D, hipStream_t s) {
+  if (type == 0) return D == 128 ? launch_units<__bf16, 128>(a, s) : launch_units<__bf16, 64>(a, s);
+  return D == 128 ? launch_units<_Float16, 128>(a, s) : launch_units<_Float16, 64>(a, s);
+}
+
+}  // namespace rcsa
