@@ -33,7 +33,8 @@ inline Divisor divisor(uint32_t d) {
   return {d, static_cast<uint32_t>((1ull << 32) * ((1ull << l) - d) / d + 1), l < 1 ? l : 1,
           l < 1 ? 0 : l - 1};
 }
-__device__ __forceinline__ int divide(int n, const Divisor& v) {
+template <typename V>
+__device__ __forceinline__ int divide(int n, V& v) {
   const uint32_t u = static_cast<uint32_t>(n), t = __umulhi(v.mul, u);
   return static_cast<int>((t + ((u - t) >> v.sh1)) >> v.sh2);
 }
@@ -46,6 +47,7 @@ struct WindowArgs {
   int B, Lq, Lk, Hq, Hk, G;
   Divisor by_G, by_Hk, by_block, by_rblocks, by_heads;  // by_heads: B * Hk
   Divisor by_half_page;             // half tiles of a page
+  int whole_tiles;                  // a page holds a multiple of 32 keys
   const int32_t *q_len, *k_len;     // [B], nullable: Lq, Lk
   const int32_t* table;             // [B][max_pages], nullable: dense k, v
   int64_t table_stride;
@@ -73,7 +75,8 @@ constexpr int kMaxPlanned = 512;    // requests whose lengths every wavefront re
 struct KeyRange {
   int lo, hi;
 };
-__device__ __forceinline__ KeyRange key_range(const WindowArgs& a, int p, int k_len) {
+template <typename A>
+__device__ __forceinline__ KeyRange key_range(A& a, int p, int k_len) {
   if (a.block == 0) return {0, k_len};
   if (p < 0) return {0, 0};
   const int e = a.block == 1 ? p + 1 : divide(p, a.by_block) * a.block + a.block;
@@ -267,7 +270,8 @@ __device__ __forceinline__ int key_of(const Place& p, int s) {
   return s >= p.steps ? -1
                       : (t < p.tiles.sink_n ? t : p.tiles.win_t0 + t - p.tiles.sink_n) * kTileKeys;
 }
-__device__ __forceinline__ KeyRange row_range(const WindowArgs& a, const Place& p, int row) {
+template <typename A>
+__device__ __forceinline__ KeyRange row_range(A& a, const Place& p, int row) {
   row = row < p.n_rows ? row : p.n_rows - 1;
   return key_range(a, divide(row, a.by_G) + p.shift, p.k_len);
 }
@@ -277,7 +281,8 @@ struct Row {
   int row, qi, head;
   bool live;
 };
-__device__ __forceinline__ Row row_of(const WindowArgs& a, const Place& p, int row) {
+template <typename A>
+__device__ __forceinline__ Row row_of(A& a, const Place& p, int row) {
   asm volatile("" : "+v"(row));
   const bool live = row < p.n_rows;
   const int at = live ? row : p.n_rows - 1, qi = divide(at, a.by_G);
@@ -289,7 +294,8 @@ __device__ __forceinline__ Row row_of(const WindowArgs& a, const Place& p, int r
 struct Step {
   int key, page0, page1;
 };
-__device__ __forceinline__ bool page_ok(const WindowArgs& a, int p) {
+template <typename A>
+__device__ __forceinline__ bool page_ok(A& a, int p) {
   return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
 }
 template <bool PAGED>
@@ -299,10 +305,13 @@ __device__ __forceinline__ Step step_of(const WindowArgs& a, const Place& p, con
   if constexpr (PAGED) {
     const int half = (r.key < 0 ? 0 : r.key) >> 4;
     const int col0 = divide(half, a.by_half_page);
-    int col1 = divide(half + 1, a.by_half_page);
-    col1 = col1 < a.max_pages ? col1 : a.max_pages - 1;
     r.page0 = ld_const(table + col0);
-    r.page1 = ld_const(table + col1);
+    if (a.whole_tiles) {  // pages of whole tiles: one entry for both halves
+      r.page1 = r.page0;
+    } else {
+      const int col1 = divide(half + 1, a.by_half_page);
+      r.page1 = ld_const(table + (col1 < a.max_pages ? col1 : a.max_pages - 1));
+    }
   }
   return r;
 }
@@ -499,9 +508,12 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowArgs& a, const Place& 
 // The end of a wavefront's rows: normalise, write the rows (or the share's partial ones and
 // their (max, sum)) and the LSE.
 template <typename T, int D, bool PAGED>
-__device__ __forceinline__ void finish_rows(const WindowArgs& a, const Place& p, RowTile<T, D>& t,
-                                            int lane, const char* kbase, const char* vbase,
-                                            const int32_t* table) {
+__device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, int lane) {
+  // (the arguments are read again: kept in scalar registers they would spill the loop's)
+  typedef const __attribute__((address_space(4))) WindowArgs Late;
+  Late* late = (Late*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(late));
+  Late& a = *late;
   typedef typename Half<T>::op4 op4;
   const int hf = lane >> 5, lr = lane & 31;
   const float l = pair_sum(t.l_run), m = t.m_run;
@@ -551,6 +563,11 @@ __device__ __forceinline__ void finish_rows(const WindowArgs& a, const Place& p,
   again |= again >> 32;
   if (static_cast<uint32_t>(again) == 0) return;
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the stores above come first)
+  const char* const kbase = static_cast<const char*>(a.k) +
+                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
+  const char* const vbase = static_cast<const char*>(a.v) +
+                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
+  const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
   for (uint32_t rows = static_cast<uint32_t>(again); rows != 0; rows &= rows - 1) {
     constexpr int N = D / 64;
     const int i = __builtin_ctz(rows);

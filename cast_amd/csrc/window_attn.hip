@@ -146,7 +146,7 @@ window_kernel(WindowArgs a) {
     iteration(std::integral_constant<int, 2>{}, j + 2);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
-  finish_rows<T, D, PAGED>(a, p, t, lane, kbase, vbase, table);
+  finish_rows<T, D, PAGED>(p, t, lane);
 }
 
 // The shares of the split row blocks joined: w_s = l_s 2^(m_s - M),
@@ -340,6 +340,7 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   a.n_pages = static_cast<int>(n_pages);
   a.page = static_cast<int>(page_size);
   if (block_table) a.by_half_page = divisor(static_cast<uint32_t>(page_size / 16));
+  a.whole_tiles = page_size % kTileKeys == 0;
   a.window = static_cast<int>(window < most ? window : 0);
   a.sinks = static_cast<int>(sinks < most ? sinks : most);
   a.block = static_cast<int>(block < most ? block : most);

@@ -99,7 +99,7 @@ window_unit_kernel(WindowArgs a) {
       return seen_bits(a, p, lr, hf, now.key, there);
     }, [&]() __attribute__((always_inline)) { next = step_of<PAGED>(a, p, table, s + 2); });
   }
-  finish_rows<T, D, PAGED>(a, p, t, lane, kbase, vbase, table);
+  finish_rows<T, D, PAGED>(p, t, lane);
 }
 
 // The units of every row joined: w_s = l_s 2^(m_s - M), out = sum w_s O_s / sum w_s.  A
