@@ -81,6 +81,25 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+__device__ __forceinline__ int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Division of n < 2^31 by an invariant: a high product and two shifts.
+struct Divisor {
+  uint32_t d, mul;
+  int sh1, sh2;
+};
+inline Divisor divisor(uint32_t d) {
+  int l = 0;
+  while ((1ull << l) < d) ++l;
+  return {d, static_cast<uint32_t>((1ull << 32) * ((1ull << l) - d) / d + 1), l < 1 ? l : 1,
+          l < 1 ? 0 : l - 1};
+}
+template <typename V>
+__device__ __forceinline__ int divide(int n, V& v) {
+  const uint32_t u = static_cast<uint32_t>(n), t = __umulhi(v.mul, u);
+  return static_cast<int>((t + ((u - t) >> v.sh1)) >> v.sh2);
+}
+
 inline int launch_status() {
   hipError_t e = hipGetLastError();
   return e == hipSuccess ? RCSA_OK : RCSA_ERR_LAUNCH;

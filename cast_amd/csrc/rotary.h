@@ -4,8 +4,6 @@
 
 namespace rcsa {
 
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
 constexpr int kMaxTokens = 32;   // tokens of a workgroup
 constexpr int kMaxDim = 512;     // channels of a head
 constexpr int kMaxHeads = 4096;
@@ -30,7 +28,9 @@ struct RotaryArgs {
   const int32_t* table;       // [B][max_pages] pages of every request's cache
   int64_t table_stride, max_pages, n_pages, page_size;
   const int32_t *starts, *lengths;
-  int tokens, lanes_log2;     // of the vector form's launch
+  // the vector form's launch: tokens of a workgroup, lanes of a head (log2), divisors
+  int tokens, lanes_log2;
+  Divisor by_heads, by_L, by_pairs;  // by_heads: Hq + Hk + Hv
 };
 
 }  // namespace rcsa

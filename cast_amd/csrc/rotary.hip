@@ -18,41 +18,23 @@
 
 namespace rcsa {
 
-// 8 consecutive elements as fp32, and back with one rounding.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]);
-template <>
-__device__ __forceinline__ void load8<__bf16>(const __bf16* p, float (&f)[8]) {
-  Vec8<u16>::load(reinterpret_cast<const u16*>(p), f);
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&f)[8]) {
-  Vec8<float>::load(p, f);
-}
-template <>
-__device__ __forceinline__ void load8<_Float16>(const _Float16* p, float (&f)[8]) {
-  const v8h r = *reinterpret_cast<const v8h*>(p);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = static_cast<float>(r[i]);
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  typedef T vec __attribute__((ext_vector_type(8)));
-  vec r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = static_cast<T>(f[i]);
-  *reinterpret_cast<vec*>(p) = r;
-}
-
 __device__ __forceinline__ float weight_at(const void* w, int dtype, int64_t i) {
   if (dtype == RCSA_F32) return static_cast<const float*>(w)[i];
   if (dtype == RCSA_F16) return static_cast<float>(static_cast<const _Float16*>(w)[i]);
   return bf16_to_f32(static_cast<const u16*>(w)[i]);
 }
-__device__ __forceinline__ void weight8(const void* w, int dtype, int64_t i, float (&f)[8]) {
-  if (dtype == RCSA_F32) load8(static_cast<const float*>(w) + i, f);
-  else if (dtype == RCSA_F16) load8(static_cast<const _Float16*>(w) + i, f);
-  else load8(static_cast<const __bf16*>(w) + i, f);
+template <typename W, int V>
+__device__ __forceinline__ void widen(const void* w, int64_t i, float (&f)[V]) {
+  typedef W vec __attribute__((ext_vector_type(V)));
+  const vec r = *reinterpret_cast<const vec*>(static_cast<const W*>(w) + i);
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = static_cast<float>(r[j]);
+}
+template <int V>
+__device__ __forceinline__ void weight_run(const void* w, int dtype, int64_t i, float (&f)[V]) {
+  if (dtype == RCSA_F32) widen<float, V>(w, i, f);
+  else if (dtype == RCSA_F16) widen<_Float16, V>(w, i, f);
+  else widen<__bf16, V>(w, i, f);
 }
 
 // cos and sin (times the scale) of pair i of the token at (b, t).
@@ -99,175 +81,235 @@ __device__ __forceinline__ TokenRows token_rows(const RotaryArgs& a, int64_t tok
   return r;
 }
 
-// The vector form: a lane holds 16 channels of a head, the 8 first and the 8
-// second channels of 8 pairs (16 channels in a row where nothing turns or the
-// pairs are interleaved), `lanes` = a power of two >= D / 16 lanes a head.  A
-// workgroup takes `tokens` tokens; its threads run over their (token, head)
-// list, queries, then keys, then values, so that no lane idles where a tensor
-// has few heads.
-template <typename T, bool INTER, int NORM>
+// The vector form.  A lane holds two runs of V channels of a head: V pairs of the half
+// layout, or 2 V / 2 interleaved ones; `lanes` = a power of two >= D / 2V lanes a head.  A
+// workgroup takes `tokens` tokens; its threads run over their (token, head) list, queries,
+// keys, then values, so that no lane idles where a tensor has few heads, U entries at a time:
+// the loads of all U are issued first, those of the first U ahead of the sines (rows
+// that are in flight, not the work on them, set the pace).  Joint norms need a token's
+// sum before its first store: a list of U entries stays in registers in between, a
+// longer one is read again.  Rows go past the caches both ways (non-temporal; us without,
+// inputs out of the caches: 44 frames x 24 heads 79 and 91, 3520 x 72 heads with joint
+// norms 34 and 40, 16391 x 48 heads 80 and 86).  A memory-bound reader of the outputs right
+// behind loses what that gains or, at 84 MB of them, 7% of the pair; the reader here is
+// the attention.
+template <typename T>
+constexpr int kWide = 16 / static_cast<int>(sizeof(T));
+// Entries of a thread.  Wide runs: two for the rotation alone (44 frames x 24 heads 80 us, one
+// 89), one with norms of heads (16391 tokens x 48 heads 82 us, two 90), three with
+// joint norms, which the list of a token should fit (3520 x 72 heads 35 us, two 43); narrow
+// runs six (14097 x 9 heads of 80 57 us, four 61).
+template <int V, int NORM>
+constexpr int kEntries = V == 2 ? 6 : (NORM == 0 ? 2 : (NORM == 1 ? 1 : 3));
+template <typename T, int V>
+struct Run {
+  typedef T vec __attribute__((ext_vector_type(V)));
+};
+template <typename T, int V, bool INTER, int NORM>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
+  typedef typename Run<T, V>::vec vec;
+  constexpr int U = kEntries<V, NORM>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int np = a.n_pairs, nt = a.tokens, nh = a.Hq + a.Hk + a.Hv;
+  const int np = a.n_pairs, nt = a.tokens, nn = a.Hq + a.Hk, nh = nn + a.Hv;
   float* const s_cos = reinterpret_cast<float*>(smem);       // [nt][np]
   float* const s_sin = s_cos + nt * np;                      // [nt][np]
   float* const s_w = s_sin + nt * np;                        // [2][D] shared weights
   float* const s_sum = s_w + (NORM ? 2 * a.D : 0);           // [nt][Hq + Hk]
-  // element offsets of every token's source and destination rows by tensor
-  __shared__ int64_t s_src[3][kMaxTokens], s_dst[3][kMaxTokens];
-  const int tid = threadIdx.x;
-  const int64_t token0 = static_cast<int64_t>(blockIdx.x) * nt;
-  const int64_t total = a.B * a.L;
-  for (int i = tid; i < nt * np; i += 256) {
-    const int64_t token = token0 + i / np;
-    if (token < total) {
-      const int64_t b = token / a.L;
-      const float2 cs = turn_of(a, b, token - b * a.L, i % np);
-      s_cos[i] = cs.x;
-      s_sin[i] = cs.y;
-    }
+  float* const s_all = s_sum + nt * nn;                      // [nt][2] sums of a token
+  // element offsets of every token's destination rows by tensor, -1: none
+  __shared__ int64_t s_dst[3][kMaxTokens];
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const int total = static_cast<int>(a.B * a.L);
+  const int token0 = static_cast<int>(blockIdx.x) * nt;
+  const int left = total - token0 < nt ? total - token0 : nt;  // tokens of this workgroup
+
+  const int lanes = 1 << a.lanes_log2;
+  const int u = tid & (lanes - 1), group = tid >> a.lanes_log2, step = threads >> a.lanes_log2;
+  const bool in_head = u * 2 * V < a.D;
+  // the lane's two runs, and whether they turn
+  int c0 = V * u, c1 = a.D / 2 + V * u;
+  bool turn0, turn1;
+  if (INTER) {
+    turn0 = c0 < 2 * np;
+    turn1 = c1 < 2 * np;
+  } else {
+    const int nu = np / V;
+    turn0 = turn1 = u < nu;
+    if (turn0) c1 = np + V * u;
+    else c0 = 2 * np + V * (u - nu), c1 = np + a.D / 2 + V * (u - nu);
   }
-  if (NORM)  // weights shared by the heads; others are read where they are used
-    for (int i = tid; i < 2 * a.D; i += 256) {
+  const int rows = left * nh;
+
+  // entry i of the list: token, tensor (0 queries, 1 keys, 2 values), head
+  struct Entry {
+    int tl, part, h;
+  };
+  auto entry = [&](int i) __attribute__((always_inline)) -> Entry {
+    const int tl = divide(i, a.by_heads), h = i - tl * nh;
+    return {tl, h < a.Hq ? 0 : (h < nn ? 1 : 2), h - (h < a.Hq ? 0 : (h < nn ? a.Hq : nn))};
+  };
+  auto source = [&](const Entry& e) __attribute__((always_inline)) -> const T* {
+    const int token = token0 + e.tl, b = divide(token, a.by_L);
+    const int64_t* const s = e.part == 0 ? a.qs : (e.part == 1 ? a.ks : a.vs);
+    return static_cast<const T*>(e.part == 0 ? a.q : (e.part == 1 ? a.k : a.v)) + b * s[0] +
+           (token - b * static_cast<int>(a.L)) * s[1] + e.h * s[2];
+  };
+  vec x[U], y[U];
+  auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + group + k * step;
+      if (in_head && i < rows) {
+        const T* const p = source(entry(i));
+        x[k] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p + c0));
+        y[k] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p + c1));
+      }
+    }
+  };
+  load(0);
+
+  for (int i = tid; i < left * np; i += threads) {
+    const int tl = divide(i, a.by_pairs), token = token0 + tl, b = divide(token, a.by_L);
+    const float2 cs = turn_of(a, b, token - b * static_cast<int>(a.L), i - tl * np);
+    s_cos[i] = cs.x;
+    s_sin[i] = cs.y;
+  }
+  if (NORM && (a.qw_h == 0 || a.kw_h == 0))  // shared by the heads (others: where used)
+    for (int i = tid; i < 2 * a.D; i += threads) {
       const void* w = i < a.D ? a.qw : a.kw;
       s_w[i] = w == nullptr ? 1.0f : weight_at(w, a.w_dtype, i < a.D ? i : i - a.D);
     }
-  if (tid < nt) {
-    const int64_t token = token0 + tid;
-    TokenRows r{0, 0, -1, -1, -1, false};
-    if (token < total) r = token_rows(a, token);
-    s_src[0][tid] = r.b * a.qs[0] + r.t * a.qs[1];
-    s_src[1][tid] = r.b * a.ks[0] + r.t * a.ks[1];
-    s_src[2][tid] = r.b * a.vs[0] + r.t * a.vs[1];
+  if (tid < left) {
+    const TokenRows r = token_rows(a, token0 + tid);
     s_dst[0][tid] = r.live ? r.q : -1;
     s_dst[1][tid] = r.live ? r.k : -1;
     s_dst[2][tid] = r.live ? r.v : -1;
   }
   __syncthreads();
 
-  const int lanes = 1 << a.lanes_log2;
-  const int u = tid & (lanes - 1);
-  const bool in_head = u * 16 < a.D;
-  const bool turns = in_head && u * 16 < 2 * np;
-  const int c0 = turns && !INTER ? 8 * u : 16 * u;       // the lane's two runs of 8 channels
-  const int c1 = turns && !INTER ? np + 8 * u : 16 * u + 8;
-  const int rows = nt * nh, step = 256 >> a.lanes_log2;
-
-  // (token, head) of list entry i; the source row and which tensor it is
-  auto entry = [&](int i, int& tl, int& h, int& part) __attribute__((always_inline)) {
-    tl = i / nh;
-    h = i - tl * nh;
-    part = h < a.Hq ? 0 : h < a.Hq + a.Hk ? 1 : 2;
-    h -= part == 0 ? 0 : part == 1 ? a.Hq : a.Hq + a.Hk;
-  };
-  auto load = [&](int tl, int h, int part, float (&x)[8], float (&y)[8])
-      __attribute__((always_inline)) {
-    const T* const p = static_cast<const T*>(part == 0 ? a.q : part == 1 ? a.k : a.v) +
-                       s_src[part][tl] +
-                       h * (part == 0 ? a.qs[2] : part == 1 ? a.ks[2] : a.vs[2]);
-    load8(p + c0, x);
-    load8(p + c1, y);
-  };
-  auto square_sum = [&](const float (&x)[8], const float (&y)[8])
-      __attribute__((always_inline)) -> float {
+  auto square_sum = [&](const vec& p, const vec& q, bool ok) __attribute__((always_inline)) -> float {
     float s = 0.0f;
+    if (ok) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s = fmaf(x[j], x[j], fmaf(y[j], y[j], s));
+      for (int j = 0; j < V; ++j) {
+        const float f = static_cast<float>(p[j]), g = static_cast<float>(q[j]);
+        s = fmaf(f, f, fmaf(g, g, s));
+      }
+    }
     for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
     return s;
   };
-
+  const bool held = rows <= U * step;  // the whole list is in registers
   if (NORM == 2) {  // the sums of every (token, head), then of every token in a fixed order
-    for (int i = tid >> a.lanes_log2; i < rows; i += step) {
-      int tl, h, part;
-      entry(i, tl, h, part);
-      float x[8] = {}, y[8] = {};
-      const int64_t dst = part < 2 ? s_dst[part][tl] : -1;
-      if (in_head && dst >= 0) load(tl, h, part, x, y);
-      const float s = square_sum(x, y);
-      if (u == 0 && part < 2) s_sum[tl * (a.Hq + a.Hk) + (part == 0 ? h : a.Hq + h)] = s;
+    for (int i0 = 0; i0 < rows; i0 += U * step) {
+      if (i0 != 0) load(i0);
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int i = i0 + group + k * step;
+        const float s = square_sum(x[k], y[k], in_head && i < rows);
+        const Entry e = entry(i);
+        if (u == 0 && i < rows && e.part < 2) s_sum[e.tl * nn + (e.part ? a.Hq : 0) + e.h] = s;
+      }
     }
     __syncthreads();
-    float s = 0.0f;
-    if (tid < 2 * nt) {
-      const float* const p = s_sum + (tid >> 1) * (a.Hq + a.Hk) + (tid & 1 ? a.Hq : 0);
-      const int n = tid & 1 ? a.Hk : a.Hq;
-      for (int h = 0; h < n; ++h) s += p[h];
+    for (int j = tid >> 4; j < 2 * left; j += threads >> 4) {  // 16 lanes a token and tensor
+      const float* const p = s_sum + (j >> 1) * nn + (j & 1 ? a.Hq : 0);
+      const int n = j & 1 ? a.Hk : a.Hq;
+      float s = 0.0f;
+      for (int h = tid & 15; h < n; h += 16) s += p[h];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, kWave);
+      if ((tid & 15) == 0) s_all[j] = s;
     }
-    __syncthreads();
-    if (tid < 2 * nt) s_sum[tid] = s;
     __syncthreads();
   }
 
-  for (int i = tid >> a.lanes_log2; i < rows; i += step) {
-    int tl, h, part;
-    entry(i, tl, h, part);
-    const int64_t dst = s_dst[part][tl];
-    const bool ok = in_head && dst >= 0;
-    float x[8] = {}, y[8] = {};
-    if (ok) load(tl, h, part, x, y);
-    if (NORM && part < 2) {  // (a row's lanes agree on part)
-      float s, n = static_cast<float>(a.D);
-      if (NORM == 2) {
-        s = s_sum[2 * tl + part];
-        n *= static_cast<float>(part == 0 ? a.Hq : a.Hk);
-      } else {
-        s = square_sum(x, y);
-      }
-      const float r = 1.0f / sqrtf(s / n + a.eps);
-      if (in_head) {
-        float w0[8], w1[8];
-        const int64_t ws = part == 0 ? a.qw_h : a.kw_h;
-        if (ws == 0) {
+  for (int i0 = 0; i0 < rows; i0 += U * step) {
+    if (i0 != 0 || (NORM == 2 && !held)) load(i0);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            w0[j] = s_w[part * a.D + c0 + j];
-            w1[j] = s_w[part * a.D + c1 + j];
-          }
+    for (int k = 0; k < U; ++k) {
+      const int i = i0 + group + k * step;
+      if (i >= rows) break;  // (a head's lanes agree)
+      const Entry e = entry(i);
+      const int64_t dst = s_dst[e.part][e.tl];
+      T* const o = static_cast<T*>(e.part == 0 ? a.qout : (e.part == 1 ? a.kout : a.vout)) + dst +
+                   e.h * (e.part == 0 ? a.qo[2] : (e.part == 1 ? a.ko[2] : a.vo[2]));
+      if (e.part == 2) {  // values as they are
+        if (in_head && dst >= 0) {
+          __builtin_nontemporal_store(x[k], reinterpret_cast<vec*>(o + c0));
+          __builtin_nontemporal_store(y[k], reinterpret_cast<vec*>(o + c1));
+        }
+        continue;
+      }
+      float p[V], q[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        p[j] = static_cast<float>(x[k][j]);
+        q[j] = static_cast<float>(y[k][j]);
+      }
+      if (NORM) {
+        float s, n = static_cast<float>(a.D);
+        if (NORM == 2) {
+          s = s_all[2 * e.tl + e.part];
+          n *= static_cast<float>(e.part ? a.Hk : a.Hq);
         } else {
-          const void* const w = part == 0 ? a.qw : a.kw;
-          weight8(w, a.w_dtype, h * ws + c0, w0);
-          weight8(w, a.w_dtype, h * ws + c1, w1);
+          s = square_sum(x[k], y[k], in_head);
         }
+        const float r = 1.0f / sqrtf(s / n + a.eps);
+        const int64_t ws = e.part ? a.kw_h : a.qw_h;
+        if (in_head) {
+          if (ws == 0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] *= r * w0[j];
-          y[j] *= r * w1[j];
+            for (int j = 0; j < V; ++j) {
+              p[j] *= r * s_w[e.part * a.D + c0 + j];
+              q[j] *= r * s_w[e.part * a.D + c1 + j];
+            }
+          } else {
+            const void* const w = e.part ? a.kw : a.qw;
+            float w0[V], w1[V];
+            weight_run<V>(w, a.w_dtype, e.h * ws + c0, w0);
+            weight_run<V>(w, a.w_dtype, e.h * ws + c1, w1);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+              p[j] *= r * w0[j];
+              q[j] *= r * w1[j];
+            }
+          }
         }
       }
+      if (!in_head || dst < 0) continue;
+      if (INTER) {  // pairs (0, 1), (2, 3) ... of either run
+        auto turn = [&](float (&f)[V], int c) __attribute__((always_inline)) {
+          const float* const cs = s_cos + e.tl * np + c / 2;
+          const float* const sn = s_sin + e.tl * np + c / 2;
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            const float f0 = f[2 * j], f1 = f[2 * j + 1];
+            f[2 * j] = f0 * cs[j] - f1 * sn[j];
+            f[2 * j + 1] = f0 * sn[j] + f1 * cs[j];
+          }
+        };
+        if (turn0) turn(p, c0);
+        if (turn1) turn(q, c1);
+      } else if (turn0) {
+        const float* const cs = s_cos + e.tl * np + V * u;
+        const float* const sn = s_sin + e.tl * np + V * u;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float f0 = p[j], f1 = q[j];
+          p[j] = f0 * cs[j] - f1 * sn[j];
+          q[j] = f0 * sn[j] + f1 * cs[j];
+        }
+      }
+      vec o0, o1;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        o0[j] = static_cast<T>(p[j]);
+        o1[j] = static_cast<T>(q[j]);
+      }
+      __builtin_nontemporal_store(o0, reinterpret_cast<vec*>(o + c0));
+      __builtin_nontemporal_store(o1, reinterpret_cast<vec*>(o + c1));
     }
-    if (!ok) continue;
-    if (turns && part < 2) {
-      const float* const cs = s_cos + tl * np + 8 * u;
-      const float* const sn = s_sin + tl * np + 8 * u;
-      float c[8], s[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        c[j] = cs[j];
-        s[j] = sn[j];
-      }
-      if (INTER) {  // pairs (0, 1), (2, 3) ... of the 16 channels
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float p = x[2 * j], q = x[2 * j + 1], m = y[2 * j], n = y[2 * j + 1];
-          x[2 * j] = p * c[j] - q * s[j];
-          x[2 * j + 1] = p * s[j] + q * c[j];
-          y[2 * j] = m * c[4 + j] - n * s[4 + j];
-          y[2 * j + 1] = m * s[4 + j] + n * c[4 + j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float p = x[j], q = y[j];
-          x[j] = p * c[j] - q * s[j];
-          y[j] = p * s[j] + q * c[j];
-        }
-      }
-    }
-    T* const o = static_cast<T*>(part == 0 ? a.qout : part == 1 ? a.kout : a.vout) + dst +
-                 h * (part == 0 ? a.qo[2] : part == 1 ? a.ko[2] : a.vo[2]);
-    store8(o + c0, x);
-    store8(o + c1, y);
   }
 }
 
@@ -332,42 +374,64 @@ __global__ void __launch_bounds__(64) rotary_any_kernel(RotaryArgs a) {
   }
 }
 
-template <typename T, bool INTER, int NORM>
-static int launch(RotaryArgs& a, hipStream_t s) {
-  const int64_t total = a.B * a.L;
-  const int nh = a.Hq + a.Hk + a.Hv;
-  const int64_t vec = 16 / static_cast<int64_t>(sizeof(T));
-  bool wide = a.D % 16 == 0 && a.D <= 256 && a.n_pairs % 8 == 0;
+// Whether rows, strides and pointers suit runs of V channels.
+template <typename T>
+static bool runs_of(const RotaryArgs& a, int V, bool inter) {
+  if (a.D % (2 * V) || a.D > 128 * V || (inter ? 2 * a.n_pairs : a.n_pairs) % V) return false;
   for (int i = 0; i < 3; ++i)
-    wide = wide && a.qs[i] % vec == 0 && a.ks[i] % vec == 0 && a.vs[i] % vec == 0 &&
-           a.qo[i] % vec == 0 && a.ko[i] % vec == 0 && a.vo[i] % vec == 0;
+    for (const int64_t* s : {a.qs, a.ks, a.vs, a.qo, a.ko, a.vo})
+      if (s[i] % V) return false;
   for (const void* p : {a.q, a.k, a.v, static_cast<const void*>(a.qout),
                         static_cast<const void*>(a.kout), static_cast<const void*>(a.vout)})
-    wide = wide && aligned16(p);
-  if (NORM) wide = wide && aligned16(a.qw) && aligned16(a.kw);
-  if (!wide) {
-    if (total >= (1ll << 31)) return RCSA_ERR_SHAPE;
-    rotary_any_kernel<T, INTER, NORM>
-        <<<dim3(static_cast<unsigned>(total), a.Hv ? 3 : a.Hk ? 2 : 1), dim3(kWave), 0, s>>>(a);
-    return launch_status();
-  }
-  a.lanes_log2 = a.D <= 16 ? 0 : a.D <= 32 ? 1 : a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4;
-  // Tokens of a workgroup: about 8 rounds of its 256 lanes, fewer where that would
-  // leave compute units without a workgroup.
-  const int64_t lanes = static_cast<int64_t>(nh) << a.lanes_log2;
-  int64_t nt = (2048 + lanes - 1) / lanes;
-  nt = nt > kMaxTokens ? kMaxTokens : nt;
-  while (nt > 1 && total / nt < 1024) nt /= 2;
+    if (reinterpret_cast<uintptr_t>(p) % (V * sizeof(T) < 16 ? V * sizeof(T) : 16)) return false;
+  const size_t w = V * (a.w_dtype == RCSA_F32 ? 4 : 2);
+  for (const void* p : {a.qw, a.kw})
+    if (reinterpret_cast<uintptr_t>(p) % (w < 16 ? w : 16)) return false;
+  return true;
+}
+
+template <typename T, int V, bool INTER, int NORM>
+static int launch_runs(RotaryArgs& a, hipStream_t s) {
+  const int64_t total = a.B * a.L;
+  const int nh = a.Hq + a.Hk + a.Hv;
+  a.lanes_log2 = 0;
+  while ((2 * V) << a.lanes_log2 < a.D) ++a.lanes_log2;
+  // Tokens of a workgroup: as many as its lanes hold at once, fewer where that would
+  // leave compute units without a workgroup; lanes: whole wavefronts that share the list
+  // evenly.
+  constexpr int U = kEntries<V, NORM>;
+  const int64_t per = static_cast<int64_t>(nh) << a.lanes_log2;
+  int64_t nt = U * 256 / per;
+  nt = nt < 1 ? 1 : (nt > kMaxTokens ? kMaxTokens : nt);
+  while (nt > 1 && total / nt < 512) nt /= 2;
   auto bytes = [&]() -> int64_t {
-    return 4 * (2 * nt * a.n_pairs + (NORM ? 2 * a.D + nt * (a.Hq + a.Hk) + 2 : 0));
+    return 4 * (2 * nt * a.n_pairs + (NORM ? 2 * a.D + nt * (a.Hq + a.Hk + 2) : 0));
   };
   while (nt > 1 && bytes() > (32 << 10)) nt /= 2;
   if (bytes() > (60 << 10)) return RCSA_ERR_SHAPE;
   a.tokens = static_cast<int>(nt);
+  a.by_heads = divisor(static_cast<uint32_t>(nh));
+  a.by_L = divisor(static_cast<uint32_t>(a.L));
+  a.by_pairs = divisor(a.n_pairs > 0 ? static_cast<uint32_t>(a.n_pairs) : 1u);
   const int64_t grid = (total + nt - 1) / nt;
-  if (grid >= (1ll << 31) || nt * nh >= (1 << 30)) return RCSA_ERR_SHAPE;
-  rotary_kernel<T, INTER, NORM><<<dim3(static_cast<unsigned>(grid)), dim3(256),
-                                  static_cast<unsigned>(bytes()), s>>>(a);
+  const int64_t rounds = (nt * per + 255) / 256;
+  const int64_t threads = ((nt * per + rounds - 1) / rounds + kWave - 1) / kWave * kWave;
+  rotary_kernel<T, V, INTER, NORM><<<dim3(static_cast<unsigned>(grid)),
+                                     dim3(static_cast<unsigned>(threads)),
+                                     static_cast<unsigned>(bytes()), s>>>(a);
+  return launch_status();
+}
+
+// Runs of 16 bytes where sizes, strides and pointers allow, of 2 channels where they allow
+// that, else element by element.
+template <typename T, bool INTER, int NORM>
+static int launch(RotaryArgs& a, hipStream_t s) {
+  if (a.B * a.L >= (1ll << 30)) return RCSA_ERR_SHAPE;
+  constexpr int W = kWide<T>;
+  if (runs_of<T>(a, W, INTER)) return launch_runs<T, W, INTER, NORM>(a, s);
+  if (runs_of<T>(a, 2, INTER)) return launch_runs<T, 2, INTER, NORM>(a, s);
+  rotary_any_kernel<T, INTER, NORM>
+      <<<dim3(static_cast<unsigned>(a.B * a.L), a.Hv ? 3 : a.Hk ? 2 : 1), dim3(kWave), 0, s>>>(a);
   return launch_status();
 }
 

@@ -20,25 +20,6 @@ typedef _Float16 v4hf __attribute__((ext_vector_type(4)));
 
 constexpr int kTileKeys = 32;
 
-__device__ __forceinline__ int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// Division of n < 2^31 by an invariant: a high product and two shifts.
-struct Divisor {
-  uint32_t d, mul;
-  int sh1, sh2;
-};
-inline Divisor divisor(uint32_t d) {
-  int l = 0;
-  while ((1ull << l) < d) ++l;
-  return {d, static_cast<uint32_t>((1ull << 32) * ((1ull << l) - d) / d + 1), l < 1 ? l : 1,
-          l < 1 ? 0 : l - 1};
-}
-template <typename V>
-__device__ __forceinline__ int divide(int n, V& v) {
-  const uint32_t u = static_cast<uint32_t>(n), t = __umulhi(v.mul, u);
-  return static_cast<int>((t + ((u - t) >> v.sh1)) >> v.sh2);
-}
-
 struct WindowArgs {
   const void *q, *k, *v;
   void* out;

@@ -696,22 +696,24 @@ int rcsa_int8_linear_group(const int8_t* x, const float* x_scale, int64_t n_line
  * channels from 2 n_pairs on pass through.  positions: int32, or int64 when
  * positions_i64, addressed with pos_strides (host array: batch, token, axis); turns fp64
  * [n_pairs]; axis int32 [n_pairs] in [0, n_axes), NULL: all 0.  The product is taken and
- * reduced in 64 bits, so far positions lose nothing.  D <= 512, H <= 4096.  Rows of
- * 16-byte aligned tensors with D a multiple of 16 (up to 256) and n_pairs of 8 move as
- * vectors; any other shape runs element by element.
+ * reduced in 64 bits, so far positions lose nothing.  D <= 512, H <= 4096, B * L <
+ * 2^30.  Rows move in runs of V
+ * channels, V = 16 bytes of the type, where D is a multiple of 2 V (up to 128 V), n_pairs
+ * (interleaved: 2 n_pairs) and all strides of V, and pointers of 16 bytes; in runs of 2
+ * where all that holds for V = 2 (pointers of two elements); else element by element.
  *
  * rcsa_norm_rope: q [B][L][Hq][D] and k [B][L][Hk][D], dims = {B, L, Hq, Hk, D},
  *   y = x * rsqrt(mean(x^2) + eps) * weight, then the rotation of rcsa_rope,
  * with the mean over a head or (across_heads) over all heads of the token; weights (NULL:
- * 1) of type weight_dtype, one [D] for all heads (stride 0) or [H][D] (stride D), 16-byte
- * aligned for the vector form.  strides: host array of 18, batch/token/head of q, k, v,
+ * 1) of type weight_dtype, one [D] for all heads (stride 0) or [H][D] (stride D).
+ * strides: host array of 18, batch/token/head of q, k, v,
  * q_out, k_out, v_out.  Without block_table k_out is [B][L][Hk][D] and v, v_out are NULL.
  * With it k_out and v_out are the pages of a cache (their strides: page, slot, head), v
  * [B][L][Hk][D] is copied beside the keys, and token t of request b goes to index
  * at = starts[b] + t (starts NULL: t), row at % page_size of page
  * block_table[b * table_stride + at / page_size]; a row whose page is not in
  * [0, n_pages), or past max_pages, is dropped.  No row may appear twice.  lengths
- * (nullable, int32 [B]): tokens t >= lengths[b] are neither read nor written.
+ * (nullable, int32 [B]): rows of tokens t >= lengths[b] are left as they were.
  */
 int rcsa_rope(const void* x, void* out, int dtype, int64_t batch, int64_t len, int64_t heads,
               int64_t head_dim, const int64_t* strides, const void* positions, int positions_i64,
