@@ -1025,7 +1025,7 @@ std::vector<at::Tensor> norm_rope(
 }
 
 // Dense (k, v [B, Lk, Hk, D]) or, with a table, paged (k, v [pages, slots, Hk, D])
-// attention over a window and the first keys; n_split -1: planned.  (out) or (out, lse).
+// attention over a window and the first keys; n_split -2: planned.  (out) or (out, lse).
 std::vector<at::Tensor> window_attention(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const c10::optional<at::Tensor>& table, const c10::optional<at::Tensor>& q_lengths,
@@ -1076,7 +1076,7 @@ std::vector<at::Tensor> window_attention(
   put_strides(v, s + 6);
   put_strides(out, s + 9);
   int64_t ns = n_split;
-  if (ns < 0) {
+  if (ns < -1) {
     int64_t most = max_keys >= 0 ? std::min(max_keys, Lk) : Lk;
     if (window > 0) most = std::min(most, window + sinks + Lq);
     check_status(a, op, a.window_attn_plan(dims, most, &ns));

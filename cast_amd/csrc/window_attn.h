@@ -45,12 +45,13 @@ struct WindowArgs {
   // round-robin.
   int xcd_items, xcd_whole;
   int descending;
-  int units;  // few rows: wavefronts of one round, 0: one unit a key head
+  int units;       // few rows in units: wavefronts of one round
   float per_unit;  // 1 / units
 };
 
 constexpr int kFewRows = 32;        // rows of a key head that one wavefront takes
 constexpr int kMaxPlanned = 512;    // requests whose lengths every wavefront reads
+constexpr int kGroupWaves = 8;      // wavefronts of a workgroup that takes a key head
 
 // The keys of a position: [0, sink) and [lo, hi).
 struct KeyRange {
@@ -113,7 +114,7 @@ __device__ __forceinline__ ItemAt item_at(const WindowArgs& a, int xcd, int in_x
   return {bh, i - bh * a.n_rblocks};
 }
 
-// Few rows: the visible tiles of all requests are dealt to units of one wavefront each,
+// Few rows, many keys: the visible tiles of all requests are dealt to units of one wavefront each,
 // `chunk` tiles of one key head at most, however uneven the lengths.  A wavefront reads
 // the lengths, one lane a request, and finds its unit among them; unit index = (units
 // of the requests before) * Hk + share * Hk + hk.
@@ -161,11 +162,6 @@ __device__ __forceinline__ int lane_prefix(int x, int lane) {  // inclusive
 // lane of the wavefront calls it; the result is uniform.
 template <bool OF_REQUEST>
 __device__ __forceinline__ Unit find_unit(const WindowArgs& a, int w, int lane) {
-  if (a.units == 0) {  // a unit for every request
-    if (w >= a.B) return {-1, 0, 0, 0, {0, 0}};
-    const Request r = request_of(a, w);
-    return {w, 0, 1, w, {uniform_int(r.k_len), uniform_int(r.q_len)}};
-  }
   if (a.B <= kWave) {  // one load of the lengths (a single request needs no lanes' sums)
     Request r{0, 0};
     if (lane < a.B) r = request_of(a, lane);
@@ -238,12 +234,11 @@ struct Half<_Float16> {
 
 // Where a wavefront's 32 rows stand: rows row0 .. of key head hk of request b, of n_rows;
 // position of query 0; the tiles [begin, begin + steps) of the rows' tiles are its
-// share's, one of `shares`, which writes rows ws_row .. of the workspace.
+// share's, one of `shares`.
 struct Place {
   int b, hk, row0, n_rows, shift, k_len;
   int shares, begin, steps;
   Tiles tiles;
-  int64_t ws_row;
 };
 // First key of step s, -1 past the last.
 __device__ __forceinline__ int key_of(const Place& p, int s) {
@@ -486,10 +481,11 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowArgs& a, const Place& 
   return (there >> hf) & 1 ? bits : 0u;
 }
 
-// The end of a wavefront's rows: normalise, write the rows (or the share's partial ones and
-// their (max, sum)) and the LSE.
+// The end of a wavefront's rows: normalise, write the rows and the LSE, or with more than one
+// share the share's partial rows to part_o [32][D] and their (max, sum) to part_ml [32].
 template <typename T, int D, bool PAGED>
-__device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, int lane) {
+__device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, int lane,
+                                            float* part_o, float2* part_ml) {
   // (the arguments are read again: kept in scalar registers they would spill the loop's)
   typedef const __attribute__((address_space(4))) WindowArgs Late;
   Late* late = (Late*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -508,10 +504,9 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, in
       bad = bad || !(fabsf(t.o_acc[dt][r]) < INFINITY);
     }
   const Row my = row_of(a, p, p.row0 + lr);
-  const int64_t wrow = p.ws_row + lr;
   if (my.live) {
     if (p.shares > 1) {
-      float* const wp = a.ws_o + wrow * D + 4 * hf;
+      float* const wp = part_o + lr * D + 4 * hf;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -520,7 +515,7 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, in
               v4f{t.o_acc[dt][4 * g], t.o_acc[dt][4 * g + 1], t.o_acc[dt][4 * g + 2],
                   t.o_acc[dt][4 * g + 3]};
       if (hf == 0)
-        a.ws_ml[wrow] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
+        part_ml[lr] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
     } else {
       T* const op = static_cast<T*>(a.out) + p.b * a.so[0] +
                     static_cast<int64_t>(my.qi) * a.so[1] + my.head * a.so[2] + 4 * hf;
@@ -543,7 +538,7 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, in
   uint64_t again = __ballot(bad && my.live && l > 0.0f && l < INFINITY);
   again |= again >> 32;
   if (static_cast<uint32_t>(again) == 0) return;
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // (the stores above come first)
+  __builtin_amdgcn_s_waitcnt(0);  // (the stores above come first)
   const char* const kbase = static_cast<const char*>(a.k) +
                             ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
   const char* const vbase = static_cast<const char*>(a.v) +
@@ -589,13 +584,14 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, in
                    r.head * a.so[2];
 #pragma unroll
     for (int c = 0; c < N; ++c) {
-      if (p.shares > 1) a.ws_o[(p.ws_row + i) * D + lane + 64 * c] = acc[c] * rinv;
+      if (p.shares > 1) part_o[i * D + lane + 64 * c] = acc[c] * rinv;
       else dst[lane + 64 * c] = static_cast<T>(acc[c] * rinv);
     }
   }
 }
 
-// Units of few rows and their join (window_units.hip); type 0: bf16, 1: fp16.
+// Few rows (window_units.hip): in units and their join, or one workgroup a key head
+// (a.units 0); type 0: bf16, 1: fp16.
 int launch_window_units(WindowArgs& a, int type, int64_t D, hipStream_t s);
 
 }  // namespace rcsa

@@ -54,7 +54,8 @@ window_kernel(WindowArgs a) {
   p.row0 = item_row0 + wave * 32;
   p.shift = p.k_len - q_len;
   const int64_t per_tail = a.xcd_items - a.xcd_whole;
-  p.ws_row = (share * per_tail * kNumXcd + xcd * per_tail + in_xcd - a.xcd_whole) * BM + wave * 32;
+  const int64_t ws_row =
+      (share * per_tail * kNumXcd + xcd * per_tail + in_xcd - a.xcd_whole) * BM + wave * 32;
 
   // uniform ranges: of the item, and of this wavefront's first and last rows
   const KeyRange w_first = row_range(a, p, p.row0), w_last = row_range(a, p, p.row0 + 31);
@@ -146,7 +147,7 @@ window_kernel(WindowArgs a) {
     iteration(std::integral_constant<int, 2>{}, j + 2);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
-  finish_rows<T, D, PAGED>(p, t, lane);
+  finish_rows<T, D, PAGED>(p, t, lane, a.ws_o + ws_row * D, a.ws_ml + ws_row);
 }
 
 // The shares of the split row blocks joined: w_s = l_s 2^(m_s - M),
@@ -214,11 +215,20 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
 static int64_t row_blocks(int64_t Lq, int64_t G) { return (Lq * G + 127) / 128; }
 
 static bool few_rows(const int64_t* d) { return d[1] * (d[3] / d[4]) <= kFewRows; }
-// Wavefronts of few rows that fit at once: two (D 64: three) to a SIMD.  Every one reads all
-// lengths to find its unit, so past kMaxPlanned requests each key head is one unit.
-static int64_t units_of_round(const int64_t* d) {
-  return d[0] > kMaxPlanned ? 0 : (d[5] == 128 ? 8 : 12) * 256;
+// Wavefronts of few rows in units that fit at once: two (D 64: three) to a SIMD.
+static int64_t units_of_round(const int64_t* d) { return (d[5] == 128 ? 8 : 12) * 256; }
+
+// A workgroup a key head takes about 6.5 us and 0.25 a tile (the loads' latency, eight
+// wavefronts) where the bandwidth does not bind; units take 11 us, their join among them, and
+// their bytes at 5 TB/s (3.3 ns a tile of D 128).  Measured, us, workgroup and units:
+// 8 heads x 256 keys 8.4, 11.1; 8 x 1024 13.1, 11.4; 32 x 1024 14.2, 14.7; 128 x 1024
+// 18.9, 23.1; 64 x 4096 41.1, 32.6; 512 x 2048 100, 117; 2048 x 1024 205, 259.  Past 256
+// tiles a single long request among short ones would hold its workgroup too long.
+static bool one_group(const int64_t* d, int64_t tiles) {
+  const int64_t heads = d[0] * d[4];
+  return tiles <= 256 && (2500 - 33 * heads * d[5] / 128) * tiles < 45000;
 }
+
 static bool window_dims(const int64_t* d) {
   for (int i = 0; i < 6; ++i)
     if (d[i] <= 0 && !(i == 2 && d[i] == 0)) return false;
@@ -243,21 +253,23 @@ static int64_t xcd_whole_of(int64_t items, int64_t n_split) {
 
 using namespace rcsa;
 
-// Few rows of a key head go to units of one wavefront (n_split 0), more to blocks of 128
-// rows.  Of these the ones past an XCD's whole rounds (one block to a compute unit; three
-// share it in time) leave compute units idle: their keys go to n_split workgroups, which
-// makes that round ceil(tail n / U) (keys / n + kFixed) tiles long.
+// Few rows of a key head go to one workgroup (n_split -1) or to units of one wavefront (0),
+// more to blocks of 128 rows.  Of these the ones past an XCD's whole rounds (one block to a
+// compute unit; three share it in time) leave compute units idle: their keys go to n_split
+// workgroups, which makes that round ceil(tail n / U) (keys / n + kFixed) tiles long.
 extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
-  *n_split = 0;
-  if (few_rows(dims)) return RCSA_OK;
+  const int64_t tiles = (max_keys + kTileKeys - 1) / kTileKeys;
+  if (few_rows(dims)) {
+    *n_split = dims[0] > kMaxPlanned || one_group(dims, tiles) ? -1 : 0;
+    return RCSA_OK;
+  }
   *n_split = 1;
   const int64_t cux = xcd_cus(), items = xcd_items_of(dims);
   const int64_t tail = items % cux;
   if (tail == 0) return RCSA_OK;
   constexpr int64_t kFixed = 16;
-  const int64_t tiles = (max_keys + kTileKeys - 1) / kTileKeys;
   int64_t best = tiles + kFixed;
   for (int64_t n = 2; n <= 16 && n * 4 <= tiles; ++n) {
     const int64_t cost = (tail * n + cux - 1) / cux * ((tiles + n - 1) / n + kFixed) +
@@ -271,12 +283,12 @@ extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int6
 }
 
 extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
-  if (!dims || !window_dims(dims) || n_split < 0 || n_split > 64) return -1;
+  if (!dims || !window_dims(dims) || n_split < -1 || n_split > 64) return -1;
   const int64_t G = dims[3] / dims[4], row = dims[5] * 4 + 8;
-  if (n_split == 0) {
-    if (!few_rows(dims)) return -1;
-    const int64_t units = units_of_round(dims);
-    return units == 0 ? 0 : (4 * units + dims[0] * dims[4]) * dims[1] * G * row;
+  if (n_split < 1) {
+    if (!few_rows(dims) || (n_split == 0 && dims[0] > kMaxPlanned)) return -1;
+    return n_split < 0 ? 0
+                       : (4 * units_of_round(dims) + dims[0] * dims[4]) * dims[1] * G * row;
   }
   const int64_t items = xcd_items_of(dims);
   return n_split == 1 ? 0 : n_split * (items - xcd_whole_of(items, n_split)) * kNumXcd * 128 * row;
@@ -299,7 +311,6 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   if (block_table && (max_pages <= 0 || n_pages <= 0 || page_size <= 0 || page_size % 16 ||
                       n_pages >= most || page_size >= most || max_pages >= most / page_size))
     return RCSA_ERR_SHAPE;
-  if (n_split < 0 || n_split > 64 || (n_split == 0 && !few_rows(dims))) return RCSA_ERR_SHAPE;
   for (int i = 0; i < 12; ++i)
     if (strides[i] < 0 || strides[i] % (i < 9 ? 8 : 4)) return RCSA_ERR_STRIDE;
   if (block_table && (strides[3] >= (1ll << 31) || strides[6] >= (1ll << 31)))
@@ -312,7 +323,7 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
       (reinterpret_cast<uintptr_t>(out) & 7u))
     return RCSA_ERR_ALIGN;
   const int64_t need = rcsa_window_attn_workspace_bytes(dims, n_split);
-  if (need > 0 && (!workspace || workspace_bytes < need)) return RCSA_ERR_SHAPE;
+  if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need))) return RCSA_ERR_SHAPE;
   WindowArgs a{};
   a.q = q;
   a.k = k;
@@ -364,7 +375,7 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   const int64_t ws_rows = need / (dims[5] * 4 + 8);
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = need ? reinterpret_cast<float2*>(a.ws_o + ws_rows * dims[5]) : nullptr;
-  if (n_split == 0) return launch_window_units(a, dtype == RCSA_BF16 ? 0 : 1, dims[5], stream);
+  if (n_split < 1) return launch_window_units(a, dtype == RCSA_BF16 ? 0 : 1, dims[5], stream);
   if (dtype == RCSA_BF16)
     return dims[5] == 128 ? launch_window<__bf16, 128>(a, stream)
                           : launch_window<__bf16, 64>(a, stream);

@@ -1,5 +1,7 @@
 // Windowed attention of few rows (one new token of each request, or a few): at most 32
-// rows of a key head, one wavefront a unit of the visible tiles of all requests.
+// rows of a key head.  Few keys: one workgroup of eight wavefronts a key head, which
+// joins their shares in LDS.  Many: one wavefront a unit of the visible tiles of all
+// requests, joined by a second launch.
 //
 // The keys and values are read once and bound the time, so what counts is bytes in
 // flight: a wavefront holds the next tile (16 KB at D 128) in registers while it works
@@ -10,19 +12,29 @@
 
 namespace rcsa {
 
-template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(64)
+template <typename T, int D, bool PAGED, bool GROUP>
+__global__ void __launch_bounds__(GROUP ? 64 * kGroupWaves : 64)
 __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 window_unit_kernel(WindowArgs a) {
   using R = RowTile<T, D>;
+  constexpr int NW = GROUP ? kGroupWaves : 1;
   constexpr int RPU = 1024 / R::KROW;          // rows of a 1 KiB load
   constexpr int UPH = 16 * R::KROW / 1024;     // loads of a half tile, K and V each
-  __shared__ __attribute__((aligned(1024))) char tile[2 * R::TILE];
-  const int lane = threadIdx.x, hf = lane >> 5, lr = lane & 31;
+  __shared__ __attribute__((aligned(1024))) char tiles[NW][2 * R::TILE];
+  __shared__ float2 s_ml[NW][kFewRows];
+  const int lane = threadIdx.x & 63, hf = lane >> 5, lr = lane & 31;
+  const int wave = GROUP ? uniform_int(static_cast<int>(threadIdx.x) >> 6) : 0;
+  char* const tile = tiles[wave];
 
   const int w = divide(static_cast<int>(blockIdx.x), a.by_Hk);
-  const Unit u = find_unit<false>(a, w, lane);
-  if (u.b < 0) return;
+  Unit u;
+  if constexpr (GROUP) {
+    const Request r = request_of(a, w);
+    u = {w, wave, kGroupWaves, 0, {uniform_int(r.k_len), uniform_int(r.q_len)}};
+  } else {
+    u = find_unit<false>(a, w, lane);
+    if (u.b < 0) return;
+  }
   Place p;
   p.b = u.b;
   p.hk = static_cast<int>(blockIdx.x) - w * a.Hk;
@@ -32,7 +44,6 @@ window_unit_kernel(WindowArgs a) {
   p.k_len = u.r.k_len;
   p.shift = u.r.k_len - u.r.q_len;
   p.shares = u.shares;
-  p.ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
   const KeyRange first = row_range(a, p, 0), last = row_range(a, p, p.n_rows - 1);
   p.tiles = tiles_of(a, first, last);
   share_of(p, u.share);
@@ -99,7 +110,44 @@ window_unit_kernel(WindowArgs a) {
       return seen_bits(a, p, lr, hf, now.key, there);
     }, [&]() __attribute__((always_inline)) { next = step_of<PAGED>(a, p, table, s + 2); });
   }
-  finish_rows<T, D, PAGED>(p, t, lane);
+  if constexpr (!GROUP) {
+    const int64_t ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
+    finish_rows<T, D, PAGED>(p, t, lane, a.ws_o + ws_row * D, a.ws_ml + ws_row);
+    return;
+  }
+  // the wavefronts' partial rows meet in LDS, each in its own tile's place
+  static_assert(kFewRows * D * 4 <= 2 * R::TILE, "partial rows fit a wavefront's tiles");
+  finish_rows<T, D, PAGED>(p, t, lane, reinterpret_cast<float*>(tile), s_ml[wave]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.n_rows * (D / 4); i += 64 * NW) {
+    const int row = i / (D / 4), c = i % (D / 4) * 4;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < NW; ++s) mx = fmaxf(mx, s_ml[s][row].x);
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NW; ++s) {
+      const float2 ml = s_ml[s][row];
+      if (ml.x == -INFINITY) continue;
+      const float f = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+      sum += f;
+      const v4f o = *reinterpret_cast<const v4f*>(tiles[s] + (row * D + c) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, o[e], acc[e]);
+    }
+    const Row r = row_of(a, p, row);
+    typename Half<T>::op4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      out[e] = static_cast<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+    *reinterpret_cast<typename Half<T>::op4*>(
+        static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(r.qi) * a.so[1] +
+        r.head * a.so[2] + c) = out;
+    if (a.lse && c == 0)
+      a.lse[(static_cast<int64_t>(p.b) * a.Hq + r.head) * a.Lq + r.qi] =
+          sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
+  }
 }
 
 // The units of every row joined: w_s = l_s 2^(m_s - M), out = sum w_s O_s / sum w_s.  A
@@ -162,14 +210,20 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
 
 template <typename T, int D>
 static int launch_units(WindowArgs& a, hipStream_t s) {
-  const int64_t n = 4ll * a.units + static_cast<int64_t>(a.B) * a.Hk;
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * a.Lq * a.G;
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hk;
+  if (a.units == 0) {
+    const dim3 grid(static_cast<unsigned>(heads)), block(64 * kGroupWaves);
+    if (a.table) window_unit_kernel<T, D, true, true><<<grid, block, 0, s>>>(a);
+    else window_unit_kernel<T, D, false, true><<<grid, block, 0, s>>>(a);
+    return launch_status();
+  }
+  const int64_t n = 4ll * a.units + heads;
+  const int64_t rows = heads * a.Lq * a.G;
   if (n >= (1ll << 31) || rows >= (1ll << 31)) return RCSA_ERR_SHAPE;
-  const dim3 grid(static_cast<unsigned>(n));
-  if (a.table) window_unit_kernel<T, D, true><<<grid, dim3(64), 0, s>>>(a);
-  else window_unit_kernel<T, D, false><<<grid, dim3(64), 0, s>>>(a);
-  if (a.units)
-    window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
+  const dim3 grid(static_cast<unsigned>(n)), block(64);
+  if (a.table) window_unit_kernel<T, D, true, false><<<grid, block, 0, s>>>(a);
+  else window_unit_kernel<T, D, false, false><<<grid, block, 0, s>>>(a);
+  window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
   return launch_status();
 }
 

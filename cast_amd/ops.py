@@ -1319,7 +1319,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
 def _shares(n_split: Optional[int], fn: str) -> int:
     if n_split is not None and n_split < 1:
         raise ValueError(f"{fn}: n_split must be positive, got {n_split}")
-    return -1 if n_split is None else int(n_split)
+    return -2 if n_split is None else int(n_split)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *,

@@ -753,12 +753,13 @@ int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, voi
  *
  * n_split 1 to 64: blocks of 128 rows of a key head (Hq / Hk heads x queries) to a
  * workgroup; the blocks past an XCD's whole rounds of its compute units have their keys
- * shared among n_split workgroups and joined by a second launch.  n_split 0, for at most 32
- * rows a key head (Lq Hq / Hk <= 32): the visible keys of all requests are dealt to
- * wavefronts in equal units, whatever the lengths, and joined (past 512 requests each key
- * head is one unit).  The workspace holds rcsa_window_attn_workspace_bytes (16-byte
- * aligned; of this call alone until it ends).  rcsa_window_attn_plan picks n_split;
- * max_keys bounds the keys that a row sees.
+ * shared among n_split workgroups and joined by a second launch.  For at most 32 rows a key
+ * head (Lq Hq / Hk <= 32), n_split -1: a key head to a workgroup, one launch; 0: the visible
+ * keys of all requests (at most 512) are dealt to wavefronts in equal units, whatever the
+ * lengths, and joined by a second launch.  The workspace holds
+ * rcsa_window_attn_workspace_bytes (-1: no such launch; 16-byte aligned, of this call alone
+ * until it ends).  rcsa_window_attn_plan picks n_split; max_keys bounds the keys that a row
+ * sees.
  */
 int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split);
 int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split);

@@ -74,6 +74,31 @@ def test_window_shapes(dev, dtype, B, Lq, Lk, Hq, Hk, D, window, sinks, block):
     _check(out, lse, q, k, v, [Lq] * B, [Lk] * B, window, sinks, block, True, 1 / math.sqrt(D))
 
 
+@pytest.mark.parametrize("n_split", [-1, 0, 1, 3])
+@pytest.mark.parametrize("D", [64, 128])
+def test_few_rows_forms(dev, D, n_split):
+    """Every form of a launch of few rows, over the torch op: a workgroup a key head, units,
+    blocks; padded, paged, with first keys, NaN in unseen values of rows that see less."""
+    from cast_amd import _lib, ops
+    ops_ = _lib.torch_ops()
+    B, T, Hq, Hk, Lk, page = 5, 4, 16, 2, 800, 48
+    q, k, v = _inputs(D + n_split, B, T, Lk, Hq, Hk, D, BF)
+    k_len, q_len = [800, 333, 4, 0, 70], [4, 2, 4, 3, 0]
+    v[0, 798, 1, 5] = float("nan")  # queries 2 and 3 of request 0 see it
+    v[4, 69] = float("inf")
+    kp, vp, table = (t.to(dev) for t in _pages(D, k, v, k_len, page))
+    ql, kl = (torch.tensor(n, dtype=torch.int32, device=dev) for n in (q_len, k_len))
+    for window, sinks in ((0, 0), (65, 40)):
+        for paged in (False, True):
+            print("few rows", D, n_split, window, paged, flush=True)
+            out = torch.full(q.shape, 9.0, dtype=BF, device=dev)
+            res = ops_.window_attention(
+                q.to(dev), kp if paged else k.to(dev), vp if paged else v.to(dev),
+                table if paged else None, ql, kl, window, sinks, 1, D ** -0.5, True, out, n_split,
+                -1)
+            _check(*res, q, k, v, q_len, k_len, window, sinks, 1, True, D ** -0.5, fill=9.0)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("n_split", [2, 3, 7, 64])
 def test_window_shares(dev, dtype, n_split):

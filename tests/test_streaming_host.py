@@ -99,7 +99,9 @@ def _window(lib, q=4096, k=4096, out=4096, dtype=0, dims=(1, 4, 8, 2, 1, 64),
     (dict(table=4096, max_pages=4, n_pages=9, page=24), SHAPE),
     (dict(table=4096, max_pages=0, n_pages=9, page=16), SHAPE),
     (dict(table=4096, max_pages=1 << 20, n_pages=9, page=1 << 12), SHAPE),
-    (dict(n_split=0), SHAPE), (dict(n_split=65), SHAPE), (dict(n_split=2), SHAPE),
+    (dict(n_split=0), SHAPE), (dict(n_split=-2), SHAPE), (dict(n_split=65), SHAPE),
+    (dict(n_split=-1, dims=(1, 40, 8, 2, 1, 64)), SHAPE),
+    (dict(n_split=0, dims=(513, 4, 8, 2, 1, 64), ws=4096, ws_bytes=1 << 40), SHAPE), (dict(n_split=2), SHAPE),
     (dict(n_split=2, ws=4096, ws_bytes=64), SHAPE),
     (dict(strides=(512, 128, 63) + (512, 64, 64) * 3), STRIDE),
     (dict(strides=(512, 128, 64, 512, 0, 64, 512, 64, 64, 512, 128, 64)), STRIDE),
@@ -114,7 +116,10 @@ def test_window_abi_refusals(lib, kw, status):
 def test_window_plan_and_workspace(lib):
     n = ctypes.c_int64(-1)
     assert lib.rcsa_window_attn_plan(_arr(1, 1, 4096, 8, 8, 128), 4096, ctypes.byref(n)) == 0
-    assert n.value == 0  # few rows: units of one wavefront
+    assert n.value == 0  # few rows, many keys: units of one wavefront
+    assert lib.rcsa_window_attn_plan(_arr(1, 1, 4096, 8, 8, 128), 512, ctypes.byref(n)) == 0
+    assert n.value == -1  # few keys: a workgroup a key head
+    assert lib.rcsa_window_attn_workspace_bytes(_arr(1, 1, 64, 8, 8, 128), -1) == 0
     assert lib.rcsa_window_attn_plan(_arr(1, 64, 4096, 8, 8, 128), 4096, ctypes.byref(n)) == 0
     assert 1 <= n.value <= 64
     assert lib.rcsa_window_attn_workspace_bytes(_arr(1, 64, 64, 8, 8, 128), 0) == -1
