@@ -379,10 +379,11 @@ struct RowTile {
 
   // One tile: `inside` when every row sees all of it, else bits() gives the lane's 16 keys.
   // prefetch() issues scalar loads for later steps: behind the first products (they return
-  // out of order, so a wait for LDS behind them would wait for them too).
-  template <typename Bits, typename Pre>
+  // out of order, so a wait for LDS behind them would wait for them too).  copies() issues
+  // a later step's OPS copies, which go out between the second products.
+  template <int OPS, typename Bits, typename Pre, typename Cp>
   __device__ __forceinline__ void step(const char* tile, float c, bool inside, Bits&& bits,
-                                       Pre&& prefetch) {
+                                       Pre&& prefetch, Cp&& copies) {
     v4i kraw[QSTEPS];
 #pragma unroll
     for (int st = 0; st < QSTEPS; ++st)
@@ -441,6 +442,7 @@ struct RowTile {
       }
     }
     l_run += part;
+    copies();
     // (the reads of the second half of the keys are in flight beside the first half's
     // products)
     auto v_group = [&](int u, op8 (&op)[NDT]) __attribute__((always_inline)) {
@@ -464,6 +466,7 @@ struct RowTile {
     for (int i = 0; i < 2 * NDT; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
       if (i < NDT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      if (i < OPS) __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
     }
   }
 };
@@ -590,8 +593,10 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, in
   }
 }
 
+// Blocks of 128 rows over pages (window_paged.hip); type 0: bf16, 1: fp16.
+void launch_window_paged(WindowArgs& a, int type, int64_t D, dim3 grid, hipStream_t s);
 // Few rows (window_units.hip): in units and their join, or one workgroup a key head
-// (a.units 0); type 0: bf16, 1: fp16.
+// (a.units 0).
 int launch_window_units(WindowArgs& a, int type, int64_t D, hipStream_t s);
 
 }  // namespace rcsa

@@ -1,154 +1,8 @@
-// Windowed attention, blocks of 128 rows: one pass over the visible keys with the
-// running maximum and sum of the softmax.
-//
-// Work: a workgroup takes 128 rows of one key head (32 a wavefront, 4
-// wavefronts) and streams the 32-key tiles that any of them sees: the tiles of
-// the first keys, then those of the window.  Three workgroups share a compute
-// unit, so that one's exponentials run beside another's matrix products.
-// A tile's K and V go global -> LDS without registers into a ring of three
-// slots; rows past the keys, and pages that are not there, land as zeros.
-// Only the tiles at the window's edges are masked; a wavefront none of whose rows
-// sees a tile only copies it.
-#include "window_attn.h"
+// Windowed attention, blocks of 128 rows: the dense form, the join of split blocks, plans and
+// the entry points (the paged form is in a source of its own: see window_paged.hip).
+#include "window_tile.h"
 
 namespace rcsa {
-
-template <typename T, int D, bool PAGED>
-__global__ void __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 3, D == 64 ? 4 : 3)))
-window_kernel(WindowArgs a) {
-  using R = RowTile<T, D>;
-  constexpr int BM = 128, STAGES = 3;
-  constexpr int RPU = 1024 / R::KROW;         // rows of a 1 KiB copy
-  constexpr int UPW = R::TILE / 1024 / 4;     // copies of a wavefront, K and V each
-  constexpr int OPS = 2 * UPW;
-  // (separate arrays and a loop unrolled over them: reads of one slot do not wait for
-  // copies in flight into the others)
-  __shared__ __attribute__((aligned(1024))) char s_0[2 * R::TILE];
-  __shared__ __attribute__((aligned(1024))) char s_1[2 * R::TILE];
-  __shared__ __attribute__((aligned(1024))) char s_2[2 * R::TILE];
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = uniform_int(tid >> 6);
-  const int hf = lane >> 5, lr = lane & 31;
-
-  // XCD x (workgroups go round-robin) runs a contiguous run of items, so that neighbours
-  // share most of their window in its L2, or every 8th from the longest on.
-  const int xcd = static_cast<int>(blockIdx.x % kNumXcd);
-  const int slot = static_cast<int>(blockIdx.x / kNumXcd);
-  const int tail = slot - a.xcd_whole;
-  Place p;
-  p.shares = tail < 0 ? 1 : a.n_split;
-  const int in_xcd = tail < 0 ? slot : a.xcd_whole + tail / a.n_split;
-  const int share = tail < 0 ? 0 : tail % a.n_split;
-  const ItemAt it = item_at(a, xcd, in_xcd);
-  if (it.bh < 0) return;
-  p.b = divide(it.bh, a.by_Hk);
-  p.hk = it.bh - p.b * a.Hk;
-  const Request rq = request_of(a, p.b);
-  const int q_len = uniform_int(rq.q_len);
-  p.k_len = uniform_int(rq.k_len);
-  p.n_rows = q_len * a.G;
-  const int item_row0 = it.rblock * BM;
-  if (item_row0 >= p.n_rows) return;
-  p.row0 = item_row0 + wave * 32;
-  p.shift = p.k_len - q_len;
-  const int64_t per_tail = a.xcd_items - a.xcd_whole;
-  const int64_t ws_row =
-      (share * per_tail * kNumXcd + xcd * per_tail + in_xcd - a.xcd_whole) * BM + wave * 32;
-
-  // uniform ranges: of the item, and of this wavefront's first and last rows
-  const KeyRange w_first = row_range(a, p, p.row0), w_last = row_range(a, p, p.row0 + 31);
-  p.tiles = tiles_of(a, row_range(a, p, item_row0), row_range(a, p, item_row0 + BM - 1));
-  share_of(p, share);
-
-  R t;
-  t.init(lane);
-  {
-    const Row r = row_of(a, p, p.row0 + lr);
-    t.load_q(static_cast<const T*>(a.q) + p.b * a.sq[0] + static_cast<int64_t>(r.qi) * a.sq[1] +
-                 r.head * a.sq[2], hf);
-  }
-
-  const char* const kbase = static_cast<const char*>(a.k) +
-                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
-  const char* const vbase = static_cast<const char*>(a.v) +
-                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
-  const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
-  const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
-
-  // Copies: wavefront w moves rows 8w .. 8w + 7 of the tile, which lie in its half w / 2,
-  // RPU rows a copy, chunks swizzled by row.
-  uint32_t k_lo[UPW], v_lo[UPW];
-#pragma unroll
-  for (int i = 0; i < UPW; ++i) {
-    const int r = (wave * UPW + i) * RPU + lane / R::CPR;  // row of the tile
-    const uint32_t in_half = static_cast<uint32_t>(r & 15);
-    k_lo[i] = in_half * krb + (((lane % R::CPR) ^ (swz_k<R::KROW>(r) & (R::CPR - 1))) * 16);
-    v_lo[i] = in_half * vrb + (((lane % R::CPR) ^ (swz_v(r) & (R::CPR - 1))) * 16);
-  }
-  struct Staged {
-    int key, there;
-  };
-  auto stage = [&](const Step& s, char* dst) __attribute__((always_inline)) -> Staged {
-    const HalfRows h = half_rows<PAGED>(a, s, wave >> 1, p.k_len, krb, vrb);
-    char* const ks = const_cast<char*>(kbase) + h.k;
-    char* const vs = const_cast<char*>(vbase) + h.v;
-    // (row strides are at least a row: a lane of row r < rows stays below)
-    const int kn = h.rows * static_cast<int>(krb), vn = h.rows * static_cast<int>(vrb);
-#pragma unroll
-    for (int i = 0; i < UPW; ++i) {
-      buffer_copy16(ks, kn, k_lo[i], dst + (wave * UPW + i) * 1024);
-      buffer_copy16(vs, vn, v_lo[i], dst + R::TILE + (wave * UPW + i) * 1024);
-    }
-    return {s.key, halves_there<PAGED>(a, s)};
-  };
-
-  // ring: step j in slot j % 3, two steps in flight; every step copies (past the
-  // list through empty ranges), so every wait counts the same operations
-  Staged st[STAGES];
-  const Step first = step_of<PAGED>(a, p, table, 0), second = step_of<PAGED>(a, p, table, 1);
-  st[0] = stage(first, s_0);
-  __builtin_amdgcn_sched_barrier(0);
-  st[1] = stage(second, s_1);
-  __builtin_amdgcn_sched_barrier(0);
-  Step next = step_of<PAGED>(a, p, table, 2);
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * OPS));  // Q has landed
-  auto iteration = [&](auto slot_c, int j) __attribute__((always_inline)) {
-    constexpr int J = decltype(slot_c)::value;
-    constexpr int F = (J + STAGES - 1) % STAGES;
-    char* const tile = J == 0 ? s_0 : J == 1 ? s_1 : s_2;
-    char* const fill = F == 0 ? s_0 : F == 1 ? s_1 : s_2;
-    wait_vm_barrier<OPS>();
-    st[F] = stage(next, fill);
-    __builtin_amdgcn_sched_barrier(0);
-    const Staged s = st[J];
-    const bool seen = s.key >= 0 && s.key < w_last.hi &&
-                      (s.key + kTileKeys > w_first.lo || s.key < a.sinks);
-    auto prefetch = [&]() __attribute__((always_inline)) {
-      next = step_of<PAGED>(a, p, table, j + STAGES);
-    };
-    if (seen) {
-      // every row of the wavefront sees the whole tile
-      const bool inside = (!PAGED || s.there == 3) && s.key + kTileKeys <= w_first.hi &&
-                          (s.key >= w_last.lo || s.key + kTileKeys <= a.sinks);
-      t.step(tile, a.scale_log2, inside, [&]() __attribute__((always_inline)) {
-        return seen_bits(a, p, p.row0 + lr, hf, s.key, s.there);
-      }, prefetch);
-    } else {
-      prefetch();
-    }
-  };
-  const int rounds = (p.steps + STAGES - 1) / STAGES;
-  for (int rd = 0; rd < rounds; ++rd) {
-    const int j = rd * STAGES;
-    iteration(std::integral_constant<int, 0>{}, j);
-    iteration(std::integral_constant<int, 1>{}, j + 1);
-    iteration(std::integral_constant<int, 2>{}, j + 2);
-  }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
-  finish_rows<T, D, PAGED>(p, t, lane, a.ws_o + ws_row * D, a.ws_ml + ws_row);
-}
 
 // The shares of the split row blocks joined: w_s = l_s 2^(m_s - M),
 // out = sum w_s O_s / sum w_s.  One thread per row and 8 channels; the shares are added in
@@ -202,7 +56,7 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
   const int64_t wgs = (a.xcd_whole + tail * a.n_split) * kNumXcd;
   if (wgs >= (1ll << 31)) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs));
-  if (a.table) window_kernel<T, D, true><<<grid, dim3(256), 0, s>>>(a);
+  if (a.table) launch_window_paged(a, std::is_same<T, __bf16>::value ? 0 : 1, D, grid, s);
   else window_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
   if (a.n_split > 1 && tail > 0) {
     const int64_t n = (tail * kNumXcd * 128 * (D / 8) + 255) / 256;
@@ -304,7 +158,8 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
                                 hipStream_t stream) {
   if (!q || !k || !v || !out || !dims || !strides) return RCSA_ERR_NULL;
   if (dtype != RCSA_BF16 && dtype != RCSA_F16) return RCSA_ERR_DTYPE;
-  if (!window_dims(dims)) return RCSA_ERR_SHAPE;
+  // (a masked logit is -inf before the scale)
+  if (!window_dims(dims) || !(sm_scale > 0.0f && sm_scale < INFINITY)) return RCSA_ERR_SHAPE;
   const int64_t most = 1ll << 30;  // positions, windows and blocks stay far from 2^31
   if (dims[2] >= most || window < 0 || sinks < 0 || block < 0) return RCSA_ERR_SHAPE;
   if (block == 0 && (window != 0 || sinks != 0)) return RCSA_ERR_SHAPE;

@@ -106,9 +106,10 @@ window_unit_kernel(WindowArgs a) {
     const int there = halves_there<PAGED>(a, now);
     const bool inside = there == 3 && now.key + kTileKeys <= first.hi &&
                         (now.key >= last.lo || now.key + kTileKeys <= a.sinks);
-    t.step(tile, a.scale_log2, inside, [&]() __attribute__((always_inline)) {
+    t.template step<0>(tile, a.scale_log2, inside, [&]() __attribute__((always_inline)) {
       return seen_bits(a, p, lr, hf, now.key, there);
-    }, [&]() __attribute__((always_inline)) { next = step_of<PAGED>(a, p, table, s + 2); });
+    }, [&]() __attribute__((always_inline)) { next = step_of<PAGED>(a, p, table, s + 2); },
+       []() __attribute__((always_inline)) {});
   }
   if constexpr (!GROUP) {
     const int64_t ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;

@@ -1310,10 +1310,17 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
         raise ValueError(f"{fn}: q {tuple(q.shape)} needs k and v [{B}, Lk, a divisor of {Hq}, "
                          f"{D}], got {tuple(k.shape)} and {tuple(v.shape)}")
     w, s, b = _window(window, sinks, block, causal, fn)
-    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    scale = _sm_scale(sm_scale, D, fn)
     res = _lib.torch_ops().window_attention(q, k, v, None, q_lengths, k_lengths, w, s, b, scale,
                                             return_lse, out, _shares(n_split, fn), -1)
     return tuple(res) if return_lse else res[0]
+
+
+def _sm_scale(sm_scale: Optional[float], D: int, fn: str) -> float:
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{fn}: sm_scale must be positive and finite, got {sm_scale}")
+    return scale
 
 
 def _shares(n_split: Optional[int], fn: str) -> int:
@@ -1351,7 +1358,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
                          f"a divisor of {Hq}, {D}], got {tuple(kp.shape)} and "
                          f"{tuple(cache.v.shape)}")
     w, s, b = _window(window, sinks, block, causal, fn)
-    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    scale = _sm_scale(sm_scale, D, fn)
     res = _lib.torch_ops().window_attention(
         q, kp, cache.v, cache.table, q_lengths, lengths, w, s, b, scale, return_lse, out,
         _shares(n_split, fn), -1 if max_length is None else int(max_length))

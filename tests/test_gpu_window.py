@@ -350,7 +350,8 @@ def test_refusals(dev):
     for kw, err in ((dict(window=0), ValueError), (dict(window=-5), ValueError),
                     (dict(sinks=-1), ValueError), (dict(block=0), ValueError),
                     (dict(causal=False, window=5), ValueError),
-                    (dict(causal=False, sinks=5), ValueError), (dict(n_split=0), ValueError),
+                    (dict(causal=False, sinks=5), ValueError), (dict(sm_scale=0.0), ValueError),
+                    (dict(sm_scale=-0.1), ValueError), (dict(n_split=0), ValueError),
                     (dict(n_split=65), RuntimeError),
                     (dict(k_lengths=torch.tensor([1, 2], device=dev)), RuntimeError),
                     (dict(k_lengths=torch.tensor([1], device=dev).int()), RuntimeError),

@@ -83,9 +83,9 @@ def test_rope_abi_refusals(lib, kw, status):
 def _window(lib, q=4096, k=4096, out=4096, dtype=0, dims=(1, 4, 8, 2, 1, 64),
             strides=(512, 128, 64, 512, 64, 64, 512, 64, 64, 512, 128, 64), table=None, ts=1,
             max_pages=0, n_pages=0, page=0, window=0, sinks=0, block=1, n_split=1, ws=None,
-            ws_bytes=0):
+            ws_bytes=0, scale=0.1):
     return lib.rcsa_window_attn(q, k, k, out, None, dtype, _arr(*dims), _arr(*strides), None, None,
-                                table, ts, max_pages, n_pages, page, window, sinks, block, 0.1,
+                                table, ts, max_pages, n_pages, page, window, sinks, block, scale,
                                 n_split, ws, ws_bytes, None)
 
 
@@ -108,7 +108,8 @@ def _window(lib, q=4096, k=4096, out=4096, dtype=0, dims=(1, 4, 8, 2, 1, 64),
     (dict(strides=(512, 128, 64, 512, 64, 64, 512, 56, 64, 512, 128, 64)), STRIDE),
     (dict(strides=(512, 128, 64, 512, 1 << 25, 64, 512, 64, 64, 512, 128, 64)), STRIDE),
     (dict(strides=(512, 128, 64, -512, 64, 64, 512, 64, 64, 512, 128, 64)), STRIDE),
-    (dict(q=4098), ALIGN), (dict(k=4104), ALIGN), (dict(out=4100), ALIGN)])
+    (dict(scale=0.0), SHAPE), (dict(scale=-1.0), SHAPE), (dict(scale=float('nan')), SHAPE),
+    (dict(scale=float('inf')), SHAPE), (dict(q=4098), ALIGN), (dict(k=4104), ALIGN), (dict(out=4100), ALIGN)])
 def test_window_abi_refusals(lib, kw, status):
     assert _window(lib, **kw) == status
 
