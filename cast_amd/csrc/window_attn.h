@@ -274,8 +274,8 @@ template <typename A>
 __device__ __forceinline__ bool page_ok(A& a, int p) {
   return static_cast<uint32_t>(p) < static_cast<uint32_t>(a.n_pages);
 }
-template <bool PAGED>
-__device__ __forceinline__ Step step_of(const WindowArgs& a, const Place& p, const int32_t* table,
+template <bool PAGED, typename A>
+__device__ __forceinline__ Step step_of(A& a, const Place& p, const int32_t* table,
                                         int s) {
   Step r{key_of(p, s), 0, 0};
   if constexpr (PAGED) {
@@ -300,8 +300,8 @@ __device__ __forceinline__ void share_of(Place& p, int share) {
   p.steps = q + (share < rem ? 1 : 0);
 }
 // Whether the step's halves are there: bits 0 and 1.
-template <bool PAGED>
-__device__ __forceinline__ int halves_there(const WindowArgs& a, const Step& s) {
+template <bool PAGED, typename A>
+__device__ __forceinline__ int halves_there(A& a, const Step& s) {
   return PAGED ? (page_ok(a, s.page0) ? 1 : 0) + (page_ok(a, s.page1) ? 2 : 0) : 3;
 }
 // The 16 rows of a half of a step: offsets of its first row, rows that are there.  (32 x
@@ -310,8 +310,8 @@ struct HalfRows {
   uint64_t k, v;
   int rows;
 };
-template <bool PAGED>
-__device__ __forceinline__ HalfRows half_rows(const WindowArgs& a, const Step& s, int half,
+template <bool PAGED, typename A>
+__device__ __forceinline__ HalfRows half_rows(A& a, const Step& s, int half,
                                               int k_len, uint32_t krb, uint32_t vrb) {
   const int key = (s.key < 0 ? 0 : s.key) + 16 * half;
   HalfRows r;
@@ -472,7 +472,8 @@ struct RowTile {
 };
 
 // The lane's 16 keys of the tile at `key` that row `row` sees, as bits.
-__device__ __forceinline__ uint32_t seen_bits(const WindowArgs& a, const Place& p, int row, int hf,
+template <typename A>
+__device__ __forceinline__ uint32_t seen_bits(A& a, const Place& p, int row, int hf,
                                               int key, int there) {
   const KeyRange kr = key_range(a, row_of(a, p, row).qi + p.shift, p.k_len);
   const int k0 = key + 16 * hf, sink = a.sinks < kr.hi ? a.sinks : kr.hi;
@@ -484,28 +485,162 @@ __device__ __forceinline__ uint32_t seen_bits(const WindowArgs& a, const Place& 
   return (there >> hf) & 1 ? bits : 0u;
 }
 
+// The launch's arguments (its first and only one) read again behind the loop: kept in scalar
+// registers through it they would spill.
+typedef const __attribute__((address_space(4))) WindowArgs LateArgs;
+__device__ __forceinline__ LateArgs& late_args() {
+  LateArgs* late = (LateArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(late));
+  return *late;
+}
+
+// The lane, counted afresh (no register holds it through the loop).
+__device__ __forceinline__ int lane_again() {
+  uint32_t none = 0;
+  asm volatile("" : "+v"(none));  // (else it is counted at the start)
+  return static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)));
+}
+
+// Rows whose products met a value that they do not see (0 * inf or 0 * NaN of a masked
+// key): a wavefront's 32 rows taken again at their known maxima m, tile by tile through
+// TILE bytes of LDS, values that are no numbers staged as 0 and added only where a row
+// sees their key.  Without pipelining, some ten times slower than the first time.
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void rows_again(LateArgs& a, const Place& p, RowTile<T, D>& t,
+                                           int lane, float m, char* lds) {
+  using R = RowTile<T, D>;
+  typedef typename R::op8 op8;
+  constexpr int RPU = 1024 / R::KROW, LOADS = R::TILE / 1024;
+  constexpr uint32_t kExp = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
+  const int hf = lane >> 5, lr = lane & 31;
+  const char* const kbase = static_cast<const char*>(a.k) +
+                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
+  const char* const vbase = static_cast<const char*>(a.v) +
+                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
+  const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
+  const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
+#pragma unroll
+  for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t.o_acc[dt][r] = 0.0f;
+  const int lrow = lane / R::CPR, chunk = lane % R::CPR;
+  // (one load at a time and fences between the products: few registers)
+  // 16-byte chunk `chunk` of row i RPU + lrow of the tile
+  auto load = [&](const char* base, uint64_t off0, uint64_t off1, int rows0, int rows1,
+                  uint32_t rb, int i) __attribute__((always_inline)) -> v4i {
+    const int row = i * RPU + lrow, in_half = row & 15;
+    const bool second = i * RPU >= 16;
+    v4i x = {0, 0, 0, 0};
+    if (in_half < (second ? rows1 : rows0))
+      x = *reinterpret_cast<const v4i*>(base + (second ? off1 : off0) +
+                                        static_cast<uint64_t>(in_half) * rb + chunk * 16);
+    return x;
+  };
+  for (int s = 0; s < p.steps; ++s) {
+    const Step st = step_of<PAGED>(a, p, table, s);
+    const HalfRows h0 = half_rows<PAGED>(a, st, 0, p.k_len, krb, vrb);
+    const HalfRows h1 = half_rows<PAGED>(a, st, 1, p.k_len, krb, vrb);
+#pragma unroll 1
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = i * RPU + lrow;
+      *reinterpret_cast<v4i*>(lds + row * R::KROW +
+                              ((chunk ^ (swz_k<R::KROW>(row) & (R::CPR - 1))) * 16)) =
+          load(kbase, h0.k, h1.k, h0.rows, h1.rows, krb, i);
+    }
+    v16f s_acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
+#pragma unroll
+    for (int q = 0; q < R::QSTEPS; ++q) {
+      s_acc = Half<T>::mfma(
+          __builtin_bit_cast(op8, *reinterpret_cast<const v4i*>(lds + t.k_off[q])), t.q_op[q],
+          s_acc);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const uint32_t own = seen_bits(a, p, p.row0 + lr, hf, st.key, halves_there<PAGED>(a, st));
+    const uint32_t other = __shfl_xor(own, 32, kWave);
+    const uint32_t seen = hf ? other | (own << 16) : own | (other << 16);
+    op8 p_op[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      p_op[r >> 3][r & 7] = static_cast<T>(
+          (own >> r) & 1u ? __builtin_amdgcn_exp2f(fmaf(s_acc[r], a.scale_log2, -m)) : 0.0f);
+    uint32_t odd = 0;  // keys of the tile with values that are no numbers
+#pragma unroll 1
+    for (int i = 0; i < LOADS; ++i) {
+      const int row = i * RPU + lrow;
+      v4i x = load(vbase, h0.v, h1.v, h0.rows, h1.rows, vrb, i);
+      bool bad = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t v = static_cast<uint32_t>(x[w]);
+        const bool lo = (v & kExp) == kExp, hi = (v & (kExp << 16)) == kExp << 16;
+        x[w] = static_cast<int>((lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u));
+        bad = bad || lo || hi;
+      }
+      const uint64_t lanes = __ballot(bad);
+#pragma unroll
+      for (int r = 0; r < RPU; ++r)  // (CPR lanes a row)
+        if ((lanes >> (r * R::CPR)) & ((1ull << R::CPR) - 1)) odd |= 1u << (i * RPU + r);
+      *reinterpret_cast<v4i*>(lds + row * R::KROW +
+                              ((chunk ^ (swz_v(row) & (R::CPR - 1))) * 16)) = x;
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int dt = 0; dt < R::NDT; ++dt) {
+        const char* const p0 = lds + t.v_off[dt] - R::TILE + 8 * u * R::KROW;
+        const auto lo = Half<T>::read_tr(p0);
+        const auto hi = Half<T>::read_tr(p0 + 4 * R::KROW);
+        t.o_acc[dt] = Half<T>::mfma(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7),
+                                    p_op[u], t.o_acc[dt]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    for (; odd != 0; odd &= odd - 1) {
+      const int j = __builtin_ctz(odd);
+      const char* const row = vbase + (j < 16 ? h0.v : h1.v) + static_cast<uint64_t>(j & 15) * vrb;
+      const bool sees = (seen >> j) & 1u;
+#pragma unroll
+      for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const typename Half<T>::op4 v = *reinterpret_cast<const typename Half<T>::op4*>(
+              row + (32 * dt + 8 * g + 4 * hf) * 2);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = static_cast<float>(v[e]);
+            if (sees && !(fabsf(f) < INFINITY)) t.o_acc[dt][4 * g + e] += f;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+}
+
 // The end of a wavefront's rows: normalise, write the rows and the LSE, or with more than one
 // share the share's partial rows to part_o [32][D] and their (max, sum) to part_ml [32].
+// lds: TILE bytes of the wavefront's own.
 template <typename T, int D, bool PAGED>
-__device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, int lane,
-                                            float* part_o, float2* part_ml) {
-  // (the arguments are read again: kept in scalar registers they would spill the loop's)
-  typedef const __attribute__((address_space(4))) WindowArgs Late;
-  Late* late = (Late*)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(late));
-  Late& a = *late;
+__device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, float* part_o,
+                                            float2* part_ml, char* lds) {
+  LateArgs& a = late_args();
+  const int lane = lane_again();
   typedef typename Half<T>::op4 op4;
   const int hf = lane >> 5, lr = lane & 31;
   const float l = pair_sum(t.l_run), m = t.m_run;
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (a NaN sum stays one)
-  bool bad = false;  // a product that is no number in a row whose sum is one
+  // a product that is no number, in a row whose sum is one
+  bool bad = false;
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      t.o_acc[dt][r] *= inv;
-      bad = bad || !(fabsf(t.o_acc[dt][r]) < INFINITY);
-    }
+    for (int r = 0; r < 16; ++r) bad = bad || !(fabsf(t.o_acc[dt][r]) < INFINITY);
+  if (__ballot(bad && l > 0.0f && l < INFINITY) != 0)
+    rows_again<T, D, PAGED>(a, p, t, lane, m == -INFINITY ? 0.0f : m, lds);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t.o_acc[dt][r] *= inv;
   const Row my = row_of(a, p, p.row0 + lr);
   if (my.live) {
     if (p.shares > 1) {
@@ -534,61 +669,6 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, in
       if (hf == 0 && a.lse)
         a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
             l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
-    }
-  }
-  // A row whose products met a value that it does not see (0 * inf or 0 * NaN of a
-  // masked key): its sum is taken again over its own keys, one row at a time.
-  uint64_t again = __ballot(bad && my.live && l > 0.0f && l < INFINITY);
-  again |= again >> 32;
-  if (static_cast<uint32_t>(again) == 0) return;
-  __builtin_amdgcn_s_waitcnt(0);  // (the stores above come first)
-  const char* const kbase = static_cast<const char*>(a.k) +
-                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
-  const char* const vbase = static_cast<const char*>(a.v) +
-                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
-  const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
-  for (uint32_t rows = static_cast<uint32_t>(again); rows != 0; rows &= rows - 1) {
-    constexpr int N = D / 64;
-    const int i = __builtin_ctz(rows);
-    const Row r = row_of(a, p, p.row0 + i);
-    const KeyRange rk = row_range(a, p, p.row0 + i);
-    const int rsink = a.sinks < rk.hi ? a.sinks : rk.hi;
-    const T* const rq = static_cast<const T*>(a.q) + p.b * a.sq[0] +
-                        static_cast<int64_t>(r.qi) * a.sq[1] + r.head * a.sq[2];
-    const float rm = __shfl(m, i, kWave), rinv = __shfl(inv, i, kWave);
-    float acc[N], qv[N];
-#pragma unroll
-    for (int c = 0; c < N; ++c) {
-      acc[c] = 0.0f;
-      qv[c] = static_cast<float>(rq[lane + 64 * c]);
-    }
-    for (int s = 0; s < p.steps; ++s)
-      for (int j = key_of(p, s), end = j + kTileKeys; j < end; ++j) {
-        if (!(j < rk.hi && (j >= rk.lo || j < rsink))) continue;
-        int64_t ko = j * a.sk[1], vo = j * a.sv[1];
-        if constexpr (PAGED) {
-          const int col = divide(j >> 4, a.by_half_page), pg = table[col];
-          if (!page_ok(a, pg)) continue;
-          const int64_t slot = j - col * a.page;
-          ko = pg * a.sk[0] + slot * a.sk[1];
-          vo = pg * a.sv[0] + slot * a.sv[1];
-        }
-        const T* const kp = reinterpret_cast<const T*>(kbase) + ko;
-        const T* const vp = reinterpret_cast<const T*>(vbase) + vo;
-        float x = 0.0f;
-#pragma unroll
-        for (int c = 0; c < N; ++c) x = fmaf(qv[c], static_cast<float>(kp[lane + 64 * c]), x);
-        const float pr = __builtin_amdgcn_exp2f(fmaf(wave_sum(x), a.scale_log2, -rm));
-#pragma unroll
-        for (int c = 0; c < N; ++c)
-          acc[c] = fmaf(pr, static_cast<float>(vp[lane + 64 * c]), acc[c]);
-      }
-    T* const dst = static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(r.qi) * a.so[1] +
-                   r.head * a.so[2];
-#pragma unroll
-    for (int c = 0; c < N; ++c) {
-      if (p.shares > 1) part_o[i * D + lane + 64 * c] = acc[c] * rinv;
-      else dst[lane + 64 * c] = static_cast<T>(acc[c] * rinv);
     }
   }
 }

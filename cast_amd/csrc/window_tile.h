@@ -150,7 +150,9 @@ window_kernel(WindowArgs a) {
     iteration(std::integral_constant<int, 2>{}, j + 2);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
-  finish_rows<T, D, PAGED>(p, t, lane, a.ws_o + ws_row * D, a.ws_ml + ws_row);
+  __builtin_amdgcn_s_barrier();  // (the ring is read: a wavefront may need a part of it)
+  finish_rows<T, D, PAGED>(p, t, a.ws_o + ws_row * D, a.ws_ml + ws_row,
+                           (wave < 2 ? s_0 : s_1) + (wave & 1) * R::TILE);
 }
 
 }  // namespace rcsa

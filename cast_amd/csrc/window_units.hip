@@ -113,12 +113,13 @@ window_unit_kernel(WindowArgs a) {
   }
   if constexpr (!GROUP) {
     const int64_t ws_row = static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
-    finish_rows<T, D, PAGED>(p, t, lane, a.ws_o + ws_row * D, a.ws_ml + ws_row);
+    finish_rows<T, D, PAGED>(p, t, late_args().ws_o + ws_row * D,
+                             late_args().ws_ml + ws_row, tile);
     return;
   }
   // the wavefronts' partial rows meet in LDS, each in its own tile's place
   static_assert(kFewRows * D * 4 <= 2 * R::TILE, "partial rows fit a wavefront's tiles");
-  finish_rows<T, D, PAGED>(p, t, lane, reinterpret_cast<float*>(tile), s_ml[wave]);
+  finish_rows<T, D, PAGED>(p, t, reinterpret_cast<float*>(tile), s_ml[wave], tile);
   __syncthreads();
   for (int i = threadIdx.x; i < p.n_rows * (D / 4); i += 64 * NW) {
     const int row = i / (D / 4), c = i % (D / 4) * 4;
