@@ -18,6 +18,7 @@
 #include <dlfcn.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <mutex>
 #include <string>
@@ -815,9 +816,30 @@ std::vector<at::Tensor> layer_call(
 
 int float_code(const char* op, const at::Tensor& t, const char* name) {
   const at::ScalarType dt = t.scalar_type();
-  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, op, ": ", name,
-              " must be bfloat16, float16 or float32");
+  TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, op, ": ", name,
+                   " must be bfloat16, float16 or float32, got ", dt);
   return dt == at::kBFloat16 ? RCSA_BF16 : dt == at::kHalf ? RCSA_F16 : RCSA_F32;
+}
+
+// An input on the call's GPU, with no gradient to compute.
+void input(const char* op, int& device, bool grads, const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), op, ": tensors must live on a HIP device, ", name, " is on ",
+              t.device());
+  TORCH_CHECK(!grads || !t.requires_grad(), op,
+              ": no gradient is computed; call it under torch.no_grad()");
+  on_device(op, device, t, name);
+}
+void input(const char* op, int& device, bool grads, const c10::optional<at::Tensor>& t,
+           const char* name) {
+  if (t.has_value()) input(op, device, grads, *t, name);
+}
+
+// Queries, keys or values [., ., H, D] of a call's dtype.
+void want_heads(const char* op, const at::Tensor& t, at::ScalarType dt, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == dt, op, ": q, k and v must share a dtype, ", name, " is ",
+                   t.scalar_type(), " beside ", dt);
+  TORCH_CHECK_VALUE(t.dim() == 4 && (t.stride(3) == 1 || t.size(3) <= 1), op, ": ", name,
+                    " must be [B, L, H, D] with a contiguous last dim, got ", t.sizes());
 }
 
 // A tensor [., ., ., D] whose rows the kernels reach by its own strides.
@@ -858,9 +880,11 @@ Turns want_turns(const char* op, const at::Tensor& positions, const at::Tensor& 
               ": positions must be [L] or [B, L], with ", n_axes, " axes last when more than one");
   want(op, turns, at::kDouble, "turns");
   want(op, axis, at::kInt, "axis");
-  TORCH_CHECK(turns.dim() == 1 && turns.is_contiguous() && 2 * turns.numel() <= D &&
+  TORCH_CHECK(turns.dim() == 1 && turns.is_contiguous() &&
                   (!axis.has_value() || (axis->is_contiguous() && axis->numel() == turns.numel())),
-              op, ": the plan turns ", 2 * turns.numel(), " channels of a head of ", D);
+              op, ": a plan holds contiguous turns and an axis for each");
+  TORCH_CHECK_VALUE(2 * turns.numel() <= D, op, ": the plan turns ", 2 * turns.numel(),
+                    " channels of a head of ", D);
   Turns r;
   r.n_axes = n_axes;
   r.n_pairs = turns.numel();
@@ -876,14 +900,15 @@ at::Tensor rope(const at::Tensor& x, const at::Tensor& positions, const at::Tens
                 double scale, const c10::optional<at::Tensor>& out_) {
   const char* op = "rope";
   const Api& a = api(op);
+  const bool grads = at::GradMode::is_enabled();
   int dev = -1;
-  on_device(op, dev, x, "x");
-  on_device(op, dev, positions, "positions");
-  on_device(op, dev, turns, "the plan");
-  on_device(op, dev, axis, "the plan");
-  on_device(op, dev, out_, "out");
+  input(op, dev, grads, x, "x");
+  input(op, dev, false, positions, "positions");
+  input(op, dev, false, turns, "the plan");
+  input(op, dev, false, axis, "the plan");
+  input(op, dev, grads, out_, "out");
   const int code = float_code(op, x, "x");
-  want_rows(op, x, x.scalar_type(), "x");
+  want_heads(op, x, x.scalar_type(), "x");
   const int64_t B = x.size(0), L = x.size(1), H = x.size(2), D = x.size(3);
   const Turns t = want_turns(op, positions, turns, axis, n_axes, B, L, D);
   const Launch l(device_of(op, dev));
@@ -915,7 +940,7 @@ void want_vector(const char* op, const c10::optional<at::Tensor>& t, int64_t B, 
               name, " must be int32 [B]");
 }
 
-// (q_out, k_out); with pages k_out is empty, keys and values are in the pages.
+// (q_out, k_out); with pages only q_out, keys and values are in the pages.
 std::vector<at::Tensor> norm_rope(
     const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& v,
     const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight,
@@ -927,26 +952,27 @@ std::vector<at::Tensor> norm_rope(
     const c10::optional<at::Tensor>& k_out_) {
   const char* op = "norm_rope";
   const Api& a = api(op);
+  const bool grads = at::GradMode::is_enabled();
   int dev = -1;
-  on_device(op, dev, q, "q");
-  on_device(op, dev, k, "k");
-  on_device(op, dev, positions, "positions");
-  on_device(op, dev, turns, "the plan");
-  for (const auto* t : {&v, &q_weight, &k_weight, &axis, &k_pages, &v_pages, &table, &starts,
-                        &lengths, &q_out_, &k_out_})
-    on_device(op, dev, *t, "an operand");
+  input(op, dev, grads, q, "q");
+  input(op, dev, grads, k, "k");
+  input(op, dev, false, positions, "positions");
+  input(op, dev, false, turns, "the plan");
+  for (const auto* t : {&v, &q_weight, &k_weight, &k_pages, &v_pages, &q_out_, &k_out_})
+    input(op, dev, grads, *t, "an operand");
+  for (const auto* t : {&axis, &table, &starts, &lengths}) input(op, dev, false, *t, "an operand");
   const int code = float_code(op, q, "q");
   const at::ScalarType dt = q.scalar_type();
-  want_rows(op, q, dt, "q");
-  want_rows(op, k, dt, "k");
+  want_heads(op, q, dt, "q");
+  want_heads(op, k, dt, "k");
   const int64_t B = q.size(0), L = q.size(1), Hq = q.size(2), Hk = k.size(2), D = q.size(3);
   TORCH_CHECK(k.size(0) == B && k.size(1) == L && k.size(3) == D, op,
               ": q and k differ in batch, tokens or channels");
   const bool paged = table.has_value();
-  TORCH_CHECK(paged == v.has_value() && paged == k_pages.has_value() &&
-                  paged == v_pages.has_value() && !(paged && k_out_.has_value()) &&
-                  (paged || !starts.has_value()), op,
-              ": v, the pages and starts go with a block table, k_out without one");
+  TORCH_CHECK_VALUE(paged == v.has_value() && paged == k_pages.has_value() &&
+                        paged == v_pages.has_value(), op, ": give v and cache together");
+  TORCH_CHECK_VALUE(paged || !starts.has_value(), op, ": starts goes with a cache");
+  TORCH_CHECK_VALUE(!paged || !k_out_.has_value(), op, ": k_out goes without a cache");
   const Turns t = want_turns(op, positions, turns, axis, n_axes, B, L, D);
   int w_code = RCSA_F32;
   int64_t ws[2] = {0, 0}, i = 0;
@@ -977,12 +1003,12 @@ std::vector<at::Tensor> norm_rope(
   put_strides(q, s);
   put_strides(k, s + 3);
   put_strides(q_out, s + 9);
-  at::Tensor k_out;
+  std::vector<at::Tensor> res{q_out};
   int64_t max_pages = 0, n_pages = 0, page = 0, table_stride = 0;
   void* kp = nullptr;
   if (paged) {
     want_table(op, *table, B);
-    want_rows(op, *v, dt, "v");
+    want_heads(op, *v, dt, "v");
     want_rows(op, *k_pages, dt, "the key pages");
     want_rows(op, *v_pages, dt, "the value pages");
     want_own(op, *k_pages, "the key pages");
@@ -999,18 +1025,18 @@ std::vector<at::Tensor> norm_rope(
     n_pages = k_pages->size(0);
     page = k_pages->size(1);
     kp = k_pages->data_ptr();
-    k_out = at::empty({0}, q.options());
   } else {
-    k_out = k_out_.has_value() ? *k_out_ : at::empty({B, L, Hk, D}, k.options());
+    const at::Tensor k_out = k_out_.has_value() ? *k_out_ : at::empty({B, L, Hk, D}, k.options());
     want_rows(op, k_out, dt, "k_out");
     want_own(op, k_out, "k_out");
     TORCH_CHECK(k_out.sizes() == k.sizes(), op, ": k_out must have k's shape");
     put_strides(k_out, s + 12);
     kp = k_out.data_ptr();
+    res.push_back(k_out);
   }
   if (q.numel() == 0 || k.numel() == 0) {
     TORCH_CHECK(B * L * D == 0, op, ": no heads");
-    return {q_out, k_out};
+    return res;
   }
   const int64_t dims[5] = {B, L, Hq, Hk, D};
   check_status(a, op, a.norm_rope(
@@ -1021,7 +1047,7 @@ std::vector<at::Tensor> norm_rope(
       ptr<const int32_t>(axis), t.n_pairs, interleaved, static_cast<float>(scale),
       ptr<const int32_t>(table), table_stride, max_pages, n_pages, page,
       ptr<const int32_t>(starts), ptr<const int32_t>(lengths), l.stream));
-  return {q_out, k_out};
+  return res;
 }
 
 // Dense (k, v [B, Lk, Hk, D]) or, with a table, paged (k, v [pages, slots, Hk, D])
@@ -1030,24 +1056,31 @@ std::vector<at::Tensor> window_attention(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const c10::optional<at::Tensor>& table, const c10::optional<at::Tensor>& q_lengths,
     const c10::optional<at::Tensor>& k_lengths, int64_t window, int64_t sinks, int64_t block,
-    double sm_scale, bool return_lse, const c10::optional<at::Tensor>& out_, int64_t n_split,
-    int64_t max_keys) {
+    c10::optional<double> sm_scale, bool return_lse, const c10::optional<at::Tensor>& out_,
+    int64_t n_split, int64_t max_keys) {
   const bool paged = table.has_value();
   const char* op = paged ? "paged_attention" : "window_attention";
   const Api& a = api(op);
+  const bool grads = at::GradMode::is_enabled();
   int dev = -1;
-  on_device(op, dev, q, "q");
-  on_device(op, dev, k, "k");
-  on_device(op, dev, v, "v");
-  for (const auto* t : {&table, &q_lengths, &k_lengths, &out_}) on_device(op, dev, *t, "an operand");
+  input(op, dev, grads, q, "q");
+  input(op, dev, grads, k, "k");
+  input(op, dev, grads, v, "v");
+  input(op, dev, grads, out_, "out");
+  for (const auto* t : {&table, &q_lengths, &k_lengths}) input(op, dev, false, *t, "an operand");
   const at::ScalarType dt = q.scalar_type();
-  TORCH_CHECK(dt == at::kBFloat16 || dt == at::kHalf, op, ": q must be bfloat16 or float16");
-  want_rows(op, q, dt, "q");
-  want_rows(op, k, dt, "k");
-  want_rows(op, v, dt, "v");
+  TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf, op,
+                   ": q, k and v must share bfloat16 or float16, q is ", dt);
+  want_heads(op, q, dt, "q");
+  want_heads(op, k, dt, "k");
+  want_heads(op, v, dt, "v");
   const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k.size(2);
-  TORCH_CHECK(k.sizes() == v.sizes() && k.size(3) == D && (paged || k.size(0) == B), op,
-              ": k and v must have one shape, and q's batch and channels");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(3) == D && (paged || k.size(0) == B) &&
+                        Hk > 0 && Hq % Hk == 0, op, ": q ", q.sizes(), " needs k and v ",
+                    paged ? "[pages, slots" : "[B, Lk", ", a divisor of its heads, ", D, "], got ",
+                    k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(!paged || k.size(1) % 16 == 0, op,
+                    ": pages must hold a multiple of 16 keys, got ", k.size(1));
   want_vector(op, q_lengths, B, "q_lengths");
   want_vector(op, k_lengths, B, "k_lengths");
   int64_t max_pages = 0, n_pages = 0, page = 0, table_stride = 0, Lk = k.size(1);
@@ -1093,7 +1126,7 @@ std::vector<at::Tensor> window_attention(
       out.data_ptr(), return_lse ? ptr<float>(res[1]) : nullptr,
       dt == at::kBFloat16 ? RCSA_BF16 : RCSA_F16, dims, s, ptr<const int32_t>(q_lengths),
       ptr<const int32_t>(k_lengths), ptr<const int32_t>(table), table_stride, max_pages, n_pages,
-      page, window, sinks, block, static_cast<float>(sm_scale), ns,
+      page, window, sinks, block, static_cast<float>(sm_scale ? *sm_scale : 1.0 / std::sqrt(D)), ns,
       ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
   return res;
 }
@@ -1162,7 +1195,7 @@ TORCH_LIBRARY(rcsa, m) {
       &norm_rope);
   m.def(
       "window_attention(Tensor q, Tensor k, Tensor v, Tensor? table, Tensor? q_lengths, "
-      "Tensor? k_lengths, int window, int sinks, int block, float sm_scale, bool return_lse, "
+      "Tensor? k_lengths, int window, int sinks, int block, float? sm_scale, bool return_lse, "
       "Tensor(a!)? out, int n_split, int max_keys) -> Tensor[]",
       &window_attention);
 }

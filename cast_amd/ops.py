@@ -1174,22 +1174,6 @@ def int8_linear_group(x_i8: torch.Tensor, x_scale: torch.Tensor, projections, *,
     return outs
 
 
-def _no_grad(fn: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{fn}: no gradient is computed; call it under torch.no_grad()")
-
-
-def _heads(x: torch.Tensor, name: str, fn: str) -> None:
-    if x.ndim != 4 or (x.stride(3) != 1 and x.shape[3] > 1):
-        raise ValueError(f"{fn}: {name} must be [B, L, H, D] with a contiguous last dim, "
-                         f"got {tuple(x.shape)}")
-
-
-def _plan_fits(plan, D: int, fn: str) -> None:
-    if plan.rotary_dim > D:
-        raise ValueError(f"{fn}: the plan turns {plan.rotary_dim} channels of a head of {D}")
-
-
 def rope(x: torch.Tensor, positions: torch.Tensor, plan, *,
          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [B, L, H, D]`` (bf16, fp16 or fp32, any strides) with its first channels turned by
@@ -1200,13 +1184,6 @@ def rope(x: torch.Tensor, positions: torch.Tensor, plan, *,
     positions undo a rotation of scale 1), as far as 64-bit angles reach.  fp32 between, one
     rounding at the end.  ``out`` (x's shape and dtype, any strides) may be ``x`` itself and
     must not overlap it otherwise."""
-    fn = "rope"
-    _require_cuda(fn, x, positions, plan.turns)
-    _no_grad(fn, x)
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"{fn}: expected bfloat16, float16 or float32, got {x.dtype}")
-    _heads(x, "x", fn)
-    _plan_fits(plan, x.shape[3], fn)
     return _lib.torch_ops().rope(x, positions, plan.turns, plan.axis, plan.n_axes,
                                  plan.interleaved, plan.scale, out)
 
@@ -1239,28 +1216,12 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan, *
     t of request b to index ``starts[b] + t`` (int32 ``[B]``; None: t), dropped where the
     table has no page for it; ``k_out`` is then None.  No two tokens may go to one row.
     ``lengths`` (int32 ``[B]``) leaves the rows of tokens ``t >= lengths[b]`` as they were."""
-    fn = "norm_rope"
-    _require_cuda(fn, q, k, positions, plan.turns)
-    _no_grad(fn, q, k, v, q_weight, k_weight)
-    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"{fn}: expected bfloat16, float16 or float32, got {q.dtype}")
-    if k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
-        raise TypeError(f"{fn}: q, k and v must share a dtype")
-    _heads(q, "q", fn)
-    _heads(k, "k", fn)
-    _plan_fits(plan, q.shape[3], fn)
-    if (cache is None) != (v is None):
-        raise ValueError(f"{fn}: give v and cache together")
-    if cache is None and starts is not None:
-        raise ValueError(f"{fn}: starts goes with a cache")
-    if cache is not None and k_out is not None:
-        raise ValueError(f"{fn}: k_out goes without a cache")
     kp, vp, table = cache if cache is not None else (None, None, None)
-    qo, ko = _lib.torch_ops().norm_rope(
-        q, k, v, q_weight, k_weight, float(eps), bool(across_heads), positions, plan.turns,
+    res = _lib.torch_ops().norm_rope(
+        q, k, v, q_weight, k_weight, eps, across_heads, positions, plan.turns,
         plan.axis, plan.n_axes, plan.interleaved, plan.scale, kp, vp, table, starts, lengths,
         q_out, k_out)
-    return qo, (ko if cache is None else None)
+    return res[0], (res[1] if cache is None else None)
 
 
 def _window(window, sinks, block, causal, fn: str) -> tuple[int, int, int]:
@@ -1295,32 +1256,22 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     not read.  A row that sees no key gives 0 (LSE -inf); a key or value that a row does not
     see does not reach it, whatever it holds.
 
-    fp32 softmax, rounded once; returns ``out [B, Lq, Hq, D]`` and, with ``return_lse``, the
-    natural log-sum-exp ``[B, Hq, Lq]``.  ``n_split`` (None: planned) shares the keys of
+    fp32 softmax, rounded once; returns ``out [B, Lq, Hq, D]`` (must not overlap q, k or v)
+    and, with ``return_lse``, the natural log-sum-exp ``[B, Hq, Lq]`` (undefined past a
+    request's queries).  ``n_split`` (None: planned) shares the keys of
     the blocks of rows that would leave compute units idle among that many workgroups."""
     fn = "window_attention"
-    _require_cuda(fn, q, k, v)
-    _no_grad(fn, q, k, v)
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"{fn}: q, k and v must share bfloat16 or float16")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _heads(t, name, fn)
-    B, _, Hq, D = q.shape
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or Hq % max(k.shape[2], 1):
-        raise ValueError(f"{fn}: q {tuple(q.shape)} needs k and v [{B}, Lk, a divisor of {Hq}, "
-                         f"{D}], got {tuple(k.shape)} and {tuple(v.shape)}")
     w, s, b = _window(window, sinks, block, causal, fn)
-    scale = _sm_scale(sm_scale, D, fn)
+    scale = _sm_scale(sm_scale, fn)
     res = _lib.torch_ops().window_attention(q, k, v, None, q_lengths, k_lengths, w, s, b, scale,
                                             return_lse, out, _shares(n_split, fn), -1)
     return tuple(res) if return_lse else res[0]
 
 
-def _sm_scale(sm_scale: Optional[float], D: int, fn: str) -> float:
-    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-    if not 0.0 < scale < math.inf:
+def _sm_scale(sm_scale: Optional[float], fn: str) -> Optional[float]:
+    if sm_scale is not None and not 0.0 < sm_scale < math.inf:
         raise ValueError(f"{fn}: sm_scale must be positive and finite, got {sm_scale}")
-    return scale
+    return None if sm_scale is None else float(sm_scale)
 
 
 def _shares(n_split: Optional[int], fn: str) -> int:
@@ -1344,22 +1295,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
     holds, if None): it only plans how the keys are shared among workgroups, a longer
     request is still read to its end."""
     fn = "paged_attention"
-    _require_cuda(fn, q, cache.k, cache.v, cache.table, lengths)
-    _no_grad(fn, q, cache.k, cache.v)
-    if q.dtype not in (torch.bfloat16, torch.float16) or cache.k.dtype != q.dtype \
-            or cache.v.dtype != q.dtype:
-        raise TypeError(f"{fn}: q and the pages must share bfloat16 or float16")
-    _heads(q, "q", fn)
-    B, _, Hq, D = q.shape
-    kp = cache.k
-    if kp.ndim != 4 or kp.shape != cache.v.shape or kp.shape[3] != D \
-            or Hq % max(kp.shape[2], 1) or kp.shape[1] % 16:
-        raise ValueError(f"{fn}: q {tuple(q.shape)} needs pages [pages, slots (a multiple of 16), "
-                         f"a divisor of {Hq}, {D}], got {tuple(kp.shape)} and "
-                         f"{tuple(cache.v.shape)}")
     w, s, b = _window(window, sinks, block, causal, fn)
-    scale = _sm_scale(sm_scale, D, fn)
+    scale = _sm_scale(sm_scale, fn)
     res = _lib.torch_ops().window_attention(
-        q, kp, cache.v, cache.table, q_lengths, lengths, w, s, b, scale, return_lse, out,
+        q, cache.k, cache.v, cache.table, q_lengths, lengths, w, s, b, scale, return_lse, out,
         _shares(n_split, fn), -1 if max_length is None else int(max_length))
     return tuple(res) if return_lse else res[0]
