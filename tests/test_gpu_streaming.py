@@ -242,3 +242,24 @@ def test_pages_past_32_bits(dev):
     assert torch.equal(fk[at], near.k[at]) and torch.equal(fv[at], v[0])
     del fk, fv, far, cache, store
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 1), (33, 33), (64, 31), (100, 0), (0, 0)])
+def test_units_of_every_length(dev, window, sinks):
+    """Few rows in units of one wavefront: requests of 0 to 255 keys, so that windows and
+    first keys begin and end anywhere in a tile."""
+    from cast_amd import _lib
+    B, T, Hq, Hk, D, page = 256, 2, 4, 2, 64, 16
+    g = torch.Generator().manual_seed(window)
+    q = torch.randn(B, T, Hq, D, generator=g).to(BF).to(dev)
+    k, v = (torch.randn(1, B, Hk, D, generator=g).to(BF).to(dev) for _ in range(2))
+    table = torch.arange(B // page, dtype=torch.int32, device=dev).expand(B, -1).contiguous()
+    lens = torch.arange(B, dtype=torch.int32, device=dev)
+    out, lse = _lib.torch_ops().window_attention(
+        q, k.view(-1, page, Hk, D), v.view(-1, page, Hk, D), table, None, lens, window, sinks, 1,
+        None, True, None, 0, -1)
+    for n in range(B):
+        seen = so.visible(T, n, window, sinks, 1, device=dev)
+        ref, rlse, tol, ltol = so.attention(q[n], k[0, :n], v[0, :n], seen, D ** -0.5, BF)
+        _same(out[n], ref, tol, (n, "rows"))
+        _same(lse[n], rlse, ltol, (n, "sums"))
