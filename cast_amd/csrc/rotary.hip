@@ -8,7 +8,10 @@
 //   x * rsqrt(mean(x^2) + eps) * w, the mean over a head or over all heads.
 //
 // HBM-bound: each element is read once, written once, and rounded once (fp32
-// between).  A position times a frequency needs more than 24 bits once the
+// between).  44 frames x 24 heads of 128 80 us, 5.9 TB/s; with joint norms and the append to
+// pages 3520 x 72 heads 35 us, 3.7 TB/s (a token's sums stand between its loads and its
+// stores, and 130 MB are few beside a launch's start and end); 32782 x 20 heads of 64 with
+// norms of heads 42 us, 3.9 TB/s; one token of a few requests 4.4 us, a launch.  A position times a frequency needs more than 24 bits once the
 // positions are far (at position 10^6 an fp32 angle is off by 0.06), so the
 // angle is a product in turns in 64 bits, reduced to [-1/2, 1/2] turns there,
 // and only then fp32: exact to an fp32 rounding at any position, with no table
