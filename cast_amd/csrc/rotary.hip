@@ -390,7 +390,7 @@ static bool runs_of(const RotaryArgs& a, int V, bool inter) {
   const size_t w = V * (a.w_dtype == RCSA_F32 ? 4 : 2);
   for (const void* p : {a.qw, a.kw})
     if (reinterpret_cast<uintptr_t>(p) % (w < 16 ? w : 16)) return false;
-  return true;
+  return a.qw_h % V == 0 && a.kw_h % V == 0;
 }
 
 template <typename T, int V, bool INTER, int NORM>
