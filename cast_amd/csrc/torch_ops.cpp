@@ -1079,6 +1079,7 @@ std::vector<at::Tensor> window_attention(
                         Hk > 0 && Hq % Hk == 0, op, ": q ", q.sizes(), " needs k and v ",
                     paged ? "[pages, slots" : "[B, Lk", ", a divisor of its heads, ", D, "], got ",
                     k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(D > 0, op, ": no channels");
   TORCH_CHECK_VALUE(!paged || k.size(1) % 16 == 0, op,
                     ": pages must hold a multiple of 16 keys, got ", k.size(1));
   want_vector(op, q_lengths, B, "q_lengths");
@@ -1111,7 +1112,7 @@ std::vector<at::Tensor> window_attention(
   int64_t ns = n_split;
   if (ns < -1) {
     int64_t most = max_keys >= 0 ? std::min(max_keys, Lk) : Lk;
-    if (window > 0) most = std::min(most, window + sinks + Lq);
+    if (window > 0 && window < Lk && sinks < Lk) most = std::min(most, window + sinks + Lq);
     check_status(a, op, a.window_attn_plan(dims, most, &ns));
   }
   at::Tensor ws;

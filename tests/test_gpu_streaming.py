@@ -263,3 +263,72 @@ def test_units_of_every_length(dev, window, sinks):
         ref, rlse, tol, ltol = so.attention(q[n], k[0, :n], v[0, :n], seen, D ** -0.5, BF)
         _same(out[n], ref, tol, (n, "rows"))
         _same(lse[n], rlse, ltol, (n, "sums"))
+
+
+def test_calls_with_nothing_to_do(dev):
+    """No requests, no positions, no heads of channels: empty results or a refusal, and
+    nothing else written."""
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    plan = rotary_plan(64, device=dev)
+    x = torch.randn(2, 3, 4, 64, device=dev).to(BF)
+    pos = torch.arange(3, device=dev)
+    pages = torch.zeros(4, 16, 4, 64, device=dev, dtype=BF)
+    table = torch.zeros(2, 2, device=dev, dtype=torch.int32)
+    cache = ops.PagedCache(pages, pages.clone(), table)
+    q, k = ops.norm_rope(x[:0], x[:0], pos, plan)
+    assert q.shape == k.shape == (0, 3, 4, 64)
+    q, k = ops.norm_rope(x[:, :0], x[:, :0], pos[:0], plan, v=x[:, :0], cache=cache)
+    assert q.shape == (2, 0, 4, 64) and k is None and (pages == 0).all()
+    out, lse = ops.window_attention(x[:0], x[:0], x[:0], return_lse=True)
+    assert out.shape == (0, 3, 4, 64) and lse.shape == (0, 4, 3)
+    out = ops.paged_attention(x[:, :0], cache, _int(dev, 5, 5))
+    assert out.shape == (2, 0, 4, 64)
+    with pytest.raises(RuntimeError, match="no channels"):
+        ops.window_attention(x[..., :0], x[..., :0], x[..., :0])
+    with pytest.raises(ValueError):
+        ops.window_attention(x, x[:, :, :0], x[:, :, :0])
+    with pytest.raises(RuntimeError, match="no heads"):
+        ops.norm_rope(x, x[:, :, :0], pos, plan)
+
+
+def test_refusals_beside_a_cache(dev):
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    plan = rotary_plan(64, device=dev)
+    x = torch.randn(2, 3, 4, 64, device=dev).to(BF)
+    pos = torch.arange(3, device=dev)
+    pages = torch.zeros(4, 16, 4, 64, device=dev, dtype=BF)
+    table = torch.zeros(2, 2, device=dev, dtype=torch.int32)
+    cache = ops.PagedCache(pages, pages.clone(), table)
+    starts = _int(dev, 0, 0)
+    for kw, err in ((dict(v=x), ValueError), (dict(cache=cache), ValueError),
+                    (dict(starts=starts), ValueError),
+                    (dict(v=x, cache=cache, k_out=x.clone()), ValueError),
+                    (dict(v=x.float(), cache=cache), TypeError),
+                    (dict(v=x[:, :2], cache=cache), RuntimeError),
+                    (dict(v=x, cache=cache, starts=starts.long()), RuntimeError),
+                    (dict(v=x, cache=cache, starts=starts[:1]), RuntimeError),
+                    (dict(v=x, cache=cache._replace(table=table[:1])), RuntimeError),
+                    (dict(v=x, cache=cache._replace(k=pages[:, :, :2])), RuntimeError),
+                    (dict(v=x, cache=cache._replace(v=pages.half())), RuntimeError),
+                    (dict(lengths=starts.cpu()), RuntimeError)):
+        with pytest.raises(err):
+            ops.norm_rope(x, x, pos, plan, **kw)
+    assert (pages == 0).all()
+
+
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_limits_of_the_rule(dev, Lq):
+    """Windows, first keys and blocks past every position, up to 64 bits: all keys in order,
+    or a block's."""
+    from cast_amd import ops
+    g = torch.Generator().manual_seed(Lq)
+    q, k, v = (torch.randn(1, n, 2, 64, generator=g).to(BF).to(dev) for n in (Lq, 90, 90))
+    want = ops.window_attention(q, k, v)
+    for most in (90, 1 << 30, (1 << 63) - 1):
+        assert torch.equal(ops.window_attention(q, k, v, window=most), want)
+        assert torch.equal(ops.window_attention(q, k, v, window=most, sinks=most), want)
+        assert torch.equal(ops.window_attention(q, k, v, window=5, sinks=most), want)
+        assert torch.equal(ops.window_attention(q, k, v, block=most),
+                           ops.window_attention(q, k, v, causal=False))
