@@ -28,9 +28,10 @@ struct RotaryArgs {
   const int32_t* table;       // [B][max_pages] pages of every request's cache
   int64_t table_stride, max_pages, n_pages, page_size;
   const int32_t *starts, *lengths;
+  Divisor by_L, by_page;
   // the vector form's launch: tokens of a workgroup, lanes of a head (log2), divisors
   int tokens, lanes_log2;
-  Divisor by_heads, by_L, by_pairs;  // by_heads: Hq + Hk + Hv
+  Divisor by_heads, by_pairs;  // by_heads: Hq + Hk + Hv
 };
 
 }  // namespace rcsa

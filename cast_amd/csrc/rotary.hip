@@ -55,30 +55,47 @@ __device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int64_t b, int64_
 }
 
 // What a token's rows are: live or not, and where its keys and values go
-// (element offsets of the row, -1: dropped).
+// (element offsets of the row, -1: dropped).  In three steps, each of which waits for the one
+// before: its request's lengths, its page, its rows.
+struct TokenAt {
+  int b, t, length, start;
+};
+__device__ __forceinline__ TokenAt token_at(const RotaryArgs& a, int token) {
+  TokenAt r;
+  r.b = divide(token, a.by_L);
+  r.t = token - r.b * static_cast<int>(a.L);
+  r.length = a.lengths == nullptr ? static_cast<int>(a.L) : a.lengths[r.b];
+  r.start = a.starts == nullptr ? 0 : a.starts[r.b];
+  return r;
+}
+// Index of the token's keys in its request's pages (-1: none, or dropped) and their page.
+struct TokenPage {
+  int at, page;
+};
+__device__ __forceinline__ TokenPage token_page(const RotaryArgs& a, const TokenAt& r) {
+  if (a.table == nullptr) return {-1, -1};
+  const int64_t at = static_cast<int64_t>(r.start) + r.t;
+  if (r.t >= r.length || at < 0 || at >= a.max_pages * a.page_size) return {-1, -1};
+  const int i = static_cast<int>(at);
+  return {i, a.table[r.b * a.table_stride + divide(i, a.by_page)]};
+}
 struct TokenRows {
-  int64_t b, t, q, k, v;
+  int64_t q, k, v;
   bool live;
 };
-__device__ __forceinline__ TokenRows token_rows(const RotaryArgs& a, int64_t token) {
+__device__ __forceinline__ TokenRows token_rows(const RotaryArgs& a, const TokenAt& p,
+                                                const TokenPage& g) {
   TokenRows r;
-  r.b = token / a.L;
-  r.t = token - r.b * a.L;
-  r.live = a.lengths == nullptr || r.t < a.lengths[r.b];
-  r.q = r.b * a.qo[0] + r.t * a.qo[1];
-  r.k = r.b * a.ko[0] + r.t * a.ko[1];
+  r.live = p.t < p.length;
+  r.q = p.b * a.qo[0] + p.t * a.qo[1];
+  r.k = p.b * a.ko[0] + p.t * a.ko[1];
   r.v = -1;
   if (a.table != nullptr) {
     r.k = -1;
-    const int64_t at = (a.starts == nullptr ? 0 : static_cast<int64_t>(a.starts[r.b])) + r.t;
-    if (r.live && at >= 0 && at < a.max_pages * a.page_size) {
-      const int64_t col = at / a.page_size;
-      const int64_t page = a.table[r.b * a.table_stride + col];
-      if (page >= 0 && page < a.n_pages) {
-        const int64_t slot = at - col * a.page_size;
-        r.k = page * a.ko[0] + slot * a.ko[1];
-        r.v = page * a.vo[0] + slot * a.vo[1];
-      }
+    if (g.page >= 0 && g.page < a.n_pages) {
+      const int64_t slot = g.at - divide(g.at, a.by_page) * static_cast<int>(a.page_size);
+      r.k = g.page * a.ko[0] + slot * a.ko[1];
+      r.v = g.page * a.vo[0] + slot * a.vo[1];
     }
   }
   return r;
@@ -169,24 +186,38 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
       }
     }
   };
+  // The first wavefronts take the sines, the second (of one: the only) the weights, the last the
+  // places of the tokens' rows, whose lengths are asked for ahead of the rows: the loads of
+  // a small call are its time.
+  const int wave = uniform_int(tid >> 6), last = (threads >> 6) - 1;
+  TokenAt at{};
+  if (wave == last) at = token_at(a, token0 + ((tid & 63) < left ? tid & 63 : 0));
   load(0);
-
+  TokenPage page{};
+  if (wave == last) page = token_page(a, at);
+  if (NORM && (last == 0 || wave == 1))  // (weights of a head's own: where they are used)
+    for (int i = tid & 63; i < 2 * a.D / V; i += kWave) {
+      const bool key = i * V >= a.D;
+      const void* const w = key ? a.kw : a.qw;
+      float f[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = 1.0f;
+      if (w != nullptr && (key ? a.kw_h : a.qw_h) == 0)
+        weight_run<V>(w, a.w_dtype, i * V - (key ? a.D : 0), f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s_w[i * V + j] = f[j];
+    }
   for (int i = tid; i < left * np; i += threads) {
     const int tl = divide(i, a.by_pairs), token = token0 + tl, b = divide(token, a.by_L);
     const float2 cs = turn_of(a, b, token - b * static_cast<int>(a.L), i - tl * np);
     s_cos[i] = cs.x;
     s_sin[i] = cs.y;
   }
-  if (NORM && (a.qw_h == 0 || a.kw_h == 0))  // shared by the heads (others: where used)
-    for (int i = tid; i < 2 * a.D; i += threads) {
-      const void* w = i < a.D ? a.qw : a.kw;
-      s_w[i] = w == nullptr ? 1.0f : weight_at(w, a.w_dtype, i < a.D ? i : i - a.D);
-    }
-  if (tid < left) {
-    const TokenRows r = token_rows(a, token0 + tid);
-    s_dst[0][tid] = r.live ? r.q : -1;
-    s_dst[1][tid] = r.live ? r.k : -1;
-    s_dst[2][tid] = r.live ? r.v : -1;
+  if (wave == last && (tid & 63) < left) {
+    const TokenRows r = token_rows(a, at, page);
+    s_dst[0][tid & 63] = r.live ? r.q : -1;
+    s_dst[1][tid & 63] = r.live ? r.k : -1;
+    s_dst[2][tid & 63] = r.live ? r.v : -1;
   }
   __syncthreads();
 
@@ -324,16 +355,17 @@ __global__ void __launch_bounds__(64) rotary_any_kernel(RotaryArgs a) {
   const int lane = threadIdx.x;
   const int64_t token = blockIdx.x;
   const int part = blockIdx.y, np = a.n_pairs;
-  const TokenRows r = token_rows(a, token);
+  const TokenAt tok = token_at(a, static_cast<int>(token));
+  const TokenRows r = token_rows(a, tok, token_page(a, tok));
   const int64_t dst = part == 0 ? r.q : part == 1 ? r.k : r.v;
   if (!r.live || dst < 0) return;  // (the whole wavefront)
   if (part < 2)
-    for (int i = lane; i < np; i += kWave) s_cs[i] = turn_of(a, r.b, r.t, i);
+    for (int i = lane; i < np; i += kWave) s_cs[i] = turn_of(a, tok.b, tok.t, i);
   __syncthreads();
   const int64_t* const in = part == 0 ? a.qs : part == 1 ? a.ks : a.vs;
   const int64_t* const on = part == 0 ? a.qo : part == 1 ? a.ko : a.vo;
   const T* const src = static_cast<const T*>(part == 0 ? a.q : part == 1 ? a.k : a.v) +
-                       r.b * in[0] + r.t * in[1];
+                       tok.b * in[0] + tok.t * in[1];
   T* const out = static_cast<T*>(part == 0 ? a.qout : part == 1 ? a.kout : a.vout) + dst;
   const int H = part == 0 ? a.Hq : part == 1 ? a.Hk : a.Hv;
   const void* const w = part == 0 ? a.qw : a.kw;
@@ -414,7 +446,6 @@ static int launch_runs(RotaryArgs& a, hipStream_t s) {
   if (bytes() > (60 << 10)) return RCSA_ERR_SHAPE;
   a.tokens = static_cast<int>(nt);
   a.by_heads = divisor(static_cast<uint32_t>(nh));
-  a.by_L = divisor(static_cast<uint32_t>(a.L));
   a.by_pairs = divisor(a.n_pairs > 0 ? static_cast<uint32_t>(a.n_pairs) : 1u);
   const int64_t grid = (total + nt - 1) / nt;
   const int64_t rounds = (nt * per + 255) / 256;
@@ -430,6 +461,8 @@ static int launch_runs(RotaryArgs& a, hipStream_t s) {
 template <typename T, bool INTER, int NORM>
 static int launch(RotaryArgs& a, hipStream_t s) {
   if (a.B * a.L >= (1ll << 30)) return RCSA_ERR_SHAPE;
+  a.by_L = divisor(static_cast<uint32_t>(a.L));
+  if (a.table) a.by_page = divisor(static_cast<uint32_t>(a.page_size));
   constexpr int W = kWide<T>;
   if (runs_of<T>(a, W, INTER)) return launch_runs<T, W, INTER, NORM>(a, s);
   if (runs_of<T>(a, 2, INTER)) return launch_runs<T, 2, INTER, NORM>(a, s);
@@ -523,7 +556,7 @@ extern "C" int rcsa_norm_rope(const void* q, const void* k, const void* v, void*
       dims[4] > kMaxDim || n_pairs > kMaxDim || n_axes > kMaxDim)
     return RCSA_ERR_SHAPE;
   if (block_table && (max_pages <= 0 || n_pages <= 0 || page_size <= 0 ||
-                      max_pages > (1ll << 40) / page_size))
+                      max_pages >= (1ll << 31) / page_size))
     return RCSA_ERR_SHAPE;
   RotaryArgs a{};
   a.q = q;
