@@ -9,9 +9,10 @@
 //
 // HBM-bound: each element is read once, written once, and rounded once (fp32
 // between).  44 frames x 24 heads of 128 80 us, 5.9 TB/s; with joint norms and the append to
-// pages 3520 x 72 heads 35 us, 3.7 TB/s (a token's sums stand between its loads and its
-// stores, and 130 MB are few beside a launch's start and end); 32782 x 20 heads of 64 with
-// norms of heads 42 us, 3.9 TB/s; one token of a few requests 4.4 us, a launch.  A position times a frequency needs more than 24 bits once the
+// pages 3520 x 72 heads 34 us, 3.8 TB/s (a token's sums stand between its loads and its
+// stores, and 130 MB are few beside a launch's start and end); with norms of heads 16391 x 48
+// heads of 128 71 us, 5.7 TB/s, 32782 x 20 heads of 64 40 us, 4.2 TB/s; one token of 8
+// requests 3.6 us, with norms and pages of 64 requests 5.7 us: a launch and its loads.  A position times a frequency needs more than 24 bits once the
 // positions are far (at position 10^6 an fp32 angle is off by 0.06), so the
 // angle is a product in turns in 64 bits, reduced to [-1/2, 1/2] turns there,
 // and only then fp32: exact to an fp32 rounding at any position, with no table
@@ -116,8 +117,9 @@ __device__ __forceinline__ TokenRows token_rows(const RotaryArgs& a, const Token
 template <typename T>
 constexpr int kWide = 16 / static_cast<int>(sizeof(T));
 // Entries of a thread.  Wide runs: two for the rotation alone (44 frames x 24 heads 80 us, one
-// 89), one with norms of heads (16391 tokens x 48 heads 82 us, two 90), three with
-// joint norms, which the list of a token should fit (3520 x 72 heads 35 us, two 43); narrow
+// 89), one with norms of heads (16391 tokens x 48 heads 71 us, two 75, three 79), three with
+// joint norms, which the list of a token should fit (3520 x 72 heads 34 us, two 42, four 38, five
+// 34; 9000 x 40 heads 51, 50, 51, 50; 3520 x 48 heads fp32 36, 41, 40, 43); narrow
 // runs six (14097 x 9 heads of 80 57 us, four 61).
 template <int V, int NORM>
 constexpr int kEntries = V == 2 ? 6 : (NORM == 0 ? 2 : (NORM == 1 ? 1 : 3));

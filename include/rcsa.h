@@ -712,8 +712,9 @@ int rcsa_int8_linear_group(const int8_t* x, const float* x_scale, int64_t n_line
  * [B][L][Hk][D] is copied beside the keys, and token t of request b goes to index
  * at = starts[b] + t (starts NULL: t), row at % page_size of page
  * block_table[b * table_stride + at / page_size]; a row whose page is not in
- * [0, n_pages), or past max_pages, is dropped.  No row may appear twice.  lengths
- * (nullable, int32 [B]): rows of tokens t >= lengths[b] are left as they were.
+ * [0, n_pages), or past max_pages, is dropped (max_pages * page_size below 2^31).  No row
+ * may appear twice.  lengths (nullable, int32 [B]): rows of tokens t >= lengths[b] are left
+ * as they were.
  */
 int rcsa_rope(const void* x, void* out, int dtype, int64_t batch, int64_t len, int64_t heads,
               int64_t head_dim, const int64_t* strides, const void* positions, int positions_i64,

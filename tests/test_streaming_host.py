@@ -80,6 +80,33 @@ def test_rope_abi_refusals(lib, kw, status):
     assert _rope(lib, **kw) == status
 
 
+def _norm(lib, q=4096, k=4096, v=None, q_out=4096, k_out=4096, v_out=None, dtype=0,
+          dims=(1, 2, 2, 2, 64), weight=None, w_dtype=0, pos=4096, n_axes=1, turns=4096, n_pairs=32,
+          table=None, max_pages=0, n_pages=0, page=0):
+    return lib.rcsa_norm_rope(q, k, v, q_out, k_out, v_out, dtype, _arr(*dims),
+                              _arr(*(256, 128, 64) * 6), weight, weight, w_dtype, 0, 0, 1e-6, 0,
+                              pos, 0, _arr(0, 1, 0), n_axes, turns, None, n_pairs, 0, 1.0, table,
+                              1, max_pages, n_pages, page, None, None, None)
+
+
+PAGES = dict(v=4096, v_out=4096, table=4096, max_pages=4, n_pages=9, page=16)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(q=None), NULL), (dict(k=None), NULL), (dict(q_out=None), NULL), (dict(k_out=None), NULL),
+    (dict(pos=None), NULL), (dict(turns=None), NULL), (dict(v=4096), NULL),
+    (dict(v_out=4096), NULL), (dict(table=4096), NULL), (dict(PAGES, table=None), NULL),
+    (dict(dtype=7), DTYPE), (dict(w_dtype=7), DTYPE), (dict(dims=(0, 2, 2, 2, 64)), SHAPE),
+    (dict(dims=(1, 0, 2, 2, 64)), SHAPE), (dict(dims=(1, 2, 0, 2, 64)), SHAPE),
+    (dict(dims=(1, 2, 2, 0, 64)), SHAPE), (dict(dims=(1, 2, 2, 5000, 64)), SHAPE),
+    (dict(dims=(1, 2, 2, 2, 513)), SHAPE), (dict(dims=(1 << 20, 1 << 20, 2, 2, 64)), SHAPE),
+    (dict(n_pairs=33), SHAPE), (dict(n_axes=0), SHAPE), (dict(PAGES, max_pages=0), SHAPE),
+    (dict(PAGES, n_pages=0), SHAPE), (dict(PAGES, page=0), SHAPE),
+    (dict(PAGES, max_pages=1 << 20, page=1 << 11), SHAPE)])
+def test_norm_abi_refusals(lib, kw, status):
+    assert _norm(lib, **kw) == status
+
+
 def _window(lib, q=4096, k=4096, out=4096, dtype=0, dims=(1, 4, 8, 2, 1, 64),
             strides=(512, 128, 64, 512, 64, 64, 512, 64, 64, 512, 128, 64), table=None, ts=1,
             max_pages=0, n_pages=0, page=0, window=0, sinks=0, block=1, n_split=1, ws=None,
