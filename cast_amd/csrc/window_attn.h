@@ -67,14 +67,19 @@ __device__ __forceinline__ KeyRange key_range(A& a, int p, int k_len) {
   return {lo < hi ? lo : hi, hi};
 }
 
-// A request's lengths, clamped to the storage.
+// A request's lengths, clamped to the storage; UNIFORM: of one request for the wavefront, by
+// scalar loads.
 struct Request {
   int k_len, q_len;
 };
+template <bool UNIFORM = false>
 __device__ __forceinline__ Request request_of(const WindowArgs& a, int b) {
   const int cap = a.table != nullptr ? a.max_pages * a.page : a.Lk;
-  int k = a.k_len == nullptr ? cap : a.k_len[b];
-  int q = a.q_len == nullptr ? a.Lq : a.q_len[b];
+  auto at = [&](const int32_t* p) __attribute__((always_inline)) -> int {
+    return UNIFORM ? ld_const(p + b) : p[b];
+  };
+  int k = a.k_len == nullptr ? cap : at(a.k_len);
+  int q = a.q_len == nullptr ? a.Lq : at(a.q_len);
   k = k < 0 ? 0 : (k > cap ? cap : k);
   q = q < 0 ? 0 : (q > a.Lq ? a.Lq : q);
   return {k, q};
@@ -164,7 +169,8 @@ template <bool OF_REQUEST>
 __device__ __forceinline__ Unit find_unit(const WindowArgs& a, int w, int lane) {
   if (a.B <= kWave) {  // one load of the lengths (a single request needs no lanes' sums)
     Request r{0, 0};
-    if (lane < a.B) r = request_of(a, lane);
+    if (a.B == 1) r = request_of<true>(a, 0);
+    else if (lane < a.B) r = request_of(a, lane);
     const int tiles = lane < a.B ? request_tiles(a, r) : -1;
     const int mine = tiles > 0 ? tiles : 0;
     const int chunk = chunk_of(a, a.B == 1 ? uniform_int(mine) : uniform_int(lane_sum(mine)));

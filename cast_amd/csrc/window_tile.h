@@ -52,7 +52,7 @@ window_kernel(WindowArgs a) {
   if (it.bh < 0) return;
   p.b = divide(it.bh, a.by_Hk);
   p.hk = it.bh - p.b * a.Hk;
-  const Request rq = request_of(a, p.b);
+  const Request rq = request_of<true>(a, p.b);
   const int q_len = uniform_int(rq.q_len);
   p.k_len = uniform_int(rq.k_len);
   p.n_rows = q_len * a.G;
