@@ -5,7 +5,7 @@
 //
 // The keys and values are read once and bound the time, so what counts is bytes in
 // flight (48 ragged requests of up to 32768 keys in pages of 16, 32 heads on 8: 326 us,
-// 5.4 TB/s, and 10 us for the join; one token over 1024 of 2500 keys 7.5 and 4.6 us, the
+// 5.4 TB/s, and 10 us for the join; one token over 1024 of 2500 keys 7.5 and 4.1 us, the
 // latency of two launches): a wavefront holds the next tile (16 KB at D 128) in registers
 // while it works on the one in its own LDS, eight wavefronts to a compute unit, no
 // barriers.  The loop is one tile long: a unit of a few tiles runs through little code that
