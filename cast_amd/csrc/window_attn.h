@@ -636,7 +636,7 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
   typedef typename Half<T>::op4 op4;
   const int hf = lane >> 5, lr = lane & 31;
   const float l = pair_sum(t.l_run), m = t.m_run;
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // (a NaN sum stays one)
+  const float inv = l > 0.0f ? 1.0f / l : l;  // (a NaN sum stays one)
   // a product that is no number, in a row whose sum is one
   bool bad = false;
 #pragma unroll
@@ -645,10 +645,11 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
     for (int r = 0; r < 16; ++r) bad = bad || !(fabsf(t.o_acc[dt][r]) < INFINITY);
   if (__ballot(bad && l > 0.0f && l < INFINITY) != 0)
     rows_again<T, D, PAGED>(a, p, t, lane, m == -INFINITY ? 0.0f : m, lds);
+  // (a select: a row that sees no key may hold 0 * inf of its neighbours' tiles)
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t.o_acc[dt][r] *= inv;
+    for (int r = 0; r < 16; ++r) t.o_acc[dt][r] = l == 0.0f ? 0.0f : t.o_acc[dt][r] * inv;
   const Row my = row_of(a, p, p.row0 + lr);
   if (my.live) {
     if (p.shares > 1) {

@@ -1,0 +1,86 @@
+"""``ops.window_attention`` and ``ops.paged_attention`` where rows, weights and shares come to
+their edges: rows that see no key beside values that are no numbers.
+
+Tolerances: the oracle's bound (see ``streaming_oracle.attention``)."""
+import pytest
+import torch
+
+from oracle import streaming_oracle as so
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+NAN, INF = float("nan"), float("inf")
+
+
+def _inputs(seed, B, Lq, Lk, Hq, Hk, D, dtype, dev):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(B, Lq, Hq, D, generator=g)
+    k = torch.randn(B, Lk, Hk, D, generator=g)
+    v = torch.randn(B, Lk, Hk, D, generator=g) + 0.5
+    return tuple(t.to(dtype).to(dev) for t in (q, k, v))
+
+
+def _within(got, ref, tol, what):
+    """Within the bound; NaN and infinities where the oracle has them."""
+    got = got.double()
+    off = (got - ref).abs()
+    same = (got == ref) | (torch.isnan(got) & torch.isnan(ref))
+    worst = torch.where(same, torch.zeros_like(off), off - tol)
+    worst = torch.nan_to_num(worst, nan=INF).max().item()
+    assert worst <= 0.0, f"{what}: {worst} past the bound"
+
+
+def _call(q, k, v, page, table, n_split, window, sinks, block, sm_scale):
+    """One request of q [1, Lq, Hq, D] over dense keys, or (page > 0) over pages of them whose
+    last page is filled up with NaN; n_split 0 and -1 are the forms of few rows."""
+    from cast_amd import _lib
+    n, Lk = k.shape[1], k.shape[1]
+    lens = None
+    if page:
+        M = max(1, -(-n // page))
+        pad = torch.full((1, M * page - n, *k.shape[2:]), NAN, dtype=k.dtype, device=k.device)
+        k, v = (torch.cat([t, pad], 1).view(M, page, *t.shape[2:]) for t in (k, v))
+        lens = torch.tensor([Lk], dtype=torch.int32, device=q.device)
+        if table is None:
+            table = torch.arange(M, dtype=torch.int32, device=q.device)[None]
+    return _lib.torch_ops().window_attention(
+        q, k, v, table if page else None, None, lens, window, sinks, block, sm_scale, True, None,
+        -2 if n_split is None else n_split, -1)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("page", [0, 16, 64])
+@pytest.mark.parametrize("Lq,Lk,window,sinks,block,n_split", [
+    (128, 10, 0, 0, 1, 1), (128, 64, 0, 0, 1, 1), (128, 64, 0, 0, 1, None), (300, 70, 0, 0, 1, 3),
+    (150, 70, 100, 0, 880, 1), (150, 70, 100, 0, 880, 2), (4, 70, 100, 0, 880, 0),
+    (4, 70, 100, 0, 880, -1), (10, 5, 0, 0, 1, 0), (10, 5, 0, 0, 1, -1), (1, 70, 32, 0, 128, 0)])
+def test_rows_without_keys_beside_no_numbers(dev, dtype, page, Lq, Lk, window, sinks, block,
+                                             n_split):
+    """Rows before the first key, or whose window lies behind the last one, give 0 and -inf,
+    whatever the values that their neighbours see, or the last tile holds."""
+    print("rows without keys", dtype, page, Lq, Lk, window, block, n_split, flush=True)
+    q, k, v = _inputs(Lq + Lk, 1, Lq, Lk, 2, 1, 64, dtype, dev)
+    v[0, Lk // 2, 0, 3], v[0, Lk - 1, 0, 9], v[0, 1, 0, 60] = INF, NAN, -INF
+    out, lse = _call(q, k, v, page, None, n_split, window, sinks, block, 0.125)
+    seen = so.visible(Lq, Lk, window, sinks, block, device=dev)
+    assert not seen.any(1).all()
+    ref, rlse, tol, ltol = so.attention(q[0], k[0], v[0], seen, 0.125, dtype)
+    _within(out[0], ref, tol, "rows")
+    _within(lse[0], rlse, ltol, "sums")
+
+
+@pytest.mark.parametrize("n_split", [None, 1, 2])
+def test_rows_of_hidden_pages_beside_no_numbers(dev, n_split):
+    """32 rows whose pages are all hidden, in a block whose last rows see an infinity."""
+    Lq, page, window = 128, 16, 16
+    q, k, v = _inputs(7, 1, Lq, Lq, 1, 1, 128, BF, dev)
+    v[0, 100, 0, 5], v[0, 3, 0, 6] = INF, NAN
+    table = torch.arange(Lq // page, dtype=torch.int32, device=dev)[None].contiguous()
+    table[0, 1:4] = -1
+    out, lse = _call(q, k, v, page, table, n_split, window, 0, 1, 0.1)
+    seen = so.visible(Lq, Lq, window, 0, 1, device=dev)
+    seen[:, page:4 * page] = False
+    assert not seen[32:64].any()
+    ref, rlse, tol, ltol = so.attention(q[0], k[0], v[0], seen, 0.1, BF)
+    _within(out[0], ref, tol, "rows")
+    _within(lse[0], rlse, ltol, "sums")
