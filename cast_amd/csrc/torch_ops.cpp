@@ -985,8 +985,7 @@ std::vector<at::Tensor> norm_rope(
       TORCH_CHECK(!any || (*w)->scalar_type() == w_dt, op, ": the weights must share a dtype");
       any = true;
       w_dt = (*w)->scalar_type();
-      TORCH_CHECK((*w)->is_contiguous() && (*w)->numel() % D == 0 &&
-                      ((*w)->numel() == D || (*w)->numel() == H * D), op,
+      TORCH_CHECK((*w)->is_contiguous() && ((*w)->numel() == D || (*w)->numel() == H * D), op,
                   ": a weight must be contiguous [D] or [H, D]");
       ws[i] = (*w)->numel() == D ? 0 : D;
     }
