@@ -682,6 +682,12 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
   }
 }
 
+// acc += w o in a join: the weight of a share far below the row's maximum underflows to 0,
+// which must not turn an infinity that the row sees into 0 * inf.
+__device__ __forceinline__ float join(float w, float o, float acc) {
+  return fmaf(w == 0.0f && !(fabsf(o) < INFINITY) ? 1.0f : w, o, acc);
+}
+
 // Blocks of 128 rows over pages (window_paged.hip); type 0: bf16, 1: fp16.
 void launch_window_paged(WindowArgs& a, int type, int64_t D, dim3 grid, hipStream_t s);
 // Few rows (window_units.hip): in units and their join, or one workgroup a key head

@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) window_merge_kernel(WindowArgs a) {
     float o[8];
     Vec8<float>::load(a.ws_o + (s * all_rows + wrow) * D + c * 8, o);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, o[j], acc[j]);
+    for (int j = 0; j < 8; ++j) acc[j] = join(w, o[j], acc[j]);
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
   typename Half<T>::op8 r;

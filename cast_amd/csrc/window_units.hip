@@ -138,7 +138,7 @@ window_unit_kernel(WindowArgs a) {
       sum += f;
       const v4f o = *reinterpret_cast<const v4f*>(tiles[s] + (row * D + c) * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, o[e], acc[e]);
+      for (int e = 0; e < 4; ++e) acc[e] = join(f, o[e], acc[e]);
     }
     const Row r = row_of(a, p, row);
     typename Half<T>::op4 out;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
     const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
     sum += w;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = fmaf(w, ov[j], acc[j]);
+    for (int j = 0; j < 8; ++j) acc[j] = join(w, ov[j], acc[j]);
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) s_acc[g][c * 8 + j] = acc[j];

@@ -1,5 +1,5 @@
 """``ops.window_attention`` and ``ops.paged_attention`` where rows, weights and shares come to
-their edges: rows that see no key beside values that are no numbers.
+their edges: rows that see no key beside values that are no numbers, shares whose weight underflows.
 
 Tolerances: the oracle's bound (see ``streaming_oracle.attention``)."""
 import pytest
@@ -82,5 +82,24 @@ def test_rows_of_hidden_pages_beside_no_numbers(dev, n_split):
     seen[:, page:4 * page] = False
     assert not seen[32:64].any()
     ref, rlse, tol, ltol = so.attention(q[0], k[0], v[0], seen, 0.1, BF)
+    _within(out[0], ref, tol, "rows")
+    _within(lse[0], rlse, ltol, "sums")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("page", [0, 48])
+@pytest.mark.parametrize("Lq,n_split", [
+    (40, 1), (40, 2), (40, 5), (4, 1), (4, 3), (4, 0), (4, -1), (4, None)])
+def test_infinities_in_a_share_of_no_weight(dev, dtype, page, Lq, n_split):
+    """The first half of the keys stands e^-256 below the second: its finite values vanish,
+    its infinities and NaN reach every row, however the keys are shared."""
+    Lk, D = 700, 64
+    q, k, v = _inputs(Lq, 1, Lq, Lk, 2, 1, D, dtype, dev)
+    q[..., 0], k[:, :350, :, 0], k[:, 350:, :, 0] = 8.0, -16.0, 16.0
+    v[0, 3, 0, 7], v[0, 40, 0, 9], v[0, 340, 0, 11], v[0, 5, 0, 20] = INF, NAN, -INF, 60000.0
+    out, lse = _call(q, k, v, page, None, n_split, 0, 0, 1, 1.0)
+    seen = so.visible(Lq, Lk, 0, 0, 1, device=dev)
+    ref, rlse, tol, ltol = so.attention(q[0], k[0], v[0], seen, 1.0, dtype)
+    assert torch.isinf(ref[..., 7]).all() and torch.isnan(ref[..., 9]).all()
     _within(out[0], ref, tol, "rows")
     _within(lse[0], rlse, ltol, "sums")
