@@ -219,6 +219,7 @@ template <>
 struct Half<__bf16> {
   typedef v8bf op8;
   typedef v4bf op4;
+  static constexpr int kShift = 0;  // (fp32's range)
   static __device__ __forceinline__ v16f mfma(op8 x, op8 y, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
   }
@@ -230,6 +231,7 @@ template <>
 struct Half<_Float16> {
   typedef v8hf op8;
   typedef v4hf op4;
+  static constexpr int kShift = 7;  // (a term: at most 2^(kTau + kShift) = 2^15)
   static __device__ __forceinline__ v16f mfma(op8 x, op8 y, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
   }
@@ -343,8 +345,11 @@ __device__ __forceinline__ HalfRows half_rows(A& a, const Step& s, int half,
 // 32 rows against staged tiles of 32 keys: S^T = K Q^T puts a query row in a lane (its
 // 16 + 16 keys in the two lane halves), so a row's maximum and sum need one lane swap,
 // and P^T is the second operand of O^T = V^T P^T as it stands.  The running maximum moves
-// only when a term passes 2^kTau.  P is rounded to the type for its product, the sums
-// keep fp32.
+// only when a term passes 2^kTau.  P is rounded to the type for its product (half a step of
+// a weight; fp32 products have a sixteenth of the rate), the sums keep fp32.
+// m_run stands kShift below the running maximum, so that terms, sums and products carry a
+// factor 2^kShift: fp16 keeps all bits of weights down to 2^-21 of the largest and some down
+// to 2^-32 (without it 2^-14 and 2^-25: 2^18 keys at 2^-25.2 lost all of their 0.7%).
 template <typename T, int D>
 struct RowTile {
   using O = Half<T>;
@@ -429,12 +434,12 @@ struct RowTile {
     };
     // (a lane's partial sum bounds its terms)
     float part = exps();
-    if (__ballot(m_run == -INFINITY || !(part <= kTauPow)) != 0) {
+    if (__ballot(m_run == -INFINITY || !(part <= kTauPow * (1 << O::kShift))) != 0) {
       float rmax = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
       rmax = pair_max(rmax);
-      const float m_blk = rmax == -INFINITY ? -INFINITY : rmax * c;
+      const float m_blk = rmax == -INFINITY ? -INFINITY : rmax * c - O::kShift;
       if (__ballot(m_blk > m_run + kTau) != 0) {
         const float m_new = fmaxf(m_run, m_blk);
         const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);

@@ -80,14 +80,14 @@ def visible(q_len, k_len, window, sinks, block, causal=True, device="cpu"):
     return (j < e) & (near | (j < sinks)) & (p[:, None] >= 0)
 
 
-def attention(q, k, v, seen, sm_scale, dtype):
+def attention(q, k, v, seen, sm_scale, dtype, weight_step=None):
     """q [Lq, H, D], k, v [Lk, Hk, D], seen [Lq, Lk].  Returns out [Lq, H, D], lse [H, Lq]
     and their bounds.  Keys and values that a row does not see do not enter.
 
     The bound of an output: its rounding; the rounding of every weight to the type (half a
-    step of sum p |v|, and the type's least step a key); a logit's fp32 error e_s (D + 2
-    roundings of its products), twice, in the weights; 2^-16 for the exponentials and the
-    sums."""
+    step of sum p |v|, and the type's least step a key, or `weight_step` of the largest
+    weight); a logit's fp32 error e_s (D + 2 roundings of its products), twice, in the
+    weights; 2^-16 for the exponentials and the sums."""
     Lq, H, D = q.shape
     Lk, Hk, _ = k.shape
     g = H // Hk
@@ -121,7 +121,8 @@ def attention(q, k, v, seen, sm_scale, dtype):
         out[:, h] = torch.where(some[:, None], o, torch.zeros_like(o))
         tol[:, h] = (o.abs() * HALF_STEP[dtype] + TINY[dtype]
                      + mass * (HALF_STEP[dtype] + 2 * e_s + 2.0 ** -16)
-                     + n * 2 * TINY[dtype] * clean.abs().amax(0, keepdim=True))
+                     + n * (2 * TINY[dtype] if weight_step is None else weight_step * p.amax(
+                         1, keepdim=True)) * clean.abs().amax(0, keepdim=True))
         lse[h] = row[:, 0]
         lse_tol[h] = e_s[:, 0] + 2.0 ** -18 * (1 + row[:, 0].abs())
     return out, lse, tol, lse_tol

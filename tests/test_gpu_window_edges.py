@@ -1,5 +1,6 @@
 """``ops.window_attention`` and ``ops.paged_attention`` where rows, weights and shares come to
-their edges: rows that see no key beside values that are no numbers, shares whose weight underflows.
+their edges: rows that see no key beside values that are no numbers, shares whose weight underflows,
+weights far below the largest.
 
 Tolerances: the oracle's bound (see ``streaming_oracle.attention``)."""
 import pytest
@@ -103,3 +104,30 @@ def test_infinities_in_a_share_of_no_weight(dev, dtype, page, Lq, n_split):
     assert torch.isinf(ref[..., 7]).all() and torch.isnan(ref[..., 9]).all()
     _within(out[0], ref, tol, "rows")
     _within(lse[0], rlse, ltol, "sums")
+
+
+@pytest.mark.parametrize("tail", [22.5, 25.2])
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("page,Lq,n_split", [
+    (0, 40, 1), (0, 40, 8), (64, 40, 2), (0, 1, 0), (64, 1, 0), (0, 1, -1), (64, 1, None)])
+def test_many_small_weights(dev, page, Lq, n_split, odd, tail):
+    """fp16: one key and 2^16 others at 2^-22.5 or 2^-25.2 of its weight, which together are a
+    part of the result: their weights keep the bits down to 2^-32 of the largest.  ``odd``:
+    beside an infinity, whose rows are taken again.
+
+    The bound: a weight's least step, half of fp16's 2^-24 at a factor of 2^7, 2^-32 of the
+    largest; the sums of up to 2048 tiles in fp32, a rounding a tile of the row's sum and two of
+    its products, 3 * 2048 * 2^-24 of the result."""
+    Lk, D = 1 + (1 << 16), 64
+    g = torch.Generator().manual_seed(Lq)
+    q, k = (torch.zeros(1, n, 1, D, device=dev, dtype=HF) for n in (Lq, Lk))
+    v = (1.0 + 0.1 * torch.randn(1, Lk, 1, D, generator=g)).to(HF).to(dev)
+    q[..., 0], k[:, 0, :, 0], v[:, 0] = 1.0, tail * 0.6931471805599453, 0.0
+    if odd:
+        v[0, 4000, 0, 17] = INF
+    out, lse = _call(q, k, v, page, None, n_split, 0, 0, 1, 1.0)
+    seen = so.visible(Lq, Lk, 0, 0, 1, device=dev)
+    ref, rlse, tol, ltol = so.attention(q[0], k[0], v[0], seen, 1.0, HF, weight_step=2.0 ** -32)
+    steps = 2049 * 2.0 ** -24
+    _within(out[0], ref, tol + 3 * steps * ref.abs(), "rows")
+    _within(lse[0], rlse, ltol + steps, "sums")
