@@ -102,6 +102,17 @@ __device__ __forceinline__ TokenRows token_rows(const RotaryArgs& a, const Token
   return r;
 }
 
+// A launch's workgroups lie in even rows of at most 2^16 (a dimension holds less than 2^32
+// threads); the few that even rows add have nothing to do.
+static dim3 grid_of(int64_t workgroups, int parts = 1) {
+  const int64_t rows = (workgroups + 65535) / 65536;
+  return dim3(static_cast<unsigned>((workgroups + rows - 1) / rows), static_cast<unsigned>(rows),
+              static_cast<unsigned>(parts));
+}
+__device__ __forceinline__ int workgroup_index() {
+  return static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x);
+}
+
 // The vector form.  A lane holds two runs of V channels of a head: V pairs of the half
 // layout, or 2 V / 2 interleaved ones; `lanes` = a power of two >= D / 2V lanes a head.  A
 // workgroup takes `tokens` tokens; its threads run over their (token, head) list, queries,
@@ -142,7 +153,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryArgs a) {
   __shared__ int64_t s_dst[3][kMaxTokens];
   const int tid = threadIdx.x, threads = blockDim.x;
   const int total = static_cast<int>(a.B * a.L);
-  const int token0 = static_cast<int>(blockIdx.x) * nt;
+  const int token0 = workgroup_index() * nt;
+  if (token0 >= total) return;
   const int left = total - token0 < nt ? total - token0 : nt;  // tokens of this workgroup
 
   const int lanes = 1 << a.lanes_log2;
@@ -355,9 +367,10 @@ template <typename T, bool INTER, int NORM>
 __global__ void __launch_bounds__(64) rotary_any_kernel(RotaryArgs a) {
   __shared__ float2 s_cs[kMaxDim / 2];
   const int lane = threadIdx.x;
-  const int64_t token = blockIdx.x;
-  const int part = blockIdx.y, np = a.n_pairs;
-  const TokenAt tok = token_at(a, static_cast<int>(token));
+  const int token = workgroup_index();
+  if (token >= static_cast<int>(a.B * a.L)) return;
+  const int part = blockIdx.z, np = a.n_pairs;
+  const TokenAt tok = token_at(a, token);
   const TokenRows r = token_rows(a, tok, token_page(a, tok));
   const int64_t dst = part == 0 ? r.q : part == 1 ? r.k : r.v;
   if (!r.live || dst < 0) return;  // (the whole wavefront)
@@ -452,8 +465,7 @@ static int launch_runs(RotaryArgs& a, hipStream_t s) {
   const int64_t grid = (total + nt - 1) / nt;
   const int64_t rounds = (nt * per + 255) / 256;
   const int64_t threads = ((nt * per + rounds - 1) / rounds + kWave - 1) / kWave * kWave;
-  rotary_kernel<T, V, INTER, NORM><<<dim3(static_cast<unsigned>(grid)),
-                                     dim3(static_cast<unsigned>(threads)),
+  rotary_kernel<T, V, INTER, NORM><<<grid_of(grid), dim3(static_cast<unsigned>(threads)),
                                      static_cast<unsigned>(bytes()), s>>>(a);
   return launch_status();
 }
@@ -469,7 +481,7 @@ static int launch(RotaryArgs& a, hipStream_t s) {
   if (runs_of<T>(a, W, INTER)) return launch_runs<T, W, INTER, NORM>(a, s);
   if (runs_of<T>(a, 2, INTER)) return launch_runs<T, 2, INTER, NORM>(a, s);
   rotary_any_kernel<T, INTER, NORM>
-      <<<dim3(static_cast<unsigned>(a.B * a.L), a.Hv ? 3 : a.Hk ? 2 : 1), dim3(kWave), 0, s>>>(a);
+      <<<grid_of(a.B * a.L, a.Hv ? 3 : a.Hk ? 2 : 1), dim3(kWave), 0, s>>>(a);
   return launch_status();
 }
 

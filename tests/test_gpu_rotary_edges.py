@@ -2,8 +2,15 @@
 import pytest
 import torch
 
+from oracle import streaming_oracle as so
+
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
+
+
+def _close(got, ref, tol, what):
+    worst = ((got.double() - ref).abs() - tol).max().item()
+    assert worst <= 0.0, f"{what}: {worst} past the bound"
 
 
 @pytest.mark.parametrize("shape", [(0,), (4, 0)])
@@ -19,3 +26,47 @@ def test_weights_of_no_channels(dev, shape):
     assert q.shape == k.shape == x.shape
     with pytest.raises(RuntimeError, match="weight"):
         ops.norm_rope(x, x, pos, plan, q_weight=torch.ones(3, device=dev, dtype=BF))
+
+
+@pytest.mark.parametrize("D,H,L", [
+    (3, 1, (1 << 26) + 77),   # element by element, a workgroup a token, past 2^32 threads
+    (128, 80, 65537 + 9),     # 16-byte runs, a workgroup a token, past one row of the grid
+    (6, 3, 65537 * 16 + 5)])  # runs of two
+def test_grids_of_many_tokens(dev, D, H, L):
+    """Every token is turned, wherever its workgroup lies in the grid."""
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    print("many tokens", D, H, L, flush=True)
+    R = D // 2 * 2
+    plan, (freq, axis) = rotary_plan(R, device=dev), so.frequencies(R)
+    x = torch.empty(1, L, H, D, device=dev, dtype=BF)
+    for i in range(0, L, 1 << 22):  # (pieces: the random numbers are fp32)
+        x[:, i:i + (1 << 22)] = torch.randn(x[:, i:i + (1 << 22)].shape, device=dev)
+    pos = torch.arange(L, device=dev, dtype=torch.int32)
+    out = torch.full_like(x, float("nan"))
+    assert ops.rope(x, pos, plan, out=out).data_ptr() == out.data_ptr()
+    assert not torch.isnan(out).any()
+    for i in sorted({0, 65500 % L, (1 << 16) % L, L // 2, max(0, (1 << 26) - 50) % L, L - 100}):
+        s = slice(i, i + 100)
+        ref, size = so.rope(x[:, s], pos[s], freq, axis, False)
+        _close(out[:, s], ref, so.rope_bound(ref, size, BF), i)
+
+
+@pytest.mark.parametrize("D,Hq,Hk", [(128, 12, 6), (5, 2, 1)])
+def test_norms_of_many_tokens(dev, D, Hq, Hk):
+    """Norms, keys and values of more tokens than a row of the grid holds: pages filled to
+    the last token."""
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    L, page = 65537 + 20, 64
+    R, M = D // 2 * 2, -(-(65537 + 20) // 64)
+    plan, (freq, axis) = rotary_plan(R, device=dev), so.frequencies(R)
+    q, k, v = (torch.randn(1, L, h, D, device=dev).to(BF) for h in (Hq, Hk, Hk))
+    kp, vp = (torch.full((M, page, Hk, D), float("nan"), device=dev, dtype=BF) for _ in range(2))
+    table = torch.arange(M, dtype=torch.int32, device=dev)[None].contiguous()
+    pos = torch.arange(L, device=dev)
+    qo, _ = ops.norm_rope(q, k, pos, plan, v=v, cache=ops.PagedCache(kp, vp, table))
+    assert torch.equal(vp.view(-1, Hk, D)[:L], v[0])
+    for got, x in ((qo, q), (kp.view(1, -1, Hk, D)[:, :L], k)):
+        ref, size = so.rope(so.norm(x, None, 1e-6, False), pos, freq, axis, False)
+        _close(got, ref, so.rope_bound(ref, size, BF, norm=True), (D, x.shape[2]))
