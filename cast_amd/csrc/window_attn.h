@@ -52,6 +52,7 @@ struct WindowArgs {
 constexpr int kFewRows = 32;        // rows of a key head that one wavefront takes
 constexpr int kMaxPlanned = 512;    // requests whose lengths every wavefront reads
 constexpr int kGroupWaves = 8;      // wavefronts of a workgroup that takes a key head
+constexpr int64_t kMaxThreads = 1ll << 32;  // a grid's dimension holds fewer
 
 // The keys of a position: [0, sink) and [lo, hi).
 struct KeyRange {

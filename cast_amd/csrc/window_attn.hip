@@ -54,7 +54,7 @@ template <typename T, int D>
 static int launch_window(WindowArgs& a, hipStream_t s) {
   const int64_t tail = a.xcd_items - a.xcd_whole;
   const int64_t wgs = (a.xcd_whole + tail * a.n_split) * kNumXcd;
-  if (wgs >= (1ll << 31)) return RCSA_ERR_SHAPE;
+  if (wgs * 256 >= kMaxThreads) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs));
   if (a.table) launch_window_paged(a, std::is_same<T, __bf16>::value ? 0 : 1, D, grid, s);
   else window_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
@@ -69,6 +69,13 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
 static int64_t row_blocks(int64_t Lq, int64_t G) { return (Lq * G + 127) / 128; }
 
 static bool few_rows(const int64_t* d) { return d[1] * (d[3] / d[4]) <= kFewRows; }
+// Whether few rows fit a launch of a workgroup a key head, or of units and their join.
+static bool group_fits(const int64_t* d) {
+  return few_rows(d) && d[0] * d[4] * (64 * kGroupWaves) < kMaxThreads;
+}
+static bool units_fit(const int64_t* d) {
+  return few_rows(d) && d[0] <= kMaxPlanned && d[0] * d[1] * d[3] * 256 < kMaxThreads;
+}
 // Wavefronts of few rows in units that fit at once: two (D 64: three) to a SIMD.
 static int64_t units_of_round(const int64_t* d) { return (d[5] == 128 ? 8 : 12) * 256; }
 
@@ -118,8 +125,9 @@ extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int6
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
   const int64_t tiles = (max_keys + kTileKeys - 1) / kTileKeys;
-  if (few_rows(dims)) {
-    *n_split = dims[0] > kMaxPlanned || one_group(dims, tiles) ? -1 : 0;
+  const bool units = units_fit(dims);
+  if (group_fits(dims) || units) {
+    *n_split = group_fits(dims) && (!units || one_group(dims, tiles)) ? -1 : 0;
     return RCSA_OK;
   }
   *n_split = 1;
@@ -143,7 +151,7 @@ extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t
   if (!dims || !window_dims(dims) || n_split < -1 || n_split > 64) return -1;
   const int64_t G = dims[3] / dims[4], row = dims[5] * 4 + 8;
   if (n_split < 1) {
-    if (!few_rows(dims) || (n_split == 0 && dims[0] > kMaxPlanned)) return -1;
+    if (!(n_split < 0 ? group_fits(dims) : units_fit(dims))) return -1;
     return n_split < 0 ? 0
                        : (4 * units_of_round(dims) + dims[0] * dims[4]) * dims[1] * G * row;
   }

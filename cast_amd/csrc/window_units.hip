@@ -243,8 +243,7 @@ static int launch_units(WindowArgs& a, hipStream_t s) {
   const int64_t each = tiles <= kLeastTiles ? 1 : (tiles + kLeastTiles - 1) / kLeastTiles;
   const int64_t any = 4ll * a.units + heads;
   const int64_t n = heads * each < any ? heads * each : any;
-  const int64_t rows = heads * a.Lq * a.G;
-  if (n >= (1ll << 31) || rows >= (1ll << 31)) return RCSA_ERR_SHAPE;
+  const int64_t rows = heads * a.Lq * a.G;  // (at most 2^24, of 256 threads: units_fit)
   const dim3 grid(static_cast<unsigned>(n)), block(64);
   if (a.table) window_unit_kernel<T, D, true, false><<<grid, block, 0, s>>>(a);
   else window_unit_kernel<T, D, false, false><<<grid, block, 0, s>>>(a);

@@ -758,7 +758,8 @@ int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, voi
  * shared among n_split workgroups and joined by a second launch.  For at most 32 rows a key
  * head (Lq Hq / Hk <= 32), n_split -1: a key head to a workgroup, one launch; 0: the visible
  * keys of all requests (at most 512) are dealt to wavefronts in equal units, whatever the
- * lengths, and joined by a second launch.  The workspace holds
+ * lengths, and joined by a second launch.  A launch has fewer than 2^32 threads: 256 a block
+ * of 128 rows, 512 a key head, 256 a row that units join.  The workspace holds
  * rcsa_window_attn_workspace_bytes (-1: no such launch; 16-byte aligned, of this call alone
  * until it ends).  rcsa_window_attn_plan picks n_split; max_keys bounds the keys that a row
  * sees.
