@@ -136,12 +136,15 @@ __device__ __forceinline__ int units_of(int tiles, int chunk) {
 // kUnitTiles tiles; beyond, units of that size, or more of them than four rounds.  A unit
 // costs about 5 us before its first tile has landed (a tile streams in 0.4 to 1), and the
 // units of a last, short round leave compute units idle.
-// (Products in fp32 that round up: a plan, the same for every wavefront.)
-constexpr int kLeastTiles = 2, kUnitTiles = 16;
-__device__ __forceinline__ int chunk_of(const WindowArgs& a, int64_t total) {
-  const float t = static_cast<float>(total) * a.Hk * 1.000001f;
-  const int one = static_cast<int>(t * a.per_unit) + 1;
-  int c = static_cast<int>(t * (0.25f * a.per_unit)) + 1;
+// (Sums and products in fp32, at most 14 roundings of 2^-24, that the factor rounds up: a plan,
+// the same for every wavefront.  The tiles of all requests pass 32 bits where tables share
+// pages; a request has at most 2^25, so that a chunk of kMostTiles leaves it whole.)
+constexpr int kLeastTiles = 2, kUnitTiles = 16, kMostTiles = 1 << 26;
+__device__ __forceinline__ int chunk_of(const WindowArgs& a, float total) {
+  const float t = total * static_cast<float>(a.Hk) * 1.000001f;
+  auto chunk = [](float x) { return static_cast<int>(fminf(x, kMostTiles)) + 1; };
+  const int one = chunk(t * a.per_unit);
+  int c = chunk(t * (0.25f * a.per_unit));
   c = c < kUnitTiles ? kUnitTiles : c;
   c = c < one ? c : one;
   return c < kLeastTiles ? kLeastTiles : c;
@@ -151,7 +154,7 @@ struct Unit {
   int before;            // units (of one key head) of the requests before b
   Request r;
 };
-__device__ __forceinline__ int lane_sum(int x) {
+__device__ __forceinline__ float lane_sum(float x) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
   return x;
@@ -174,7 +177,8 @@ __device__ __forceinline__ Unit find_unit(const WindowArgs& a, int w, int lane) 
     else if (lane < a.B) r = request_of(a, lane);
     const int tiles = lane < a.B ? request_tiles(a, r) : -1;
     const int mine = tiles > 0 ? tiles : 0;
-    const int chunk = chunk_of(a, a.B == 1 ? uniform_int(mine) : uniform_int(lane_sum(mine)));
+    const float own = static_cast<float>(a.B == 1 ? uniform_int(mine) : mine);
+    const int chunk = uniform_int(chunk_of(a, a.B == 1 ? own : lane_sum(own)));
     const int n = units_of(tiles, chunk);
     const int upto = a.B == 1 ? n : lane_prefix(n, lane);
     int l = w;
@@ -187,10 +191,10 @@ __device__ __forceinline__ Unit find_unit(const WindowArgs& a, int w, int lane) 
     const int shares = at(n), before = at(upto) - shares;
     return {l, w - before, shares, before, {at(r.k_len), at(r.q_len)}};
   }
-  int64_t total = 0;
+  float total = 0.0f;
   for (int b0 = 0; b0 < a.B; b0 += kWave) {
     const int t = b0 + lane < a.B ? request_tiles(a, request_of(a, b0 + lane)) : 0;
-    total += lane_sum(t > 0 ? t : 0);
+    total += lane_sum(static_cast<float>(t > 0 ? t : 0));
   }
   const int chunk = uniform_int(chunk_of(a, total));
   int before = 0;

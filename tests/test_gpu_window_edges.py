@@ -131,3 +131,30 @@ def test_many_small_weights(dev, page, Lq, n_split, odd, tail):
     steps = 2049 * 2.0 ** -24
     _within(out[0], ref, tol + 3 * steps * ref.abs(), "rows")
     _within(lse[0], rlse, ltol + steps, "sums")
+
+
+def test_plan_of_2_31_tiles(dev):
+    """64 requests of 2^30 - 16 keys each, over a table whose entries repeat eight pages: the
+    plan counts 2^31 tiles, and every unit finds its place.
+
+    The bound: units of 2^31 / (4 * 3072) tiles, a rounding a tile of the row's sum and two of
+    its products in fp32; a weight's half step; logits as in the oracle."""
+    from cast_amd import _lib
+    B, page, N, D = 64, 16, 8, 64
+    M = (1 << 26) - 1
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(B, 1, 1, D, generator=g).to(BF).to(dev)
+    k, v = (torch.randn(N, page, 1, D, generator=g).to(BF).to(dev) for _ in range(2))
+    table = (torch.arange(M, dtype=torch.int32, device=dev) % N)[None].expand(B, M)
+    lens = torch.full((B,), M * page, dtype=torch.int32, device=dev)
+    out, lse = _lib.torch_ops().window_attention(q, k, v, table, None, lens, 0, 0, 1, 0.125, True,
+                                                 None, 0, -1)
+    times = torch.tensor([M // N + (i < M % N) for i in range(N)], device=dev).double()
+    s = q[:, 0, 0].double() @ k.view(-1, D).double().T.contiguous() * 0.125
+    s = s + times.log().repeat_interleave(page)
+    row = torch.logsumexp(s, 1, keepdim=True)
+    p, vv = torch.exp(s - row), v.view(-1, D).double()
+    steps = 2.0 ** 31 / (4 * 3072) * 2.0 ** -24
+    tol = (p @ vv.abs()) * (2.0 ** -7 + 3 * steps) + 1e-4
+    _within(out[:, 0, 0], p @ vv, tol, "rows")
+    _within(lse[:, 0, 0], row[:, 0], torch.full_like(row[:, 0], steps + 1e-3), "sums")
