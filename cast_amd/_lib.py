@@ -82,6 +82,7 @@ SIGNATURES: dict[str, list] = {
                                   _P],
     "rcsa_window_attn_plan": [_P, _I, ctypes.POINTER(c_int64)],
     "rcsa_window_attn_workspace_bytes": [_P, _I],
+    "rcsa_window_attn_workspace_bytes_for": [_P, _I, _I, _I, _I],
     "rcsa_window_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _P] + [_I] * 7 + [c_float, _I, _P, _I,
                                                                              _P],
     "rcsa_pack_tokens": [_P, c_int, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P],
@@ -115,7 +116,8 @@ def load() -> ctypes.CDLL:
                       else c_int64 if name in ("rcsa_attn_workspace_bytes",
                                                "rcsa_attn_noalloc_scratch_bytes",
                                                "rcsa_order_lists_max_blocks",
-                                               "rcsa_window_attn_workspace_bytes")
+                                               "rcsa_window_attn_workspace_bytes",
+                                               "rcsa_window_attn_workspace_bytes_for")
                       else c_int)
     _lib = lib
     return lib

@@ -52,7 +52,7 @@ struct Api {
   decltype(&rcsa_rope) rope = nullptr;
   decltype(&rcsa_norm_rope) norm_rope = nullptr;
   decltype(&rcsa_window_attn_plan) window_attn_plan = nullptr;
-  decltype(&rcsa_window_attn_workspace_bytes) window_attn_workspace_bytes = nullptr;
+  decltype(&rcsa_window_attn_workspace_bytes_for) window_attn_workspace_bytes = nullptr;
   decltype(&rcsa_window_attn) window_attn = nullptr;
 };
 
@@ -89,7 +89,7 @@ void bind_library(const std::string& path) {
   bind_one(h, "rcsa_rope", api.rope);
   bind_one(h, "rcsa_norm_rope", api.norm_rope);
   bind_one(h, "rcsa_window_attn_plan", api.window_attn_plan);
-  bind_one(h, "rcsa_window_attn_workspace_bytes", api.window_attn_workspace_bytes);
+  bind_one(h, "rcsa_window_attn_workspace_bytes_for", api.window_attn_workspace_bytes);
   bind_one(h, "rcsa_window_attn", api.window_attn);
   g_api = api;
   g_bound = true;
@@ -1115,8 +1115,7 @@ std::vector<at::Tensor> window_attention(
     check_status(a, op, a.window_attn_plan(dims, most, &ns));
   }
   at::Tensor ws;
-  int64_t ws_bytes = 0;
-  ws_bytes = a.window_attn_workspace_bytes(dims, ns);
+  const int64_t ws_bytes = a.window_attn_workspace_bytes(dims, ns, Lk, window, sinks);
   TORCH_CHECK(ws_bytes >= 0, op, ": no launch of ", ns, " shares for q ", q.sizes(), ", k ",
               k.sizes());
   if (ws_bytes > 0) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));

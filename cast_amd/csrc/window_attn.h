@@ -701,7 +701,7 @@ __device__ __forceinline__ float join(float w, float o, float acc) {
 // Blocks of 128 rows over pages (window_paged.hip); type 0: bf16, 1: fp16.
 void launch_window_paged(WindowArgs& a, int type, int64_t D, dim3 grid, hipStream_t s);
 // Few rows (window_units.hip): in units and their join, or one workgroup a key head
-// (a.units 0).
-int launch_window_units(WindowArgs& a, int type, int64_t D, hipStream_t s);
+// (a.units 0); `units` of them are launched.
+int launch_window_units(WindowArgs& a, int type, int64_t D, int64_t units, hipStream_t s);
 
 }  // namespace rcsa

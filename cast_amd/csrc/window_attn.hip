@@ -68,6 +68,8 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
 // Blocks of rows of a key head.
 static int64_t row_blocks(int64_t Lq, int64_t G) { return (Lq * G + 127) / 128; }
 
+constexpr int64_t kMostKeys = 1ll << 30;
+
 static bool few_rows(const int64_t* d) { return d[1] * (d[3] / d[4]) <= kFewRows; }
 // Whether few rows fit a launch of a workgroup a key head, or of units and their join.
 static bool group_fits(const int64_t* d) {
@@ -78,6 +80,23 @@ static bool units_fit(const int64_t* d) {
 }
 // Wavefronts of few rows in units that fit at once: two (D 64: three) to a SIMD.
 static int64_t units_of_round(const int64_t* d) { return (d[5] == 128 ? 8 : 12) * 256; }
+
+// Units that a launch of few rows can have, over requests of at most `storage` keys: of their
+// storage, or of the window and first keys of Lq positions; of any length the plan's (see
+// chunk_of).  (A grid for any length: 16 x 32 heads x 256 keys 15.3 us, so 14.7; 64 x 512 keys
+// of 8 heads 15.6 and 15.2; long ones are the same.)
+static int64_t units_of_launch(const int64_t* d, int64_t storage, int64_t window, int64_t sinks) {
+  int64_t tiles = (storage + kTileKeys - 1) / kTileKeys;
+  if (window > 0) {
+    const int64_t seen =
+        (window + d[1]) / kTileKeys + 2 + (sinks + kTileKeys - 1) / kTileKeys;
+    tiles = seen < tiles ? seen : tiles;
+  }
+  const int64_t heads = d[0] * d[4];
+  const int64_t each = tiles <= kLeastTiles ? 1 : (tiles + kLeastTiles - 1) / kLeastTiles;
+  const int64_t any = 4 * units_of_round(d) + heads;
+  return heads * each < any ? heads * each : any;
+}
 
 // A workgroup a key head takes about 6.5 us and 0.25 a tile (the loads' latency, eight
 // wavefronts) where the bandwidth does not bind; units take 11 us, their join among them, and
@@ -147,16 +166,25 @@ extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int6
   return RCSA_OK;
 }
 
-extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
+extern "C" int64_t rcsa_window_attn_workspace_bytes_for(const int64_t* dims, int64_t n_split,
+                                                        int64_t storage, int64_t window,
+                                                        int64_t sinks) {
   if (!dims || !window_dims(dims) || n_split < -1 || n_split > 64) return -1;
+  if (storage < 0 || storage > kMostKeys || window < 0 || sinks < 0) return -1;
+  if (window >= kMostKeys) window = 0;
+  if (sinks > kMostKeys) sinks = kMostKeys;
   const int64_t G = dims[3] / dims[4], row = dims[5] * 4 + 8;
   if (n_split < 1) {
     if (!(n_split < 0 ? group_fits(dims) : units_fit(dims))) return -1;
     return n_split < 0 ? 0
-                       : (4 * units_of_round(dims) + dims[0] * dims[4]) * dims[1] * G * row;
+                       : units_of_launch(dims, storage, window, sinks) * dims[1] * G * row;
   }
   const int64_t items = xcd_items_of(dims);
   return n_split == 1 ? 0 : n_split * (items - xcd_whole_of(items, n_split)) * kNumXcd * 128 * row;
+}
+
+extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
+  return rcsa_window_attn_workspace_bytes_for(dims, n_split, kMostKeys, 0, 0);
 }
 
 extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
@@ -171,7 +199,7 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   if (dtype != RCSA_BF16 && dtype != RCSA_F16) return RCSA_ERR_DTYPE;
   // (a masked logit is -inf before the scale)
   if (!window_dims(dims) || !(sm_scale > 0.0f && sm_scale < INFINITY)) return RCSA_ERR_SHAPE;
-  const int64_t most = 1ll << 30;  // positions, windows and blocks stay far from 2^31
+  const int64_t most = kMostKeys;  // positions, windows and blocks stay far from 2^31
   if (dims[2] >= most || window < 0 || sinks < 0 || block < 0) return RCSA_ERR_SHAPE;
   if (block == 0 && (window != 0 || sinks != 0)) return RCSA_ERR_SHAPE;
   if (block_table && (max_pages <= 0 || n_pages <= 0 || page_size <= 0 || page_size % 16 ||
@@ -188,7 +216,9 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(workspace) ||
       (reinterpret_cast<uintptr_t>(out) & 7u))
     return RCSA_ERR_ALIGN;
-  const int64_t need = rcsa_window_attn_workspace_bytes(dims, n_split);
+  const int64_t storage = block_table ? max_pages * page_size : dims[2];
+  const int64_t need =
+      rcsa_window_attn_workspace_bytes_for(dims, n_split, storage, window, sinks);
   if (need < 0 || (need > 0 && (!workspace || workspace_bytes < need))) return RCSA_ERR_SHAPE;
   WindowArgs a{};
   a.q = q;
@@ -241,7 +271,9 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   const int64_t ws_rows = need / (dims[5] * 4 + 8);
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = need ? reinterpret_cast<float2*>(a.ws_o + ws_rows * dims[5]) : nullptr;
-  if (n_split < 1) return launch_window_units(a, dtype == RCSA_BF16 ? 0 : 1, dims[5], stream);
+  if (n_split < 1)
+    return launch_window_units(a, dtype == RCSA_BF16 ? 0 : 1, dims[5],
+                               units_of_launch(dims, storage, a.window, a.sinks), stream);
   if (dtype == RCSA_BF16)
     return dims[5] == 128 ? launch_window<__bf16, 128>(a, stream)
                           : launch_window<__bf16, 64>(a, stream);

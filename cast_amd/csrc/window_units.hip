@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
 }
 
 template <typename T, int D>
-static int launch_units(WindowArgs& a, hipStream_t s) {
+static int launch_units(WindowArgs& a, int64_t units, hipStream_t s) {
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hk;
   if (a.units == 0) {
     const dim3 grid(static_cast<unsigned>(heads)), block(64 * kGroupWaves);
@@ -230,30 +230,20 @@ static int launch_units(WindowArgs& a, hipStream_t s) {
     else window_unit_kernel<T, D, false, true><<<grid, block, 0, s>>>(a);
     return launch_status();
   }
-  // units of a key head that a request can have: of its storage, or of its window and first
-  // keys (a grid for any length: 16 x 32 heads x 256 keys 15.3 us, so 14.7; 64 x 512 keys
-  // of 8 heads 15.6 and 15.2; long ones are the same)
-  const int64_t cap = a.table ? static_cast<int64_t>(a.max_pages) * a.page : a.Lk;
-  int64_t tiles = (cap + kTileKeys - 1) / kTileKeys;
-  if (a.window > 0) {
-    const int64_t seen = (static_cast<int64_t>(a.window) + a.Lq) / kTileKeys + 2 +
-                         (static_cast<int64_t>(a.sinks) + kTileKeys - 1) / kTileKeys;
-    tiles = seen < tiles ? seen : tiles;
-  }
-  const int64_t each = tiles <= kLeastTiles ? 1 : (tiles + kLeastTiles - 1) / kLeastTiles;
-  const int64_t any = 4ll * a.units + heads;
-  const int64_t n = heads * each < any ? heads * each : any;
   const int64_t rows = heads * a.Lq * a.G;  // (at most 2^24, of 256 threads: units_fit)
-  const dim3 grid(static_cast<unsigned>(n)), block(64);
+  const dim3 grid(static_cast<unsigned>(units)), block(64);
   if (a.table) window_unit_kernel<T, D, true, false><<<grid, block, 0, s>>>(a);
   else window_unit_kernel<T, D, false, false><<<grid, block, 0, s>>>(a);
   window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
   return launch_status();
 }
 
-int launch_window_units(WindowArgs& a, int type, int64_t D, hipStream_t s) {
-  if (type == 0) return D == 128 ? launch_units<__bf16, 128>(a, s) : launch_units<__bf16, 64>(a, s);
-  return D == 128 ? launch_units<_Float16, 128>(a, s) : launch_units<_Float16, 64>(a, s);
+int launch_window_units(WindowArgs& a, int type, int64_t D, int64_t units, hipStream_t s) {
+  if (type == 0)
+    return D == 128 ? launch_units<__bf16, 128>(a, units, s)
+                    : launch_units<__bf16, 64>(a, units, s);
+  return D == 128 ? launch_units<_Float16, 128>(a, units, s)
+                  : launch_units<_Float16, 64>(a, units, s);
 }
 
 }  // namespace rcsa

@@ -760,12 +760,16 @@ int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, voi
  * keys of all requests (at most 512) are dealt to wavefronts in equal units, whatever the
  * lengths, and joined by a second launch.  A launch has fewer than 2^32 threads: 256 a block
  * of 128 rows, 512 a key head, 256 a row that units join.  The workspace holds
- * rcsa_window_attn_workspace_bytes (-1: no such launch; 16-byte aligned, of this call alone
- * until it ends).  rcsa_window_attn_plan picks n_split; max_keys bounds the keys that a row
+ * rcsa_window_attn_workspace_bytes_for (-1: no such launch; 16-byte aligned, of this call
+ * alone until it ends) of the keys that a request's storage holds (Lk, or max_pages *
+ * page_size) and the call's window and sinks; rcsa_window_attn_workspace_bytes is enough for
+ * any of them.  rcsa_window_attn_plan picks n_split; max_keys bounds the keys that a row
  * sees.
  */
 int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split);
 int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t n_split);
+int64_t rcsa_window_attn_workspace_bytes_for(const int64_t* dims, int64_t n_split,
+                                             int64_t storage, int64_t window, int64_t sinks);
 int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
                      int dtype, const int64_t* dims, const int64_t* strides,
                      const int32_t* q_lengths, const int32_t* k_lengths,

@@ -158,3 +158,30 @@ def test_plan_of_2_31_tiles(dev):
     tol = (p @ vv.abs()) * (2.0 ** -7 + 3 * steps) + 1e-4
     _within(out[:, 0, 0], p @ vv, tol, "rows")
     _within(lse[:, 0, 0], row[:, 0], torch.full_like(row[:, 0], steps + 1e-3), "sums")
+
+
+@pytest.mark.parametrize("Lk,window,sinks", [
+    (1, 0, 0), (64, 0, 0), (65, 0, 0), (4000, 0, 0), (4000, 100, 40), (4000, 1, 0),
+    (200000, 0, 0)])
+def test_units_stay_in_their_workspace(dev, Lk, window, sinks):
+    """A call over the C ABI with a workspace of just its size: what lies behind it stays, the
+    result is that of the torch call."""
+    import ctypes
+    from cast_amd import _lib
+    lib = _lib.load()
+    B, Lq, Hq, Hk, D = 2, 3, 8, 2, 128
+    q, k, v = _inputs(Lk, B, Lq, Lk, Hq, Hk, D, BF, dev)
+    dims = (ctypes.c_int64 * 6)(B, Lq, Lk, Hq, Hk, D)
+    need = lib.rcsa_window_attn_workspace_bytes_for(dims, 0, Lk, window, sinks)
+    assert need > 0
+    ws = torch.full((need + (1 << 20),), 0x5a, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(q)
+    strides = (ctypes.c_int64 * 12)(*(s for t in (q, k, v, out) for s in t.stride()[:3]))
+    assert lib.rcsa_window_attn(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None, 0, dims, strides, None,
+        None, None, 0, 0, 0, 0, window, sinks, 1, 0.1, 0, ws.data_ptr(), need,
+        torch.cuda.current_stream().cuda_stream) == 0
+    want = _lib.torch_ops().window_attention(q, k, v, None, None, None, window, sinks, 1, 0.1,
+                                             False, None, 0, -1)[0]
+    assert torch.equal(out, want)
+    assert (ws[need:] == 0x5a).all()

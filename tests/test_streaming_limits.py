@@ -28,7 +28,7 @@ def _plan(lib, dims, keys):
 
 def _launch(lib, dims, n_split, ws=None, ws_bytes=0):
     """The status of a launch whose pointers lead nowhere: a refusal comes before it."""
-    strides = (64, 64, 64) * 4
+    strides = (dims[5],) * 12
     return lib.rcsa_window_attn(4096, 4096, 4096, 4096, None, 0, _arr(*dims), _arr(*strides), None,
                                 None, None, 0, 0, 0, 0, 0, 0, 1, 0.1, n_split, ws, ws_bytes, None)
 
@@ -48,3 +48,25 @@ def test_window_launches_stay_below_2_32_threads(lib):
     blocks = (1 << 19, 1, 8, 32, 32, 64)    # 2^24 blocks of rows
     assert lib.rcsa_window_attn_workspace_bytes(_arr(*blocks), 1) == 0
     assert _launch(lib, blocks, 1) == SHAPE
+
+
+def test_units_workspace_goes_by_the_storage(lib):
+    """Rows of the units that a storage or window can have, never more than for any length;
+    a byte less is refused."""
+    def size(dims, storage, window=0, sinks=0):
+        return lib.rcsa_window_attn_workspace_bytes_for(_arr(*dims), 0, storage, window, sinks)
+
+    dims, row = (2, 4, 64, 16, 4, 128), 4 * 4 * (128 * 4 + 8)
+    any_length = lib.rcsa_window_attn_workspace_bytes(_arr(*dims), 0)
+    assert any_length == (4 * 8 * 256 + 2 * 4) * row
+    assert size(dims, 0) == size(dims, 64) == 2 * 4 * row          # one unit a key head
+    assert size(dims, 65) == size(dims, 128) == 2 * 4 * 2 * row    # two tiles a unit
+    assert size(dims, 1 << 30) == any_length
+    assert size(dims, 1 << 30, 1 << 40, 1 << 40) == any_length     # a window past all
+    assert size(dims, 1 << 30, 60, 4) == 2 * 4 * 3 * row           # 5 tiles and the first
+    assert all(size(dims, n) <= any_length for n in range(0, 1 << 20, 997))
+    assert size(dims, -1) == size(dims, (1 << 30) + 1) == size(dims, 64, -1) == -1
+    assert size(dims, 64, 0, -1) == -1
+    need = size(dims, 64)
+    assert _launch(lib, dims, 0, 4096, need - 1) == SHAPE
+    assert _launch(lib, dims, 0, None, need) == SHAPE
