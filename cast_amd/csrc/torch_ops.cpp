@@ -821,12 +821,15 @@ int float_code(const char* op, const at::Tensor& t, const char* name) {
   return dt == at::kBFloat16 ? RCSA_BF16 : dt == at::kHalf ? RCSA_F16 : RCSA_F32;
 }
 
-// An input on the call's GPU, with no gradient to compute.
+// An input on the call's GPU, with no gradient to compute (nor, which no_grad leaves on, a
+// forward-mode tangent).
 void input(const char* op, int& device, bool grads, const at::Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), op, ": tensors must live on a HIP device, ", name, " is on ",
               t.device());
   TORCH_CHECK(!grads || !t.requires_grad(), op,
               ": no gradient is computed; call it under torch.no_grad()");
+  TORCH_CHECK(!t._fw_grad(0).defined(), op,
+              ": no forward-mode gradient is computed; unpack the dual tensor ", name);
   on_device(op, device, t, name);
 }
 void input(const char* op, int& device, bool grads, const c10::optional<at::Tensor>& t,

@@ -70,3 +70,29 @@ def test_norms_of_many_tokens(dev, D, Hq, Hk):
     for got, x in ((qo, q), (kp.view(1, -1, Hk, D)[:, :L], k)):
         ref, size = so.rope(so.norm(x, None, 1e-6, False), pos, freq, axis, False)
         _close(got, ref, so.rope_bound(ref, size, BF, norm=True), (D, x.shape[2]))
+
+
+def test_forward_mode_gradients_are_refused(dev):
+    """A dual tensor's tangent is not dropped silently, with or without no_grad."""
+    from torch.autograd import forward_ad
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    plan = rotary_plan(64, device=dev)
+    x = torch.randn(2, 16, 4, 64, device=dev).to(BF)
+    pos = torch.arange(16, device=dev)
+    pages = torch.zeros(4, 16, 4, 64, device=dev, dtype=BF)
+    table = torch.zeros(2, 1, device=dev, dtype=torch.int32)
+    lens = torch.ones(2, device=dev, dtype=torch.int32)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.rope(d, pos, plan), lambda: ops.rope(x, pos, plan, out=d),
+                     lambda: ops.norm_rope(d, x, pos, plan), lambda: ops.norm_rope(x, d, pos, plan),
+                     lambda: ops.norm_rope(x, x, pos, plan, q_weight=d[0, 0]),
+                     lambda: ops.window_attention(d, x, x), lambda: ops.window_attention(x, x, d),
+                     lambda: ops.paged_attention(d, ops.PagedCache(pages, pages, table), lens)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        y = forward_ad.unpack_dual(d).primal
+        assert torch.equal(ops.rope(y, pos, plan), ops.rope(x, pos, plan))
