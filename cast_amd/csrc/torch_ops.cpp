@@ -858,6 +858,32 @@ void want_own(const char* op, const at::Tensor& t, const char* name) {
     TORCH_CHECK(t.stride(i) > 0 || t.size(i) <= 1, op, ": ", name, " must not be expanded");
 }
 
+// Whether two tensors certainly share memory: they begin at one element, or one of them is
+// dense and holds the other's first or last element.  (Interleaved views, such as the parts of
+// a fused projection, are not told apart further.)
+bool share_memory(const char* op, const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto first = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
+  auto end = [&](const at::Tensor& t) {
+    return first(t) + static_cast<uintptr_t>(span(op, t, "a tensor")) * t.element_size();
+  };
+  auto holds = [&](const at::Tensor& t, const at::Tensor& u) {
+    return t.is_non_overlapping_and_dense() &&
+           ((first(t) <= first(u) && first(u) < end(t)) || (first(t) < end(u) && end(u) <= end(t)));
+  };
+  return first(a) == first(b) || holds(a, b) || holds(b, a);
+}
+
+// A given output does not overlap another operand (`same`: unless it is that very tensor).
+void want_apart(const char* op, const at::Tensor& out, const char* name, const at::Tensor& t,
+                const char* other, bool same = false) {
+  bool alike = same && out.data_ptr() == t.data_ptr() && out.sizes() == t.sizes();
+  for (int64_t i = 0; alike && i < t.dim(); ++i)
+    alike = t.size(i) <= 1 || t.stride(i) == out.stride(i);
+  TORCH_CHECK_VALUE(alike || !share_memory(op, out, t), op, ": ", name, " must not overlap ",
+                    other);
+}
+
 // (the stride of a dimension of one element says nothing)
 void put_strides(const at::Tensor& t, int64_t* s) {
   for (int64_t i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
@@ -919,6 +945,7 @@ at::Tensor rope(const at::Tensor& x, const at::Tensor& positions, const at::Tens
   want_rows(op, out, x.scalar_type(), "out");
   want_own(op, out, "out");
   TORCH_CHECK(out.sizes() == x.sizes(), op, ": out must have x's shape");
+  if (out_.has_value()) want_apart(op, out, "out", x, "x unless it is x", true);
   if (x.numel() == 0) return out;
   int64_t s[6];
   put_strides(x, s);
@@ -1001,6 +1028,11 @@ std::vector<at::Tensor> norm_rope(
   want_rows(op, q_out, dt, "q_out");
   want_own(op, q_out, "q_out");
   TORCH_CHECK(q_out.sizes() == q.sizes(), op, ": q_out must have q's shape");
+  if (q_out_.has_value()) {
+    want_apart(op, q_out, "q_out", q, "q unless it is q", true);
+    want_apart(op, q_out, "q_out", k, "k");
+    if (v.has_value()) want_apart(op, q_out, "q_out", *v, "v");
+  }
   int64_t s[18] = {};
   put_strides(q, s);
   put_strides(k, s + 3);
@@ -1019,6 +1051,13 @@ std::vector<at::Tensor> norm_rope(
     TORCH_CHECK(k_pages->sizes() == v_pages->sizes() && k_pages->size(2) == Hk &&
                     k_pages->size(3) == D && k_pages->size(0) > 0 && k_pages->size(1) > 0, op,
                 ": the pages must be [pages, slots, ", Hk, ", ", D, "]");
+    want_apart(op, *k_pages, "the key pages", *v_pages, "the value pages");
+    want_apart(op, *k_pages, "the key pages", q, "q");
+    want_apart(op, *v_pages, "the value pages", q, "q");
+    if (q_out_.has_value()) {
+      want_apart(op, q_out, "q_out", *k_pages, "the key pages");
+      want_apart(op, q_out, "q_out", *v_pages, "the value pages");
+    }
     put_strides(*v, s + 6);
     put_strides(*k_pages, s + 12);
     put_strides(*v_pages, s + 15);
@@ -1032,6 +1071,11 @@ std::vector<at::Tensor> norm_rope(
     want_rows(op, k_out, dt, "k_out");
     want_own(op, k_out, "k_out");
     TORCH_CHECK(k_out.sizes() == k.sizes(), op, ": k_out must have k's shape");
+    if (k_out_.has_value()) {
+      want_apart(op, k_out, "k_out", k, "k unless it is k", true);
+      want_apart(op, k_out, "k_out", q, "q");
+      want_apart(op, k_out, "k_out", q_out, "q_out");
+    }
     put_strides(k_out, s + 12);
     kp = k_out.data_ptr();
     res.push_back(k_out);
@@ -1102,6 +1146,11 @@ std::vector<at::Tensor> window_attention(
   want_rows(op, out, dt, "out");
   want_own(op, out, "out");
   TORCH_CHECK(out.sizes() == q.sizes(), op, ": out must have q's shape");
+  if (out_.has_value()) {
+    want_apart(op, out, "out", q, "q");
+    want_apart(op, out, "out", k, "k");
+    want_apart(op, out, "out", v, "v");
+  }
   std::vector<at::Tensor> res{out};
   if (return_lse) res.push_back(at::empty({B, Hq, Lq}, q.options().dtype(at::kFloat)));
   if (q.numel() == 0) return res;

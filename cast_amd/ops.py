@@ -1183,7 +1183,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, plan, *,
     ``[B, L]``, with the plan's axes last when it has more than one; any sign (negated
     positions undo a rotation of scale 1), as far as 64-bit angles reach.  fp32 between, one
     rounding at the end.  ``out`` (x's shape and dtype, any strides) may be ``x`` itself and
-    must not overlap it otherwise."""
+    must not overlap it otherwise (refused, but for interleaved views, which are not told
+    apart)."""
     return _lib.torch_ops().rope(x, positions, plan.turns, plan.axis, plan.n_axes,
                                  plan.interleaved, plan.scale, out)
 
@@ -1210,7 +1211,8 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan, *
     ``x * rsqrt(mean(x^2) + eps) * weight``, the mean over a head or, with
     ``across_heads``, over all heads of a token (the reference normalises the whole
     projection, P/matrix_curvature_phase_frame_weave.py:5391-5393); a weight is ``[D]`` or
-    ``[H, D]`` (None: 1).  Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be q / k.
+    ``[H, D]`` (None: 1).  Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be q / k and
+    overlap nothing else.
 
     With ``cache`` the keys, and ``v [B, L, Hk, D]`` as it is, go to the cache instead: token
     t of request b to index ``starts[b] + t`` (int32 ``[B]``; None: t), dropped where the

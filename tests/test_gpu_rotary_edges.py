@@ -96,3 +96,46 @@ def test_forward_mode_gradients_are_refused(dev):
                 call()
         y = forward_ad.unpack_dual(d).primal
         assert torch.equal(ops.rope(y, pos, plan), ops.rope(x, pos, plan))
+
+
+def test_outputs_that_overlap_are_refused(dev):
+    """An output may be its own input, or a part of a fused projection beside it; shifted,
+    turned or another operand's memory is refused before anything is written."""
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    plan = rotary_plan(64, device=dev)
+    pos = torch.arange(16, device=dev)
+    store = torch.randn(2 * 17 * 4 * 64, device=dev).to(BF)
+    x, shifted = store[:8192].view(2, 16, 4, 64), store[64:8256].view(2, 16, 4, 64)
+    k, v = torch.randn(2, 2, 16, 4, 64, device=dev).to(BF)
+    pages = torch.randn(2, 16, 4, 64, device=dev).to(BF)
+    table = torch.arange(2, device=dev, dtype=torch.int32)[:, None].contiguous()
+    lens = torch.full((2,), 16, device=dev, dtype=torch.int32)
+    cache = ops.PagedCache(pages, pages.clone(), table)
+    was = store.clone(), k.clone(), v.clone(), pages.clone()
+    for call in (lambda: ops.rope(x, pos, plan, out=shifted),
+                 lambda: ops.rope(x[:, :4], pos[:4], plan, out=x[:, :4].transpose(1, 2)),
+                 lambda: ops.norm_rope(x, k, pos, plan, q_out=shifted),
+                 lambda: ops.norm_rope(x, k, pos, plan, q_out=k),
+                 lambda: ops.norm_rope(x, k, pos, plan, k_out=x),
+                 lambda: ops.norm_rope(x, k, pos, plan, q_out=v, k_out=v),
+                 lambda: ops.norm_rope(x, k, pos, plan, v=v, cache=cache, q_out=v),
+                 lambda: ops.norm_rope(x, k, pos, plan, v=v, cache=cache, q_out=pages),
+                 lambda: ops.norm_rope(x, k, pos, plan, v=v, cache=cache._replace(v=pages)),
+                 lambda: ops.norm_rope(pages, k, pos, plan, v=v, cache=cache),
+                 lambda: ops.window_attention(x, k, v, out=x),
+                 lambda: ops.window_attention(x, k, v, out=shifted),
+                 lambda: ops.window_attention(x, k, v, out=k),
+                 lambda: ops.window_attention(x, k, v, out=v),
+                 lambda: ops.window_attention(x[:, 3:5], k, v, out=k[:, 3:5]),
+                 lambda: ops.paged_attention(x, cache, lens, out=pages)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip((store, k, v, pages), was))
+    fused = torch.randn(2, 16, 4, 4, 64, device=dev).to(BF)
+    q, k, v, o = fused.unbind(2)
+    want = ops.window_attention(*(t.contiguous() for t in (q, k, v)))
+    assert torch.equal(ops.window_attention(q, k, v, out=o), want)
+    want = ops.norm_rope(q.contiguous(), k.contiguous(), pos, plan)
+    assert ops.norm_rope(q, k, pos, plan, q_out=q, k_out=k)[0].data_ptr() == q.data_ptr()
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1])
