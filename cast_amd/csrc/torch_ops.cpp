@@ -1015,8 +1015,10 @@ std::vector<at::Tensor> norm_rope(
       TORCH_CHECK(!any || (*w)->scalar_type() == w_dt, op, ": the weights must share a dtype");
       any = true;
       w_dt = (*w)->scalar_type();
-      TORCH_CHECK((*w)->is_contiguous() && ((*w)->numel() == D || (*w)->numel() == H * D), op,
-                  ": a weight must be contiguous [D] or [H, D]");
+      const int64_t d = (*w)->dim();  // (flat, or channels last)
+      TORCH_CHECK((*w)->is_contiguous() && ((*w)->numel() == D || (*w)->numel() == H * D) &&
+                      (d == 1 || (d > 1 && (*w)->size(d - 1) == D)), op,
+                  ": a weight must be contiguous [D] or [H, D], got ", (*w)->sizes());
       ws[i] = (*w)->numel() == D ? 0 : D;
     }
     ++i;

@@ -1210,8 +1210,8 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan, *
 
     ``x * rsqrt(mean(x^2) + eps) * weight``, the mean over a head or, with
     ``across_heads``, over all heads of a token (the reference normalises the whole
-    projection, P/matrix_curvature_phase_frame_weave.py:5391-5393); a weight is ``[D]`` or
-    ``[H, D]`` (None: 1).  Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be q / k and
+    projection, P/matrix_curvature_phase_frame_weave.py:5391-5393); a weight is ``[D]``,
+    ``[H, D]`` or, flat, ``[H * D]`` (None: 1).  Returns ``(q_out, k_out)``; ``q_out`` / ``k_out`` may be q / k and
     overlap nothing else.
 
     With ``cache`` the keys, and ``v [B, L, Hk, D]`` as it is, go to the cache instead: token

@@ -139,3 +139,28 @@ def test_outputs_that_overlap_are_refused(dev):
     want = ops.norm_rope(q.contiguous(), k.contiguous(), pos, plan)
     assert ops.norm_rope(q, k, pos, plan, q_out=q, k_out=k)[0].data_ptr() == q.data_ptr()
     assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_weight_shapes(dev):
+    """[D], [H, D] and the flat [H * D] of a projection's norm; a turned or split shape of as
+    many elements is refused."""
+    from cast_amd import ops
+    from cast_amd.rotary import rotary_plan
+    H, D = 4, 64
+    plan = rotary_plan(D, device=dev)
+    pos = torch.arange(5, device=dev)
+    x = torch.randn(2, 5, H, D, device=dev).to(BF)
+    w = torch.randn(H, D, device=dev).to(BF)
+    for across in (False, True):
+        kw = dict(across_heads=across)
+        want = ops.norm_rope(x, x, pos, plan, q_weight=w, k_weight=w, **kw)
+        for shape in ((H * D,), (1, 1, H, D), (2, H // 2, D)):
+            got = ops.norm_rope(x, x, pos, plan, q_weight=w.view(shape), k_weight=w.view(shape),
+                                **kw)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), shape
+        one = ops.norm_rope(x, x, pos, plan, q_weight=w[0], **kw)[0]
+        assert torch.equal(ops.norm_rope(x, x, pos, plan, q_weight=w[:1], **kw)[0], one)
+        for shape in ((D, H), (H, D, 1), (2 * H, D // 2), (8, 8), (D, 1)):
+            n = shape[0] * shape[1] * (shape[2] if len(shape) > 2 else 1)
+            with pytest.raises(RuntimeError, match="weight"):
+                ops.norm_rope(x, x, pos, plan, q_weight=w.view(-1)[:n].view(shape), **kw)
