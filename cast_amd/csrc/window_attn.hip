@@ -197,8 +197,9 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
                                 hipStream_t stream) {
   if (!q || !k || !v || !out || !dims || !strides) return RCSA_ERR_NULL;
   if (dtype != RCSA_BF16 && dtype != RCSA_F16) return RCSA_ERR_DTYPE;
-  // (a masked logit is -inf before the scale)
-  if (!window_dims(dims) || !(sm_scale > 0.0f && sm_scale < INFINITY)) return RCSA_ERR_SHAPE;
+  // (a masked logit is -inf before the scale; a zero one stays zero under a finite one)
+  const float scale_log2 = sm_scale * 1.4426950408889634f;
+  if (!window_dims(dims) || !(sm_scale > 0.0f && scale_log2 < INFINITY)) return RCSA_ERR_SHAPE;
   const int64_t most = kMostKeys;  // positions, windows and blocks stay far from 2^31
   if (dims[2] >= most || window < 0 || sinks < 0 || block < 0) return RCSA_ERR_SHAPE;
   if (block == 0 && (window != 0 || sinks != 0)) return RCSA_ERR_SHAPE;
@@ -251,7 +252,7 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   a.window = static_cast<int>(window < most ? window : 0);
   a.sinks = static_cast<int>(sinks < most ? sinks : most);
   a.block = static_cast<int>(block < most ? block : most);
-  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   a.n_rblocks = static_cast<int>(row_blocks(a.Lq, a.G));
   a.n_items = static_cast<int64_t>(a.B) * a.Hk * a.n_rblocks;
   a.n_split = static_cast<int>(n_split);

@@ -746,7 +746,7 @@ int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, voi
  *   j < min(e, k_len) and (j >= e - window or j < sinks), e = (floor(p / block) + 1) block;
  * window 0: no window; block 1: by token, n: by blocks of n positions (frames), 0: every
  * key (window and sinks 0).  A page that is not in [0, n_pages) hides its keys.
- *   out = softmax(sm_scale q k) v in fp32 (sm_scale > 0), rounded once; lse (nullable)
+ *   out = softmax(sm_scale q k) v in fp32 (0 < sm_scale < 2^127), rounded once; lse (nullable)
  * [B][Hq][Lq] the natural log of the row's sum; a row that sees nothing gives 0 and -inf.
  * What a row does not see does not reach it, NaN and infinities included.  Rows i >= q_len
  * of both are left as they were.  out must not overlap q, k or v.  q, k, v rows 16-byte, out

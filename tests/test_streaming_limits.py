@@ -26,11 +26,11 @@ def _plan(lib, dims, keys):
     return n.value
 
 
-def _launch(lib, dims, n_split, ws=None, ws_bytes=0):
+def _launch(lib, dims, n_split, ws=None, ws_bytes=0, scale=0.1):
     """The status of a launch whose pointers lead nowhere: a refusal comes before it."""
     strides = (dims[5],) * 12
     return lib.rcsa_window_attn(4096, 4096, 4096, 4096, None, 0, _arr(*dims), _arr(*strides), None,
-                                None, None, 0, 0, 0, 0, 0, 0, 1, 0.1, n_split, ws, ws_bytes, None)
+                                None, None, 0, 0, 0, 0, 0, 0, 1, scale, n_split, ws, ws_bytes, None)
 
 
 def test_window_launches_stay_below_2_32_threads(lib):
@@ -70,3 +70,10 @@ def test_units_workspace_goes_by_the_storage(lib):
     need = size(dims, 64)
     assert _launch(lib, dims, 0, 4096, need - 1) == SHAPE
     assert _launch(lib, dims, 0, None, need) == SHAPE
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38, 1e-46])
+def test_scales_that_leave_fp32_are_refused(lib, scale):
+    """The kernels take the scale times log2 e in fp32: infinite there, a logit of 0 would be
+    NaN; 0 in fp32, it is no scale."""
+    assert _launch(lib, (1, 4, 8, 2, 1, 64), 1, scale=scale) == SHAPE
