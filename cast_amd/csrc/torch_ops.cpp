@@ -858,20 +858,29 @@ void want_own(const char* op, const at::Tensor& t, const char* name) {
     TORCH_CHECK(t.stride(i) > 0 || t.size(i) <= 1, op, ": ", name, " must not be expanded");
 }
 
+// The bytes from a tensor's first element to its last one, and whether all are its own.
+struct Extent {
+  uintptr_t first, end;
+  bool dense;
+};
+Extent extent(const char* op, const at::Tensor& t) {
+  Extent e;
+  e.dense = t.is_non_overlapping_and_dense();
+  e.first = reinterpret_cast<uintptr_t>(t.data_ptr());
+  e.end = e.first + static_cast<uintptr_t>(e.dense ? t.numel() : span(op, t, "a tensor")) *
+                        t.element_size();
+  return e;
+}
+
 // Whether two tensors certainly share memory: they begin at one element, or one of them is
 // dense and holds the other's first or last element.  (Interleaved views, such as the parts of
 // a fused projection, are not told apart further.)
 bool share_memory(const char* op, const at::Tensor& a, const at::Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
-  auto first = [](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); };
-  auto end = [&](const at::Tensor& t) {
-    return first(t) + static_cast<uintptr_t>(span(op, t, "a tensor")) * t.element_size();
-  };
-  auto holds = [&](const at::Tensor& t, const at::Tensor& u) {
-    return t.is_non_overlapping_and_dense() &&
-           ((first(t) <= first(u) && first(u) < end(t)) || (first(t) < end(u) && end(u) <= end(t)));
-  };
-  return first(a) == first(b) || holds(a, b) || holds(b, a);
+  const Extent x = extent(op, a), y = extent(op, b);
+  if (x.end <= y.first || y.end <= x.first) return false;
+  return x.first == y.first || (x.dense && (x.first < y.first || y.end <= x.end)) ||
+         (y.dense && (y.first < x.first || x.end <= y.end));
 }
 
 // A given output does not overlap another operand (`same`: unless it is that very tensor).
