@@ -83,7 +83,8 @@ __device__ __forceinline__ float wave_max(float v) {
 
 __device__ __forceinline__ int uniform_int(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Division of n < 2^31 by an invariant: a high product and two shifts.
+// Division of n < 2^31 by an invariant: a high product and two shifts (Granlund and
+// Montgomery, "Division by invariant integers using multiplication", 1994).
 struct Divisor {
   uint32_t d, mul;
   int sh1, sh2;

@@ -12,12 +12,12 @@
 // pages 3520 x 72 heads 34 us, 3.8 TB/s (a token's sums stand between its loads and its
 // stores, and 130 MB are few beside a launch's start and end); with norms of heads 16391 x 48
 // heads of 128 71 us, 5.7 TB/s, 32782 x 20 heads of 64 40 us, 4.2 TB/s; one token of 8
-// requests 3.6 us, with norms and pages of 64 requests 5.7 us: a launch and its loads.  A position times a frequency needs more than 24 bits once the
-// positions are far (at position 10^6 an fp32 angle is off by 0.06), so the
-// angle is a product in turns in 64 bits, reduced to [-1/2, 1/2] turns there,
-// and only then fp32: exact to an fp32 rounding at any position, with no table
-// to read.  The sines are taken once per token and pair into LDS and shared by
-// all heads of the token.
+// requests 3.6 us, with norms and pages of 64 requests 5.7 us: a launch and its loads.
+// A position times a frequency needs more than 24 bits once the positions are far (at
+// position 10^6 an fp32 angle is off by 0.06), so the angle is a product in turns in 64
+// bits, reduced to [-1/2, 1/2] turns there, and only then fp32: exact to an fp32 rounding at
+// any position, with no table to read.  The sines are taken once per token and pair into LDS
+// and shared by all heads of the token.
 #include "rotary.h"
 
 namespace rcsa {
@@ -131,7 +131,8 @@ constexpr int kWide = 16 / static_cast<int>(sizeof(T));
 // 89), one with norms of heads (16391 tokens x 48 heads 71 us, two 75, three 79), three with
 // joint norms, which the list of a token should fit (3520 x 72 heads 34 us, two 42, four 38, five
 // 34; 9000 x 40 heads 51, 50, 51, 50; 3520 x 48 heads fp32 36, 41, 40, 43); narrow
-// runs six (14097 x 9 heads of 80 57 us, four 61).
+// runs six (3 x 14097 x 9 heads of 80 56 us, four 61): 4 bytes a lane move at 2.2 TB/s, half of
+// what the wide runs reach.
 template <int V, int NORM>
 constexpr int kEntries = V == 2 ? 6 : (NORM == 0 ? 2 : (NORM == 1 ? 1 : 3));
 template <typename T, int V>

@@ -520,9 +520,9 @@ __device__ __forceinline__ int lane_again() {
 // Rows whose products met a value that they do not see (0 * inf or 0 * NaN of a masked
 // key): a wavefront's 32 rows taken again at their known maxima m, tile by tile through
 // TILE bytes of LDS, values that are no numbers staged as 0 and added only where a row
-// sees their key.  One load at a time, forty times slower than the first time (32K causal
-// tokens x 32 heads, every head's first value infinite: 43 ms, without it 7.7); batches of loads
-// spill.
+// sees their key.  One load at a time, five to seven times the first pass (32K causal
+// tokens x 32 heads, every head's first value infinite, so that all rows are taken again: on
+// 8 key heads 43 ms in all, without it 7.4, on 32 57 and 7.3); batches of loads spill.
 template <typename T, int D, bool PAGED>
 __device__ __forceinline__ void rows_again(LateArgs& a, const Place& p, RowTile<T, D>& t,
                                            int lane, float m, char* lds) {

@@ -8,9 +8,11 @@
 // A tile's K and V go global -> LDS without registers into a ring of three
 // slots; rows past the keys, and pages that are not there, land as zeros.
 // Bound by the matrix products at the card's power limit: 44 frames of 880 tokens, a window of
-// 12 and an anchor, 24 heads 4.0-4.2 ms by box, 1110-1190 TFLOP/s (a 16384^3 product 1362), the
-// matrix pipe 75% busy at 1.6 GHz; window 4096 over 32773 tokens, 32 heads on 8 1.8-1.9 ms,
-// 1090-1150 TFLOP/s, 71%; four frames on 44 in pages 770-790 us, 1020 TFLOP/s, 62%.
+// 12 and an anchor, 24 heads 3.9-4.2 ms by card, 1110-1200 TFLOP/s (a 16384^3 product 1362), the
+// matrix pipe 75% busy at 1.45-1.6 GHz; window 4096 over 32773 tokens, 32 heads on 8 1.8-1.9 ms,
+// 1090-1160 TFLOP/s, 72%.  Four frames on 44 in pages, 992 workgroups on 768 places, 755-795 us,
+// 1010-1060 TFLOP/s, 61%.  D 64 has half the products a key beside the same exponentials: 16384
+// tokens x 16 heads, window 4096, 288 us, 835 TFLOP/s, 51%.
 // Only the tiles at the window's edges are masked.  A wavefront also works on the few
 // tiles that none of its rows sees: with a branch around the work the copies could not
 // go out between the matrix products (four frames against 20 of 44 708 us so, 722 with

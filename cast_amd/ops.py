@@ -1192,7 +1192,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, plan, *,
 class PagedCache(NamedTuple):
     """Keys and values in pages, and the pages of every request: key j of request b is row
     ``j % slots`` of page ``table[b, j // slots]``; an entry outside the pages hides its
-    keys."""
+    keys.  :func:`norm_rope` fills pages of any size and type, :func:`paged_attention` reads
+    bf16 or fp16 pages of a multiple of 16 keys and D 64 or 128."""
     k: torch.Tensor      # [pages, slots, Hk, D]
     v: torch.Tensor      # [pages, slots, Hk, D]
     table: torch.Tensor  # int32 [B, pages of a request]
@@ -1217,7 +1218,8 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan, *
     With ``cache`` the keys, and ``v [B, L, Hk, D]`` as it is, go to the cache instead: token
     t of request b to index ``starts[b] + t`` (int32 ``[B]``; None: t), dropped where the
     table has no page for it; ``k_out`` is then None.  No two tokens may go to one row.
-    ``lengths`` (int32 ``[B]``) leaves the rows of tokens ``t >= lengths[b]`` as they were."""
+    ``lengths`` (int32 ``[B]``) leaves the rows of tokens ``t >= lengths[b]`` as they were
+    (give ``q_out``; a fresh one holds nothing there)."""
     kp, vp, table = cache if cache is not None else (None, None, None)
     res = _lib.torch_ops().norm_rope(
         q, k, v, q_weight, k_weight, eps, across_heads, positions, plan.turns,
@@ -1258,8 +1260,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     not read.  A row that sees no key gives 0 (LSE -inf); a key or value that a row does not
     see does not reach it, whatever it holds.
 
-    fp32 softmax, rounded once; returns ``out [B, Lq, Hq, D]`` (must not overlap q, k or v)
-    and, with ``return_lse``, the natural log-sum-exp ``[B, Hq, Lq]`` (undefined past a
+    fp32 softmax, its weights rounded to the type for their product with v, the result rounded
+    once; returns ``out [B, Lq, Hq, D]`` (must not overlap q, k or v) and, with ``return_lse``, the natural log-sum-exp ``[B, Hq, Lq]`` (undefined past a
     request's queries).  ``n_split`` (None: planned) shares the keys of
     the blocks of rows that would leave compute units idle among that many workgroups."""
     fn = "window_attention"
@@ -1293,7 +1295,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
     of each request, the new ones among them.  Pages hold a multiple of 16 keys.
 
     Pages that no row sees are not read, so their table entries may be anything; an entry
-    outside the pages hides its keys.  ``max_length`` bounds the lengths (what the table
+    outside the pages hides its keys; tables may share pages.  ``max_length`` bounds the lengths (what the table
     holds, if None): it only plans how the keys are shared among workgroups, a longer
     request is still read to its end."""
     fn = "paged_attention"

@@ -697,10 +697,10 @@ int rcsa_int8_linear_group(const int8_t* x, const float* x_scale, int64_t n_line
  * positions_i64, addressed with pos_strides (host array: batch, token, axis); turns fp64
  * [n_pairs]; axis int32 [n_pairs] in [0, n_axes), NULL: all 0.  The product is taken and
  * reduced in 64 bits, so far positions lose nothing.  D <= 512, H <= 4096, B * L <
- * 2^30.  Rows move in runs of V
- * channels, V = 16 bytes of the type, where D is a multiple of 2 V (up to 128 V), n_pairs
- * (interleaved: 2 n_pairs) and all strides of V, and pointers of 16 bytes; in runs of 2
- * where all that holds for V = 2 (pointers of two elements); else element by element.
+ * 2^30.  Rows move in runs of V channels, V = 16 bytes of the type, where D is a multiple
+ * of 2 V (up to 128 V), n_pairs (interleaved: 2 n_pairs) and all strides of V, and pointers
+ * of 16 bytes; in runs of 2 where all that holds for V = 2 (pointers of two elements); else
+ * element by element.
  *
  * rcsa_norm_rope: q [B][L][Hq][D] and k [B][L][Hk][D], dims = {B, L, Hq, Hk, D},
  *   y = x * rsqrt(mean(x^2) + eps) * weight, then the rotation of rcsa_rope,
@@ -748,6 +748,7 @@ int rcsa_norm_rope(const void* q, const void* k, const void* v, void* q_out, voi
  * key (window and sinks 0).  A page that is not in [0, n_pages) hides its keys.
  *   out = softmax(sm_scale q k) v in fp32 (0 < sm_scale < 2^127), rounded once; lse (nullable)
  * [B][Hq][Lq] the natural log of the row's sum; a row that sees nothing gives 0 and -inf.
+ * B < 2^20, Lq < 2^24, Lk (or max_pages * page_size) < 2^30, Hq < 2^16.
  * What a row does not see does not reach it, NaN and infinities included.  Rows i >= q_len
  * of both are left as they were.  out must not overlap q, k or v.  q, k, v rows 16-byte, out
  * rows 8-byte aligned; the token (slot) strides of k and v are at least D and below 2^25
