@@ -20,6 +20,8 @@ RCSA_OK = 0
 RCSA_BF16 = 0
 RCSA_F32 = 1
 RCSA_F16 = 2
+RCSA_CODE_INT8 = 0
+RCSA_CODE_E4M3 = 1
 RCSA_ORDER_INDEX = 0
 RCSA_ORDER_RANK = 1
 RCSA_ORDER_RANK_LOCAL = 2
@@ -85,6 +87,9 @@ SIGNATURES: dict[str, list] = {
     "rcsa_window_attn_workspace_bytes_for": [_P, _I, _I, _I, _I],
     "rcsa_window_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _P] + [_I] * 7 + [c_float, _I, _P, _I,
                                                                              _P],
+    "rcsa_append_cache": [_P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P, _P, _P] + [_I] * 5
+                         + [_P],
+    "rcsa_read_cache": [_P, _P, c_int, _P, _P, _P, _P, c_int, _P, _P, _P, _P, _P] + [_I] * 5 + [_P],
     "rcsa_pack_tokens": [_P, c_int, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P, _P],
     "rcsa_unpack_tokens": [_P, _I, _I, _I, _I, _P, _I, _P, _P],
     "rcsa_status_string": [c_int],

@@ -9,8 +9,8 @@
 // bad layout.  Every tensor is checked to span the elements the call's dims
 // and strides reach, so no argument combination makes a kernel read or write
 // past the tensors it was given.  Nothing here synchronises, and nothing but
-// layer_call, order_lists, valid_bits, rope, norm_rope and window_attention, which
-// allocate their outputs (and the last its workspace), allocates device memory.
+// layer_call, order_lists, valid_bits, rope, norm_rope, read_cache and window_attention,
+// which allocate their outputs (and the last its workspace), allocates device memory.
 //
 // The C ABI is bound at load time (rcsa::bind_library) from the library the
 // Python side loaded, so one librcsa.so serves both the ctypes binding and
@@ -54,6 +54,8 @@ struct Api {
   decltype(&rcsa_window_attn_plan) window_attn_plan = nullptr;
   decltype(&rcsa_window_attn_workspace_bytes_for) window_attn_workspace_bytes = nullptr;
   decltype(&rcsa_window_attn) window_attn = nullptr;
+  decltype(&rcsa_append_cache) append_cache = nullptr;
+  decltype(&rcsa_read_cache) read_cache = nullptr;
 };
 
 std::mutex g_mu;
@@ -91,6 +93,8 @@ void bind_library(const std::string& path) {
   bind_one(h, "rcsa_window_attn_plan", api.window_attn_plan);
   bind_one(h, "rcsa_window_attn_workspace_bytes_for", api.window_attn_workspace_bytes);
   bind_one(h, "rcsa_window_attn", api.window_attn);
+  bind_one(h, "rcsa_append_cache", api.append_cache);
+  bind_one(h, "rcsa_read_cache", api.read_cache);
   g_api = api;
   g_bound = true;
 }
@@ -1107,6 +1111,166 @@ std::vector<at::Tensor> norm_rope(
   return res;
 }
 
+// ---- A cache in 8 bits (cast_amd/ops.py: QuantizedCache, append_cache, read_cache) ----
+
+// Codes [pages, slots, H, D], scales [pages, blocks, H] and the table of B requests.
+struct Cache8 {
+  int code;
+  int64_t max_pages, n_pages, page, block, table_stride;
+};
+void put_scale_strides(const at::Tensor& t, int64_t* s) {
+  for (int64_t i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+Cache8 want_cache8(const char* op, const at::Tensor& k, const at::Tensor& v,
+                   const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& table,
+                   int64_t B) {
+  const at::ScalarType dt = k.scalar_type();
+  TORCH_CHECK_TYPE(dt == at::kChar || dt == at::kFloat8_e4m3fn, op,
+                   ": the cache's codes must be int8 or float8_e4m3fn, got ", dt);
+  TORCH_CHECK_TYPE(v.scalar_type() == dt, op, ": the cache's codes must share a dtype, v is ",
+                   v.scalar_type(), " beside ", dt);
+  TORCH_CHECK_VALUE(k.dim() == 4 && (k.stride(3) == 1 || k.size(3) <= 1) &&
+                        k.sizes() == v.sizes() && v.stride(3) == k.stride(3) && k.numel() > 0, op,
+                    ": the cache's codes must be [pages, slots, H, D] alike, with a contiguous "
+                    "last dim, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_VALUE(k_scale.dim() == 3 && k_scale.sizes() == v_scale.sizes() &&
+                        k_scale.size(0) == k.size(0) && k_scale.size(2) == k.size(2) &&
+                        k_scale.size(1) > 0 && k.size(1) % k_scale.size(1) == 0 &&
+                        k.size(1) / k_scale.size(1) % 16 == 0, op,
+                    ": the scales must be [pages, blocks, H] of blocks of a multiple of 16 slots, "
+                    "got ", k_scale.sizes(), " and ", v_scale.sizes(), " beside codes ", k.sizes());
+  TORCH_CHECK_TYPE(k_scale.scalar_type() == at::kFloat && v_scale.scalar_type() == at::kFloat, op,
+                   ": the scales must be float32");
+  want_table(op, table, B);
+  return {dt == at::kChar ? RCSA_CODE_INT8 : RCSA_CODE_E4M3, table.size(1), k.size(0), k.size(1),
+          k.size(1) / k_scale.size(1), table.stride(0)};
+}
+
+void append_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_codes,
+                  const at::Tensor& v_codes, const at::Tensor& k_scale, const at::Tensor& v_scale,
+                  const at::Tensor& table, const c10::optional<at::Tensor>& starts,
+                  const c10::optional<at::Tensor>& lengths,
+                  const c10::optional<at::Tensor>& offsets) {
+  const char* op = "append_cache";
+  const Api& a = api(op);
+  const bool grads = at::GradMode::is_enabled();
+  int dev = -1;
+  input(op, dev, grads, k, "k");
+  input(op, dev, grads, v, "v");
+  for (const auto* t : {&k_codes, &v_codes, &k_scale, &v_scale})
+    input(op, dev, grads, *t, "the cache");
+  input(op, dev, false, table, "the block table");
+  for (const auto* t : {&starts, &lengths, &offsets}) input(op, dev, false, *t, "an operand");
+  const int code = float_code(op, k, "k");
+  const bool packed = offsets.has_value();
+  TORCH_CHECK_VALUE(!packed || !lengths.has_value(), op, ": give lengths or offsets");
+  TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type(), op, ": k and v must share a dtype, v is ",
+                   v.scalar_type(), " beside ", k.scalar_type());
+  const int64_t nd = packed ? 3 : 4;
+  TORCH_CHECK_VALUE(k.dim() == nd && k.sizes() == v.sizes() &&
+                        (k.size(nd - 1) <= 1 || (k.stride(nd - 1) == 1 && v.stride(nd - 1) == 1)),
+                    op, ": k and v must be ", packed ? "[T, H, D]" : "[B, L, H, D]",
+                    " alike, with a contiguous last dim, got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(!packed || (offsets->dim() == 1 && offsets->size(0) > 0), op,
+              ": offsets must be int32 [B + 1]");
+  const int64_t B = packed ? offsets->size(0) - 1 : k.size(0), L = k.size(nd - 3),
+                H = k.size(nd - 2), D = k.size(nd - 1);
+  want_vector(op, starts, B, "starts");
+  want_vector(op, lengths, B, "lengths");
+  if (packed) want_vector(op, offsets, B + 1, "offsets");
+  const Cache8 c = want_cache8(op, k_codes, v_codes, k_scale, v_scale, table, B);
+  TORCH_CHECK_VALUE(k_codes.size(2) == H && k_codes.size(3) == D, op, ": the cache holds [",
+                    k_codes.size(2), ", ", k_codes.size(3), "] a key, k is ", k.sizes());
+  const std::pair<const at::Tensor*, const char*> outs[4] = {
+      {&k_codes, "the key codes"}, {&v_codes, "the value codes"}, {&k_scale, "the key scales"},
+      {&v_scale, "the value scales"}};
+  for (int i = 0; i < 4; ++i) {
+    want_own(op, *outs[i].first, outs[i].second);
+    want_apart(op, *outs[i].first, outs[i].second, k, "k");
+    want_apart(op, *outs[i].first, outs[i].second, v, "v");
+    want_apart(op, *outs[i].first, outs[i].second, table, "the block table");
+    for (int j = 0; j < i; ++j)
+      want_apart(op, *outs[i].first, outs[i].second, *outs[j].first, outs[j].second);
+  }
+  const Launch l(device_of(op, dev));
+  if (B == 0 || L == 0) return;
+  int64_t s[18] = {};
+  for (int i = 0; i < 2; ++i) {
+    const at::Tensor& x = i == 0 ? k : v;
+    for (int64_t d = 4 - nd; d < 3; ++d)
+      s[3 * i + d] = x.size(d - (4 - nd)) > 1 ? x.stride(d - (4 - nd)) : 0;
+  }
+  put_strides(k_codes, s + 6);
+  put_strides(v_codes, s + 9);
+  put_scale_strides(k_scale, s + 12);
+  put_scale_strides(v_scale, s + 15);
+  const int64_t dims[4] = {B, L, H, D};
+  check_status(a, op, a.append_cache(
+      k.data_ptr(), v.data_ptr(), code, dims, s, ptr<const int32_t>(offsets),
+      ptr<const int32_t>(starts), ptr<const int32_t>(lengths), k_codes.data_ptr(),
+      v_codes.data_ptr(), c.code, k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+      table.data_ptr<int32_t>(), c.table_stride, c.max_pages, c.n_pages, c.page, c.block,
+      l.stream));
+}
+
+// Keys starts[b] + t, t < size, of every request into k_out, v_out [B, size, H, D].
+std::vector<at::Tensor> read_cache(
+    const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& k_scale,
+    const at::Tensor& v_scale, const at::Tensor& table, const at::Tensor& lengths, int64_t size,
+    const c10::optional<at::Tensor>& starts, at::ScalarType dtype,
+    const c10::optional<at::Tensor>& k_out_, const c10::optional<at::Tensor>& v_out_) {
+  const char* op = "read_cache";
+  const Api& a = api(op);
+  const bool grads = at::GradMode::is_enabled();
+  int dev = -1;
+  for (const auto* t : {&k_codes, &v_codes, &k_scale, &v_scale})
+    input(op, dev, grads, *t, "the cache");
+  input(op, dev, false, table, "the block table");
+  input(op, dev, false, lengths, "lengths");
+  input(op, dev, false, starts, "starts");
+  input(op, dev, grads, k_out_, "k_out");
+  input(op, dev, grads, v_out_, "v_out");
+  const int64_t B = lengths.dim() == 1 ? lengths.size(0) : -1;
+  want_vector(op, lengths, B, "lengths");
+  want_vector(op, starts, B, "starts");
+  TORCH_CHECK_VALUE(size >= 0, op, ": size must not be negative, got ", size);
+  TORCH_CHECK_VALUE(k_out_.has_value() == v_out_.has_value(), op, ": give k and v outputs together");
+  const Cache8 c = want_cache8(op, k_codes, v_codes, k_scale, v_scale, table, B);
+  const int64_t H = k_codes.size(2), D = k_codes.size(3);
+  const Launch l(device_of(op, dev));
+  const auto options = k_codes.options().dtype(dtype);
+  const at::Tensor k_out = k_out_.has_value() ? *k_out_ : at::empty({B, size, H, D}, options);
+  const at::Tensor v_out = v_out_.has_value() ? *v_out_ : at::empty({B, size, H, D}, options);
+  const int code = float_code(op, k_out, "k_out");
+  const std::pair<const at::Tensor*, const char*> outs[2] = {{&k_out, "k_out"}, {&v_out, "v_out"}};
+  for (const auto& o : outs) {
+    want_rows(op, *o.first, k_out.scalar_type(), o.second);
+    want_own(op, *o.first, o.second);
+    TORCH_CHECK(o.first->size(0) == B && o.first->size(1) == size && o.first->size(2) == H &&
+                    o.first->size(3) == D, op, ": ", o.second, " must be [", B, ", ", size, ", ",
+                H, ", ", D, "], got ", o.first->sizes());
+    if (!k_out_.has_value()) continue;
+    for (const auto* t : {&k_codes, &v_codes, &k_scale, &v_scale, &table})
+      want_apart(op, *o.first, o.second, *t, "the cache");
+  }
+  if (k_out_.has_value()) want_apart(op, k_out, "k_out", v_out, "v_out");
+  if (k_out.numel() == 0) return {k_out, v_out};
+  int64_t s[18];
+  put_strides(k_codes, s);
+  put_strides(v_codes, s + 3);
+  put_scale_strides(k_scale, s + 6);
+  put_scale_strides(v_scale, s + 9);
+  put_strides(k_out, s + 12);
+  put_strides(v_out, s + 15);
+  const int64_t dims[4] = {B, size, H, D};
+  check_status(a, op, a.read_cache(
+      k_codes.data_ptr(), v_codes.data_ptr(), c.code, k_scale.data_ptr<float>(),
+      v_scale.data_ptr<float>(), k_out.data_ptr(), v_out.data_ptr(), code, dims, s,
+      ptr<const int32_t>(starts), lengths.data_ptr<int32_t>(), table.data_ptr<int32_t>(),
+      c.table_stride, c.max_pages, c.n_pages, c.page, c.block, l.stream));
+  return {k_out, v_out};
+}
+
 // Dense (k, v [B, Lk, Hk, D]) or, with a table, paged (k, v [pages, slots, Hk, D])
 // attention over a window and the first keys; n_split -2: planned.  (out) or (out, lse).
 std::vector<at::Tensor> window_attention(
@@ -1260,4 +1424,14 @@ TORCH_LIBRARY(rcsa, m) {
       "Tensor? k_lengths, int window, int sinks, int block, float? sm_scale, bool return_lse, "
       "Tensor(a!)? out, int n_split, int max_keys) -> Tensor[]",
       &window_attention);
+  m.def(
+      "append_cache(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) v_codes, "
+      "Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor table, Tensor? starts, Tensor? lengths, "
+      "Tensor? offsets) -> ()",
+      &append_cache);
+  m.def(
+      "read_cache(Tensor k_codes, Tensor v_codes, Tensor k_scale, Tensor v_scale, Tensor table, "
+      "Tensor lengths, int size, Tensor? starts, ScalarType dtype, Tensor(a!)? k_out, "
+      "Tensor(b!)? v_out) -> Tensor[]",
+      &read_cache);
 }

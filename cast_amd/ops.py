@@ -21,7 +21,7 @@ __all__ = [
     "pool_query", "pool_key", "block_scores", "select_topk", "quantize_key",
     "sparse_attn_bf16", "sparse_attn_int8", "pack_tokens", "unpack_tokens", "row_budgets",
     "quantize_key_select", "order_lists", "rope", "norm_rope", "PagedCache",
-    "window_attention", "paged_attention",
+    "window_attention", "paged_attention", "QuantizedCache", "append_cache", "read_cache",
 ]
 
 
@@ -1197,6 +1197,58 @@ class PagedCache(NamedTuple):
     k: torch.Tensor      # [pages, slots, Hk, D]
     v: torch.Tensor      # [pages, slots, Hk, D]
     table: torch.Tensor  # int32 [B, pages of a request]
+
+
+class QuantizedCache(NamedTuple):
+    """A :class:`PagedCache` in 8 bits: code c of a block of tokens and head with scale s stands
+    for c * s.  The block of row r of a page is ``r // (slots // blocks)``, a multiple of 16
+    rows.  :func:`append_cache` fills it, :func:`read_cache` and :func:`paged_attention` read
+    it."""
+    k: torch.Tensor        # int8 or float8_e4m3fn [pages, slots, Hk, D]
+    v: torch.Tensor        # alike
+    k_scale: torch.Tensor  # float32 [pages, blocks, Hk]
+    v_scale: torch.Tensor  # alike
+    table: torch.Tensor    # int32 [B, pages of a request]
+
+
+def append_cache(k: torch.Tensor, v: torch.Tensor, cache: QuantizedCache,
+                 starts: Optional[torch.Tensor] = None, *,
+                 lengths: Optional[torch.Tensor] = None,
+                 offsets: Optional[torch.Tensor] = None) -> QuantizedCache:
+    """Quantises ``k, v [B, L, Hk, D]`` (bf16, fp16 or fp32, rows 16-byte aligned, D a multiple
+    of 8) as they are written to the cache (``rcsa_append_cache``); returns the cache.
+
+    Token t of request b becomes key ``starts[b] + t`` (int32 ``[B]``; None: t), for the first
+    ``lengths[b]`` tokens of a padded batch; packed requests have ``k, v [T, Hk, D]`` and
+    ``offsets`` (int32 ``[B + 1]``, not decreasing): rows ``offsets[b]`` to ``offsets[b + 1]`` are
+    request b's.  Keys that the table has no page for are dropped.
+
+    A block that gets new tokens takes the scale max(s0, own, 2^-100): own is max |x| of its new
+    values of the head / 127 (int8) or the least power of two p with max |x| <= 448 p (e4m3), s0
+    its scale if it holds keys before the new ones, else 0.  New codes are x / s to the
+    nearest; where the scale grew, the codes before become c * s0 / s, rounded once more (half
+    a step of the new scale).  Infinities saturate, NaN becomes 0.  An append ends its
+    request: rows of a block behind the new ones hold nothing any more.  No two tokens may go to
+    one key, nor two requests to one block."""
+    _lib.torch_ops().append_cache(k, v, cache.k, cache.v, cache.k_scale, cache.v_scale,
+                                  cache.table, starts, lengths, offsets)
+    return cache
+
+
+def read_cache(cache: QuantizedCache, lengths: torch.Tensor, *, size: int,
+               starts: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
+               out: Optional[tuple[torch.Tensor, torch.Tensor]] = None):
+    """Keys ``starts[b] + t`` (int32 ``[B]``; None: t) below ``lengths[b]`` (int32 ``[B]``), t <
+    ``size``, and their values, as dense ``(k, v) [B, size, Hk, D]`` of ``dtype`` (bf16, fp16 or
+    fp32), e.g. for the woven layers (``rcsa_read_cache``): c * s in fp32, rounded once.
+
+    Keys that the table has no page for give 0.  ``out = (k, v)`` (any strides, rows 16-byte
+    aligned, their dtype) takes them; its rows past a request's keys stay as they were, those of
+    fresh outputs hold nothing."""
+    ko, vo = out if out is not None else (None, None)
+    return tuple(_lib.torch_ops().read_cache(cache.k, cache.v, cache.k_scale, cache.v_scale,
+                                             cache.table, lengths, int(size), starts, dtype, ko,
+                                             vo))
 
 
 def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan, *,

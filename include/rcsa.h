@@ -43,6 +43,10 @@ enum {
  * entry points also take fp16). */
 enum { RCSA_BF16 = 0, RCSA_F32 = 1, RCSA_F16 = 2 };
 
+/* Element type codes of a cache in 8 bits: int8 in [-127, 127], or e4m3 (4 exponent, 3
+ * mantissa bits, up to 448, no infinities). */
+enum { RCSA_CODE_INT8 = 0, RCSA_CODE_E4M3 = 1 };
+
 /* Selection output order. */
 enum {
   RCSA_ORDER_INDEX = 0, /* ascending block index (what the attention kernel streams best) */
@@ -778,6 +782,54 @@ int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, flo
                      int64_t n_pages, int64_t page_size, int64_t window, int64_t sinks,
                      int64_t block, float sm_scale, int64_t n_split, void* workspace,
                      int64_t workspace_bytes, hipStream_t stream);
+
+/*
+ * A paged cache in 8 bits, one scale for each block of tokens and head.  No reference kernel:
+ * the reference holds its keys and values in 16 bits.
+ *
+ * Pages of codes [n_pages][page_size][H][D] (int8 or e4m3) and fp32 scales
+ * [n_pages][page_size / block_size][H], of keys and of values: key j of request b is row
+ * j % page_size of page block_table[b * table_stride + j / page_size], code c of a block and
+ * head with scale s stands for c * s.  block_size (a multiple of 16, at most 65536) divides
+ * page_size.  A page that is not in [0, n_pages), or past max_pages, hides its keys.  D is a
+ * multiple of 8, at most 1024; max_pages * page_size < 2^30.
+ *
+ * rcsa_append_cache: k, v [B][L][H][D] (bf16, fp16 or fp32), dims = {B, L, H, D}; token t of
+ * request b becomes key starts[b] + t (starts NULL: t), lengths (nullable, int32 [B]) of them,
+ * those on hidden or negative keys are dropped.  With offsets (int32 [B + 1], not decreasing,
+ * lengths NULL) the requests are packed: k, v [L][H][D], request b the rows offsets[b] ..
+ * offsets[b + 1].  A block that gets new tokens takes the scale
+ *   s = max(s0, own, 2^-100), own = fp32(a / 127) (int8), the least power of two p with
+ *   a <= 448 p (e4m3), a = max |x| of the block's new finite values of the head,
+ * s0 its scale if keys before the new ones are in it (a scale that is no positive finite number
+ * counts as 0), else 0; new codes are x / s to the nearest, ties to even (e4m3 with a scale
+ * that is no power of two: of the fp32 quotient); infinities saturate, NaN becomes 0.  Where
+ * s > s0 the codes of the keys before become c s0 / s, rounded alike.  Rows of a block behind
+ * the new ones hold nothing any more: an append ends its request.  No two tokens of a call may
+ * go to one key, nor two requests to one block.
+ *
+ * rcsa_read_cache: rows t of k_out, v_out [B][L][H][D] (bf16, fp16 or fp32) become keys
+ * starts[b] + t (NULL: t) of request b, c * s in fp32 rounded once, as far as they are below
+ * lengths[b] (int32 [B]); hidden keys give 0, the rows of keys from lengths[b] on, or past the
+ * table, are left as they were.
+ *
+ * strides: host array of 18, in elements: batch, token, head of k, v (append) or page, slot, head
+ * of the codes of keys, values (read) first; then page, slot, head of the codes (append) or page, block,
+ * head of the scales (read); then page, block, head of the scales (append) or batch, token, head of
+ * k_out, v_out (read).  Rows of k, v, k_out, v_out are 16-byte, of the codes 8-byte aligned.
+ */
+int rcsa_append_cache(const void* k, const void* v, int dtype, const int64_t* dims,
+                      const int64_t* strides, const int32_t* offsets, const int32_t* starts,
+                      const int32_t* lengths, void* k_codes, void* v_codes, int code,
+                      float* k_scales, float* v_scales, const int32_t* block_table,
+                      int64_t table_stride, int64_t max_pages, int64_t n_pages,
+                      int64_t page_size, int64_t block_size, hipStream_t stream);
+int rcsa_read_cache(const void* k_codes, const void* v_codes, int code, const float* k_scales,
+                    const float* v_scales, void* k_out, void* v_out, int dtype,
+                    const int64_t* dims, const int64_t* strides, const int32_t* starts,
+                    const int32_t* lengths, const int32_t* block_table, int64_t table_stride,
+                    int64_t max_pages, int64_t n_pages, int64_t page_size, int64_t block_size,
+                    hipStream_t stream);
 
 #ifdef __cplusplus
 }
