@@ -87,6 +87,8 @@ SIGNATURES: dict[str, list] = {
     "rcsa_window_attn_workspace_bytes_for": [_P, _I, _I, _I, _I],
     "rcsa_window_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _P] + [_I] * 7 + [c_float, _I, _P, _I,
                                                                              _P],
+    "rcsa_cached_attn": [_P, _P, _P, c_int, _P, _P, _P, _P, c_int] + [_P] * 6 + [_I] * 8
+                        + [c_float, _I, _P, _I, _P],
     "rcsa_append_cache": [_P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P, _P, _P] + [_I] * 5
                          + [_P],
     "rcsa_read_cache": [_P, _P, c_int, _P, _P, _P, _P, c_int, _P, _P, _P, _P, _P] + [_I] * 5 + [_P],

@@ -1,0 +1,326 @@
+// Attention over pages of 8-bit codes, blocks of 128 rows: window_tile.h's work with a tile's
+// codes taken through registers, where they become fp16 on their way to LDS (once a
+// workgroup, not once a wavefront), two tiles ahead of the products.
+#include "cached_attn.h"
+
+namespace rcsa {
+
+// RowTile's step with a scale for each half of a tile's keys (a lane half's 16).
+template <int D>
+struct CodeTile : RowTile<_Float16, D> {
+  using R = RowTile<_Float16, D>;
+  using O = Half<_Float16>;
+  float c_row;  // logit of q . c, times the key's scale, in log2 units
+  int v_exp;    // accumulators are in units of 2^v_exp
+
+  template <typename Bits, typename Pre, typename Cp>
+  __device__ __forceinline__ void step8(const char* tile, const Scales& sc, int hf, bool inside,
+                                        Bits&& bits, Pre&& prefetch, Cp&& copies) {
+    v4i kraw[R::QSTEPS];
+#pragma unroll
+    for (int st = 0; st < R::QSTEPS; ++st)
+      kraw[st] = *reinterpret_cast<const v4i*>(tile + this->k_off[st]);
+    v16f s_acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < R::QSTEPS; ++st)
+      s_acc = O::mfma(__builtin_bit_cast(v8hf, kraw[st]), this->q_op[st], s_acc);
+    __builtin_amdgcn_sched_group_barrier(0x100, R::QSTEPS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    prefetch();
+    int e_new = v_exp;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = static_cast<int>(__float_as_uint(sc.v[h]) >> 23) - 126;  // 2^e > the scale
+      e_new = sc.v[h] > 0.0f && e > e_new ? e : e_new;
+    }
+    if (e_new != v_exp) {
+      const int down = v_exp - e_new;
+      const float f = down < -126 ? 0.0f : power_of(down);
+#pragma unroll
+      for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
+      v_exp = e_new;
+    }
+    const float c = c_row * (hf ? sc.k[1] : sc.k[0]);
+    const float f = (hf ? sc.v[1] : sc.v[0]) * power_of(-v_exp);
+    float rv[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
+    if (!inside) {
+      const uint32_t seen = bits();
+      // (a scale of 0 would make NaN of -inf)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rv[r] = ((seen >> r) & 1u) ? rv[r] * c : -INFINITY;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rv[r] *= c;
+    }
+    v8hf p_op[2];
+    auto exps = [&]() __attribute__((always_inline)) -> float {
+      const float bias = this->m_run == -INFINITY ? 0.0f : -this->m_run;
+      float lsum[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int jj = 0; jj < 8; ++jj) {
+          const float e = __builtin_amdgcn_exp2f(rv[8 * u + jj] + bias);
+          p_op[u][jj] = static_cast<_Float16>(e * f);
+          if (u == 0 && jj < 4) lsum[jj] = e;
+          else lsum[jj & 3] += e;
+        }
+      return (lsum[0] + lsum[1]) + (lsum[2] + lsum[3]);
+    };
+    float part = exps();
+    if (__ballot(this->m_run == -INFINITY || !(part <= kTauPow * (1 << O::kShift))) != 0) {
+      float rmax = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
+      rmax = pair_max(rmax);
+      const float m_blk = rmax == -INFINITY ? -INFINITY : rmax - O::kShift;
+      if (__ballot(m_blk > this->m_run + kTau) != 0) {
+        const float m_new = fmaxf(this->m_run, m_blk);
+        const float alpha =
+            m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(this->m_run - m_new);
+        this->l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= alpha;
+        this->m_run = m_new;
+        part = exps();
+      }
+    }
+    this->l_run += part;
+    copies();
+    auto v_group = [&](int u, v8hf (&op)[R::NDT]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int dt = 0; dt < R::NDT; ++dt) {
+        const char* const p0 = tile + this->v_off[dt] + 8 * u * R::KROW;
+        const auto lo = O::read_tr(p0);
+        const auto hi = O::read_tr(p0 + 4 * R::KROW);
+        op[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    };
+    v8hf vop[2][R::NDT];
+    v_group(0, vop[0]);
+    v_group(1, vop[1]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int dt = 0; dt < R::NDT; ++dt)
+        this->o_acc[dt] = O::mfma(vop[u][dt], p_op[u], this->o_acc[dt]);
+  }
+};
+
+template <typename T, bool E4M3, int D>
+__global__ void __launch_bounds__(256)
+__attribute__((amdgpu_waves_per_eu(2, 2)))
+cached_tile_kernel(WindowArgs a) {
+  using C = CodeTile<D>;
+  using R = RowTile<_Float16, D>;
+  typedef typename Half<T>::op8 op8;
+  constexpr int BM = 128;
+  // a wavefront moves rows 8 w .. 8 w + 7 of a tile: a lane BPL bytes of one of them
+  constexpr int BPL = D / 8, CHUNKS = BPL / 8;  // (16-byte chunks of the fp16 row)
+  __shared__ __attribute__((aligned(1024))) char s_0[2 * R::TILE];
+  __shared__ __attribute__((aligned(1024))) char s_1[2 * R::TILE];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uniform_int(tid >> 6);
+  const int hf = lane >> 5, lr = lane & 31;
+
+  const int xcd = static_cast<int>(blockIdx.x % kNumXcd);
+  const int slot = static_cast<int>(blockIdx.x / kNumXcd);
+  const int tail = slot - a.xcd_whole;
+  Place p;
+  p.shares = tail < 0 ? 1 : a.n_split;
+  const int in_xcd = tail < 0 ? slot : a.xcd_whole + tail / a.n_split;
+  const int share = tail < 0 ? 0 : tail % a.n_split;
+  const ItemAt it = item_at(a, xcd, in_xcd);
+  if (it.bh < 0) return;
+  p.b = divide(it.bh, a.by_Hk);
+  p.hk = it.bh - p.b * a.Hk;
+  const Request rq = request_of<true>(a, p.b);
+  const int q_len = uniform_int(rq.q_len);
+  p.k_len = uniform_int(rq.k_len);
+  p.n_rows = q_len * a.G;
+  const int item_row0 = it.rblock * BM;
+  if (item_row0 >= p.n_rows) return;
+  p.row0 = item_row0 + wave * 32;
+  p.shift = p.k_len - q_len;
+  const int64_t per_tail = a.xcd_items - a.xcd_whole;
+  const int64_t ws_row =
+      (share * per_tail * kNumXcd + xcd * per_tail + in_xcd - a.xcd_whole) * BM + wave * 32;
+  const KeyRange w_first = row_range(a, p, p.row0), w_last = row_range(a, p, p.row0 + 31);
+  p.tiles = tiles_of(a, row_range(a, p, item_row0), row_range(a, p, item_row0 + BM - 1));
+  share_of(p, share);
+
+  C t;
+  t.init(lane);
+  t.v_exp = -126;
+  {
+    const Row r = row_of(a, p, p.row0 + lr);
+    const T* const row = static_cast<const T*>(a.q) + p.b * a.sq[0] +
+                         static_cast<int64_t>(r.qi) * a.sq[1] + r.head * a.sq[2];
+    op8 raw[R::QSTEPS];
+    float most = 0.0f;
+#pragma unroll
+    for (int st = 0; st < R::QSTEPS; ++st) {
+      raw[st] = *reinterpret_cast<const op8*>(row + (hf * R::QSTEPS + st) * 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(static_cast<float>(raw[st][i])));
+    }
+    const int k = row_shift(pair_max(most));
+    const float up = power_of(k);
+#pragma unroll
+    for (int st = 0; st < R::QSTEPS; ++st) t.q_op[st] = scaled8<T>(raw[st], up);
+    t.c_row = a.scale_log2 * power_of(-k);
+  }
+
+  const char* const kbase = static_cast<const char*>(a.k) + p.hk * a.sk[2];
+  const char* const vbase = static_cast<const char*>(a.v) + p.hk * a.sv[2];
+  const uint32_t krb = static_cast<uint32_t>(a.sk[1]), vrb = static_cast<uint32_t>(a.sv[1]);
+  const int32_t* const table = a.table + p.b * a.table_stride;
+
+  // the lane's bytes of a tile: row 8 wave + lane / 8, which lies in half wave / 2
+  const int trow = 8 * wave + (lane >> 3), in_half = trow & 15;
+  const int k_lo = in_half * static_cast<int>(krb) + (lane & 7) * BPL;
+  const int v_lo = in_half * static_cast<int>(vrb) + (lane & 7) * BPL;
+  int k_at[CHUNKS], v_at[CHUNKS];
+#pragma unroll
+  for (int i = 0; i < CHUNKS; ++i) {
+    const int chunk = (lane & 7) * CHUNKS + i;
+    k_at[i] = trow * R::KROW + ((chunk ^ (swz_k<R::KROW>(trow) & (R::CPR - 1))) * 16);
+    v_at[i] = R::TILE + trow * R::KROW + ((chunk ^ (swz_v(trow) & (R::CPR - 1))) * 16);
+  }
+  struct Staged {
+    v4i k, v;  // (D 64: the first two words)
+  };
+  auto load = [&](const Step& s) __attribute__((always_inline)) -> Staged {
+    const HalfRows h = code_rows(a, s, wave >> 1, krb, vrb);
+    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(kbase) + h.k, 0, 16 * static_cast<int>(krb), kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<char*>(vbase) + h.v, 0, 16 * static_cast<int>(vrb), kRsrcWord3);
+    Staged x;
+    if constexpr (BPL == 16) {
+      x.k = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lo, 0, 0));
+      x.v = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vr, v_lo, 0, 0));
+    } else {
+      const auto k2 = __builtin_amdgcn_raw_buffer_load_b64(kr, k_lo, 0, 0);
+      const auto v2 = __builtin_amdgcn_raw_buffer_load_b64(vr, v_lo, 0, 0);
+      x.k = v4i{static_cast<int>(k2[0]), static_cast<int>(k2[1]), 0, 0};
+      x.v = v4i{static_cast<int>(v2[0]), static_cast<int>(v2[1]), 0, 0};
+    }
+    return x;
+  };
+  auto put = [&](const Staged& x, char* dst) __attribute__((always_inline)) {
+    v8hf k[2], v[2];
+    v4i fv = x.v;
+#pragma unroll
+    for (int i = 0; i < BPL / 4; ++i)
+      fv[i] = static_cast<int>(Widen<E4M3>::finite(static_cast<uint32_t>(fv[i])));
+    widen16<E4M3>(x.k, k[0], k[1]);
+    widen16<E4M3>(fv, v[0], v[1]);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      *reinterpret_cast<v8hf*>(dst + k_at[i]) = k[i];
+      *reinterpret_cast<v8hf*>(dst + v_at[i]) = v[i];
+    }
+  };
+
+  // Two slots: tile j in slot j % 2, written during step j - 1 (all wavefronts have left step
+  // j - 2 by then), its codes asked for during step j - 2.
+  Step cur = step_of<true>(a, p, table, 0), next = step_of<true>(a, p, table, 1);
+  Scales sc = scales_of(a, p, cur);
+  put(load(cur), s_0);
+  Staged st = load(next);
+  auto iteration = [&](auto slot_c, int j) __attribute__((always_inline)) {
+    constexpr int J = decltype(slot_c)::value;
+    char* const tile = J == 0 ? s_0 : s_1;
+    char* const fill = J == 0 ? s_1 : s_0;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const Step now = cur;
+    const Scales ns = sc;
+    cur = next;
+    const int there = halves_there<true>(a, now);
+    const bool inside = now.key >= 0 && there == 3 && now.key + kTileKeys <= w_first.hi &&
+                        (now.key >= w_last.lo || now.key + kTileKeys <= a.sinks);
+    t.step8(
+        tile, ns, hf, inside,
+        [&]() __attribute__((always_inline)) {
+          return now.key < 0 ? 0u : seen_bits(a, p, p.row0 + lr, hf, now.key, there);
+        },
+        [&]() __attribute__((always_inline)) {
+          sc = scales_of(a, p, cur);
+          next = step_of<true>(a, p, table, j + 2);
+        },
+        [&]() __attribute__((always_inline)) {
+          put(st, fill);
+          st = load(next);
+        });
+  };
+  const int rounds = (p.steps + 1) / 2;
+  for (int rd = 0; rd < rounds; ++rd) {
+    iteration(std::integral_constant<int, 0>{}, 2 * rd);
+    iteration(std::integral_constant<int, 1>{}, 2 * rd + 1);
+  }
+
+  // the end of the wavefront's rows
+  const float l = pair_sum(t.l_run), m = t.m_run;
+  const float unit = power_of(t.v_exp);
+  const float inv = l > 0.0f ? unit / l : l;  // (a NaN sum stays one)
+#pragma unroll
+  for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) t.o_acc[dt][r] = l == 0.0f ? 0.0f : t.o_acc[dt][r] * inv;
+  const Row my = row_of(a, p, p.row0 + lr);
+  if (!my.live) return;
+  if (p.shares > 1) {
+    float* const wp = a.ws_o + (ws_row + lr) * D + 4 * hf;
+#pragma unroll
+    for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<v4f*>(wp + 32 * dt + 8 * g) =
+            v4f{t.o_acc[dt][4 * g], t.o_acc[dt][4 * g + 1], t.o_acc[dt][4 * g + 2],
+                t.o_acc[dt][4 * g + 3]};
+    if (hf == 0)
+      a.ws_ml[ws_row + lr] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
+    return;
+  }
+  T* const op = static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(my.qi) * a.so[1] +
+                my.head * a.so[2] + 4 * hf;
+#pragma unroll
+  for (int dt = 0; dt < R::NDT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      typename Half<T>::op4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(t.o_acc[dt][4 * g + e]);
+      *reinterpret_cast<typename Half<T>::op4*>(op + 32 * dt + 8 * g) = w;
+    }
+  if (hf == 0 && a.lse)
+    a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
+        l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+}
+
+template <typename T>
+static void launch_type(WindowArgs& a, bool e4m3, int64_t D, dim3 grid, hipStream_t s) {
+  const dim3 block(256);
+  if (e4m3 && D == 128) cached_tile_kernel<T, true, 128><<<grid, block, 0, s>>>(a);
+  else if (e4m3) cached_tile_kernel<T, true, 64><<<grid, block, 0, s>>>(a);
+  else if (D == 128) cached_tile_kernel<T, false, 128><<<grid, block, 0, s>>>(a);
+  else cached_tile_kernel<T, false, 64><<<grid, block, 0, s>>>(a);
+}
+
+void launch_cached_tile(WindowArgs& a, int type, bool e4m3, int64_t D, dim3 grid, hipStream_t s) {
+  if (type == 0) launch_type<__bf16>(a, e4m3, D, grid, s);
+  else launch_type<_Float16>(a, e4m3, D, grid, s);
+}
+
+}  // namespace rcsa

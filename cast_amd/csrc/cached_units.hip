@@ -1,0 +1,311 @@
+// Attention of few rows over pages of 8-bit codes (one new token of each request, or a few): at
+// most 32 rows of a key head, dealt as in window_units.hip to workgroups of eight wavefronts
+// or to units of one.
+//
+// Codes go from memory to the matrix operands through registers alone: a lane of S = K Q^T
+// holds a key's channels, which are contiguous; a lane of O^T = V^T P^T holds D / 32
+// neighbouring channels of the 16 keys whose weights it has, one load a key (a load
+// instruction covers two whole rows), turned byte by byte into operands.
+#include "cached_attn.h"
+
+namespace rcsa {
+
+template <typename T, bool E4M3, int D, bool GROUP>
+__global__ void __launch_bounds__(GROUP ? 64 * kGroupWaves : 64)
+__attribute__((amdgpu_waves_per_eu(2, 2)))
+cached_unit_kernel(WindowArgs a) {
+  constexpr int NW = GROUP ? kGroupWaves : 1;
+  constexpr int KL = D / 32, NDT = D / 32;  // loads of a key's half row; channels of a lane
+  typedef typename Half<T>::op8 op8;
+  __shared__ __attribute__((aligned(16))) float s_o[GROUP ? NW : 1][GROUP ? kFewRows * D : 4];
+  __shared__ float2 s_ml[NW][kFewRows];
+  const int lane = threadIdx.x & 63, hf = lane >> 5, lr = lane & 31;
+  const int wave = GROUP ? uniform_int(static_cast<int>(threadIdx.x) >> 6) : 0;
+
+  const int w = divide(static_cast<int>(blockIdx.x), a.by_Hk);
+  Unit u;
+  if constexpr (GROUP) {
+    const Request r = request_of<true>(a, w);
+    u = {w, wave, kGroupWaves, 0, {uniform_int(r.k_len), uniform_int(r.q_len)}};
+  } else {
+    u = find_unit<false>(a, w, lane);
+    if (u.b < 0) return;
+  }
+  Place p;
+  p.b = u.b;
+  p.hk = static_cast<int>(blockIdx.x) - w * a.Hk;
+  p.row0 = 0;
+  p.n_rows = u.r.q_len * a.G;
+  if (p.n_rows == 0) return;
+  p.k_len = u.r.k_len;
+  p.shift = u.r.k_len - u.r.q_len;
+  p.shares = u.shares;
+  const KeyRange first = row_range(a, p, 0), last = row_range(a, p, p.n_rows - 1);
+  p.tiles = tiles_of(a, first, last);
+  share_of(p, u.share);
+
+  const char* const kbase = static_cast<const char*>(a.k) + p.hk * a.sk[2];
+  const char* const vbase = static_cast<const char*>(a.v) + p.hk * a.sv[2];
+  const uint32_t krb = static_cast<uint32_t>(a.sk[1]), vrb = static_cast<uint32_t>(a.sv[1]);
+  const int32_t* const table = a.table + p.b * a.table_stride;
+
+  // The lane's row of the queries: step st of the products takes the channels of 8 bytes st & 1
+  // of load st / 2.
+  const Row my = row_of(a, p, lr);
+  v8hf q_op[2 * KL];
+  float c_row;
+  {
+    const T* const row = static_cast<const T*>(a.q) + p.b * a.sq[0] +
+                         static_cast<int64_t>(my.qi) * a.sq[1] + my.head * a.sq[2];
+    op8 raw[2 * KL];
+    float most = 0.0f;
+#pragma unroll
+    for (int st = 0; st < 2 * KL; ++st) {
+      raw[st] = *reinterpret_cast<const op8*>(row + (st >> 1) * 32 + hf * 16 + (st & 1) * 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(static_cast<float>(raw[st][i])));
+    }
+    const int k = row_shift(pair_max(most));
+    const float up = power_of(k);
+#pragma unroll
+    for (int st = 0; st < 2 * KL; ++st) q_op[st] = scaled8<T>(raw[st], up);
+    c_row = a.scale_log2 * power_of(-k);
+  }
+
+  // A step's codes: the lane's key of the tile is lr (16 bytes at hf * 16 of every 32), its
+  // channels of key 8 (r / 4) + 4 hf + r % 4 are NDT lr and the next ones.
+  struct Tile {
+    v4i k[KL];
+    uint32_t v[16];
+  };
+  auto load_k = [&](const Step& s, v4i (&k)[KL]) __attribute__((always_inline)) {
+    const HalfRows h0 = code_rows(a, s, 0, krb, vrb), h1 = code_rows(a, s, 1, krb, vrb);
+    const char* const at = kbase + (lr < 16 ? h0.k : h1.k) + static_cast<uint64_t>(lr & 15) * krb +
+                           hf * 16;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) k[i] = *reinterpret_cast<const v4i*>(at + 32 * i);
+  };
+  auto load_v = [&](const Step& s, uint32_t (&v)[16]) __attribute__((always_inline)) {
+    const int at = static_cast<int>(4 * hf * vrb + NDT * lr);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const HalfRows r = code_rows(a, s, h, krb, vrb);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(vbase) + r.v, 0, 16 * static_cast<int>(vrb), kRsrcWord3);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int off = (8 * (j >> 2) + (j & 3)) * static_cast<int>(vrb);
+        if constexpr (NDT == 4)
+          v[8 * h + j] = static_cast<uint32_t>(
+              __builtin_amdgcn_raw_buffer_load_b32(rs, at, off, 0));
+        else
+          v[8 * h + j] = static_cast<uint16_t>(
+              __builtin_amdgcn_raw_buffer_load_b16(rs, at, off, 0));
+      }
+    }
+  };
+
+  Step cur = step_of<true>(a, p, table, 0), next = step_of<true>(a, p, table, 1);
+  Tile t;
+  load_k(cur, t.k);
+  load_v(cur, t.v);
+  Scales sc = scales_of(a, p, cur);
+  v16f o_acc[NDT];
+#pragma unroll
+  for (int x = 0; x < NDT; ++x)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o_acc[x][r] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+  int v_exp = -126;  // accumulators are in units of 2^v_exp
+  constexpr int kShift = Half<_Float16>::kShift;
+
+  for (int s = 0; s < p.steps; ++s) {
+    const Step now = cur;
+    const Scales ns = sc;
+    v16f s_acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      v8hf lo, hi;
+      widen16<E4M3>(t.k[i], lo, hi);
+      s_acc = Half<_Float16>::mfma(lo, q_op[2 * i], s_acc);
+      s_acc = Half<_Float16>::mfma(hi, q_op[2 * i + 1], s_acc);
+    }
+    cur = next;
+    const bool more = s + 1 < p.steps;
+    if (more) {
+      load_k(cur, t.k);
+      sc = scales_of(a, p, cur);
+      next = step_of<true>(a, p, table, s + 2);
+    }
+    // logits in log2 units: r < 8 of the first half's keys, the others of the second's
+    const float c0 = c_row * ns.k[0], c1 = c_row * ns.k[1];
+    float rv[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) rv[r] = s_acc[r] * (r < 8 ? c0 : c1);
+    const int there = halves_there<true>(a, now);
+    const bool inside = there == 3 && now.key + kTileKeys <= first.hi &&
+                        (now.key >= last.lo || now.key + kTileKeys <= a.sinks);
+    if (!inside) {
+      const uint32_t seen = seen_keys(a, p, lr, now.key, there) >> (4 * hf);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        rv[r] = (seen >> (8 * (r >> 2) + (r & 3))) & 1u ? rv[r] : -INFINITY;
+    }
+    // the scales of the values, relative to the largest so far
+    int e_new = v_exp;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = static_cast<int>(__float_as_uint(ns.v[h]) >> 23) - 126;  // 2^e > the scale
+      e_new = ns.v[h] > 0.0f && e > e_new ? e : e_new;
+    }
+    if (e_new != v_exp) {
+      const int down = v_exp - e_new;
+      const float f = down < -126 ? 0.0f : power_of(down);
+#pragma unroll
+      for (int x = 0; x < NDT; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[x][r] *= f;
+      v_exp = e_new;
+    }
+    const float f0 = ns.v[0] * power_of(-v_exp), f1 = ns.v[1] * power_of(-v_exp);
+    v8hf p_op[2];
+    auto exps = [&]() __attribute__((always_inline)) -> float {
+      const float bias = m_run == -INFINITY ? 0.0f : -m_run;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(rv[r] + bias);
+        p_op[r >> 3][r & 7] = static_cast<_Float16>(e * (r < 8 ? f0 : f1));
+        sum[r & 3] += e;
+      }
+      return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    float part = exps();
+    if (__ballot(m_run == -INFINITY || !(part <= kTauPow * (1 << kShift))) != 0) {
+      float rmax = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
+      rmax = pair_max(rmax);
+      const float m_blk = rmax == -INFINITY ? -INFINITY : rmax - kShift;
+      if (__ballot(m_blk > m_run + kTau) != 0) {
+        const float m_new = fmaxf(m_run, m_blk);
+        const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+        l_run *= alpha;
+#pragma unroll
+        for (int x = 0; x < NDT; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o_acc[x][r] *= alpha;
+        m_run = m_new;
+        part = exps();
+      }
+    }
+    l_run += part;
+    uint32_t tamed[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) tamed[r] = Widen<E4M3>::tame(Widen<E4M3>::finite(t.v[r]));
+    if (more) load_v(cur, t.v);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 0; x < NDT; ++x)
+        o_acc[x] = Half<_Float16>::mfma(column8<E4M3>(x, tamed + 8 * h), p_op[h], o_acc[x]);
+  }
+
+  // The end of the rows: lane (row, hf) holds channels 32 g' + ... : register r of product x is
+  // channel NDT (8 (r / 4) + 4 hf + r % 4) + x.
+  const float l = pair_sum(l_run);
+  const float unit = power_of(v_exp);
+  const float inv = l > 0.0f ? unit / l : l;  // (a NaN sum stays one)
+  auto value = [&](int r, int x) __attribute__((always_inline)) -> float {
+    return l == 0.0f ? 0.0f : o_acc[x][r] * (1 << Widen<E4M3>::kShift) * inv;
+  };
+  const bool live = lr < p.n_rows;
+  if (GROUP || p.shares > 1) {
+    const int64_t ws_row = GROUP ? 0 : static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
+    float* const part_o = GROUP ? s_o[wave] : a.ws_o + ws_row * D;
+    float2* const part_ml = GROUP ? s_ml[wave] : a.ws_ml + ws_row;
+    if (live) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float* const at = part_o + lr * D + NDT * (8 * (r >> 2) + 4 * hf + (r & 3));
+#pragma unroll
+        for (int x = 0; x < NDT; ++x) at[x] = value(r, x);
+      }
+      if (hf == 0)
+        part_ml[lr] = make_float2(l > 0.0f ? m_run : (l == 0.0f ? -INFINITY : l), l);
+    }
+  } else if (live) {
+    T* const op = static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(my.qi) * a.so[1] +
+                  my.head * a.so[2];
+#pragma unroll
+    for (int r = 0; r < 16; r += 4 / NDT) {
+      typename Half<T>::op4 w4;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) w4[x] = static_cast<T>(value(r + x / NDT, x % NDT));
+      *reinterpret_cast<typename Half<T>::op4*>(
+          op + NDT * (8 * (r >> 2) + 4 * hf + (r & 3))) = w4;
+    }
+    if (hf == 0 && a.lse)
+      a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
+          l == 0.0f ? -INFINITY : (m_run + __log2f(l)) * 0.69314718055994531f;
+  }
+  if constexpr (GROUP) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.n_rows * (D / 4); i += 64 * NW) {
+      const int row = i / (D / 4), c = i % (D / 4) * 4;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int s = 0; s < NW; ++s) mx = fmaxf(mx, s_ml[s][row].x);
+      v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      float sum = 0.0f;
+#pragma unroll
+      for (int s = 0; s < NW; ++s) {
+        const float2 ml = s_ml[s][row];
+        if (ml.x == -INFINITY) continue;
+        const float f = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
+        sum += f;
+        const v4f o = *reinterpret_cast<const v4f*>(s_o[s] + row * D + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = join(f, o[e], acc[e]);
+      }
+      const Row r = row_of(a, p, row);
+      typename Half<T>::op4 out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+      *reinterpret_cast<typename Half<T>::op4*>(
+          static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(r.qi) * a.so[1] +
+          r.head * a.so[2] + c) = out;
+      if (a.lse && c == 0)
+        a.lse[(static_cast<int64_t>(p.b) * a.Hq + r.head) * a.Lq + r.qi] =
+            sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
+    }
+  }
+}
+
+template <typename T, bool E4M3, int D>
+static int launch(WindowArgs& a, int64_t units, hipStream_t s) {
+  if (a.units == 0) {
+    const dim3 grid(static_cast<unsigned>(a.B * a.Hk)), block(64 * kGroupWaves);
+    cached_unit_kernel<T, E4M3, D, true><<<grid, block, 0, s>>>(a);
+    return launch_status();
+  }
+  cached_unit_kernel<T, E4M3, D, false>
+      <<<dim3(static_cast<unsigned>(units)), dim3(64), 0, s>>>(a);
+  return launch_unit_merge(a, std::is_same<T, __bf16>::value ? 0 : 1, D, s);
+}
+
+template <typename T>
+static int launch_type(WindowArgs& a, bool e4m3, int64_t D, int64_t units, hipStream_t s) {
+  if (e4m3) return D == 128 ? launch<T, true, 128>(a, units, s) : launch<T, true, 64>(a, units, s);
+  return D == 128 ? launch<T, false, 128>(a, units, s) : launch<T, false, 64>(a, units, s);
+}
+
+int launch_cached_units(WindowArgs& a, int type, bool e4m3, int64_t D, int64_t units,
+                        hipStream_t s) {
+  return type == 0 ? launch_type<__bf16>(a, e4m3, D, units, s)
+                   : launch_type<_Float16>(a, e4m3, D, units, s);
+}
+
+}  // namespace rcsa

@@ -54,6 +54,7 @@ struct Api {
   decltype(&rcsa_window_attn_plan) window_attn_plan = nullptr;
   decltype(&rcsa_window_attn_workspace_bytes_for) window_attn_workspace_bytes = nullptr;
   decltype(&rcsa_window_attn) window_attn = nullptr;
+  decltype(&rcsa_cached_attn) cached_attn = nullptr;
   decltype(&rcsa_append_cache) append_cache = nullptr;
   decltype(&rcsa_read_cache) read_cache = nullptr;
 };
@@ -93,6 +94,7 @@ void bind_library(const std::string& path) {
   bind_one(h, "rcsa_window_attn_plan", api.window_attn_plan);
   bind_one(h, "rcsa_window_attn_workspace_bytes_for", api.window_attn_workspace_bytes);
   bind_one(h, "rcsa_window_attn", api.window_attn);
+  bind_one(h, "rcsa_cached_attn", api.cached_attn);
   bind_one(h, "rcsa_append_cache", api.append_cache);
   bind_one(h, "rcsa_read_cache", api.read_cache);
   g_api = api;
@@ -1272,13 +1274,15 @@ std::vector<at::Tensor> read_cache(
 }
 
 // Dense (k, v [B, Lk, Hk, D]) or, with a table, paged (k, v [pages, slots, Hk, D])
-// attention over a window and the first keys; n_split -2: planned.  (out) or (out, lse).
+// attention over a window and the first keys; pages may be codes with their scales; n_split
+// -2: planned.  (out) or (out, lse).
 std::vector<at::Tensor> window_attention(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
     const c10::optional<at::Tensor>& table, const c10::optional<at::Tensor>& q_lengths,
     const c10::optional<at::Tensor>& k_lengths, int64_t window, int64_t sinks, int64_t block,
     c10::optional<double> sm_scale, bool return_lse, const c10::optional<at::Tensor>& out_,
-    int64_t n_split, int64_t max_keys) {
+    int64_t n_split, int64_t max_keys, const c10::optional<at::Tensor>& k_scale,
+    const c10::optional<at::Tensor>& v_scale) {
   const bool paged = table.has_value();
   const char* op = paged ? "paged_attention" : "window_attention";
   const Api& a = api(op);
@@ -1289,12 +1293,22 @@ std::vector<at::Tensor> window_attention(
   input(op, dev, grads, v, "v");
   input(op, dev, grads, out_, "out");
   for (const auto* t : {&table, &q_lengths, &k_lengths}) input(op, dev, false, *t, "an operand");
+  const bool codes = k_scale.has_value();
+  TORCH_CHECK_VALUE(codes == v_scale.has_value() && (paged || !codes), op,
+                    ": give both scales, with pages");
+  input(op, dev, grads, k_scale, "the cache");
+  input(op, dev, grads, v_scale, "the cache");
   const at::ScalarType dt = q.scalar_type();
-  TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf, op,
-                   ": q, k and v must share bfloat16 or float16, q is ", dt);
+  TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf, op, codes ? ": q must be" :
+                   ": q, k and v must share", " bfloat16 or float16, q is ", dt);
   want_heads(op, q, dt, "q");
-  want_heads(op, k, dt, "k");
-  want_heads(op, v, dt, "v");
+  Cache8 c8{};
+  if (codes) {
+    c8 = want_cache8(op, k, v, *k_scale, *v_scale, *table, q.size(0));
+  } else {
+    want_heads(op, k, dt, "k");
+    want_heads(op, v, dt, "v");
+  }
   const int64_t B = q.size(0), Lq = q.size(1), Hq = q.size(2), D = q.size(3), Hk = k.size(2);
   TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(3) == D && (paged || k.size(0) == B) &&
                         Hk > 0 && Hq % Hk == 0, op, ": q ", q.sizes(), " needs k and v ",
@@ -1325,6 +1339,10 @@ std::vector<at::Tensor> window_attention(
     want_apart(op, out, "out", q, "q");
     want_apart(op, out, "out", k, "k");
     want_apart(op, out, "out", v, "v");
+    if (codes) {
+      want_apart(op, out, "out", *k_scale, "the key scales");
+      want_apart(op, out, "out", *v_scale, "the value scales");
+    }
   }
   std::vector<at::Tensor> res{out};
   if (return_lse) res.push_back(at::empty({B, Hq, Lq}, q.options().dtype(at::kFloat)));
@@ -1346,13 +1364,27 @@ std::vector<at::Tensor> window_attention(
   TORCH_CHECK(ws_bytes >= 0, op, ": no launch of ", ns, " shares for q ", q.sizes(), ", k ",
               k.sizes());
   if (ws_bytes > 0) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+  const double scale = sm_scale ? *sm_scale : 1.0 / std::sqrt(D);
+  if (codes) {
+    int64_t ss[6];
+    put_scale_strides(*k_scale, ss);
+    put_scale_strides(*v_scale, ss + 3);
+    check_status(a, op, a.cached_attn(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), c8.code, k_scale->data_ptr<float>(),
+        v_scale->data_ptr<float>(), out.data_ptr(), return_lse ? ptr<float>(res[1]) : nullptr,
+        dt == at::kBFloat16 ? RCSA_BF16 : RCSA_F16, dims, s, ss, ptr<const int32_t>(q_lengths),
+        ptr<const int32_t>(k_lengths), ptr<const int32_t>(table), table_stride, max_pages, n_pages,
+        page, c8.block, window, sinks, block, static_cast<float>(scale), ns,
+        ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
+    return res;
+  }
   const bool none = !paged && Lk == 0;  // no keys: no key memory either
   check_status(a, op, a.window_attn(
       q.data_ptr(), none ? q.data_ptr() : k.data_ptr(), none ? q.data_ptr() : v.data_ptr(),
       out.data_ptr(), return_lse ? ptr<float>(res[1]) : nullptr,
       dt == at::kBFloat16 ? RCSA_BF16 : RCSA_F16, dims, s, ptr<const int32_t>(q_lengths),
       ptr<const int32_t>(k_lengths), ptr<const int32_t>(table), table_stride, max_pages, n_pages,
-      page, window, sinks, block, static_cast<float>(sm_scale ? *sm_scale : 1.0 / std::sqrt(D)), ns,
+      page, window, sinks, block, static_cast<float>(scale), ns,
       ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
   return res;
 }
@@ -1422,7 +1454,8 @@ TORCH_LIBRARY(rcsa, m) {
   m.def(
       "window_attention(Tensor q, Tensor k, Tensor v, Tensor? table, Tensor? q_lengths, "
       "Tensor? k_lengths, int window, int sinks, int block, float? sm_scale, bool return_lse, "
-      "Tensor(a!)? out, int n_split, int max_keys) -> Tensor[]",
+      "Tensor(a!)? out, int n_split, int max_keys, Tensor? k_scale=None, Tensor? v_scale=None) "
+      "-> Tensor[]",
       &window_attention);
   m.def(
       "append_cache(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) v_codes, "

@@ -45,6 +45,11 @@ struct WindowArgs {
   // round-robin.
   int xcd_items, xcd_whole;
   int descending;
+  // pages of 8-bit codes: their scales [page][block][head], 16 keys of a block
+  const float *ks, *vs;
+  int64_t sks[3], svs[3];
+  Divisor by_half_mark;
+  int e4m3;        // the codes' type; -1: 16-bit keys and values
   int units;       // few rows in units: wavefronts of one round
   float per_unit;  // 1 / units
 };
@@ -703,5 +708,6 @@ void launch_window_paged(WindowArgs& a, int type, int64_t D, dim3 grid, hipStrea
 // Few rows (window_units.hip): in units and their join, or one workgroup a key head
 // (a.units 0); `units` of them are launched.
 int launch_window_units(WindowArgs& a, int type, int64_t D, int64_t units, hipStream_t s);
+int launch_unit_merge(WindowArgs& a, int type, int64_t D, hipStream_t s);
 
 }  // namespace rcsa

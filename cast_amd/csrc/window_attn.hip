@@ -1,5 +1,6 @@
 // Windowed attention, blocks of 128 rows: the dense form, the join of split blocks, plans and
 // the entry points (the paged form is in a source of its own: see window_paged.hip).
+#include "cached_attn.h"
 #include "window_tile.h"
 
 namespace rcsa {
@@ -56,7 +57,9 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
   const int64_t wgs = (a.xcd_whole + tail * a.n_split) * kNumXcd;
   if (wgs * 256 >= kMaxThreads) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs));
-  if (a.table) launch_window_paged(a, std::is_same<T, __bf16>::value ? 0 : 1, D, grid, s);
+  constexpr int type = std::is_same<T, __bf16>::value ? 0 : 1;
+  if (a.e4m3 >= 0) launch_cached_tile(a, type, a.e4m3 == 1, D, grid, s);
+  else if (a.table) launch_window_paged(a, type, D, grid, s);
   else window_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
   if (a.n_split > 1 && tail > 0) {
     const int64_t n = (tail * kNumXcd * 128 * (D / 8) + 255) / 256;
@@ -187,14 +190,20 @@ extern "C" int64_t rcsa_window_attn_workspace_bytes(const int64_t* dims, int64_t
   return rcsa_window_attn_workspace_bytes_for(dims, n_split, kMostKeys, 0, 0);
 }
 
-extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
-                                int dtype, const int64_t* dims, const int64_t* strides,
-                                const int32_t* q_lengths, const int32_t* k_lengths,
-                                const int32_t* block_table, int64_t table_stride,
-                                int64_t max_pages, int64_t n_pages, int64_t page_size,
-                                int64_t window, int64_t sinks, int64_t block, float sm_scale,
-                                int64_t n_split, void* workspace, int64_t workspace_bytes,
-                                hipStream_t stream) {
+// Pages of codes: their type, scales and the keys of a scale.
+struct CodePages {
+  bool e4m3;
+  const float *ks, *vs;
+  const int64_t* strides;  // page, block, head of both
+  int64_t block_size;
+};
+
+static int run(const void* q, const void* k, const void* v, void* out, float* lse, int dtype,
+               const CodePages* codes, const int64_t* dims, const int64_t* strides,
+               const int32_t* q_lengths, const int32_t* k_lengths, const int32_t* block_table,
+               int64_t table_stride, int64_t max_pages, int64_t n_pages, int64_t page_size,
+               int64_t window, int64_t sinks, int64_t block, float sm_scale, int64_t n_split,
+               void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   if (!q || !k || !v || !out || !dims || !strides) return RCSA_ERR_NULL;
   if (dtype != RCSA_BF16 && dtype != RCSA_F16) return RCSA_ERR_DTYPE;
   // (a masked logit is -inf before the scale; a zero one stays zero under a finite one)
@@ -207,7 +216,8 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
                       n_pages >= most || page_size >= most || max_pages >= most / page_size))
     return RCSA_ERR_SHAPE;
   for (int i = 0; i < 12; ++i)
-    if (strides[i] < 0 || strides[i] % (i < 9 ? 8 : 4)) return RCSA_ERR_STRIDE;
+    if (strides[i] < 0 || strides[i] % (i < 3 ? 8 : i < 9 ? (codes ? 16 : 8) : 4))
+      return RCSA_ERR_STRIDE;
   if (block_table && (strides[3] >= (1ll << 31) || strides[6] >= (1ll << 31)))
     return RCSA_ERR_STRIDE;
   // (rows of keys do not overlap; the stride of a single one says nothing)
@@ -269,15 +279,63 @@ extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, voi
   a.xcd_whole = static_cast<int>(xcd_whole_of(xcd_items, n_split));
   // rows without a window see more keys the later they stand
   a.descending = a.window == 0 && a.block != 0;
+  if (codes) {
+    a.ks = codes->ks;
+    a.vs = codes->vs;
+    for (int i = 0; i < 3; ++i) {
+      a.sks[i] = codes->strides[i];
+      a.svs[i] = codes->strides[3 + i];
+    }
+    a.by_half_mark = divisor(static_cast<uint32_t>(codes->block_size / 16));
+  }
   const int64_t ws_rows = need / (dims[5] * 4 + 8);
   a.ws_o = static_cast<float*>(workspace);
   a.ws_ml = need ? reinterpret_cast<float2*>(a.ws_o + ws_rows * dims[5]) : nullptr;
-  if (n_split < 1)
-    return launch_window_units(a, dtype == RCSA_BF16 ? 0 : 1, dims[5],
-                               units_of_launch(dims, storage, a.window, a.sinks), stream);
+  const int type = dtype == RCSA_BF16 ? 0 : 1;
+  if (n_split < 1) {
+    const int64_t units = units_of_launch(dims, storage, a.window, a.sinks);
+    return codes ? launch_cached_units(a, type, codes->e4m3, dims[5], units, stream)
+                 : launch_window_units(a, type, dims[5], units, stream);
+  }
+  a.e4m3 = codes ? (codes->e4m3 ? 1 : 0) : -1;
   if (dtype == RCSA_BF16)
     return dims[5] == 128 ? launch_window<__bf16, 128>(a, stream)
                           : launch_window<__bf16, 64>(a, stream);
   return dims[5] == 128 ? launch_window<_Float16, 128>(a, stream)
                         : launch_window<_Float16, 64>(a, stream);
+}
+
+extern "C" int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, float* lse,
+                                int dtype, const int64_t* dims, const int64_t* strides,
+                                const int32_t* q_lengths, const int32_t* k_lengths,
+                                const int32_t* block_table, int64_t table_stride,
+                                int64_t max_pages, int64_t n_pages, int64_t page_size,
+                                int64_t window, int64_t sinks, int64_t block, float sm_scale,
+                                int64_t n_split, void* workspace, int64_t workspace_bytes,
+                                hipStream_t stream) {
+  return run(q, k, v, out, lse, dtype, nullptr, dims, strides, q_lengths, k_lengths, block_table,
+             table_stride, max_pages, n_pages, page_size, window, sinks, block, sm_scale, n_split,
+             workspace, workspace_bytes, stream);
+}
+
+extern "C" int rcsa_cached_attn(const void* q, const void* k_codes, const void* v_codes, int code,
+                                const float* k_scales, const float* v_scales, void* out,
+                                float* lse, int dtype, const int64_t* dims,
+                                const int64_t* strides, const int64_t* scale_strides,
+                                const int32_t* q_lengths, const int32_t* k_lengths,
+                                const int32_t* block_table, int64_t table_stride,
+                                int64_t max_pages, int64_t n_pages, int64_t page_size,
+                                int64_t block_size, int64_t window, int64_t sinks, int64_t block,
+                                float sm_scale, int64_t n_split, void* workspace,
+                                int64_t workspace_bytes, hipStream_t stream) {
+  if (!k_scales || !v_scales || !scale_strides || !block_table) return RCSA_ERR_NULL;
+  if (code != RCSA_CODE_INT8 && code != RCSA_CODE_E4M3) return RCSA_ERR_DTYPE;
+  if (block_size <= 0 || block_size % 16 || page_size <= 0 || page_size % block_size)
+    return RCSA_ERR_SHAPE;
+  for (int i = 0; i < 6; ++i)
+    if (scale_strides[i] < 0) return RCSA_ERR_STRIDE;
+  const CodePages codes = {code == RCSA_CODE_E4M3, k_scales, v_scales, scale_strides, block_size};
+  return run(q, k_codes, v_codes, out, lse, dtype, &codes, dims, strides, q_lengths, k_lengths,
+             block_table, table_stride, max_pages, n_pages, page_size, window, sinks, block,
+             sm_scale, n_split, workspace, workspace_bytes, stream);
 }

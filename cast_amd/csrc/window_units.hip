@@ -222,6 +222,14 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
 }
 
 template <typename T, int D>
+static int merge(WindowArgs& a, hipStream_t s) {
+  // (at most 2^24 rows, of 256 threads: units_fit)
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * a.Lq * a.G;
+  window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
+  return launch_status();
+}
+
+template <typename T, int D>
 static int launch_units(WindowArgs& a, int64_t units, hipStream_t s) {
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hk;
   if (a.units == 0) {
@@ -230,12 +238,15 @@ static int launch_units(WindowArgs& a, int64_t units, hipStream_t s) {
     else window_unit_kernel<T, D, false, true><<<grid, block, 0, s>>>(a);
     return launch_status();
   }
-  const int64_t rows = heads * a.Lq * a.G;  // (at most 2^24, of 256 threads: units_fit)
   const dim3 grid(static_cast<unsigned>(units)), block(64);
   if (a.table) window_unit_kernel<T, D, true, false><<<grid, block, 0, s>>>(a);
   else window_unit_kernel<T, D, false, false><<<grid, block, 0, s>>>(a);
-  window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
-  return launch_status();
+  return merge<T, D>(a, s);
+}
+
+int launch_unit_merge(WindowArgs& a, int type, int64_t D, hipStream_t s) {
+  if (type == 0) return D == 128 ? merge<__bf16, 128>(a, s) : merge<__bf16, 64>(a, s);
+  return D == 128 ? merge<_Float16, 128>(a, s) : merge<_Float16, 64>(a, s);
 }
 
 int launch_window_units(WindowArgs& a, int type, int64_t D, int64_t units, hipStream_t s) {

@@ -1336,7 +1336,7 @@ def _shares(n_split: Optional[int], fn: str) -> int:
     return -2 if n_split is None else int(n_split)
 
 
-def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *,
+def paged_attention(q: torch.Tensor, cache: PagedCache | QuantizedCache, lengths: torch.Tensor, *,
                     q_lengths: Optional[torch.Tensor] = None, window: Optional[int] = None,
                     sinks: int = 0, block: int = 1, causal: bool = True,
                     sm_scale: Optional[float] = None, return_lse: bool = False,
@@ -1346,6 +1346,11 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
     (one new token, or a chunk), over a :class:`PagedCache`: ``lengths`` (int32 ``[B]``) keys
     of each request, the new ones among them.  Pages hold a multiple of 16 keys.
 
+    Over a :class:`QuantizedCache` (``rcsa_cached_attn``) keys and values are the c * s that its
+    codes stand for; q and the products are of 16 bits, the weights of fp16 with their value's scale.
+    A scale that is no positive number below 2^126 counts as 0, and so does a value's e4m3 code
+    that holds no number (:func:`append_cache` writes none).
+
     Pages that no row sees are not read, so their table entries may be anything; an entry
     outside the pages hides its keys; tables may share pages.  ``max_length`` bounds the lengths (what the table
     holds, if None): it only plans how the keys are shared among workgroups, a longer
@@ -1353,7 +1358,8 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, lengths: torch.Tensor, *
     fn = "paged_attention"
     w, s, b = _window(window, sinks, block, causal, fn)
     scale = _sm_scale(sm_scale, fn)
+    scales = (cache.k_scale, cache.v_scale) if isinstance(cache, QuantizedCache) else ()
     res = _lib.torch_ops().window_attention(
         q, cache.k, cache.v, cache.table, q_lengths, lengths, w, s, b, scale, return_lse, out,
-        _shares(n_split, fn), -1 if max_length is None else int(max_length))
+        _shares(n_split, fn), -1 if max_length is None else int(max_length), *scales)
     return tuple(res) if return_lse else res[0]

@@ -831,6 +831,26 @@ int rcsa_read_cache(const void* k_codes, const void* v_codes, int code, const fl
                     int64_t max_pages, int64_t n_pages, int64_t page_size, int64_t block_size,
                     hipStream_t stream);
 
+/*
+ * rcsa_cached_attn: rcsa_window_attn over such pages; q and out bf16 or fp16, D 64 or 128,
+ *   out = softmax(sm_scale q . (c_k s_k)) (c_v s_v).
+ * Arguments as there, with the type of the codes, their scales (scale_strides: host array of 6,
+ * page, block, head of the scales of keys and of values) and block_size; block_table and
+ * k_lengths are wanted.  A scale that is no positive number below 2^126 counts as 0; a value
+ * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.
+ * Token (slot) strides and pointers of the codes are multiples of 16.  The plan and the workspace
+ * are rcsa_window_attn's.
+ */
+int rcsa_cached_attn(const void* q, const void* k_codes, const void* v_codes, int code,
+                     const float* k_scales, const float* v_scales, void* out, float* lse,
+                     int dtype, const int64_t* dims, const int64_t* strides,
+                     const int64_t* scale_strides, const int32_t* q_lengths,
+                     const int32_t* k_lengths, const int32_t* block_table, int64_t table_stride,
+                     int64_t max_pages, int64_t n_pages, int64_t page_size, int64_t block_size,
+                     int64_t window, int64_t sinks, int64_t block, float sm_scale,
+                     int64_t n_split, void* workspace, int64_t workspace_bytes,
+                     hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

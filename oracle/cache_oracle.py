@@ -70,3 +70,19 @@ def read(v, scales, table, block, lo, hi):
         if 0 <= page < n_pages:
             out[j - lo] = v[page, row] * scales[page, row // block, :, None]
     return out
+
+
+def attention(q, k, v, v_top, seen, sm_scale, dtype):
+    """``streaming_oracle.attention`` of the values that codes stand for (k, v in fp64), and the
+    bounds of a kernel that rounds a weight times its block's scale to fp16: half a step, 2^-11,
+    of it; the type's least half step, 2^-25, where the largest weight is 2^7 at least and a
+    scale's unit at most twice the largest scale, so 2^-31 of the largest weight and of
+    ``v_top``, the largest scale times the largest code; and the result's own rounding."""
+    from oracle import streaming_oracle as so
+    top = float(v.abs().max()) if v.numel() else 0.0
+    step = 2.0 ** -31 * (v_top / top if top > 0.0 else 0.0)
+    out, lse, tol, ltol = so.attention(q, k, v, seen, sm_scale, torch.float16, weight_step=step)
+    tol = tol + out.abs() * (so.HALF_STEP[dtype] - so.HALF_STEP[torch.float16])
+    if dtype == torch.bfloat16:
+        tol = (tol - so.TINY[torch.float16]).clamp(min=0.0)  # (without keys it is not in it)
+    return out, lse, tol, ltol
