@@ -87,6 +87,9 @@ SIGNATURES: dict[str, list] = {
     "rcsa_window_attn_workspace_bytes_for": [_P, _I, _I, _I, _I],
     "rcsa_window_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _P] + [_I] * 7 + [c_float, _I, _P, _I,
                                                                              _P],
+    "rcsa_packed_attn_plan": [_P, _I, ctypes.POINTER(c_int64)],
+    "rcsa_packed_attn_workspace_bytes": [_P, _I],
+    "rcsa_packed_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _I, _I, _I, c_float, _I, _P, _I, _P],
     "rcsa_cached_attn": [_P, _P, _P, c_int, _P, _P, _P, _P, c_int] + [_P] * 6 + [_I] * 8
                         + [c_float, _I, _P, _I, _P],
     "rcsa_append_cache": [_P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P, _P, _P] + [_I] * 5
@@ -124,7 +127,8 @@ def load() -> ctypes.CDLL:
                                                "rcsa_attn_noalloc_scratch_bytes",
                                                "rcsa_order_lists_max_blocks",
                                                "rcsa_window_attn_workspace_bytes",
-                                               "rcsa_window_attn_workspace_bytes_for")
+                                               "rcsa_window_attn_workspace_bytes_for",
+                                               "rcsa_packed_attn_workspace_bytes")
                       else c_int)
     _lib = lib
     return lib

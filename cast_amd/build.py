@@ -56,6 +56,7 @@ FILE_FLAGS = {
     "sparse_attn_shapes.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
     "sparse_attn_bf16_cu3.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
     "window_attn.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "window_packed.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
     "window_paged.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
 }
 

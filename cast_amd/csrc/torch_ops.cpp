@@ -9,8 +9,9 @@
 // bad layout.  Every tensor is checked to span the elements the call's dims
 // and strides reach, so no argument combination makes a kernel read or write
 // past the tensors it was given.  Nothing here synchronises, and nothing but
-// layer_call, order_lists, valid_bits, rope, norm_rope, read_cache and window_attention,
-// which allocate their outputs (and the last its workspace), allocates device memory.
+// layer_call, order_lists, valid_bits, rope, norm_rope, read_cache, window_attention
+// and packed_attention, which allocate their outputs (and the last two their workspace),
+// allocates device memory.
 //
 // The C ABI is bound at load time (rcsa::bind_library) from the library the
 // Python side loaded, so one librcsa.so serves both the ctypes binding and
@@ -55,6 +56,9 @@ struct Api {
   decltype(&rcsa_window_attn_workspace_bytes_for) window_attn_workspace_bytes = nullptr;
   decltype(&rcsa_window_attn) window_attn = nullptr;
   decltype(&rcsa_cached_attn) cached_attn = nullptr;
+  decltype(&rcsa_packed_attn_plan) packed_attn_plan = nullptr;
+  decltype(&rcsa_packed_attn_workspace_bytes) packed_attn_workspace_bytes = nullptr;
+  decltype(&rcsa_packed_attn) packed_attn = nullptr;
   decltype(&rcsa_append_cache) append_cache = nullptr;
   decltype(&rcsa_read_cache) read_cache = nullptr;
 };
@@ -95,6 +99,9 @@ void bind_library(const std::string& path) {
   bind_one(h, "rcsa_window_attn_workspace_bytes_for", api.window_attn_workspace_bytes);
   bind_one(h, "rcsa_window_attn", api.window_attn);
   bind_one(h, "rcsa_cached_attn", api.cached_attn);
+  bind_one(h, "rcsa_packed_attn_plan", api.packed_attn_plan);
+  bind_one(h, "rcsa_packed_attn_workspace_bytes", api.packed_attn_workspace_bytes);
+  bind_one(h, "rcsa_packed_attn", api.packed_attn);
   bind_one(h, "rcsa_append_cache", api.append_cache);
   bind_one(h, "rcsa_read_cache", api.read_cache);
   g_api = api;
@@ -1389,6 +1396,88 @@ std::vector<at::Tensor> window_attention(
   return res;
 }
 
+// Attention over packed requests; n_split 0: planned.  (out) or (out, lse).
+std::vector<at::Tensor> packed_attention(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
+    const c10::optional<at::Tensor>& k_offsets_, int64_t window, int64_t sinks, int64_t block,
+    c10::optional<double> sm_scale, bool return_lse, const c10::optional<at::Tensor>& out_,
+    int64_t n_split) {
+  const char* op = "packed_attention";
+  const Api& a = api(op);
+  const bool grads = at::GradMode::is_enabled();
+  int dev = -1;
+  input(op, dev, grads, q, "q");
+  input(op, dev, grads, k, "k");
+  input(op, dev, grads, v, "v");
+  input(op, dev, grads, out_, "out");
+  input(op, dev, false, offsets, "offsets");
+  input(op, dev, false, k_offsets_, "k_offsets");
+  const at::ScalarType dt = q.scalar_type();
+  TORCH_CHECK_TYPE(dt == at::kBFloat16 || dt == at::kHalf, op,
+                   ": q, k and v must share bfloat16 or float16, q is ", dt);
+  const std::pair<const at::Tensor*, const char*> ins[3] = {{&q, "q"}, {&k, "k"}, {&v, "v"}};
+  for (const auto& t : ins) {
+    TORCH_CHECK_TYPE(t.first->scalar_type() == dt, op, ": q, k and v must share a dtype, ", t.second,
+                     " is ", t.first->scalar_type(), " beside ", dt);
+    TORCH_CHECK_VALUE(t.first->dim() == 3 && (t.first->stride(2) == 1 || t.first->size(2) <= 1), op,
+                      ": ", t.second, " must be [T, H, D] with a contiguous last dim, got ",
+                      t.first->sizes());
+  }
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), Tk = k.size(0), Hk = k.size(1);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(2) == D && Hk > 0 && Hq % Hk == 0, op, ": q ",
+                    q.sizes(), " needs k and v [Tk, a divisor of its heads, ", D, "], got ",
+                    k.sizes(), " and ", v.sizes());
+  TORCH_CHECK(D > 0, op, ": no channels");
+  TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) > 0, op, ": offsets must be int32 [B + 1]");
+  const int64_t B = offsets.size(0) - 1;
+  const at::Tensor& k_offsets = k_offsets_.has_value() ? *k_offsets_ : offsets;
+  for (const auto* t : {&offsets, &k_offsets}) {
+    want(op, *t, at::kInt, "offsets");
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == B + 1 && t->is_contiguous(), op,
+                ": offsets must be int32 [B + 1]");
+  }
+  TORCH_CHECK_VALUE(k_offsets_.has_value() || T == Tk, op,
+                    ": k and v have the rows of q unless k_offsets is given");
+  const Launch l(device_of(op, dev));
+  const at::Tensor out = out_.has_value() ? *out_ : at::empty({T, Hq, D}, q.options());
+  want(op, out, dt, "out");
+  TORCH_CHECK(out.sizes() == q.sizes() && (out.stride(2) == 1 || D <= 1), op,
+              ": out must have q's shape and a contiguous last dim");
+  want_own(op, out, "out");
+  if (out_.has_value()) {
+    want_apart(op, out, "out", q, "q");
+    want_apart(op, out, "out", k, "k");
+    want_apart(op, out, "out", v, "v");
+  }
+  std::vector<at::Tensor> res{out};
+  if (return_lse) res.push_back(at::empty({Hq, T}, q.options().dtype(at::kFloat)));
+  if (q.numel() == 0 || B == 0) return res;
+  const int64_t dims[6] = {B, T, Tk, Hq, Hk, D};
+  int64_t s[8], i = 0;
+  for (const at::Tensor* t : {&q, &k, &v, &out})
+    for (int64_t d = 0; d < 2; ++d) s[i++] = t->size(d) > 1 ? t->stride(d) : 0;
+  int64_t ns = n_split;
+  if (ns < 1) {
+    int64_t most = Tk;
+    if (window > 0 && window < Tk && sinks < Tk) most = std::min(most, window + sinks + 128);
+    check_status(a, op, a.packed_attn_plan(dims, most, &ns));
+  }
+  at::Tensor ws;
+  const int64_t ws_bytes = a.packed_attn_workspace_bytes(dims, ns);
+  TORCH_CHECK(ws_bytes >= 0, op, ": no launch of ", ns, " shares for q ", q.sizes(), ", k ",
+              k.sizes(), " and ", B, " requests");
+  if (ws_bytes > 0) ws = at::empty({ws_bytes}, q.options().dtype(at::kByte));
+  const bool none = Tk == 0;  // no keys: no key memory either
+  check_status(a, op, a.packed_attn(
+      q.data_ptr(), none ? q.data_ptr() : k.data_ptr(), none ? q.data_ptr() : v.data_ptr(),
+      out.data_ptr(), return_lse ? ptr<float>(res[1]) : nullptr,
+      dt == at::kBFloat16 ? RCSA_BF16 : RCSA_F16, dims, s, offsets.data_ptr<int32_t>(),
+      k_offsets.data_ptr<int32_t>(), window, sinks, block,
+      static_cast<float>(sm_scale ? *sm_scale : 1.0 / std::sqrt(D)), ns,
+      ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, l.stream));
+  return res;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(rcsa, m) {
@@ -1457,6 +1546,11 @@ TORCH_LIBRARY(rcsa, m) {
       "Tensor(a!)? out, int n_split, int max_keys, Tensor? k_scale=None, Tensor? v_scale=None) "
       "-> Tensor[]",
       &window_attention);
+  m.def(
+      "packed_attention(Tensor q, Tensor k, Tensor v, Tensor offsets, Tensor? k_offsets, "
+      "int window, int sinks, int block, float? sm_scale, bool return_lse, Tensor(a!)? out, "
+      "int n_split) -> Tensor[]",
+      &packed_attention);
   m.def(
       "append_cache(Tensor k, Tensor v, Tensor(a!) k_codes, Tensor(b!) v_codes, "
       "Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor table, Tensor? starts, Tensor? lengths, "

@@ -9,8 +9,10 @@
 //   out = softmax_j(sm_scale q . k_j) v,  lse = log sum_j exp(sm_scale q . k_j).
 // The G = Hq / Hk query heads of a key head are rows of one problem: row r is
 // query r / G of head hk * G + r % G, so every staged key serves all of them and
-// a tile of rows spans few positions.
+// a tile of rows spans few positions.  Packed requests stand behind each other in q and in k
+// and v; the batch and key lengths of the dense form are their offsets.
 #pragma once
+#include "packed.h"
 #include "sparse_attn_kernel.h"
 
 namespace rcsa {
@@ -19,6 +21,7 @@ typedef _Float16 v8hf __attribute__((ext_vector_type(8)));
 typedef _Float16 v4hf __attribute__((ext_vector_type(4)));
 
 constexpr int kTileKeys = 32;
+constexpr int kDense = 0, kPaged = 1, kPacked = 2;  // forms of keys and values
 
 struct WindowArgs {
   const void *q, *k, *v;
@@ -50,6 +53,10 @@ struct WindowArgs {
   int64_t sks[3], svs[3];
   Divisor by_half_mark;
   int e4m3;        // the codes' type; -1: 16-bit keys and values
+  // packed: rows of the requests in q and in k, v ([B + 1] each), a request's row blocks
+  // numbered through n_ranks
+  const int32_t *q_off, *k_off;
+  int n_ranks;
   int units;       // few rows in units: wavefronts of one round
   float per_unit;  // 1 / units
 };
@@ -255,9 +262,26 @@ struct Half<_Float16> {
 // share's, one of `shares`.
 struct Place {
   int b, hk, row0, n_rows, shift, k_len;
+  int q0, k0;  // packed: the request's first rows
   int shares, begin, steps;
   Tiles tiles;
 };
+// Where a request's queries and outputs (s: strides), and the keys or values of its key head,
+// begin, in elements.
+template <int FORM, typename S>
+__device__ __forceinline__ int64_t rows_at(const Place& p, S& s) {
+  return FORM == kPacked ? p.q0 * s[1] : p.b * s[0];
+}
+template <int FORM, typename S>
+__device__ __forceinline__ int64_t keys_at(const Place& p, S& s) {
+  return (FORM == kPaged ? 0 : FORM == kPacked ? p.k0 * s[1] : p.b * s[0]) + p.hk * s[2];
+}
+// Its place in lse ([B][Hq][Lq], packed [Hq][Lq]).
+template <int FORM, typename A>
+__device__ __forceinline__ int64_t lse_at(A& a, const Place& p, int head, int qi) {
+  return FORM == kPacked ? static_cast<int64_t>(head) * a.Lq + p.q0 + qi
+                         : (static_cast<int64_t>(p.b) * a.Hq + head) * a.Lq + qi;
+}
 // First key of step s, -1 past the last.
 __device__ __forceinline__ int key_of(const Place& p, int s) {
   const int t = p.begin + s;
@@ -528,18 +552,17 @@ __device__ __forceinline__ int lane_again() {
 // sees their key.  One load at a time, five to seven times the first pass (32K causal
 // tokens x 32 heads, every head's first value infinite, so that all rows are taken again: on
 // 8 key heads 43 ms in all, without it 7.4, on 32 57 and 7.3); batches of loads spill.
-template <typename T, int D, bool PAGED>
+template <typename T, int D, int FORM>
 __device__ __forceinline__ void rows_again(LateArgs& a, const Place& p, RowTile<T, D>& t,
                                            int lane, float m, char* lds) {
   using R = RowTile<T, D>;
   typedef typename R::op8 op8;
+  constexpr bool PAGED = FORM == kPaged;
   constexpr int RPU = 1024 / R::KROW, LOADS = R::TILE / 1024;
   constexpr uint32_t kExp = std::is_same<T, __bf16>::value ? 0x7f80u : 0x7c00u;
   const int hf = lane >> 5, lr = lane & 31;
-  const char* const kbase = static_cast<const char*>(a.k) +
-                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
-  const char* const vbase = static_cast<const char*>(a.v) +
-                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
+  const char* const kbase = static_cast<const char*>(a.k) + keys_at<FORM>(p, a.sk) * 2;
+  const char* const vbase = static_cast<const char*>(a.v) + keys_at<FORM>(p, a.sv) * 2;
   const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
   const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
 #pragma unroll
@@ -643,7 +666,7 @@ __device__ __forceinline__ void rows_again(LateArgs& a, const Place& p, RowTile<
 // The end of a wavefront's rows: normalise, write the rows and the LSE, or with more than one
 // share the share's partial rows to part_o [32][D] and their (max, sum) to part_ml [32].
 // lds: TILE bytes of the wavefront's own.
-template <typename T, int D, bool PAGED>
+template <typename T, int D, int FORM>
 __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, float* part_o,
                                             float2* part_ml, char* lds) {
   LateArgs& a = late_args();
@@ -659,7 +682,7 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
 #pragma unroll
     for (int r = 0; r < 16; ++r) bad = bad || !(fabsf(t.o_acc[dt][r]) < INFINITY);
   if (__ballot(bad && l > 0.0f && l < INFINITY) != 0)
-    rows_again<T, D, PAGED>(a, p, t, lane, m == -INFINITY ? 0.0f : m, lds);
+    rows_again<T, D, FORM>(a, p, t, lane, m == -INFINITY ? 0.0f : m, lds);
   // (a select: a row that sees no key may hold 0 * inf of its neighbours' tiles)
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -679,7 +702,7 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
       if (hf == 0)
         part_ml[lr] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
     } else {
-      T* const op = static_cast<T*>(a.out) + p.b * a.so[0] +
+      T* const op = static_cast<T*>(a.out) + rows_at<FORM>(p, a.so) +
                     static_cast<int64_t>(my.qi) * a.so[1] + my.head * a.so[2] + 4 * hf;
 #pragma unroll
       for (int dt = 0; dt < D / 32; ++dt)
@@ -691,10 +714,110 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
           *reinterpret_cast<op4*>(op + 32 * dt + 8 * g) = w;
         }
       if (hf == 0 && a.lse)
-        a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
+        a.lse[lse_at<FORM>(a, p, my.head, my.qi)] =
             l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
     }
   }
+}
+
+// Packed requests.  A row block's number is its rank, in one of two orders.
+//
+// In their order (windows, whose blocks cost alike; no order among positions; more than
+// kMaxRanked requests): request b has the ranks from floor(q_off[b] G / 128) + b on, one more at
+// most than it has blocks.
+// Longest first, where rows see every key before them and B <= kMaxRanked: the level of block i
+// of a request is i and the blocks that its earlier keys would fill, and ranks go through the
+// levels from the highest on, at one level through the requests.  The rank's level
+// is searched by counting the blocks at or above one, a lane a request.
+constexpr int kMaxRanked = 512;
+
+__device__ __forceinline__ int lanes_sum(int x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
+  return uniform_int(x);
+}
+struct Packed {
+  int b, rblock;  // b -1: no such block
+};
+__device__ __forceinline__ Packed packed_at(const WindowArgs& a, int rank, int lane) {
+  auto blocks_of = [&](int b, int* level) __attribute__((always_inline)) -> int {
+    const RowsOf q = rows_of(a.q_off, b, a.Lq), k = rows_of(a.k_off, b, a.Lk);
+    const int before = k.count - q.count;
+    *level = static_cast<int>((before > 0 ? static_cast<int64_t>(before) * a.G : 0) >> 7);
+    return (q.count * a.G + 127) >> 7;
+  };
+  if (!a.descending) {
+    auto first = [&](int b) __attribute__((always_inline)) -> int64_t {
+      int o = a.q_off[b];
+      o = o < 0 ? 0 : (o > a.Lq ? a.Lq : o);
+      return ((static_cast<int64_t>(o) * a.G) >> 7) + b;
+    };
+    const int b = request_at(a.B, rank, lane, first);
+    if (b < 0) return {-1, 0};
+    int level;
+    const int rblock = static_cast<int>(rank - first(b));
+    return {rblock < blocks_of(b, &level) ? b : -1, rblock};
+  }
+  constexpr int PER = kMaxRanked / kWave;
+  int n[PER], at[PER], top = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    n[i] = at[i] = 0;
+    if (i * kWave < a.B && i * kWave + lane < a.B) n[i] = blocks_of(i * kWave + lane, &at[i]);
+    top = n[i] > 0 && at[i] + n[i] > top ? at[i] + n[i] : top;
+  }
+  auto from = [&](int level) __attribute__((always_inline)) -> int {  // blocks at it or above
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int x = at[i] + n[i] - level;
+      c += x < 0 ? 0 : (x < n[i] ? x : n[i]);
+    }
+    return lanes_sum(c);
+  };
+  int lo = 0, hi = top;  // from(lo) > rank >= from(hi)
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const int other = __shfl_xor(hi, o, kWave);
+    hi = other > hi ? other : hi;
+  }
+  hi = uniform_int(hi);
+  if (from(0) <= rank) return {-1, 0};
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (from(mid) > rank) lo = mid;
+    else hi = mid;
+  }
+  int skip = rank - from(lo + 1);  // requests with a block at level lo before the rank's
+  for (int i = 0; i < PER; ++i) {
+    int ni = 0, ai = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (j == i) {
+        ni = n[j];
+        ai = at[j];
+      }
+    const bool has = ai <= lo && lo < ai + ni;
+    const uint64_t with = __ballot(has);
+    const int c = __builtin_popcountll(with);
+    if (skip < c) {
+      const int mine = static_cast<int>(__builtin_amdgcn_mbcnt_hi(
+          static_cast<uint32_t>(with >> 32),
+          __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(with), 0)));
+      const int l = __builtin_ctzll(__ballot(has && mine == skip));
+      return {i * kWave + l, lo - __builtin_amdgcn_readlane(ai, l)};
+    }
+    skip -= c;
+  }
+  return {-1, 0};
+}
+// The rows of block `rblock` of packed request b: lengths and first rows (n_rows 0: none).
+__device__ __forceinline__ int packed_place(const WindowArgs& a, Place& p) {
+  const RowsOf q = rows_of(a.q_off, p.b, a.Lq), k = rows_of(a.k_off, p.b, a.Lk);
+  p.q0 = uniform_int(q.first);
+  p.k0 = uniform_int(k.first);
+  p.k_len = uniform_int(k.count);
+  return uniform_int(q.count);
 }
 
 // acc += w o in a join: the weight of a share far below the row's maximum underflows to 0,
@@ -705,6 +828,8 @@ __device__ __forceinline__ float join(float w, float o, float acc) {
 
 // Blocks of 128 rows over pages (window_paged.hip); type 0: bf16, 1: fp16.
 void launch_window_paged(WindowArgs& a, int type, int64_t D, dim3 grid, hipStream_t s);
+// Packed requests, whole or in shares and their join (window_packed.hip).
+int launch_window_packed(WindowArgs& a, int type, int64_t D, hipStream_t s);
 // Few rows (window_units.hip): in units and their join, or one workgroup a key head
 // (a.units 0); `units` of them are launched.
 int launch_window_units(WindowArgs& a, int type, int64_t D, int64_t units, hipStream_t s);

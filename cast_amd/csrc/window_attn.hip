@@ -60,7 +60,7 @@ static int launch_window(WindowArgs& a, hipStream_t s) {
   constexpr int type = std::is_same<T, __bf16>::value ? 0 : 1;
   if (a.e4m3 >= 0) launch_cached_tile(a, type, a.e4m3 == 1, D, grid, s);
   else if (a.table) launch_window_paged(a, type, D, grid, s);
-  else window_kernel<T, D, false><<<grid, dim3(256), 0, s>>>(a);
+  else window_kernel<T, D, kDense><<<grid, dim3(256), 0, s>>>(a);
   if (a.n_split > 1 && tail > 0) {
     const int64_t n = (tail * kNumXcd * 128 * (D / 8) + 255) / 256;
     window_merge_kernel<T, D><<<dim3(static_cast<unsigned>(n)), dim3(256), 0, s>>>(a);

@@ -7,7 +7,7 @@ namespace rcsa {
 
 template <typename T, int D>
 static void launch(WindowArgs& a, dim3 grid, hipStream_t s) {
-  window_kernel<T, D, true><<<grid, dim3(256), 0, s>>>(a);
+  window_kernel<T, D, kPaged><<<grid, dim3(256), 0, s>>>(a);
 }
 
 void launch_window_paged(WindowArgs& a, int type, int64_t D, dim3 grid, hipStream_t s) {

@@ -22,11 +22,12 @@
 
 namespace rcsa {
 
-template <typename T, int D, bool PAGED>
+template <typename T, int D, int FORM>
 __global__ void __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 3, D == 64 ? 4 : 3)))
 window_kernel(WindowArgs a) {
   using R = RowTile<T, D>;
+  constexpr bool PAGED = FORM == kPaged;
   constexpr int BM = 128, STAGES = 3;
   constexpr int RPU = 1024 / R::KROW;         // rows of a 1 KiB copy
   constexpr int UPW = R::TILE / 1024 / 4;     // copies of a wavefront, K and V each
@@ -43,28 +44,44 @@ window_kernel(WindowArgs a) {
 
   // XCD x (workgroups go round-robin) runs a contiguous run of items, so that neighbours
   // share most of their window in its L2, or every 8th from the longest on.
-  const int xcd = static_cast<int>(blockIdx.x % kNumXcd);
-  const int slot = static_cast<int>(blockIdx.x / kNumXcd);
-  const int tail = slot - a.xcd_whole;
   Place p;
-  p.shares = tail < 0 ? 1 : a.n_split;
-  const int in_xcd = tail < 0 ? slot : a.xcd_whole + tail / a.n_split;
-  const int share = tail < 0 ? 0 : tail % a.n_split;
-  const ItemAt it = item_at(a, xcd, in_xcd);
-  if (it.bh < 0) return;
-  p.b = divide(it.bh, a.by_Hk);
-  p.hk = it.bh - p.b * a.Hk;
-  const Request rq = request_of<true>(a, p.b);
-  const int q_len = uniform_int(rq.q_len);
-  p.k_len = uniform_int(rq.k_len);
+  int share, q_len, item_row0;
+  int64_t ws_row;
+  if constexpr (FORM == kPacked) {
+    // the key heads of a row block side by side, its shares a grid apart
+    const int each = a.n_ranks * a.Hk, id = static_cast<int>(blockIdx.x);
+    share = id / each;
+    const int item = id - share * each, rank = divide(item, a.by_Hk);
+    const Packed it = packed_at(a, rank, lane);
+    if (it.b < 0) return;
+    p.shares = a.n_split;
+    p.b = it.b;
+    p.hk = item - rank * a.Hk;
+    q_len = packed_place(a, p);
+    item_row0 = it.rblock * BM;
+    ws_row = static_cast<int64_t>(id) * BM + wave * 32;
+  } else {
+    const int xcd = static_cast<int>(blockIdx.x % kNumXcd);
+    const int slot = static_cast<int>(blockIdx.x / kNumXcd);
+    const int tail = slot - a.xcd_whole;
+    p.shares = tail < 0 ? 1 : a.n_split;
+    const int in_xcd = tail < 0 ? slot : a.xcd_whole + tail / a.n_split;
+    share = tail < 0 ? 0 : tail % a.n_split;
+    const ItemAt it = item_at(a, xcd, in_xcd);
+    if (it.bh < 0) return;
+    p.b = divide(it.bh, a.by_Hk);
+    p.hk = it.bh - p.b * a.Hk;
+    const Request rq = request_of<true>(a, p.b);
+    q_len = uniform_int(rq.q_len);
+    p.k_len = uniform_int(rq.k_len);
+    item_row0 = it.rblock * BM;
+    const int64_t per_tail = a.xcd_items - a.xcd_whole;
+    ws_row = (share * per_tail * kNumXcd + xcd * per_tail + in_xcd - a.xcd_whole) * BM + wave * 32;
+  }
   p.n_rows = q_len * a.G;
-  const int item_row0 = it.rblock * BM;
   if (item_row0 >= p.n_rows) return;
   p.row0 = item_row0 + wave * 32;
   p.shift = p.k_len - q_len;
-  const int64_t per_tail = a.xcd_items - a.xcd_whole;
-  const int64_t ws_row =
-      (share * per_tail * kNumXcd + xcd * per_tail + in_xcd - a.xcd_whole) * BM + wave * 32;
 
   // uniform ranges: of the item, and of this wavefront's first and last rows
   const KeyRange w_first = row_range(a, p, p.row0), w_last = row_range(a, p, p.row0 + 31);
@@ -75,14 +92,12 @@ window_kernel(WindowArgs a) {
   t.init(lane);
   {
     const Row r = row_of(a, p, p.row0 + lr);
-    t.load_q(static_cast<const T*>(a.q) + p.b * a.sq[0] + static_cast<int64_t>(r.qi) * a.sq[1] +
-                 r.head * a.sq[2], hf);
+    t.load_q(static_cast<const T*>(a.q) + rows_at<FORM>(p, a.sq) +
+                 static_cast<int64_t>(r.qi) * a.sq[1] + r.head * a.sq[2], hf);
   }
 
-  const char* const kbase = static_cast<const char*>(a.k) +
-                            ((PAGED ? 0 : p.b * a.sk[0]) + p.hk * a.sk[2]) * 2;
-  const char* const vbase = static_cast<const char*>(a.v) +
-                            ((PAGED ? 0 : p.b * a.sv[0]) + p.hk * a.sv[2]) * 2;
+  const char* const kbase = static_cast<const char*>(a.k) + keys_at<FORM>(p, a.sk) * 2;
+  const char* const vbase = static_cast<const char*>(a.v) + keys_at<FORM>(p, a.sv) * 2;
   const uint32_t krb = static_cast<uint32_t>(a.sk[1] * 2), vrb = static_cast<uint32_t>(a.sv[1] * 2);
   const int32_t* const table = PAGED ? a.table + p.b * a.table_stride : nullptr;
 
@@ -157,7 +172,7 @@ window_kernel(WindowArgs a) {
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
   __builtin_amdgcn_s_barrier();  // (the ring is read: a wavefront may need a part of it)
-  finish_rows<T, D, PAGED>(p, t, a.ws_o + ws_row * D, a.ws_ml + ws_row,
+  finish_rows<T, D, FORM>(p, t, a.ws_o + ws_row * D, a.ws_ml + ws_row,
                            (wave < 2 ? s_0 : s_1) + (wave & 1) * R::TILE);
 }
 

@@ -21,7 +21,7 @@ __all__ = [
     "pool_query", "pool_key", "block_scores", "select_topk", "quantize_key",
     "sparse_attn_bf16", "sparse_attn_int8", "pack_tokens", "unpack_tokens", "row_budgets",
     "quantize_key_select", "order_lists", "rope", "norm_rope", "PagedCache",
-    "window_attention", "paged_attention", "QuantizedCache", "append_cache", "read_cache",
+    "window_attention", "paged_attention", "packed_attention", "QuantizedCache", "append_cache", "read_cache",
 ]
 
 
@@ -1321,6 +1321,30 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     scale = _sm_scale(sm_scale, fn)
     res = _lib.torch_ops().window_attention(q, k, v, None, q_lengths, k_lengths, w, s, b, scale,
                                             return_lse, out, _shares(n_split, fn), -1)
+    return tuple(res) if return_lse else res[0]
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, *,
+                     k_offsets: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                     sinks: int = 0, block: int = 1, causal: bool = True,
+                     sm_scale: Optional[float] = None, return_lse: bool = False,
+                     out: Optional[torch.Tensor] = None, n_split: Optional[int] = None):
+    """:func:`window_attention` of requests that follow each other without padding
+    (``rcsa_packed_attn``): ``q [T, Hq, D]``, ``k, v [Tk, Hk, D]``.
+
+    Request b has the queries ``offsets[b]`` to ``offsets[b + 1]`` (int32 ``[B + 1]``, not
+    decreasing; held within the rows) and the keys ``k_offsets[b]`` to ``k_offsets[b + 1]`` (None:
+    ``offsets``, whole prompts), of which its queries are the last positions.  The lengths are
+    read on the device: a captured call follows them.  Rows before ``offsets[0]`` and from
+    ``offsets[B]`` on stay as they were (give ``out``).
+
+    Returns ``out [T, Hq, D]`` and, with ``return_lse``, ``[Hq, T]``.  ``n_split`` (None: planned)
+    workgroups share the keys of every block of 128 rows."""
+    fn = "packed_attention"
+    w, s, b = _window(window, sinks, block, causal, fn)
+    scale = _sm_scale(sm_scale, fn)
+    res = _lib.torch_ops().packed_attention(q, k, v, offsets, k_offsets, w, s, b, scale,
+                                            return_lse, out, max(0, _shares(n_split, fn)))
     return tuple(res) if return_lse else res[0]
 
 

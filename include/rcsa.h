@@ -784,6 +784,29 @@ int rcsa_window_attn(const void* q, const void* k, const void* v, void* out, flo
                      int64_t workspace_bytes, hipStream_t stream);
 
 /*
+ * rcsa_packed_attn: rcsa_window_attn over packed requests, without padding: dims = {B, T, Tk, Hq,
+ * Hk, D}, q [T][Hq][D] and out alike, k, v [Tk][Hk][D]; request b has the queries q_offsets[b] ..
+ * q_offsets[b + 1] and the keys k_offsets[b] .. k_offsets[b + 1] (int32 [B + 1] each, not
+ * decreasing, held within the rows; equal for whole prompts), of which its queries are the last
+ * positions.  strides: host array of 8, row and head stride of q, k, v, out.  lse (nullable)
+ * [Hq][T].  window, sinks, block, types, alignments and what rows see as there; rows before
+ * q_offsets[0] and behind q_offsets[B] are left as they were.  T Hq / Hk < 2^30, and (T Hq / Hk /
+ * 128 + B) Hk < 2^24.
+ *
+ * n_split 1 to 64 workgroups share the keys of every block of 128 rows, joined by a second
+ * launch where they are more than one; the workspace holds rcsa_packed_attn_workspace_bytes
+ * (-1: no such launch; 16-byte aligned, of this call alone until it ends).
+ * rcsa_packed_attn_plan picks n_split; max_keys bounds the keys that a row sees.
+ */
+int rcsa_packed_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split);
+int64_t rcsa_packed_attn_workspace_bytes(const int64_t* dims, int64_t n_split);
+int rcsa_packed_attn(const void* q, const void* k, const void* v, void* out, float* lse,
+                     int dtype, const int64_t* dims, const int64_t* strides,
+                     const int32_t* q_offsets, const int32_t* k_offsets, int64_t window,
+                     int64_t sinks, int64_t block, float sm_scale, int64_t n_split,
+                     void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/*
  * A paged cache in 8 bits, one scale for each block of tokens and head.  No reference kernel:
  * the reference holds its keys and values in 16 bits.
  *
