@@ -57,6 +57,7 @@ FILE_FLAGS = {
     "sparse_attn_bf16_cu3.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
     "window_attn.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
     "window_packed.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "cached_tile.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
     "window_paged.hip": ["-mllvm", "-amdgpu-sched-strategy=max-memory-clause"],
 }
 

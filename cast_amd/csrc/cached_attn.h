@@ -130,42 +130,70 @@ __device__ __forceinline__ int row_shift(float most) {
   return k > 100 ? 100 : k;
 }
 
-// The scales of a step's two halves of 16 keys: of a page that is there, as the cache holds them
-// if they are positive numbers below 2^126, else 0.
+// A step: its first key, and the pages of its two halves of 16 keys.
+struct CodeStep {
+  int key, page0, page1;
+};
+// The first row of a half in its page.
+template <typename A>
+__device__ __forceinline__ int slot_of(A& a, int key, int half) {
+  const int k = (key < 0 ? 0 : key);
+  const int slot = k - divide(k >> 4, a.by_half_page) * a.page;
+  return half == 0 ? slot : (slot + 16 < a.page ? slot + 16 : 0);
+}
+template <typename A>
+__device__ __forceinline__ CodeStep code_step(A& a, const Place& p, const int32_t* table, int s) {
+  CodeStep r;
+  r.key = key_of(p, s);
+  const int key = r.key < 0 ? 0 : r.key;
+  const int col = divide(key >> 4, a.by_half_page);
+  r.page0 = ld_const(table + col);
+  r.page1 = r.page0;
+  if (!a.whole_tiles && key - col * a.page + 16 >= a.page)
+    r.page1 = ld_const(table + (col + 1 < a.max_pages ? col + 1 : a.max_pages - 1));
+  return r;
+}
+template <typename A>
+__device__ __forceinline__ int halves_there(A& a, const CodeStep& s) {
+  return (page_ok(a, s.page0) ? 1 : 0) + (page_ok(a, s.page1) ? 2 : 0);
+}
+// Where the first rows of a half of a step are (page 0's where it is not there: its codes are
+// not seen, but read).  (32 x 32-bit products: a page spans less than 4 GiB.)
+struct HalfAt {
+  uint64_t k, v;
+};
+template <typename A>
+__device__ __forceinline__ HalfAt half_at(A& a, const CodeStep& s, int half, uint32_t krb,
+                                          uint32_t vrb) {
+  const int pg = half ? s.page1 : s.page0;
+  const uint32_t slot = static_cast<uint32_t>(slot_of(a, s.key, half));
+  const uint32_t at = s.key >= 0 && page_ok(a, pg) ? static_cast<uint32_t>(pg) : 0u;
+  return {static_cast<uint64_t>(at) * static_cast<uint32_t>(a.sk[0]) +
+              static_cast<uint64_t>(slot) * krb,
+          static_cast<uint64_t>(at) * static_cast<uint32_t>(a.sv[0]) +
+              static_cast<uint64_t>(slot) * vrb};
+}
+// The scales of a step's two halves: of a page that is there, as the cache holds them if they are
+// positive numbers below 2^126, else 0.  ks, vs: of the key head.
 struct Scales {
   float k[2], v[2];
 };
 template <typename A>
-__device__ __forceinline__ Scales scales_of(A& a, const Place& p, const Step& s) {
+__device__ __forceinline__ Scales scales_of(A& a, const CodeStep& s, const float* ks,
+                                            const float* vs) {
   Scales r;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int key = (s.key < 0 ? 0 : s.key) + 16 * h;
     const int pg = h ? s.page1 : s.page0;
     const bool there = s.key >= 0 && page_ok(a, pg);
-    const int half = key >> 4, col = divide(half, a.by_half_page);
-    const int mark = divide(half - col * (a.page >> 4), a.by_half_mark);
-    const uint64_t at = there ? static_cast<uint32_t>(pg) : 0u;
-    const float k = ld_const(a.ks + at * a.sks[0] + mark * a.sks[1] + p.hk * a.sks[2]);
-    const float v = ld_const(a.vs + at * a.svs[0] + mark * a.svs[1] + p.hk * a.svs[2]);
+    const int mark = divide(slot_of(a, s.key, h) >> 4, a.by_half_mark);
+    const int at = there ? pg : 0;
+    const float k = ld_const(ks + (at * a.sks[0] + mark * a.sks[1]));
+    const float v = ld_const(vs + (at * a.svs[0] + mark * a.svs[1]));
     r.k[h] = there && k > 0.0f && k < 0x1p126f ? k : 0.0f;
     r.v[h] = there && v > 0.0f && v < 0x1p126f ? v : 0.0f;
   }
   return r;
-}
-
-// Where the first rows of a half of a step are (page 0's where it is not there: its codes are
-// not seen, but read).
-template <typename A>
-__device__ __forceinline__ HalfRows code_rows(A& a, const Step& s, int half, uint32_t krb,
-                                              uint32_t vrb) {
-  const int key = (s.key < 0 ? 0 : s.key) + 16 * half;
-  const int pg = half ? s.page1 : s.page0;
-  const int col = divide(key >> 4, a.by_half_page);
-  const uint32_t slot = static_cast<uint32_t>(key - col * a.page);
-  const uint64_t at = s.key >= 0 && page_ok(a, pg) ? static_cast<uint32_t>(pg) : 0u;
-  return {at * static_cast<uint64_t>(a.sk[0]) + static_cast<uint64_t>(slot) * krb,
-          at * static_cast<uint64_t>(a.sv[0]) + static_cast<uint64_t>(slot) * vrb, 16};
 }
 
 // The 32 keys of the tile at `key` that row `row` sees, as bits.

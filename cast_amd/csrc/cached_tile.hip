@@ -13,13 +13,16 @@ struct CodeTile : RowTile<_Float16, D> {
   float c_row;  // logit of q . c, times the key's scale, in log2 units
   int v_exp;    // accumulators are in units of 2^v_exp
 
-  template <typename Bits, typename Pre, typename Cp>
+  template <typename Bits, typename Pre>
   __device__ __forceinline__ void step8(const char* tile, const Scales& sc, int hf, bool inside,
-                                        Bits&& bits, Pre&& prefetch, Cp&& copies) {
+                                        Bits&& bits, Pre&& prefetch) {
+    // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
     v4i kraw[R::QSTEPS];
+    int k0 = this->k_off[0];
+    asm volatile("" : "+v"(k0));
 #pragma unroll
     for (int st = 0; st < R::QSTEPS; ++st)
-      kraw[st] = *reinterpret_cast<const v4i*>(tile + this->k_off[st]);
+      kraw[st] = *reinterpret_cast<const v4i*>(tile + (k0 ^ (st * 16)));
     v16f s_acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
@@ -45,30 +48,27 @@ struct CodeTile : RowTile<_Float16, D> {
         for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
       v_exp = e_new;
     }
-    const float c = c_row * (hf ? sc.k[1] : sc.k[0]);
-    const float f = (hf ? sc.v[1] : sc.v[0]) * power_of(-v_exp);
+    const float c = fmaxf(c_row * (hf ? sc.k[1] : sc.k[0]), 0x1p-126f);  // (0 * -inf is NaN)
+    const float f = fmaxf((hf ? sc.v[1] : sc.v[0]) * power_of(-v_exp), 0x1p-60f);
+    const float log_f = __builtin_amdgcn_logf(f);
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
     if (!inside) {
       const uint32_t seen = bits();
-      // (a scale of 0 would make NaN of -inf)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) rv[r] = ((seen >> r) & 1u) ? rv[r] * c : -INFINITY;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) rv[r] *= c;
+      for (int r = 0; r < 16; ++r) rv[r] = ((seen >> r) & 1u) ? rv[r] : -INFINITY;
     }
     v8hf p_op[2];
     auto exps = [&]() __attribute__((always_inline)) -> float {
-      const float bias = this->m_run == -INFINITY ? 0.0f : -this->m_run;
+      const float bias = log_f + (this->m_run == -INFINITY ? 0.0f : -this->m_run);
       float lsum[4];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int jj = 0; jj < 8; ++jj) {
-          const float e = __builtin_amdgcn_exp2f(rv[8 * u + jj] + bias);
-          p_op[u][jj] = static_cast<_Float16>(e * f);
+          const float e = __builtin_amdgcn_exp2f(fmaf(rv[8 * u + jj], c, bias));
+          p_op[u][jj] = static_cast<_Float16>(e);
           if (u == 0 && jj < 4) lsum[jj] = e;
           else lsum[jj & 3] += e;
         }
@@ -79,7 +79,7 @@ struct CodeTile : RowTile<_Float16, D> {
       float rmax = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
-      rmax = pair_max(rmax);
+      rmax = pair_max(rmax * c);
       const float m_blk = rmax == -INFINITY ? -INFINITY : rmax - O::kShift;
       if (__ballot(m_blk > this->m_run + kTau) != 0) {
         const float m_new = fmaxf(this->m_run, m_blk);
@@ -94,12 +94,13 @@ struct CodeTile : RowTile<_Float16, D> {
         part = exps();
       }
     }
-    this->l_run += part;
-    copies();
+    this->l_run = fmaf(part, __builtin_amdgcn_rcpf(f), this->l_run);
+    int v0 = this->v_off[0];
+    asm volatile("" : "+v"(v0));
     auto v_group = [&](int u, v8hf (&op)[R::NDT]) __attribute__((always_inline)) {
 #pragma unroll
       for (int dt = 0; dt < R::NDT; ++dt) {
-        const char* const p0 = tile + this->v_off[dt] + 8 * u * R::KROW;
+        const char* const p0 = tile + (v0 ^ (dt * 64)) + 8 * u * R::KROW;
         const auto lo = O::read_tr(p0);
         const auto hi = O::read_tr(p0 + 4 * R::KROW);
         op[dt] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -118,16 +119,18 @@ struct CodeTile : RowTile<_Float16, D> {
 
 template <typename T, bool E4M3, int D>
 __global__ void __launch_bounds__(256)
-__attribute__((amdgpu_waves_per_eu(2, 2)))
+__attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 3, D == 64 ? 4 : 3)))
 cached_tile_kernel(WindowArgs a) {
   using C = CodeTile<D>;
   using R = RowTile<_Float16, D>;
   typedef typename Half<T>::op8 op8;
   constexpr int BM = 128;
-  // a wavefront moves rows 8 w .. 8 w + 7 of a tile: a lane BPL bytes of one of them
+  // bytes of a row that a lane widens
   constexpr int BPL = D / 8, CHUNKS = BPL / 8;  // (16-byte chunks of the fp16 row)
   __shared__ __attribute__((aligned(1024))) char s_0[2 * R::TILE];
   __shared__ __attribute__((aligned(1024))) char s_1[2 * R::TILE];
+  __shared__ __attribute__((aligned(1024))) char r_0[8192];
+  __shared__ __attribute__((aligned(1024))) char r_1[8192];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uniform_int(tid >> 6);
@@ -186,82 +189,89 @@ cached_tile_kernel(WindowArgs a) {
   const uint32_t krb = static_cast<uint32_t>(a.sk[1]), vrb = static_cast<uint32_t>(a.sv[1]);
   const int32_t* const table = a.table + p.b * a.table_stride;
 
-  // the lane's bytes of a tile: row 8 wave + lane / 8, which lies in half wave / 2
-  const int trow = 8 * wave + (lane >> 3), in_half = trow & 15;
-  const int k_lo = in_half * static_cast<int>(krb) + (lane & 7) * BPL;
-  const int v_lo = in_half * static_cast<int>(vrb) + (lane & 7) * BPL;
-  int k_at[CHUNKS], v_at[CHUNKS];
-#pragma unroll
-  for (int i = 0; i < CHUNKS; ++i) {
-    const int chunk = (lane & 7) * CHUNKS + i;
-    k_at[i] = trow * R::KROW + ((chunk ^ (swz_k<R::KROW>(trow) & (R::CPR - 1))) * 16);
-    v_at[i] = R::TILE + trow * R::KROW + ((chunk ^ (swz_v(trow) & (R::CPR - 1))) * 16);
-  }
-  struct Staged {
-    v4i k, v;  // (D 64: the first two words)
+  // Copies: a wavefront moves rows 8 w .. 8 w + 7 of a tile, which lie in its half w / 2, as they
+  // are into its part of a slot (D 64: the lanes past them zeros), 16 bytes a lane.
+  constexpr int LPR = D / 16;  // lanes of a row
+  const int in_half = (8 * wave + lane / LPR) & 15;
+  const uint32_t none = lane < 8 * LPR ? 0u : 0x80000000u;
+  const uint32_t k_lo = (in_half * krb + lane % LPR * 16) | none;
+  const uint32_t v_lo = (in_half * vrb + lane % LPR * 16) | none;
+  auto stage = [&](const CodeStep& s, char* dst) __attribute__((always_inline)) {
+    const HalfAt h = half_at(a, s, wave >> 1, krb, vrb);
+    buffer_copy16(const_cast<char*>(kbase) + h.k, 16 * static_cast<int>(krb), k_lo,
+                  dst + wave * 2048);
+    buffer_copy16(const_cast<char*>(vbase) + h.v, 16 * static_cast<int>(vrb), v_lo,
+                  dst + wave * 2048 + 1024);
   };
-  auto load = [&](const Step& s) __attribute__((always_inline)) -> Staged {
-    const HalfRows h = code_rows(a, s, wave >> 1, krb, vrb);
-    const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(kbase) + h.k, 0, 16 * static_cast<int>(krb), kRsrcWord3);
-    const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<char*>(vbase) + h.v, 0, 16 * static_cast<int>(vrb), kRsrcWord3);
-    Staged x;
-    if constexpr (BPL == 16) {
-      x.k = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lo, 0, 0));
-      x.v = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(vr, v_lo, 0, 0));
-    } else {
-      const auto k2 = __builtin_amdgcn_raw_buffer_load_b64(kr, k_lo, 0, 0);
-      const auto v2 = __builtin_amdgcn_raw_buffer_load_b64(vr, v_lo, 0, 0);
-      x.k = v4i{static_cast<int>(k2[0]), static_cast<int>(k2[1]), 0, 0};
-      x.v = v4i{static_cast<int>(v2[0]), static_cast<int>(v2[1]), 0, 0};
-    }
-    return x;
-  };
-  auto put = [&](const Staged& x, char* dst) __attribute__((always_inline)) {
-    v8hf k[2], v[2];
-    v4i fv = x.v;
+  // Its own copies, landed, become fp16 in the tile: lane l BPL bytes of row 8 w + l / 8.
+  const int trow = 8 * wave + (lane >> 3);
+  const int raw = wave * 2048 + lane * BPL;
+  const int chunk = (lane & 7) * CHUNKS;  // (the next chunk: one bit up)
+  const int k_at = trow * R::KROW + ((chunk ^ (swz_k<R::KROW>(trow) & (R::CPR - 1))) * 16);
+  const int v_at = R::TILE + trow * R::KROW + ((chunk ^ (swz_v(trow) & (R::CPR - 1))) * 16);
+  auto widen = [&](const char* src, char* dst) __attribute__((always_inline)) {
+    auto half = [&](const char* from, int at, bool values) __attribute__((always_inline)) {
+      v4i w = {0, 0, 0, 0};
+      if constexpr (BPL == 16) {
+        w = *reinterpret_cast<const v4i*>(from);
+      } else {
+        const auto two = *reinterpret_cast<const v2u*>(from);
+        w[0] = static_cast<int>(two[0]);
+        w[1] = static_cast<int>(two[1]);
+      }
+      if (values)
 #pragma unroll
-    for (int i = 0; i < BPL / 4; ++i)
-      fv[i] = static_cast<int>(Widen<E4M3>::finite(static_cast<uint32_t>(fv[i])));
-    widen16<E4M3>(x.k, k[0], k[1]);
-    widen16<E4M3>(fv, v[0], v[1]);
-#pragma unroll
-    for (int i = 0; i < CHUNKS; ++i) {
-      *reinterpret_cast<v8hf*>(dst + k_at[i]) = k[i];
-      *reinterpret_cast<v8hf*>(dst + v_at[i]) = v[i];
-    }
+        for (int i = 0; i < BPL / 4; ++i)
+          w[i] = static_cast<int>(Widen<E4M3>::finite(static_cast<uint32_t>(w[i])));
+      v8hf o[2];
+      widen16<E4M3>(w, o[0], o[1]);
+      *reinterpret_cast<v8hf*>(dst + at) = o[0];
+      if constexpr (CHUNKS == 2) *reinterpret_cast<v8hf*>(dst + (at ^ 16)) = o[1];
+    };
+    half(src + raw, k_at, false);
+    half(src + raw + 1024, v_at, true);
   };
 
-  // Two slots: tile j in slot j % 2, written during step j - 1 (all wavefronts have left step
-  // j - 2 by then), its codes asked for during step j - 2.
-  Step cur = step_of<true>(a, p, table, 0), next = step_of<true>(a, p, table, 1);
-  Scales sc = scales_of(a, p, cur);
-  put(load(cur), s_0);
-  Staged st = load(next);
+  // Tile j is in slot j % 2 as fp16, written during step j - 1 (every wavefront has left step
+  // j - 2 by then); its codes landed in raw slot j % 2, asked for during step j - 3.
+  const float* const ks = a.ks + p.hk * a.sks[2];
+  const float* const vs = a.vs + p.hk * a.svs[2];
+  CodeStep e0 = code_step(a, p, table, 0), e1 = code_step(a, p, table, 1);
+  CodeStep e2 = code_step(a, p, table, 2), e3 = code_step(a, p, table, 3);
+  stage(e0, r_0);
+  __builtin_amdgcn_sched_barrier(0);
+  stage(e1, r_1);
+  __builtin_amdgcn_sched_barrier(0);
+  Scales sc = scales_of(a, e0, ks, vs);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));
+  widen(r_0, s_0);
+  __builtin_amdgcn_sched_barrier(0);  // (its codes are in registers)
+  stage(e2, r_0);
   auto iteration = [&](auto slot_c, int j) __attribute__((always_inline)) {
     constexpr int J = decltype(slot_c)::value;
     char* const tile = J == 0 ? s_0 : s_1;
     char* const fill = J == 0 ? s_1 : s_0;
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const Step now = cur;
+    char* const codes = J == 0 ? r_1 : r_0;
+    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    widen(codes, fill);
+    __builtin_amdgcn_sched_barrier(0);
+    stage(e3, codes);
+    __builtin_amdgcn_sched_barrier(0);
+    const int key = e0.key, there = halves_there(a, e0);
     const Scales ns = sc;
-    cur = next;
-    const int there = halves_there<true>(a, now);
-    const bool inside = now.key >= 0 && there == 3 && now.key + kTileKeys <= w_first.hi &&
-                        (now.key >= w_last.lo || now.key + kTileKeys <= a.sinks);
+    e0 = e1;
+    e1 = e2;
+    e2 = e3;
+    const bool inside = key >= 0 && there == 3 && key + kTileKeys <= w_first.hi &&
+                        (key >= w_last.lo || key + kTileKeys <= a.sinks);
     t.step8(
         tile, ns, hf, inside,
         [&]() __attribute__((always_inline)) {
-          return now.key < 0 ? 0u : seen_bits(a, p, p.row0 + lr, hf, now.key, there);
+          return key < 0 ? 0u : seen_bits(late_args(), p, p.row0 + lr, hf, key, there);
         },
         [&]() __attribute__((always_inline)) {
-          sc = scales_of(a, p, cur);
-          next = step_of<true>(a, p, table, j + 2);
-        },
-        [&]() __attribute__((always_inline)) {
-          put(st, fill);
-          st = load(next);
+          sc = scales_of(a, e0, ks, vs);
+          e3 = code_step(a, p, table, j + 4);
         });
   };
   const int rounds = (p.steps + 1) / 2;
@@ -269,8 +279,10 @@ cached_tile_kernel(WindowArgs a) {
     iteration(std::integral_constant<int, 0>{}, 2 * rd);
     iteration(std::integral_constant<int, 1>{}, 2 * rd + 1);
   }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
 
   // the end of the wavefront's rows
+  LateArgs& e = late_args();
   const float l = pair_sum(t.l_run), m = t.m_run;
   const float unit = power_of(t.v_exp);
   const float inv = l > 0.0f ? unit / l : l;  // (a NaN sum stays one)
@@ -278,10 +290,10 @@ cached_tile_kernel(WindowArgs a) {
   for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) t.o_acc[dt][r] = l == 0.0f ? 0.0f : t.o_acc[dt][r] * inv;
-  const Row my = row_of(a, p, p.row0 + lr);
+  const Row my = row_of(e, p, p.row0 + lr);
   if (!my.live) return;
   if (p.shares > 1) {
-    float* const wp = a.ws_o + (ws_row + lr) * D + 4 * hf;
+    float* const wp = e.ws_o + (ws_row + lr) * D + 4 * hf;
 #pragma unroll
     for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
@@ -290,22 +302,22 @@ cached_tile_kernel(WindowArgs a) {
             v4f{t.o_acc[dt][4 * g], t.o_acc[dt][4 * g + 1], t.o_acc[dt][4 * g + 2],
                 t.o_acc[dt][4 * g + 3]};
     if (hf == 0)
-      a.ws_ml[ws_row + lr] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
+      e.ws_ml[ws_row + lr] = make_float2(l > 0.0f ? m : (l == 0.0f ? -INFINITY : l), l);
     return;
   }
-  T* const op = static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(my.qi) * a.so[1] +
-                my.head * a.so[2] + 4 * hf;
+  T* const op = static_cast<T*>(e.out) + p.b * e.so[0] + static_cast<int64_t>(my.qi) * e.so[1] +
+                my.head * e.so[2] + 4 * hf;
 #pragma unroll
   for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       typename Half<T>::op4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = static_cast<T>(t.o_acc[dt][4 * g + e]);
+      for (int i = 0; i < 4; ++i) w[i] = static_cast<T>(t.o_acc[dt][4 * g + i]);
       *reinterpret_cast<typename Half<T>::op4*>(op + 32 * dt + 8 * g) = w;
     }
-  if (hf == 0 && a.lse)
-    a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
+  if (hf == 0 && e.lse)
+    e.lse[(static_cast<int64_t>(p.b) * e.Hq + my.head) * e.Lq + my.qi] =
         l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 

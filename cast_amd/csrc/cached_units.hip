@@ -78,18 +78,18 @@ cached_unit_kernel(WindowArgs a) {
     v4i k[KL];
     uint32_t v[16];
   };
-  auto load_k = [&](const Step& s, v4i (&k)[KL]) __attribute__((always_inline)) {
-    const HalfRows h0 = code_rows(a, s, 0, krb, vrb), h1 = code_rows(a, s, 1, krb, vrb);
+  auto load_k = [&](const CodeStep& s, v4i (&k)[KL]) __attribute__((always_inline)) {
+    const HalfAt h0 = half_at(a, s, 0, krb, vrb), h1 = half_at(a, s, 1, krb, vrb);
     const char* const at = kbase + (lr < 16 ? h0.k : h1.k) + static_cast<uint64_t>(lr & 15) * krb +
                            hf * 16;
 #pragma unroll
     for (int i = 0; i < KL; ++i) k[i] = *reinterpret_cast<const v4i*>(at + 32 * i);
   };
-  auto load_v = [&](const Step& s, uint32_t (&v)[16]) __attribute__((always_inline)) {
+  auto load_v = [&](const CodeStep& s, uint32_t (&v)[16]) __attribute__((always_inline)) {
     const int at = static_cast<int>(4 * hf * vrb + NDT * lr);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const HalfRows r = code_rows(a, s, h, krb, vrb);
+      const HalfAt r = half_at(a, s, h, krb, vrb);
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<char*>(vbase) + r.v, 0, 16 * static_cast<int>(vrb), kRsrcWord3);
 #pragma unroll
@@ -105,11 +105,13 @@ cached_unit_kernel(WindowArgs a) {
     }
   };
 
-  Step cur = step_of<true>(a, p, table, 0), next = step_of<true>(a, p, table, 1);
+  const float* const ks = a.ks + p.hk * a.sks[2];
+  const float* const vs = a.vs + p.hk * a.svs[2];
+  CodeStep cur = code_step(a, p, table, 0), next = code_step(a, p, table, 1);
   Tile t;
   load_k(cur, t.k);
   load_v(cur, t.v);
-  Scales sc = scales_of(a, p, cur);
+  Scales sc = scales_of(a, cur, ks, vs);
   v16f o_acc[NDT];
 #pragma unroll
   for (int x = 0; x < NDT; ++x)
@@ -120,7 +122,7 @@ cached_unit_kernel(WindowArgs a) {
   constexpr int kShift = Half<_Float16>::kShift;
 
   for (int s = 0; s < p.steps; ++s) {
-    const Step now = cur;
+    const int key = cur.key, there = halves_there(a, cur);
     const Scales ns = sc;
     v16f s_acc;
 #pragma unroll
@@ -136,19 +138,18 @@ cached_unit_kernel(WindowArgs a) {
     const bool more = s + 1 < p.steps;
     if (more) {
       load_k(cur, t.k);
-      sc = scales_of(a, p, cur);
-      next = step_of<true>(a, p, table, s + 2);
+      sc = scales_of(a, cur, ks, vs);
+      next = code_step(a, p, table, s + 2);
     }
     // logits in log2 units: r < 8 of the first half's keys, the others of the second's
     const float c0 = c_row * ns.k[0], c1 = c_row * ns.k[1];
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r] * (r < 8 ? c0 : c1);
-    const int there = halves_there<true>(a, now);
-    const bool inside = there == 3 && now.key + kTileKeys <= first.hi &&
-                        (now.key >= last.lo || now.key + kTileKeys <= a.sinks);
+    const bool inside = there == 3 && key + kTileKeys <= first.hi &&
+                        (key >= last.lo || key + kTileKeys <= a.sinks);
     if (!inside) {
-      const uint32_t seen = seen_keys(a, p, lr, now.key, there) >> (4 * hf);
+      const uint32_t seen = seen_keys(late_args(), p, lr, key, there) >> (4 * hf);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         rv[r] = (seen >> (8 * (r >> 2) + (r & 3))) & 1u ? rv[r] : -INFINITY;

@@ -50,7 +50,7 @@ struct WindowArgs {
   int descending;
   // pages of 8-bit codes: their scales [page][block][head], 16 keys of a block
   const float *ks, *vs;
-  int64_t sks[3], svs[3];
+  int sks[3], svs[3];  // (their last one is below 2^29)
   Divisor by_half_mark;
   int e4m3;        // the codes' type; -1: 16-bit keys and values
   // packed: rows of the requests in q and in k, v ([B + 1] each), a request's row blocks

@@ -283,8 +283,8 @@ static int run(const void* q, const void* k, const void* v, void* out, float* ls
     a.ks = codes->ks;
     a.vs = codes->vs;
     for (int i = 0; i < 3; ++i) {
-      a.sks[i] = codes->strides[i];
-      a.svs[i] = codes->strides[3 + i];
+      a.sks[i] = static_cast<int>(codes->strides[i]);
+      a.svs[i] = static_cast<int>(codes->strides[3 + i]);
     }
     a.by_half_mark = divisor(static_cast<uint32_t>(codes->block_size / 16));
   }
@@ -332,8 +332,19 @@ extern "C" int rcsa_cached_attn(const void* q, const void* k_codes, const void* 
   if (code != RCSA_CODE_INT8 && code != RCSA_CODE_E4M3) return RCSA_ERR_DTYPE;
   if (block_size <= 0 || block_size % 16 || page_size <= 0 || page_size % block_size)
     return RCSA_ERR_SHAPE;
-  for (int i = 0; i < 6; ++i)
-    if (scale_strides[i] < 0) return RCSA_ERR_STRIDE;
+  if (!dims || n_pages <= 0 || n_pages >= kMostKeys || dims[4] <= 0 || dims[4] >= (1 << 16))
+    return dims ? RCSA_ERR_SHAPE : RCSA_ERR_NULL;
+  for (int i = 0; i < 6; i += 3) {  // (offsets of scales are 32-bit, of bytes)
+    constexpr int64_t most = 1ll << 29;
+    const int64_t n[3] = {n_pages, page_size / block_size, dims[4]};
+    int64_t last = 0;
+    for (int j = 0; j < 3; ++j) {
+      if (scale_strides[i + j] < 0) return RCSA_ERR_STRIDE;
+      if (n[j] > 1 && scale_strides[i + j] > (most - 1) / (n[j] - 1)) return RCSA_ERR_STRIDE;
+      last += (n[j] - 1) * scale_strides[i + j];
+    }
+    if (last >= most) return RCSA_ERR_STRIDE;
+  }
   const CodePages codes = {code == RCSA_CODE_E4M3, k_scales, v_scales, scale_strides, block_size};
   return run(q, k_codes, v_codes, out, lse, dtype, &codes, dims, strides, q_lengths, k_lengths,
              block_table, table_stride, max_pages, n_pages, page_size, window, sinks, block,
