@@ -130,70 +130,179 @@ __device__ __forceinline__ int row_shift(float most) {
   return k > 100 ? 100 : k;
 }
 
-// A step: its first key, and the pages of its two halves of 16 keys.
-struct CodeStep {
-  int key, page0, page1;
-};
-// The first row of a half in its page.
-template <typename A>
-__device__ __forceinline__ int slot_of(A& a, int key, int half) {
-  const int k = (key < 0 ? 0 : key);
-  const int slot = k - divide(k >> 4, a.by_half_page) * a.page;
-  return half == 0 ? slot : (slot + 16 < a.page ? slot + 16 : 0);
-}
-template <typename A>
-__device__ __forceinline__ CodeStep code_step(A& a, const Place& p, const int32_t* table, int s) {
-  CodeStep r;
-  r.key = key_of(p, s);
-  const int key = r.key < 0 ? 0 : r.key;
-  const int col = divide(key >> 4, a.by_half_page);
-  r.page0 = ld_const(table + col);
-  r.page1 = r.page0;
-  if (!a.whole_tiles && key - col * a.page + 16 >= a.page)
-    r.page1 = ld_const(table + (col + 1 < a.max_pages ? col + 1 : a.max_pages - 1));
-  return r;
-}
-template <typename A>
-__device__ __forceinline__ int halves_there(A& a, const CodeStep& s) {
-  return (page_ok(a, s.page0) ? 1 : 0) + (page_ok(a, s.page1) ? 2 : 0);
-}
-// Where the first rows of a half of a step are (page 0's where it is not there: its codes are
-// not seen, but read).  (32 x 32-bit products: a page spans less than 4 GiB.)
-struct HalfAt {
-  uint64_t k, v;
-};
-template <typename A>
-__device__ __forceinline__ HalfAt half_at(A& a, const CodeStep& s, int half, uint32_t krb,
-                                          uint32_t vrb) {
-  const int pg = half ? s.page1 : s.page0;
-  const uint32_t slot = static_cast<uint32_t>(slot_of(a, s.key, half));
-  const uint32_t at = s.key >= 0 && page_ok(a, pg) ? static_cast<uint32_t>(pg) : 0u;
-  return {static_cast<uint64_t>(at) * static_cast<uint32_t>(a.sk[0]) +
-              static_cast<uint64_t>(slot) * krb,
-          static_cast<uint64_t>(at) * static_cast<uint32_t>(a.sv[0]) +
-              static_cast<uint64_t>(slot) * vrb};
-}
-// The scales of a step's two halves: of a page that is there, as the cache holds them if they are
-// positive numbers below 2^126, else 0.  ks, vs: of the key head.
+// A share's tiles one after the other: where the codes of the present one are, and which scales
+// are its.  All of it is scalar work, which takes its turn with the vector work of a wavefront:
+// WHOLE (pages and blocks of whole tiles) steps along a page by additions and looks into
+// the table where a page ends, a page ahead; otherwise the two halves of 16 keys are looked up
+// each on their own.  Past the share's last tile, and on pages that are not there, the codes
+// stand where some page's are: they are read, and not seen.
+template <bool WHOLE>
 struct Scales {
-  float k[2], v[2];
+  static constexpr int N = WHOLE ? 1 : 2;
+  float k[N], v[N];
 };
-template <typename A>
-__device__ __forceinline__ Scales scales_of(A& a, const CodeStep& s, const float* ks,
-                                            const float* vs) {
-  Scales r;
+template <bool WHOLE>
+struct TileRef {
+  static constexpr int N = WHOLE ? 1 : 2;
+  int key, there;  // the first key, -1: no tile; which halves are there (bits)
+  int k[N], v[N];  // where their scales are
+};
+template <bool WHOLE, typename A>
+struct CodeStream {
+  A& a;
+  const int32_t* table;
+  int hk, page, mark;
+  uint32_t krb, vrb;
+  int left, sinks, window;  // tiles left, those of the first keys, the window's first key
+  int col, slot, in_mark, ahead;
+  const char *kp, *vp;
+  int page1, slot1;
+  TileRef<WHOLE> ref;
+
+  __device__ __forceinline__ CodeStream(A& args, const Place& p)
+      : a(args),
+        table(args.table + p.b * args.table_stride),
+        hk(p.hk),
+        page(args.page),
+        mark(args.mark),
+        krb(static_cast<uint32_t>(args.sk[1])),
+        vrb(static_cast<uint32_t>(args.sv[1])) {
+    left = p.steps;
+    sinks = p.tiles.sink_n - p.begin;
+    window = p.tiles.win_t0 * kTileKeys;
+    slot1 = page1 = ahead = 0;
+    const int first = sinks > 0 ? p.begin * kTileKeys : window - sinks * kTileKeys;
+    jump(args, left > 0 ? first : -1);
+  }
+  template <typename X>
+  __device__ __forceinline__ int entry(X& x, int c) const {
+    return ld_const(table + (c < x.max_pages ? c : x.max_pages - 1));
+  }
+  // Row `at_slot` of a page (page 0's where it is not there).  (32 x 32-bit products: a page
+  // spans less than 4 GiB.)
+  struct At {
+    const char *k, *v;
+  };
+  template <typename X>
+  __device__ __forceinline__ At row_at(X& x, bool there, int pg, int at_slot) const {
+    const uint32_t at = there ? static_cast<uint32_t>(pg) : 0u;
+    const uint32_t row = static_cast<uint32_t>(at_slot);
+    return {static_cast<const char*>(x.k) + hk * x.sk[2] +
+                static_cast<uint64_t>(at) * static_cast<uint32_t>(x.sk[0]) +
+                static_cast<uint64_t>(row) * krb,
+            static_cast<const char*>(x.v) + hk * x.sv[2] +
+                static_cast<uint64_t>(at) * static_cast<uint32_t>(x.sv[0]) +
+                static_cast<uint64_t>(row) * vrb};
+  }
+  template <typename X>
+  __device__ __forceinline__ void on_page(X& x, int h, int pg, int at_slot) {
+    const bool there = ref.key >= 0 && page_ok(x, pg);
+    if (h == 0) {
+      const At at = row_at(x, there, pg, at_slot);
+      kp = at.k;
+      vp = at.v;
+    }
+    const int nth = divide(at_slot >> 4, x.by_half_mark), at = there ? pg : 0;
+    ref.k[h] = at * x.sks[0] + nth * x.sks[1];
+    ref.v[h] = at * x.svs[0] + nth * x.svs[1];
+    if constexpr (WHOLE) {
+      ref.there = there ? 3 : 0;
+      in_mark = at_slot - nth * mark;
+    } else {
+      ref.there = h == 0 ? (there ? 1 : 0) : ref.there + (there ? 2 : 0);
+    }
+  }
+  template <typename X>
+  __device__ __forceinline__ void jump(X& x, int key) {
+    ref.key = key;
+    const int k = key < 0 ? 0 : key;
+    col = divide(k >> 4, x.by_half_page);
+    slot = k - col * page;
+    const int page0 = entry(x, col);
+    on_page(x, 0, page0, slot);
+    if constexpr (WHOLE) {
+      ahead = entry(x, col + 1);
+    } else {
+      const bool same = slot + 16 < page;
+      slot1 = same ? slot + 16 : 0;
+      page1 = same ? page0 : entry(x, col + 1);
+      on_page(x, 1, page1, slot1);
+    }
+  }
+  __device__ __forceinline__ void next() {
+    --left;
+    --sinks;
+    if constexpr (WHOLE) {
+      // (arguments that only a new page needs are read again there: scalar registers are short)
+      if (left <= 0) {
+        ref.key = -1;
+        return;
+      }
+      if (sinks == 0) {
+        jump(late_args(), window);
+        return;
+      }
+      ref.key += kTileKeys;
+      slot += kTileKeys;
+      if (slot >= page) {
+        LateArgs& x = late_args();
+        ++col;
+        slot = 0;
+        on_page(x, 0, ahead, 0);
+        ahead = entry(x, col + 1);
+        return;
+      }
+      kp += kTileKeys * krb;
+      vp += kTileKeys * vrb;
+      in_mark += kTileKeys;
+      if (in_mark >= mark) {
+        LateArgs& x = late_args();
+        in_mark = 0;
+        ref.k[0] += x.sks[1];
+        ref.v[0] += x.svs[1];
+      }
+    } else {
+      jump(a, left <= 0 ? -1 : sinks == 0 ? window : ref.key + kTileKeys);
+    }
+  }
+  // The first rows of a half.
+  __device__ __forceinline__ At half(int h) const {
+    if constexpr (WHOLE) {
+      return {kp + h * 16 * krb, vp + h * 16 * vrb};
+    } else {
+      return h == 0 ? At{kp, vp} : row_at(a, ref.there & 2, page1, slot1);
+    }
+  }
+};
+// A positive number below 2^126, or 0.
+__device__ __forceinline__ float scale_or_0(float s) {
+  const uint32_t u = __float_as_uint(s);
+  return u - 1u < 0x7e800000u - 1u ? s : 0.0f;
+}
+// The scales of a tile (ks, vs: of the key head), 0 for a half that is not there.
+template <bool WHOLE>
+__device__ __forceinline__ Scales<WHOLE> scales_of(const TileRef<WHOLE>& t, const float* ks,
+                                                   const float* vs) {
+  Scales<WHOLE> r;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int pg = h ? s.page1 : s.page0;
-    const bool there = s.key >= 0 && page_ok(a, pg);
-    const int mark = divide(slot_of(a, s.key, h) >> 4, a.by_half_mark);
-    const int at = there ? pg : 0;
-    const float k = ld_const(ks + (at * a.sks[0] + mark * a.sks[1]));
-    const float v = ld_const(vs + (at * a.svs[0] + mark * a.svs[1]));
-    r.k[h] = there && k > 0.0f && k < 0x1p126f ? k : 0.0f;
-    r.v[h] = there && v > 0.0f && v < 0x1p126f ? v : 0.0f;
+  for (int h = 0; h < TileRef<WHOLE>::N; ++h) {
+    r.k[h] = scale_or_0(ld_const(ks + t.k[h]));
+    r.v[h] = (t.there >> h) & 1 ? scale_or_0(ld_const(vs + t.v[h])) : 0.0f;
   }
   return r;
+}
+// The unit 2^e of the accumulators: above the scales of all values so far.
+struct Unit2 {
+  uint32_t bits;  // of 2^e
+  float inv;      // 2^-e
+};
+__device__ __forceinline__ Unit2 least_unit() { return {1u << 23, 0x1p126f}; }
+// The least power of two above scale s, and the factor from unit u to it.
+__device__ __forceinline__ float raise_unit(Unit2& u, float s) {
+  const uint32_t e = (__float_as_uint(s) >> 23) + 1u;  // (at most 253)
+  const uint32_t down = e - (u.bits >> 23);
+  u = {e << 23, __uint_as_float((254u - e) << 23)};
+  return down >= 127u ? 0.0f : __uint_as_float((127u - down) << 23);
 }
 
 // The 32 keys of the tile at `key` that row `row` sees, as bits.

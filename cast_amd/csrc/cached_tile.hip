@@ -11,10 +11,10 @@ struct CodeTile : RowTile<_Float16, D> {
   using R = RowTile<_Float16, D>;
   using O = Half<_Float16>;
   float c_row;  // logit of q . c, times the key's scale, in log2 units
-  int v_exp;    // accumulators are in units of 2^v_exp
+  Unit2 unit;   // of the accumulators
 
-  template <typename Bits, typename Pre>
-  __device__ __forceinline__ void step8(const char* tile, const Scales& sc, int hf, bool inside,
+  template <bool WHOLE, typename Bits, typename Pre>
+  __device__ __forceinline__ void step8(const char* tile, const Scales<WHOLE>& sc, int hf, bool inside,
                                         Bits&& bits, Pre&& prefetch) {
     // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
     v4i kraw[R::QSTEPS];
@@ -33,23 +33,20 @@ struct CodeTile : RowTile<_Float16, D> {
     __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
     __builtin_amdgcn_sched_barrier(0);
     prefetch();
-    int e_new = v_exp;
+    constexpr int N = Scales<WHOLE>::N;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = static_cast<int>(__float_as_uint(sc.v[h]) >> 23) - 126;  // 2^e > the scale
-      e_new = sc.v[h] > 0.0f && e > e_new ? e : e_new;
-    }
-    if (e_new != v_exp) {
-      const int down = v_exp - e_new;
-      const float f = down < -126 ? 0.0f : power_of(down);
+    for (int h = 0; h < N; ++h)
+      if (__float_as_uint(sc.v[h]) >= unit.bits) {
+        const float f = raise_unit(unit, sc.v[h]);
 #pragma unroll
-      for (int dt = 0; dt < R::NDT; ++dt)
+        for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
-      v_exp = e_new;
-    }
-    const float c = fmaxf(c_row * (hf ? sc.k[1] : sc.k[0]), 0x1p-126f);  // (0 * -inf is NaN)
-    const float f = fmaxf((hf ? sc.v[1] : sc.v[0]) * power_of(-v_exp), 0x1p-60f);
+          for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
+      }
+    const float ks = N == 1 ? sc.k[0] : hf ? sc.k[N - 1] : sc.k[0];
+    const float vs = N == 1 ? sc.v[0] : hf ? sc.v[N - 1] : sc.v[0];
+    const float c = fmaxf(c_row * ks, 0x1p-126f);  // (0 * -inf is NaN)
+    const float f = fmaxf(vs * unit.inv, 0x1p-60f);
     const float log_f = __builtin_amdgcn_logf(f);
     float rv[16];
 #pragma unroll
@@ -117,7 +114,7 @@ struct CodeTile : RowTile<_Float16, D> {
   }
 };
 
-template <typename T, bool E4M3, int D>
+template <typename T, bool E4M3, int D, bool WHOLE>
 __global__ void __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 3, D == 64 ? 4 : 3)))
 cached_tile_kernel(WindowArgs a) {
@@ -164,7 +161,7 @@ cached_tile_kernel(WindowArgs a) {
 
   C t;
   t.init(lane);
-  t.v_exp = -126;
+  t.unit = least_unit();
   {
     const Row r = row_of(a, p, p.row0 + lr);
     const T* const row = static_cast<const T*>(a.q) + p.b * a.sq[0] +
@@ -184,10 +181,8 @@ cached_tile_kernel(WindowArgs a) {
     t.c_row = a.scale_log2 * power_of(-k);
   }
 
-  const char* const kbase = static_cast<const char*>(a.k) + p.hk * a.sk[2];
-  const char* const vbase = static_cast<const char*>(a.v) + p.hk * a.sv[2];
-  const uint32_t krb = static_cast<uint32_t>(a.sk[1]), vrb = static_cast<uint32_t>(a.sv[1]);
-  const int32_t* const table = a.table + p.b * a.table_stride;
+  CodeStream<WHOLE, WindowArgs> codes(a, p);
+  const uint32_t krb = codes.krb, vrb = codes.vrb;
 
   // Copies: a wavefront moves rows 8 w .. 8 w + 7 of a tile, which lie in its half w / 2, as they
   // are into its part of a slot (D 64: the lanes past them zeros), 16 bytes a lane.
@@ -196,11 +191,10 @@ cached_tile_kernel(WindowArgs a) {
   const uint32_t none = lane < 8 * LPR ? 0u : 0x80000000u;
   const uint32_t k_lo = (in_half * krb + lane % LPR * 16) | none;
   const uint32_t v_lo = (in_half * vrb + lane % LPR * 16) | none;
-  auto stage = [&](const CodeStep& s, char* dst) __attribute__((always_inline)) {
-    const HalfAt h = half_at(a, s, wave >> 1, krb, vrb);
-    buffer_copy16(const_cast<char*>(kbase) + h.k, 16 * static_cast<int>(krb), k_lo,
-                  dst + wave * 2048);
-    buffer_copy16(const_cast<char*>(vbase) + h.v, 16 * static_cast<int>(vrb), v_lo,
+  auto stage = [&](char* dst) __attribute__((always_inline)) {
+    const auto h = codes.half(wave >> 1);
+    buffer_copy16(const_cast<char*>(h.k), 16 * static_cast<int>(krb), k_lo, dst + wave * 2048);
+    buffer_copy16(const_cast<char*>(h.v), 16 * static_cast<int>(vrb), v_lo,
                   dst + wave * 2048 + 1024);
   };
   // Its own copies, landed, become fp16 in the tile: lane l BPL bytes of row 8 w + l / 8.
@@ -236,56 +230,60 @@ cached_tile_kernel(WindowArgs a) {
   // j - 2 by then); its codes landed in raw slot j % 2, asked for during step j - 3.
   const float* const ks = a.ks + p.hk * a.sks[2];
   const float* const vs = a.vs + p.hk * a.svs[2];
-  CodeStep e0 = code_step(a, p, table, 0), e1 = code_step(a, p, table, 1);
-  CodeStep e2 = code_step(a, p, table, 2), e3 = code_step(a, p, table, 3);
-  stage(e0, r_0);
+  typedef TileRef<WHOLE> Ref;
+  Ref e0 = codes.ref, e1, e2;
+  stage(r_0);
   __builtin_amdgcn_sched_barrier(0);
-  stage(e1, r_1);
+  codes.next();
+  e1 = codes.ref;
+  stage(r_1);
   __builtin_amdgcn_sched_barrier(0);
-  Scales sc = scales_of(a, e0, ks, vs);
+  codes.next();
+  e2 = codes.ref;
+  Scales<WHOLE> sc = scales_of(e0, ks, vs);
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));
   widen(r_0, s_0);
   __builtin_amdgcn_sched_barrier(0);  // (its codes are in registers)
-  stage(e2, r_0);
-  auto iteration = [&](auto slot_c, int j) __attribute__((always_inline)) {
+  stage(r_0);
+  codes.next();
+  auto iteration = [&](auto slot_c) __attribute__((always_inline)) {
     constexpr int J = decltype(slot_c)::value;
     char* const tile = J == 0 ? s_0 : s_1;
     char* const fill = J == 0 ? s_1 : s_0;
-    char* const codes = J == 0 ? r_1 : r_0;
+    char* const raw_slot = J == 0 ? r_1 : r_0;
     asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    widen(codes, fill);
+    widen(raw_slot, fill);
     __builtin_amdgcn_sched_barrier(0);
-    stage(e3, codes);
+    stage(raw_slot);
     __builtin_amdgcn_sched_barrier(0);
-    const int key = e0.key, there = halves_there(a, e0);
-    const Scales ns = sc;
+    const int key = e0.key, there = e0.there;
+    const Scales<WHOLE> ns = sc;
     e0 = e1;
     e1 = e2;
-    e2 = e3;
+    e2 = codes.ref;
     const bool inside = key >= 0 && there == 3 && key + kTileKeys <= w_first.hi &&
                         (key >= w_last.lo || key + kTileKeys <= a.sinks);
-    t.step8(
+    t.template step8<WHOLE>(
         tile, ns, hf, inside,
         [&]() __attribute__((always_inline)) {
           return key < 0 ? 0u : seen_bits(late_args(), p, p.row0 + lr, hf, key, there);
         },
         [&]() __attribute__((always_inline)) {
-          sc = scales_of(a, e0, ks, vs);
-          e3 = code_step(a, p, table, j + 4);
+          sc = scales_of(e0, ks, vs);
+          codes.next();
         });
   };
   const int rounds = (p.steps + 1) / 2;
   for (int rd = 0; rd < rounds; ++rd) {
-    iteration(std::integral_constant<int, 0>{}, 2 * rd);
-    iteration(std::integral_constant<int, 1>{}, 2 * rd + 1);
+    iteration(std::integral_constant<int, 0>{});
+    iteration(std::integral_constant<int, 1>{});
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));  // trailing copies land before the slots are freed
 
   // the end of the wavefront's rows
   LateArgs& e = late_args();
   const float l = pair_sum(t.l_run), m = t.m_run;
-  const float unit = power_of(t.v_exp);
-  const float inv = l > 0.0f ? unit / l : l;  // (a NaN sum stays one)
+  const float inv = l > 0.0f ? __uint_as_float(t.unit.bits) / l : l;  // (a NaN sum stays one)
 #pragma unroll
   for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
@@ -321,13 +319,18 @@ cached_tile_kernel(WindowArgs a) {
         l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
+template <typename T, bool E4M3, int D>
+static void launch(WindowArgs& a, dim3 grid, hipStream_t s) {
+  const dim3 block(256);
+  if (a.whole_tiles && a.mark % kTileKeys == 0)
+    cached_tile_kernel<T, E4M3, D, true><<<grid, block, 0, s>>>(a);
+  else
+    cached_tile_kernel<T, E4M3, D, false><<<grid, block, 0, s>>>(a);
+}
 template <typename T>
 static void launch_type(WindowArgs& a, bool e4m3, int64_t D, dim3 grid, hipStream_t s) {
-  const dim3 block(256);
-  if (e4m3 && D == 128) cached_tile_kernel<T, true, 128><<<grid, block, 0, s>>>(a);
-  else if (e4m3) cached_tile_kernel<T, true, 64><<<grid, block, 0, s>>>(a);
-  else if (D == 128) cached_tile_kernel<T, false, 128><<<grid, block, 0, s>>>(a);
-  else cached_tile_kernel<T, false, 64><<<grid, block, 0, s>>>(a);
+  if (e4m3) D == 128 ? launch<T, true, 128>(a, grid, s) : launch<T, true, 64>(a, grid, s);
+  else D == 128 ? launch<T, false, 128>(a, grid, s) : launch<T, false, 64>(a, grid, s);
 }
 
 void launch_cached_tile(WindowArgs& a, int type, bool e4m3, int64_t D, dim3 grid, hipStream_t s) {

@@ -10,7 +10,7 @@
 
 namespace rcsa {
 
-template <typename T, bool E4M3, int D, bool GROUP>
+template <typename T, bool E4M3, int D, bool WHOLE, bool GROUP>
 __global__ void __launch_bounds__(GROUP ? 64 * kGroupWaves : 64)
 __attribute__((amdgpu_waves_per_eu(2, 2)))
 cached_unit_kernel(WindowArgs a) {
@@ -44,17 +44,12 @@ cached_unit_kernel(WindowArgs a) {
   p.tiles = tiles_of(a, first, last);
   share_of(p, u.share);
 
-  const char* const kbase = static_cast<const char*>(a.k) + p.hk * a.sk[2];
-  const char* const vbase = static_cast<const char*>(a.v) + p.hk * a.sv[2];
-  const uint32_t krb = static_cast<uint32_t>(a.sk[1]), vrb = static_cast<uint32_t>(a.sv[1]);
-  const int32_t* const table = a.table + p.b * a.table_stride;
-
   // The lane's row of the queries: step st of the products takes the channels of 8 bytes st & 1
   // of load st / 2.
-  const Row my = row_of(a, p, lr);
   v8hf q_op[2 * KL];
   float c_row;
   {
+    const Row my = row_of(a, p, lr);
     const T* const row = static_cast<const T*>(a.q) + p.b * a.sq[0] +
                          static_cast<int64_t>(my.qi) * a.sq[1] + my.head * a.sq[2];
     op8 raw[2 * KL];
@@ -78,52 +73,62 @@ cached_unit_kernel(WindowArgs a) {
     v4i k[KL];
     uint32_t v[16];
   };
-  auto load_k = [&](const CodeStep& s, v4i (&k)[KL]) __attribute__((always_inline)) {
-    const HalfAt h0 = half_at(a, s, 0, krb, vrb), h1 = half_at(a, s, 1, krb, vrb);
-    const char* const at = kbase + (lr < 16 ? h0.k : h1.k) + static_cast<uint64_t>(lr & 15) * krb +
-                           hf * 16;
+  CodeStream<WHOLE, WindowArgs> codes(a, p);
+  const uint32_t krb = codes.krb, vrb = codes.vrb;
+  auto load_k = [&](v4i (&k)[KL]) __attribute__((always_inline)) {
+    const char* at;
+    if constexpr (WHOLE) {
+      at = codes.kp + (lr * krb + hf * 16);
+    } else {
+      const auto h0 = codes.half(0), h1 = codes.half(1);
+      at = (lr < 16 ? h0.k : h1.k) + ((lr & 15) * krb + hf * 16);
+    }
 #pragma unroll
     for (int i = 0; i < KL; ++i) k[i] = *reinterpret_cast<const v4i*>(at + 32 * i);
   };
-  auto load_v = [&](const CodeStep& s, uint32_t (&v)[16]) __attribute__((always_inline)) {
-    const int at = static_cast<int>(4 * hf * vrb + NDT * lr);
+  int v_lo[4];  // rows 4 hf + 0 .. 3; the others are 8, 16 and 24 further
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v_lo[j] = static_cast<int>((4 * hf + j) * vrb + NDT * lr);
+  auto load_v = [&](uint32_t (&v)[16]) __attribute__((always_inline)) {
+    const char* from = codes.half(0).v;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const HalfAt r = half_at(a, s, h, krb, vrb);
+      if (!WHOLE && h == 1) from = codes.half(1).v;
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<char*>(vbase) + r.v, 0, 16 * static_cast<int>(vrb), kRsrcWord3);
+          const_cast<char*>(from), 0, (WHOLE ? 32 : 16) * static_cast<int>(vrb), kRsrcWord3);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int off = (8 * (j >> 2) + (j & 3)) * static_cast<int>(vrb);
+        const int off = (8 * (j >> 2) + (WHOLE ? 16 * h : 0)) * static_cast<int>(vrb);
         if constexpr (NDT == 4)
           v[8 * h + j] = static_cast<uint32_t>(
-              __builtin_amdgcn_raw_buffer_load_b32(rs, at, off, 0));
+              __builtin_amdgcn_raw_buffer_load_b32(rs, v_lo[j & 3], off, 0));
         else
           v[8 * h + j] = static_cast<uint16_t>(
-              __builtin_amdgcn_raw_buffer_load_b16(rs, at, off, 0));
+              __builtin_amdgcn_raw_buffer_load_b16(rs, v_lo[j & 3], off, 0));
       }
     }
   };
 
   const float* const ks = a.ks + p.hk * a.sks[2];
   const float* const vs = a.vs + p.hk * a.svs[2];
-  CodeStep cur = code_step(a, p, table, 0), next = code_step(a, p, table, 1);
   Tile t;
-  load_k(cur, t.k);
-  load_v(cur, t.v);
-  Scales sc = scales_of(a, cur, ks, vs);
+  load_k(t.k);
+  load_v(t.v);
+  TileRef<WHOLE> cur = codes.ref;
+  Scales<WHOLE> sc = scales_of(cur, ks, vs);
+  codes.next();
   v16f o_acc[NDT];
 #pragma unroll
   for (int x = 0; x < NDT; ++x)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o_acc[x][r] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;
-  int v_exp = -126;  // accumulators are in units of 2^v_exp
+  Unit2 unit = least_unit();  // of the accumulators
   constexpr int kShift = Half<_Float16>::kShift;
 
   for (int s = 0; s < p.steps; ++s) {
-    const int key = cur.key, there = halves_there(a, cur);
-    const Scales ns = sc;
+    const int key = cur.key, there = cur.there;
+    const Scales<WHOLE> ns = sc;
     v16f s_acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
@@ -134,15 +139,15 @@ cached_unit_kernel(WindowArgs a) {
       s_acc = Half<_Float16>::mfma(lo, q_op[2 * i], s_acc);
       s_acc = Half<_Float16>::mfma(hi, q_op[2 * i + 1], s_acc);
     }
-    cur = next;
     const bool more = s + 1 < p.steps;
     if (more) {
-      load_k(cur, t.k);
-      sc = scales_of(a, cur, ks, vs);
-      next = code_step(a, p, table, s + 2);
+      load_k(t.k);
+      cur = codes.ref;
+      sc = scales_of(cur, ks, vs);
     }
     // logits in log2 units: r < 8 of the first half's keys, the others of the second's
-    const float c0 = c_row * ns.k[0], c1 = c_row * ns.k[1];
+    constexpr int N = Scales<WHOLE>::N;
+    const float c0 = c_row * ns.k[0], c1 = c_row * ns.k[N - 1];
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r] * (r < 8 ? c0 : c1);
@@ -155,22 +160,16 @@ cached_unit_kernel(WindowArgs a) {
         rv[r] = (seen >> (8 * (r >> 2) + (r & 3))) & 1u ? rv[r] : -INFINITY;
     }
     // the scales of the values, relative to the largest so far
-    int e_new = v_exp;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int e = static_cast<int>(__float_as_uint(ns.v[h]) >> 23) - 126;  // 2^e > the scale
-      e_new = ns.v[h] > 0.0f && e > e_new ? e : e_new;
-    }
-    if (e_new != v_exp) {
-      const int down = v_exp - e_new;
-      const float f = down < -126 ? 0.0f : power_of(down);
+    for (int h = 0; h < N; ++h)
+      if (__float_as_uint(ns.v[h]) >= unit.bits) {
+        const float f = raise_unit(unit, ns.v[h]);
 #pragma unroll
-      for (int x = 0; x < NDT; ++x)
+        for (int x = 0; x < NDT; ++x)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o_acc[x][r] *= f;
-      v_exp = e_new;
-    }
-    const float f0 = ns.v[0] * power_of(-v_exp), f1 = ns.v[1] * power_of(-v_exp);
+          for (int r = 0; r < 16; ++r) o_acc[x][r] *= f;
+      }
+    const float f0 = ns.v[0] * unit.inv, f1 = ns.v[N - 1] * unit.inv;
     v8hf p_op[2];
     auto exps = [&]() __attribute__((always_inline)) -> float {
       const float bias = m_run == -INFINITY ? 0.0f : -m_run;
@@ -206,7 +205,10 @@ cached_unit_kernel(WindowArgs a) {
     uint32_t tamed[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) tamed[r] = Widen<E4M3>::tame(Widen<E4M3>::finite(t.v[r]));
-    if (more) load_v(cur, t.v);
+    if (more) {
+      load_v(t.v);
+      codes.next();
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -216,17 +218,18 @@ cached_unit_kernel(WindowArgs a) {
 
   // The end of the rows: lane (row, hf) holds channels 32 g' + ... : register r of product x is
   // channel NDT (8 (r / 4) + 4 hf + r % 4) + x.
+  LateArgs& e = late_args();
+  const Row my = row_of(e, p, lr);
   const float l = pair_sum(l_run);
-  const float unit = power_of(v_exp);
-  const float inv = l > 0.0f ? unit / l : l;  // (a NaN sum stays one)
+  const float inv = l > 0.0f ? __uint_as_float(unit.bits) / l : l;  // (a NaN sum stays one)
   auto value = [&](int r, int x) __attribute__((always_inline)) -> float {
     return l == 0.0f ? 0.0f : o_acc[x][r] * (1 << Widen<E4M3>::kShift) * inv;
   };
   const bool live = lr < p.n_rows;
   if (GROUP || p.shares > 1) {
-    const int64_t ws_row = GROUP ? 0 : static_cast<int64_t>(blockIdx.x) * a.Lq * a.G;
-    float* const part_o = GROUP ? s_o[wave] : a.ws_o + ws_row * D;
-    float2* const part_ml = GROUP ? s_ml[wave] : a.ws_ml + ws_row;
+    const int64_t ws_row = GROUP ? 0 : static_cast<int64_t>(blockIdx.x) * e.Lq * e.G;
+    float* const part_o = GROUP ? s_o[wave] : e.ws_o + ws_row * D;
+    float2* const part_ml = GROUP ? s_ml[wave] : e.ws_ml + ws_row;
     if (live) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -238,8 +241,8 @@ cached_unit_kernel(WindowArgs a) {
         part_ml[lr] = make_float2(l > 0.0f ? m_run : (l == 0.0f ? -INFINITY : l), l);
     }
   } else if (live) {
-    T* const op = static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(my.qi) * a.so[1] +
-                  my.head * a.so[2];
+    T* const op = static_cast<T*>(e.out) + p.b * e.so[0] + static_cast<int64_t>(my.qi) * e.so[1] +
+                  my.head * e.so[2];
 #pragma unroll
     for (int r = 0; r < 16; r += 4 / NDT) {
       typename Half<T>::op4 w4;
@@ -248,8 +251,8 @@ cached_unit_kernel(WindowArgs a) {
       *reinterpret_cast<typename Half<T>::op4*>(
           op + NDT * (8 * (r >> 2) + 4 * hf + (r & 3))) = w4;
     }
-    if (hf == 0 && a.lse)
-      a.lse[(static_cast<int64_t>(p.b) * a.Hq + my.head) * a.Lq + my.qi] =
+    if (hf == 0 && e.lse)
+      e.lse[(static_cast<int64_t>(p.b) * e.Hq + my.head) * e.Lq + my.qi] =
           l == 0.0f ? -INFINITY : (m_run + __log2f(l)) * 0.69314718055994531f;
   }
   if constexpr (GROUP) {
@@ -269,38 +272,44 @@ cached_unit_kernel(WindowArgs a) {
         sum += f;
         const v4f o = *reinterpret_cast<const v4f*>(s_o[s] + row * D + c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = join(f, o[e], acc[e]);
+        for (int i = 0; i < 4; ++i) acc[i] = join(f, o[i], acc[i]);
       }
-      const Row r = row_of(a, p, row);
+      const Row r = row_of(e, p, row);
       typename Half<T>::op4 out;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(sum == 0.0f ? 0.0f : acc[e] / sum);
+      for (int i = 0; i < 4; ++i) out[i] = static_cast<T>(sum == 0.0f ? 0.0f : acc[i] / sum);
       *reinterpret_cast<typename Half<T>::op4*>(
-          static_cast<T*>(a.out) + p.b * a.so[0] + static_cast<int64_t>(r.qi) * a.so[1] +
-          r.head * a.so[2] + c) = out;
-      if (a.lse && c == 0)
-        a.lse[(static_cast<int64_t>(p.b) * a.Hq + r.head) * a.Lq + r.qi] =
+          static_cast<T*>(e.out) + p.b * e.so[0] + static_cast<int64_t>(r.qi) * e.so[1] +
+          r.head * e.so[2] + c) = out;
+      if (e.lse && c == 0)
+        e.lse[(static_cast<int64_t>(p.b) * e.Hq + r.head) * e.Lq + r.qi] =
             sum == 0.0f ? -INFINITY : (mx + __log2f(sum)) * 0.69314718055994531f;
     }
   }
 }
 
-template <typename T, bool E4M3, int D>
+template <typename T, bool E4M3, int D, bool WHOLE>
 static int launch(WindowArgs& a, int64_t units, hipStream_t s) {
   if (a.units == 0) {
     const dim3 grid(static_cast<unsigned>(a.B * a.Hk)), block(64 * kGroupWaves);
-    cached_unit_kernel<T, E4M3, D, true><<<grid, block, 0, s>>>(a);
+    cached_unit_kernel<T, E4M3, D, WHOLE, true><<<grid, block, 0, s>>>(a);
     return launch_status();
   }
-  cached_unit_kernel<T, E4M3, D, false>
+  cached_unit_kernel<T, E4M3, D, WHOLE, false>
       <<<dim3(static_cast<unsigned>(units)), dim3(64), 0, s>>>(a);
   return launch_unit_merge(a, std::is_same<T, __bf16>::value ? 0 : 1, D, s);
 }
 
+template <typename T, bool E4M3, int D>
+static int launch_form(WindowArgs& a, int64_t units, hipStream_t s) {
+  return a.whole_tiles && a.mark % kTileKeys == 0 ? launch<T, E4M3, D, true>(a, units, s)
+                                                  : launch<T, E4M3, D, false>(a, units, s);
+}
 template <typename T>
 static int launch_type(WindowArgs& a, bool e4m3, int64_t D, int64_t units, hipStream_t s) {
-  if (e4m3) return D == 128 ? launch<T, true, 128>(a, units, s) : launch<T, true, 64>(a, units, s);
-  return D == 128 ? launch<T, false, 128>(a, units, s) : launch<T, false, 64>(a, units, s);
+  if (e4m3)
+    return D == 128 ? launch_form<T, true, 128>(a, units, s) : launch_form<T, true, 64>(a, units, s);
+  return D == 128 ? launch_form<T, false, 128>(a, units, s) : launch_form<T, false, 64>(a, units, s);
 }
 
 int launch_cached_units(WindowArgs& a, int type, bool e4m3, int64_t D, int64_t units,

@@ -52,6 +52,7 @@ struct WindowArgs {
   const float *ks, *vs;
   int sks[3], svs[3];  // (their last one is below 2^29)
   Divisor by_half_mark;
+  int mark;
   int e4m3;        // the codes' type; -1: 16-bit keys and values
   // packed: rows of the requests in q and in k, v ([B + 1] each), a request's row blocks
   // numbered through n_ranks

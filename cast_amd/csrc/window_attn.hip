@@ -286,6 +286,7 @@ static int run(const void* q, const void* k, const void* v, void* out, float* ls
       a.sks[i] = static_cast<int>(codes->strides[i]);
       a.svs[i] = static_cast<int>(codes->strides[3 + i]);
     }
+    a.mark = static_cast<int>(codes->block_size);
     a.by_half_mark = divisor(static_cast<uint32_t>(codes->block_size / 16));
   }
   const int64_t ws_rows = need / (dims[5] * 4 + 8);
