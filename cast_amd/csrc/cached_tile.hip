@@ -12,27 +12,12 @@ struct CodeTile : RowTile<_Float16, D> {
   using O = Half<_Float16>;
   float c_row;  // logit of q . c, times the key's scale, in log2 units
   Unit2 unit;   // of the accumulators
+  // what a tile's scales give: logits, log2 of a weight's factor and its reciprocal
+  float c, log_f, inv_f;
 
-  template <bool WHOLE, typename Bits, typename Pre>
-  __device__ __forceinline__ void step8(const char* tile, const Scales<WHOLE>& sc, int hf, bool inside,
-                                        Bits&& bits, Pre&& prefetch) {
-    // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
-    v4i kraw[R::QSTEPS];
-    int k0 = this->k_off[0];
-    asm volatile("" : "+v"(k0));
-#pragma unroll
-    for (int st = 0; st < R::QSTEPS; ++st)
-      kraw[st] = *reinterpret_cast<const v4i*>(tile + (k0 ^ (st * 16)));
-    v16f s_acc;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
-#pragma unroll
-    for (int st = 0; st < R::QSTEPS; ++st)
-      s_acc = O::mfma(__builtin_bit_cast(v8hf, kraw[st]), this->q_op[st], s_acc);
-    __builtin_amdgcn_sched_group_barrier(0x100, R::QSTEPS, 0);
-    __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    prefetch();
+  // (a branch of its own: scales change where a block ends)
+  template <bool WHOLE>
+  __device__ __forceinline__ void take(const Scales<WHOLE>& sc, int hf) {
     constexpr int N = Scales<WHOLE>::N;
 #pragma unroll
     for (int h = 0; h < N; ++h)
@@ -45,9 +30,36 @@ struct CodeTile : RowTile<_Float16, D> {
       }
     const float ks = N == 1 ? sc.k[0] : hf ? sc.k[N - 1] : sc.k[0];
     const float vs = N == 1 ? sc.v[0] : hf ? sc.v[N - 1] : sc.v[0];
-    const float c = fmaxf(c_row * ks, 0x1p-126f);  // (0 * -inf is NaN)
+    c = fmaxf(c_row * ks, 0x1p-126f);  // (0 * -inf is NaN)
     const float f = fmaxf(vs * unit.inv, 0x1p-60f);
-    const float log_f = __builtin_amdgcn_logf(f);
+    log_f = __builtin_amdgcn_logf(f);
+    inv_f = __builtin_amdgcn_rcpf(f);
+  }
+
+  template <bool WHOLE, typename Bits, typename Pre>
+  __device__ __forceinline__ void step8(const char* tile, const Scales<WHOLE>& sc, bool changed,
+                                        int hf, bool inside,
+                                        Bits&& bits, Pre&& prefetch) {
+    // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
+    v4i kraw[R::QSTEPS];
+    constexpr int HELD = 4;
+    int far = 64;
+    asm volatile("" : "+s"(far));
+#pragma unroll
+    for (int st = 0; st < R::QSTEPS; ++st)
+      kraw[st] = *reinterpret_cast<const v4i*>(
+          tile + (st < HELD ? this->k_off[st] : this->k_off[st - HELD] ^ far));
+    v16f s_acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
+#pragma unroll
+    for (int st = 0; st < R::QSTEPS; ++st)
+      s_acc = O::mfma(__builtin_bit_cast(v8hf, kraw[st]), this->q_op[st], s_acc);
+    __builtin_amdgcn_sched_group_barrier(0x100, R::QSTEPS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    prefetch();
+    if (!WHOLE || changed) take<WHOLE>(sc, hf);
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
@@ -91,7 +103,7 @@ struct CodeTile : RowTile<_Float16, D> {
         part = exps();
       }
     }
-    this->l_run = fmaf(part, __builtin_amdgcn_rcpf(f), this->l_run);
+    this->l_run = fmaf(part, inv_f, this->l_run);
     int v0 = this->v_off[0];
     asm volatile("" : "+v"(v0));
     auto v_group = [&](int u, v8hf (&op)[R::NDT]) __attribute__((always_inline)) {
@@ -246,6 +258,7 @@ cached_tile_kernel(WindowArgs a) {
   __builtin_amdgcn_sched_barrier(0);  // (its codes are in registers)
   stage(r_0);
   codes.next();
+  uint32_t had_k = ~0u, had_v = ~0u;  // (the scales of the tile before: none)
   auto iteration = [&](auto slot_c) __attribute__((always_inline)) {
     constexpr int J = decltype(slot_c)::value;
     char* const tile = J == 0 ? s_0 : s_1;
@@ -258,13 +271,16 @@ cached_tile_kernel(WindowArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     const int key = e0.key, there = e0.there;
     const Scales<WHOLE> ns = sc;
+    const bool changed = __float_as_uint(ns.k[0]) != had_k || __float_as_uint(ns.v[0]) != had_v;
+    had_k = __float_as_uint(ns.k[0]);
+    had_v = __float_as_uint(ns.v[0]);
     e0 = e1;
     e1 = e2;
     e2 = codes.ref;
     const bool inside = key >= 0 && there == 3 && key + kTileKeys <= w_first.hi &&
                         (key >= w_last.lo || key + kTileKeys <= a.sinks);
     t.template step8<WHOLE>(
-        tile, ns, hf, inside,
+        tile, ns, changed, hf, inside,
         [&]() __attribute__((always_inline)) {
           return key < 0 ? 0u : seen_bits(late_args(), p, p.row0 + lr, hf, key, there);
         },
