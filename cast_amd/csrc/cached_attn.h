@@ -49,29 +49,16 @@ struct Widen<true> {  // e4m3
   }
 };
 
-// Sixteen codes as two operands of eight.
+// Eight codes as an operand.
 template <bool E4M3>
-__device__ __forceinline__ void widen16(v4i w, v8hf& lo, v8hf& hi) {
+__device__ __forceinline__ v8hf widen8(uint32_t w0, uint32_t w1) {
   using W = Widen<E4M3>;
-  v2hf p[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t t = W::tame(static_cast<uint32_t>(w[i]));
-    p[2 * i] = W::pair(t, false);
-    p[2 * i + 1] = W::pair(t, true);
-  }
-  struct Two {
-    v2hf p[8];
+  const uint32_t t0 = W::tame(w0), t1 = W::tame(w1);
+  struct Four {
+    v2hf p[4];
   };
-  struct Ops {
-    v8hf lo, hi;
-  };
-  Two two;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) two.p[i] = p[i];
-  const Ops o = __builtin_bit_cast(Ops, two);
-  lo = o.lo;
-  hi = o.hi;
+  return __builtin_bit_cast(
+      v8hf, Four{{W::pair(t0, false), W::pair(t0, true), W::pair(t1, false), W::pair(t1, true)}});
 }
 
 // Column x of four words, byte by byte, as one word of four: column(x, w0 .. w3).

@@ -134,8 +134,6 @@ cached_tile_kernel(WindowArgs a) {
   using R = RowTile<_Float16, D>;
   typedef typename Half<T>::op8 op8;
   constexpr int BM = 128;
-  // bytes of a row that a lane widens
-  constexpr int BPL = D / 8, CHUNKS = BPL / 8;  // (16-byte chunks of the fp16 row)
   __shared__ __attribute__((aligned(1024))) char s_0[2 * R::TILE];
   __shared__ __attribute__((aligned(1024))) char s_1[2 * R::TILE];
   __shared__ __attribute__((aligned(1024))) char r_0[8192];
@@ -209,33 +207,23 @@ cached_tile_kernel(WindowArgs a) {
     buffer_copy16(const_cast<char*>(h.v), 16 * static_cast<int>(vrb), v_lo,
                   dst + wave * 2048 + 1024);
   };
-  // Its own copies, landed, become fp16 in the tile: lane l BPL bytes of row 8 w + l / 8.
-  const int trow = 8 * wave + (lane >> 3);
-  const int raw = wave * 2048 + lane * BPL;
-  const int chunk = (lane & 7) * CHUNKS;  // (the next chunk: one bit up)
+  // Its own copies, landed, become fp16 in the tile: lane l the 8 codes of chunk l % CPR of rows
+  // 8 w + l / CPR and, D 128, the one 4 further (its swizzle: K's chunk ^ 4).  Whole rows at a
+  // time, so that the writes of a row meet no bank twice.
+  const int trow = 8 * wave + lane / R::CPR, chunk = lane % R::CPR;
+  const int raw = wave * 2048 + lane * 8;
   const int k_at = trow * R::KROW + ((chunk ^ (swz_k<R::KROW>(trow) & (R::CPR - 1))) * 16);
   const int v_at = R::TILE + trow * R::KROW + ((chunk ^ (swz_v(trow) & (R::CPR - 1))) * 16);
   auto widen = [&](const char* src, char* dst) __attribute__((always_inline)) {
-    auto half = [&](const char* from, int at, bool values) __attribute__((always_inline)) {
-      v4i w = {0, 0, 0, 0};
-      if constexpr (BPL == 16) {
-        w = *reinterpret_cast<const v4i*>(from);
-      } else {
-        const auto two = *reinterpret_cast<const v2u*>(from);
-        w[0] = static_cast<int>(two[0]);
-        w[1] = static_cast<int>(two[1]);
-      }
-      if (values)
 #pragma unroll
-        for (int i = 0; i < BPL / 4; ++i)
-          w[i] = static_cast<int>(Widen<E4M3>::finite(static_cast<uint32_t>(w[i])));
-      v8hf o[2];
-      widen16<E4M3>(w, o[0], o[1]);
-      *reinterpret_cast<v8hf*>(dst + at) = o[0];
-      if constexpr (CHUNKS == 2) *reinterpret_cast<v8hf*>(dst + (at ^ 16)) = o[1];
-    };
-    half(src + raw, k_at, false);
-    half(src + raw + 1024, v_at, true);
+    for (int i = 0; i < D / 64; ++i) {
+      const v2u k = *reinterpret_cast<const v2u*>(src + raw + 512 * i);
+      const v2u v = *reinterpret_cast<const v2u*>(src + raw + 1024 + 512 * i);
+      *reinterpret_cast<v8hf*>(dst + (i == 0 ? k_at : (k_at ^ 64) + 4 * R::KROW)) =
+          widen8<E4M3>(k[0], k[1]);
+      *reinterpret_cast<v8hf*>(dst + v_at + i * 4 * R::KROW) =
+          widen8<E4M3>(Widen<E4M3>::finite(v[0]), Widen<E4M3>::finite(v[1]));
+    }
   };
 
   // Tile j is in slot j % 2 as fp16, written during step j - 1 (every wavefront has left step

@@ -134,10 +134,12 @@ cached_unit_kernel(WindowArgs a) {
     for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
 #pragma unroll
     for (int i = 0; i < KL; ++i) {
-      v8hf lo, hi;
-      widen16<E4M3>(t.k[i], lo, hi);
-      s_acc = Half<_Float16>::mfma(lo, q_op[2 * i], s_acc);
-      s_acc = Half<_Float16>::mfma(hi, q_op[2 * i + 1], s_acc);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        s_acc = Half<_Float16>::mfma(
+            widen8<E4M3>(static_cast<uint32_t>(t.k[i][2 * j]),
+                         static_cast<uint32_t>(t.k[i][2 * j + 1])),
+            q_op[2 * i + j], s_acc);
     }
     const bool more = s + 1 < p.steps;
     if (more) {
