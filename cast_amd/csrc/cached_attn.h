@@ -24,41 +24,60 @@ struct Widen;
 
 template <>
 struct Widen<false> {  // int8
-  static constexpr int kShift = 9;  // columns() gives c 2^-9
   static __device__ __forceinline__ uint32_t tame(uint32_t w) { return w ^ 0x80808080u; }
-  // c + 128 beneath the exponent of 1024, less 1152: exact
-  static __device__ __forceinline__ v2hf pair(uint32_t tamed, bool hi) {
-    const uint32_t p = hi ? __builtin_amdgcn_perm(0x64646464u, tamed, 0x04030402u)
-                          : __builtin_amdgcn_perm(0x64646464u, tamed, 0x04010400u);
-    return __builtin_bit_cast(v2hf, p) - static_cast<_Float16>(1152.0f);
+  // (c + kMore) / kUnit: a byte c + 128 alone is the subnormal number (c + 128) 2^-24.  For
+  // products whose other side's sum is known.
+  static constexpr float kUnit = 0x1p24f, kMore = 128.0f;
+  static __device__ __forceinline__ v2hf biased(uint32_t tamed, bool hi) {
+    return __builtin_bit_cast(v2hf, hi ? __builtin_amdgcn_perm(0u, tamed, 0x0c030c02u)
+                                       : __builtin_amdgcn_perm(0u, tamed, 0x0c010c00u));
+  }
+  // c 2^-kShift from (c + 128) 2^-24, exactly
+  static constexpr int kShift = 9;
+  static __device__ __forceinline__ v2hf centred(v2hf b) {
+    const v2hf up = {static_cast<_Float16>(32768.0f), static_cast<_Float16>(32768.0f)};
+    const v2hf less = {static_cast<_Float16>(-0.25f), static_cast<_Float16>(-0.25f)};
+    return __builtin_elementwise_fma(b, up, less);
   }
   static __device__ __forceinline__ uint32_t finite(uint32_t w) { return w; }
+  static __device__ __forceinline__ bool odd(uint32_t, uint32_t) { return false; }
 };
 template <>
 struct Widen<true> {  // e4m3
-  static constexpr int kShift = 0;
   static __device__ __forceinline__ uint32_t tame(uint32_t w) { return w; }
-  static __device__ __forceinline__ v2hf pair(uint32_t w, bool hi) {
+  static constexpr float kUnit = 1.0f, kMore = 0.0f;
+  static __device__ __forceinline__ v2hf biased(uint32_t w, bool hi) {
     return hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w), 1.0f, true)
               : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w), 1.0f, false);
   }
+  static constexpr int kShift = 0;
+  static __device__ __forceinline__ v2hf centred(v2hf b) { return b; }
   // Codes that hold no number (0x7f, 0xff) as 0: a weight of 0 would not hide them.
   static __device__ __forceinline__ uint32_t finite(uint32_t w) {
     const uint32_t none = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
     return w & ~((none >> 7) * 255u);
   }
+  // Whether a lane of the wavefront has one.
+  static __device__ __forceinline__ bool odd(uint32_t w0, uint32_t w1) {
+    const uint32_t a = (w0 & 0x7f7f7f7fu) + 0x01010101u, b = (w1 & 0x7f7f7f7fu) + 0x01010101u;
+    return __ballot(((a | b) & 0x80808080u) != 0) != 0;
+  }
 };
 
-// Eight codes as an operand.
-template <bool E4M3>
+// Eight codes as an operand, (c + kMore) / kUnit or, centred, c 2^-kShift.
+template <bool E4M3, bool CENTRED>
 __device__ __forceinline__ v8hf widen8(uint32_t w0, uint32_t w1) {
   using W = Widen<E4M3>;
-  const uint32_t t0 = W::tame(w0), t1 = W::tame(w1);
   struct Four {
     v2hf p[4];
   };
-  return __builtin_bit_cast(
-      v8hf, Four{{W::pair(t0, false), W::pair(t0, true), W::pair(t1, false), W::pair(t1, true)}});
+  Four f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f.p[i] = W::biased(W::tame(i < 2 ? w0 : w1), i & 1);
+    if constexpr (CENTRED) f.p[i] = W::centred(f.p[i]);
+  }
+  return __builtin_bit_cast(v8hf, f);
 }
 
 // Column x of four words, byte by byte, as one word of four: column(x, w0 .. w3).
@@ -81,18 +100,15 @@ __device__ __forceinline__ v8hf column8(int x, const uint32_t* w) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t c = byte_column(x, w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-      f.p[2 * i] = Widen<true>::pair(c, false);
-      f.p[2 * i + 1] = Widen<true>::pair(c, true);
+      f.p[2 * i] = Widen<true>::biased(c, false);
+      f.p[2 * i + 1] = Widen<true>::biased(c, true);
     }
   } else {
-    // a byte c + 128 alone is the subnormal (c + 128) 2^-24
     const uint32_t s = 0x0c040c00u + 0x00010001u * static_cast<uint32_t>(x);
-    const v2hf up = {static_cast<_Float16>(32768.0f), static_cast<_Float16>(32768.0f)};
-    const v2hf less = {static_cast<_Float16>(-0.25f), static_cast<_Float16>(-0.25f)};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      f.p[i] = __builtin_elementwise_fma(
-          __builtin_bit_cast(v2hf, __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], s)), up, less);
+      f.p[i] = Widen<false>::centred(
+          __builtin_bit_cast(v2hf, __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], s)));
   }
   return __builtin_bit_cast(v8hf, f);
 }
@@ -109,6 +125,16 @@ __device__ __forceinline__ v8hf scaled8(typename Half<T>::op8 v, float up) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = static_cast<_Float16>(static_cast<float>(v[i]) * up);
   return o;
+}
+// The sum of a lane's share of a row.
+template <int N>
+__device__ __forceinline__ float sum_of(const v8hf (&q)[N]) {
+  float sum = 0.0f;
+#pragma unroll
+  for (int st = 0; st < N; ++st)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += static_cast<float>(q[st][i]);
+  return sum;
 }
 // k with 2^14 <= most 2^k < 2^15, at most 100 (rows of zeros, and of no numbers: 0).
 __device__ __forceinline__ int row_shift(float most) {

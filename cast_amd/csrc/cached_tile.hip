@@ -10,10 +10,13 @@ template <int D>
 struct CodeTile : RowTile<_Float16, D> {
   using R = RowTile<_Float16, D>;
   using O = Half<_Float16>;
-  float c_row;  // logit of q . c, times the key's scale, in log2 units
+  // The products are q . (c + 128) 2^-24 for int8 codes: a logit in log2 units is the product
+  // times c_row times the key's scale, and c_less times it.
+  float c_row, c_less;
   Unit2 unit;   // of the accumulators
-  // what a tile's scales give: logits, log2 of a weight's factor and its reciprocal
-  float c, log_f, inv_f;
+  // what a tile's scales give: a product's factor, what is added to it (c_less times the key's
+  // scale and log2 of the weights' factor f), 1 / f
+  float c, more, inv_f;
 
   // (a branch of its own: scales change where a block ends)
   template <bool WHOLE>
@@ -32,7 +35,7 @@ struct CodeTile : RowTile<_Float16, D> {
     const float vs = N == 1 ? sc.v[0] : hf ? sc.v[N - 1] : sc.v[0];
     c = fmaxf(c_row * ks, 0x1p-126f);  // (0 * -inf is NaN)
     const float f = fmaxf(vs * unit.inv, 0x1p-60f);
-    log_f = __builtin_amdgcn_logf(f);
+    more = fmaf(c_less, ks, __builtin_amdgcn_logf(f));
     inv_f = __builtin_amdgcn_rcpf(f);
   }
 
@@ -42,7 +45,7 @@ struct CodeTile : RowTile<_Float16, D> {
                                         Bits&& bits, Pre&& prefetch) {
     // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
     v4i kraw[R::QSTEPS];
-    constexpr int HELD = 4;
+    constexpr int HELD = 8;
     int far = 64;
     asm volatile("" : "+s"(far));
 #pragma unroll
@@ -70,7 +73,7 @@ struct CodeTile : RowTile<_Float16, D> {
     }
     v8hf p_op[2];
     auto exps = [&]() __attribute__((always_inline)) -> float {
-      const float bias = log_f + (this->m_run == -INFINITY ? 0.0f : -this->m_run);
+      const float bias = more + (this->m_run == -INFINITY ? 0.0f : -this->m_run);
       float lsum[4];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -88,7 +91,7 @@ struct CodeTile : RowTile<_Float16, D> {
       float rmax = -INFINITY;
 #pragma unroll
       for (int r = 0; r < 16; ++r) rmax = fmaxf(rmax, rv[r]);
-      rmax = pair_max(rmax * c);
+      rmax = pair_max(fmaf(rmax, c, more + __builtin_amdgcn_logf(inv_f)));
       const float m_blk = rmax == -INFINITY ? -INFINITY : rmax - O::kShift;
       if (__ballot(m_blk > this->m_run + kTau) != 0) {
         const float m_new = fmaxf(this->m_run, m_blk);
@@ -188,7 +191,9 @@ cached_tile_kernel(WindowArgs a) {
     const float up = power_of(k);
 #pragma unroll
     for (int st = 0; st < R::QSTEPS; ++st) t.q_op[st] = scaled8<T>(raw[st], up);
-    t.c_row = a.scale_log2 * power_of(-k);
+    const float unit = a.scale_log2 * power_of(-k);
+    t.c_row = unit * Widen<E4M3>::kUnit;
+    t.c_less = E4M3 ? 0.0f : -Widen<E4M3>::kMore * unit * pair_sum(sum_of<R::QSTEPS>(t.q_op));
   }
 
   CodeStream<WHOLE, WindowArgs> codes(a, p);
@@ -218,11 +223,14 @@ cached_tile_kernel(WindowArgs a) {
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) {
       const v2u k = *reinterpret_cast<const v2u*>(src + raw + 512 * i);
-      const v2u v = *reinterpret_cast<const v2u*>(src + raw + 1024 + 512 * i);
+      v2u v = *reinterpret_cast<const v2u*>(src + raw + 1024 + 512 * i);
+      if (Widen<E4M3>::odd(v[0], v[1]))
+#pragma unroll
+        for (int j = 0; j < 2; ++j) v[j] = Widen<E4M3>::finite(v[j]);
       *reinterpret_cast<v8hf*>(dst + (i == 0 ? k_at : (k_at ^ 64) + 4 * R::KROW)) =
-          widen8<E4M3>(k[0], k[1]);
+          widen8<E4M3, false>(k[0], k[1]);
       *reinterpret_cast<v8hf*>(dst + v_at + i * 4 * R::KROW) =
-          widen8<E4M3>(Widen<E4M3>::finite(v[0]), Widen<E4M3>::finite(v[1]));
+          widen8<E4M3, true>(v[0], v[1]);
     }
   };
 
@@ -253,10 +261,6 @@ cached_tile_kernel(WindowArgs a) {
     char* const fill = J == 0 ? s_1 : s_0;
     char* const raw_slot = J == 0 ? r_1 : r_0;
     asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    widen(raw_slot, fill);
-    __builtin_amdgcn_sched_barrier(0);
-    stage(raw_slot);
-    __builtin_amdgcn_sched_barrier(0);
     const int key = e0.key, there = e0.there;
     const Scales<WHOLE> ns = sc;
     const bool changed = __float_as_uint(ns.k[0]) != had_k || __float_as_uint(ns.v[0]) != had_v;
@@ -273,6 +277,9 @@ cached_tile_kernel(WindowArgs a) {
           return key < 0 ? 0u : seen_bits(late_args(), p, p.row0 + lr, hf, key, there);
         },
         [&]() __attribute__((always_inline)) {
+          widen(raw_slot, fill);
+          __builtin_amdgcn_sched_barrier(0);
+          stage(raw_slot);
           sc = scales_of(e0, ks, vs);
           codes.next();
         });
@@ -291,7 +298,8 @@ cached_tile_kernel(WindowArgs a) {
 #pragma unroll
   for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) t.o_acc[dt][r] = l == 0.0f ? 0.0f : t.o_acc[dt][r] * inv;
+    for (int r = 0; r < 16; ++r)
+      t.o_acc[dt][r] = l == 0.0f ? 0.0f : t.o_acc[dt][r] * (1 << Widen<E4M3>::kShift) * inv;
   const Row my = row_of(e, p, p.row0 + lr);
   if (!my.live) return;
   if (p.shares > 1) {

@@ -47,7 +47,7 @@ cached_unit_kernel(WindowArgs a) {
   // The lane's row of the queries: step st of the products takes the channels of 8 bytes st & 1
   // of load st / 2.
   v8hf q_op[2 * KL];
-  float c_row;
+  float c_row, less;  // of the products q . (c + kMore) / kUnit: a factor, and what is added
   {
     const Row my = row_of(a, p, lr);
     const T* const row = static_cast<const T*>(a.q) + p.b * a.sq[0] +
@@ -64,7 +64,9 @@ cached_unit_kernel(WindowArgs a) {
     const float up = power_of(k);
 #pragma unroll
     for (int st = 0; st < 2 * KL; ++st) q_op[st] = scaled8<T>(raw[st], up);
-    c_row = a.scale_log2 * power_of(-k);
+    const float unit = a.scale_log2 * power_of(-k);
+    c_row = unit * Widen<E4M3>::kUnit;
+    less = E4M3 ? 0.0f : -Widen<E4M3>::kMore / Widen<E4M3>::kUnit * pair_sum(sum_of<2 * KL>(q_op));
   }
 
   // A step's codes: the lane's key of the tile is lr (16 bytes at hf * 16 of every 32), its
@@ -137,7 +139,7 @@ cached_unit_kernel(WindowArgs a) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         s_acc = Half<_Float16>::mfma(
-            widen8<E4M3>(static_cast<uint32_t>(t.k[i][2 * j]),
+            widen8<E4M3, false>(static_cast<uint32_t>(t.k[i][2 * j]),
                          static_cast<uint32_t>(t.k[i][2 * j + 1])),
             q_op[2 * i + j], s_acc);
     }
@@ -152,7 +154,7 @@ cached_unit_kernel(WindowArgs a) {
     const float c0 = c_row * ns.k[0], c1 = c_row * ns.k[N - 1];
     float rv[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) rv[r] = s_acc[r] * (r < 8 ? c0 : c1);
+    for (int r = 0; r < 16; ++r) rv[r] = (s_acc[r] + less) * (r < 8 ? c0 : c1);
     const bool inside = there == 3 && key + kTileKeys <= first.hi &&
                         (key >= last.lo || key + kTileKeys <= a.sinks);
     if (!inside) {
