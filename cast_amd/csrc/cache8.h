@@ -5,6 +5,8 @@
 // A block's tokens follow each other in one page; page j / page of a request's table holds
 // key j in row j % page, and that row's block is row / block.
 #pragma once
+#include <type_traits>
+
 #include "rcsa_common.h"
 
 namespace rcsa {
@@ -20,17 +22,18 @@ template <>
 struct Code8<false> {
   // The scale of a block whose largest value is `most`: most / 127, rounded to fp32.
   static __device__ __forceinline__ float scale_for(float most) { return most / 127.0f; }
-  // The codes nearest x / s, ties to even.  x * inv is off by 2^-23 of it, so that the whole
-  // number next to it is the quotient's or one beside; the remainder x - q s is exact (fp32
-  // values on a grid no finer than half of s's last place, below 2^24 steps of it), so that
-  // comparing it with s / 2 decides as the real quotient would.  Infinities saturate, NaN
+  // The codes nearest x / s, ties to even.  t = x * inv is off by 2^-22 of it, below 2^-15, so
+  // that the whole number next to t is the quotient's unless t is that near the border of two
+  // codes.  Where a lane has such a t (one value in 2000), the remainder x - q s decides: it
+  // is exact (fp32 values on a grid no finer than half of s's last place, below 2^24 steps of
+  // it).  t + 1.5 2^23 is t rounded, its code in the lowest byte.  Infinities saturate, NaN
   // becomes 0.
   struct To {
-    float s, inv, half;
-    __device__ __forceinline__ To(float scale) : s(scale), inv(1.0f / scale), half(0.5f * scale) {}
-    __device__ __forceinline__ int one(float x) const {
-      float q = __builtin_rintf(x * inv);
-      q = fminf(fmaxf(q, -127.0f), 127.0f);
+    float s, inv;
+    __device__ __forceinline__ explicit To(float scale) : s(scale), inv(1.0f / scale) {}
+    __device__ __forceinline__ int exactly(float x) const {
+      const float half = 0.5f * s;
+      const float q = fminf(fmaxf(__builtin_rintf(x * inv), -127.0f), 127.0f);
       const float r = fmaf(-q, s, x), far = fabsf(r);
       const int c = static_cast<int>(q);
       const bool move = far > half || (far == half && (c & 1));
@@ -38,9 +41,34 @@ struct Code8<false> {
       d = d > 127 ? 127 : (d < -127 ? -127 : d);
       return x == x ? d : 0;
     }
-    __device__ __forceinline__ uint32_t four(const float* x) const {
-      return (one(x[0]) & 255) | (one(x[1]) & 255) << 8 | (one(x[2]) & 255) << 16 |
-             static_cast<uint32_t>(one(x[3])) << 24;
+    // `plain`: no infinity or NaN among the values of the wavefront
+    __device__ __forceinline__ uint2 eight(const float* x, bool plain) const {
+      constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+      float u[8], off = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float t = x[i] * inv;
+        u[i] = t + kMagic;
+        off = fmaxf(off, fabsf(t - (u[i] - kMagic)));
+      }
+      uint2 w;
+      if (!plain || __ballot(off > 0.4999f) != 0) {
+        auto four = [&](const float* y) __attribute__((always_inline)) -> uint32_t {
+          return (exactly(y[0]) & 255) | (exactly(y[1]) & 255) << 8 | (exactly(y[2]) & 255) << 16 |
+                 static_cast<uint32_t>(exactly(y[3])) << 24;
+        };
+        w = make_uint2(four(x), four(x + 4));
+      } else {
+        auto four = [&](const float* y) __attribute__((always_inline)) -> uint32_t {
+          const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y[1]), __float_as_uint(y[0]),
+                                                    0x0c0c0400u);
+          const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(y[3]), __float_as_uint(y[2]),
+                                                    0x0c0c0400u);
+          return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+        };
+        w = make_uint2(four(u), four(u + 4));
+      }
+      return w;
     }
   };
   static __device__ __forceinline__ void values(uint32_t w, float* x) {
@@ -76,17 +104,25 @@ struct Code8<true> {
   struct To {
     float s, inv;
     bool power;
-    __device__ __forceinline__ To(float scale)
+    __device__ __forceinline__ explicit To(float scale)
         : s(scale), inv(1.0f / scale), power((__float_as_uint(scale) & 0x7fffffu) == 0) {}
-    __device__ __forceinline__ float one(float x) const {
-      const float y = power ? x * inv : x / s;
-      const float z = fminf(fmaxf(y, -448.0f), 448.0f);
-      return x == x ? z : 0.0f;
+    static __device__ __forceinline__ uint32_t four(const float* y) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true));
     }
-    __device__ __forceinline__ uint32_t four(const float* x) const {
-      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(one(x[0]), one(x[1]), 0, false);
-      return static_cast<uint32_t>(
-          __builtin_amdgcn_cvt_pk_fp8_f32(one(x[2]), one(x[3]), lo, true));
+    __device__ __forceinline__ uint2 eight(const float* x, bool plain) const {
+      float y[8];
+      if (plain && power) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[i] * inv;  // (at most 448)
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float z = power ? x[i] * inv : x[i] / s;
+          y[i] = x[i] == x[i] ? fminf(fmaxf(z, -448.0f), 448.0f) : 0.0f;
+        }
+      }
+      return make_uint2(four(y), four(y + 4));
     }
   };
   static __device__ __forceinline__ void values(uint32_t w, float* x) {
@@ -102,15 +138,19 @@ struct Code8<true> {
     const double f = static_cast<double>(s0) / s;  // (a power of two, of scale_for's)
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(x[i] * f);
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true));
+    return To::four(x);
   }
 };
 
-// Eight consecutive values of a tensor of type T as fp32, and back (rounded once).
+// Eight consecutive values of a tensor of type T as fp32, and back (rounded once); their
+// largest size, which infinities and NaN exceed every number with, as bits of the type (fp32's
+// its own).
 template <typename T>
 struct Run8 {
   typedef T V __attribute__((ext_vector_type(8)));
+  static constexpr uint32_t kInfinity =
+      std::is_same<T, __bf16>::value ? 0x7f80u : std::is_same<T, _Float16>::value ? 0x7c00u
+                                                                                  : 0x7f800000u;
   static __device__ __forceinline__ void floats(const V& v, float* x) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(v[i]);
@@ -120,6 +160,40 @@ struct Run8 {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = static_cast<T>(x[i]);
     return v;
+  }
+  // Of 16-bit types two running maxima in a word.
+  static __device__ __forceinline__ void most(const V& v, uint32_t& m) {
+    if constexpr (sizeof(T) == 2) {
+      typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+      struct Words {
+        uint32_t w[4];
+      };
+      const Words w = __builtin_bit_cast(Words, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v2us a = __builtin_bit_cast(v2us, w.w[i] & 0x7fff7fffu);
+        m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(a, __builtin_bit_cast(v2us, m)));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t a = __float_as_uint(static_cast<float>(v[i])) & 0x7fffffffu;
+        m = a > m ? a : m;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return a > b ? a : b;
+  }
+  // The larger of a word's two (fp32: itself).
+  static __device__ __forceinline__ uint32_t one_of(uint32_t m) {
+    return sizeof(T) == 2 ? larger(m & 0xffffu, m >> 16) : m;
+  }
+  static __device__ __forceinline__ float value(uint32_t bits) {
+    if constexpr (std::is_same<T, __bf16>::value) return __uint_as_float(bits << 16);
+    else if constexpr (std::is_same<T, _Float16>::value)
+      return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(bits)));
+    else return __uint_as_float(bits);
   }
 };
 

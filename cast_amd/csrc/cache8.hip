@@ -34,16 +34,28 @@ __device__ __forceinline__ int64_t first_item(const AppendArgs& a, int b) {
   return divide(o, a.by_block) + 2ll * b;
 }
 
-template <typename T, bool E4M3, bool PACKED, int THREADS>
+__device__ __forceinline__ uint32_t wave_most(uint32_t m) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint32_t other = __shfl_xor(m, o, kWave);
+    m = other > m ? other : m;
+  }
+  return m;
+}
+
+// A workgroup takes a block's keys or values of one head (BOTH: one after the other, for
+// blocks that a wavefront holds twice): one pass over them, the largest first, HELD runs of 8
+// channels a thread in registers, more of them read again.
+template <typename T, bool E4M3, bool PACKED, int THREADS, bool BOTH>
 __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
   using C = Code8<E4M3>;
   using R = Run8<T>;
   typedef typename R::V V;
-  constexpr int HELD = 8;  // runs of a thread that stay in registers
+  constexpr int HELD = BOTH ? 4 : 8, KV = BOTH ? 2 : 1;
   const int tid = threadIdx.x, lane = tid & 63;
   const int id = static_cast<int>(blockIdx.x);
   const int at = divide(id, a.by_heads), head = id - at * a.H;
-  const int kv = at & 1, all = at >> 1;
+  const int kv0 = BOTH ? 0 : at & 1, all = BOTH ? at : at >> 1;
   int b, item, row0, count;
   if constexpr (PACKED) {
     b = request_at(a.B, all, lane, [&](int i) __attribute__((always_inline)) {
@@ -77,77 +89,103 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
   const int to = hi - first < a.block ? static_cast<int>(hi - first) : a.block;
   const int col = divide(n, a.by_page_blocks), in_page = n - col * a.page_blocks;
   const int page = a.table[b * a.table_stride + col];
-  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.n_pages)) return;
 
-  const T* const x = static_cast<const T*>(a.x[kv]) + (PACKED ? 0 : b * a.sx[kv][0]) +
-                     head * a.sx[kv][2] + (row0 + first + from - start) * a.sx[kv][1];
-  char* const codes = a.codes[kv] + page * a.sc[kv][0] + head * a.sc[kv][2] +
-                      static_cast<int64_t>(in_page) * a.block * a.sc[kv][1];
-  float* const scale = a.scales[kv] + page * a.ss[kv][0] + in_page * a.ss[kv][1] +
-                       head * a.ss[kv][2];
-  float s0 = 0.0f;
-  if (from > 0) {
-    s0 = *scale;
-    s0 = s0 > 0.0f && s0 < INFINITY ? s0 : 0.0f;
-  }
-
-  const int64_t xs = a.sx[kv][1], cs = a.sc[kv][1];
+  // (the new values do not wait for the table)
   const int runs = (to - from) * a.runs;
-  auto load = [&](int i) __attribute__((always_inline)) -> V {
+  auto source = [&](int kv) __attribute__((always_inline)) -> const T* {
+    return static_cast<const T*>(a.x[kv]) + (PACKED ? 0 : b * a.sx[kv][0]) + head * a.sx[kv][2] +
+           (row0 + first + from - start) * a.sx[kv][1];
+  };
+  auto load = [&](int kv, const T* x, int i) __attribute__((always_inline)) -> V {
     const int row = divide(i, a.by_runs);
-    return *reinterpret_cast<const V*>(x + row * xs + (i - row * a.runs) * 8);
+    return *reinterpret_cast<const V*>(x + row * a.sx[kv][1] + (i - row * a.runs) * 8);
   };
-  float most = 0.0f;
-  auto look = [&](const V& v) __attribute__((always_inline)) {
-    float f[8];
-    R::floats(v, f);
+  V held[KV][HELD];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float m = fabsf(f[e]);
-      most = fmaxf(most, m < INFINITY ? m : 0.0f);
-    }
-  };
-  V held[HELD];
+  for (int j = 0; j < KV; ++j) {
+    const int kv = BOTH ? j : kv0;
+    const T* const x = source(kv);
 #pragma unroll
-  for (int k = 0; k < HELD; ++k)
-    if (tid + k * THREADS < runs) held[k] = load(tid + k * THREADS);
-#pragma unroll
-  for (int k = 0; k < HELD; ++k)
-    if (tid + k * THREADS < runs) look(held[k]);
-  for (int i = tid + HELD * THREADS; i < runs; i += THREADS) look(load(i));
-  most = wave_max(most);
-  if constexpr (THREADS > kWave) {
-    __shared__ float s_most[THREADS / kWave];
-    if (lane == 0) s_most[tid / kWave] = most;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / kWave; ++w) most = fmaxf(most, s_most[w]);
+    for (int k = 0; k < HELD; ++k)
+      if (tid + k * THREADS < runs) held[j][k] = load(kv, x, tid + k * THREADS);
   }
-  const float own = C::scale_for(most);
-  const float s = fmaxf(fmaxf(s0, own), kLeastScale);
-
-  const typename C::To to_code(s);
-  auto store = [&](int i, const V& v) __attribute__((always_inline)) {
-    const int row = divide(i, a.by_runs);
-    float f[8];
-    R::floats(v, f);
-    *reinterpret_cast<uint2*>(codes + (from + row) * cs + (i - row * a.runs) * 8) =
-        make_uint2(to_code.four(f), to_code.four(f + 4));
-  };
+  if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.n_pages)) return;
 #pragma unroll
-  for (int k = 0; k < HELD; ++k)
-    if (tid + k * THREADS < runs) store(tid + k * THREADS, held[k]);
-  for (int i = tid + HELD * THREADS; i < runs; i += THREADS) store(i, load(i));
-  if (s != s0) {  // (a block's first scale, or a larger one)
-    for (int i = tid; i < from * a.runs; i += THREADS) {
-      const int row = divide(i, a.by_runs);
-      uint2* const p = reinterpret_cast<uint2*>(codes + row * cs + (i - row * a.runs) * 8);
-      const uint2 w = *p;
-      *p = make_uint2(C::again(w.x, s0, s), C::again(w.y, s0, s));
+  for (int j = 0; j < KV; ++j) {
+    const int kv = BOTH ? j : kv0;
+    const T* const x = source(kv);
+    char* const codes = a.codes[kv] + page * a.sc[kv][0] + head * a.sc[kv][2] +
+                        static_cast<int64_t>(in_page) * a.block * a.sc[kv][1];
+    float* const scale = a.scales[kv] + page * a.ss[kv][0] + in_page * a.ss[kv][1] +
+                         head * a.ss[kv][2];
+    float s0 = 0.0f;
+    if (from > 0) {
+      s0 = *scale;
+      s0 = s0 > 0.0f && s0 < INFINITY ? s0 : 0.0f;
     }
-    // (every thread has read the block's old scale before the barrier, or, of one wavefront,
-    // before this store)
-    if (tid == 0) *scale = s;
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (tid + k * THREADS < runs) R::most(held[j][k], m);
+    for (int i = tid + HELD * THREADS; i < runs; i += THREADS) R::most(load(kv, x, i), m);
+    __shared__ uint32_t s_most[2][THREADS / kWave];
+    auto block_most = [&](uint32_t mine, int nth) __attribute__((always_inline)) -> uint32_t {
+      uint32_t r = wave_most(mine);
+      if constexpr (THREADS > kWave) {
+        if (lane == 0) s_most[nth][tid / kWave] = r;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / kWave; ++w) r = R::larger(r, s_most[nth][w]);
+      }
+      return r;
+    };
+    uint32_t bits = block_most(R::one_of(m), 0);
+    const bool plain = bits < R::kInfinity;
+    if (!plain) {  // the largest number beside infinities and NaN
+      uint32_t f = 0;
+      auto look = [&](const V& v) __attribute__((always_inline)) {
+        float x8[8];
+        R::floats(v, x8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float size = fabsf(x8[e]);
+          const uint32_t u = size < INFINITY ? __float_as_uint(size) : 0u;
+          f = u > f ? u : f;
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < HELD; ++k)
+        if (tid + k * THREADS < runs) look(held[j][k]);
+      for (int i = tid + HELD * THREADS; i < runs; i += THREADS) look(load(kv, x, i));
+      bits = block_most(f, 1);
+    }
+    const float own = C::scale_for(plain ? R::value(bits) : __uint_as_float(bits));
+    const float s = fmaxf(fmaxf(s0, own), kLeastScale);
+
+    const typename C::To to_code(s);
+    auto store = [&](int i, const V& v) __attribute__((always_inline)) {
+      const int row = divide(i, a.by_runs);
+      float f[8];
+      R::floats(v, f);
+      *reinterpret_cast<uint2*>(codes + (from + row) * a.sc[kv][1] + (i - row * a.runs) * 8) =
+          to_code.eight(f, plain);
+    };
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (tid + k * THREADS < runs) store(tid + k * THREADS, held[j][k]);
+    for (int i = tid + HELD * THREADS; i < runs; i += THREADS) store(i, load(kv, x, i));
+    if (s != s0) {  // (a block's first scale, or a larger one)
+      for (int i = tid; i < from * a.runs; i += THREADS) {
+        const int row = divide(i, a.by_runs);
+        uint2* const p =
+            reinterpret_cast<uint2*>(codes + row * a.sc[kv][1] + (i - row * a.runs) * 8);
+        const uint2 w = *p;
+        *p = make_uint2(C::again(w.x, s0, s), C::again(w.y, s0, s));
+      }
+      // (every thread has read the block's old scale before the barrier, or, of one
+      // wavefront, before this store)
+      if (tid == 0) *scale = s;
+    }
   }
 }
 
@@ -161,57 +199,101 @@ struct ReadArgs {
   const int32_t *starts, *lengths, *table;
   int64_t table_stride;
   int B, L, H, max_pages, n_pages, page, block, runs;  // runs: of 8 channels in a head
-  Divisor by_heads, by_runs, by_L, by_page, by_block;
-  int64_t total;            // runs of the keys
+  int tokens, groups;       // tokens of a workgroup, workgroups of a request
+  int columns, side;        // runs of a token that a workgroup takes, tokens side by side
+  Divisor by_runs, by_columns, by_page, by_block, by_groups;
 };
 
+constexpr int kReadTokens = 64, kReadThreads = 512;  // of a workgroup, at most
+
+// A workgroup takes some tokens of a request, keys or values: its first threads find where the
+// tokens are; then a thread goes through every `side`-th of them in one run of 8 channels, U
+// at a time, so that a run's place is found once and its scale read where a block begins.
+// The values pass the caches.
 template <typename T, bool E4M3>
-__global__ void __launch_bounds__(256) read_kernel(ReadArgs a) {
+__global__ void __launch_bounds__(kReadThreads) read_kernel(ReadArgs a) {
   using C = Code8<E4M3>;
   using R = Run8<T>;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= a.total) return;
-  const int kv = static_cast<int>(blockIdx.y);
-  const int row = static_cast<int>(i / (a.runs * a.H));       // b, token
-  const int in_row = static_cast<int>(i - static_cast<int64_t>(row) * a.runs * a.H);
-  const int head = divide(in_row, a.by_runs), run = in_row - head * a.runs;
-  const int b = divide(row, a.by_L), t = row - b * a.L;
+  typedef unsigned int v2i __attribute__((ext_vector_type(2)));
+  constexpr int U = 4;
+  __shared__ int64_t s_codes[kReadTokens], s_scale[kReadTokens];  // codes -1: no page
+  const int tid = threadIdx.x, kv = static_cast<int>(blockIdx.y);
+  const int b = divide(static_cast<int>(blockIdx.x), a.by_groups);
+  const int t0 = (static_cast<int>(blockIdx.x) - b * a.groups) * a.tokens;
+  // keys first + t, t from lo to hi - 1, are wanted and there may be some
+  const int64_t first = a.starts == nullptr ? 0 : a.starts[b];
   const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page;
-  const int64_t start = a.starts == nullptr ? 0 : a.starts[b];
-  const int64_t j = start + t, len = a.lengths[b];
-  if (j < 0 || j >= len || j >= cap) return;
-  const int col = divide(static_cast<int>(j), a.by_page), slot = static_cast<int>(j) - col * a.page;
-  const int page = a.table[b * a.table_stride + col];
-  float f[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) f[e] = 0.0f;
-  if (static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages)) {
-    const uint2 w = *reinterpret_cast<const uint2*>(a.codes[kv] + page * a.sc[kv][0] +
-                                                    slot * a.sc[kv][1] + head * a.sc[kv][2] +
-                                                    run * 8);
-    const float s = a.scales[kv][page * a.ss[kv][0] + divide(slot, a.by_block) * a.ss[kv][1] +
-                                 head * a.ss[kv][2]];
-    C::values(w.x, f);
-    C::values(w.y, f + 4);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] *= s;
+  const int64_t len = a.lengths[b] < cap ? a.lengths[b] : cap;
+  const int64_t end = len - first < a.L ? len - first : a.L;
+  const int64_t from = -first > t0 ? -first : t0;
+  const int64_t to = end < t0 + a.tokens ? end : t0 + a.tokens;
+  if (from >= to) return;
+  const int lo = static_cast<int>(from), hi = static_cast<int>(to);
+  if (tid < hi - lo) {
+    const int j = static_cast<int>(first + lo + tid);
+    const int col = divide(j, a.by_page), slot = j - col * a.page;
+    const int page = a.table[b * a.table_stride + col];
+    const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+    s_codes[tid] = there ? page * a.sc[kv][0] + slot * a.sc[kv][1] : -1;
+    s_scale[tid] = page * a.ss[kv][0] + divide(slot, a.by_block) * a.ss[kv][1];
   }
-  *reinterpret_cast<typename R::V*>(static_cast<T*>(a.out[kv]) + b * a.so[kv][0] +
-                                    t * a.so[kv][1] + head * a.so[kv][2] + run * 8) = R::of(f);
+  __syncthreads();
+  const int beside = divide(tid, a.by_columns);
+  const int c = static_cast<int>(blockIdx.z) * a.columns + tid - beside * a.columns;
+  if (beside >= a.side || c >= a.runs * a.H) return;
+  const int head = divide(c, a.by_runs), run = c - head * a.runs;
+  const char* const codes = a.codes[kv] + head * a.sc[kv][2] + run * 8;
+  const float* const scales = a.scales[kv] + head * a.ss[kv][2];
+  T* const out = static_cast<T*>(a.out[kv]) + b * a.so[kv][0] + lo * a.so[kv][1] +
+                 head * a.so[kv][2] + run * 8;
+  const int n = hi - lo;
+  int64_t had = -1;
+  float s = 0.0f;
+  for (int t = beside; t < n; t += U * a.side) {
+    v2i w[U];
+    int64_t at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int tu = t + u * a.side;
+      at[u] = -1;
+      if (tu < n) at[u] = s_codes[tu];
+      w[u] = v2i{0, 0};
+      if (at[u] >= 0)
+        w[u] = *reinterpret_cast<const v2i*>(codes + at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int tu = t + u * a.side;
+      if (tu >= n) break;
+      if (at[u] >= 0 && s_scale[tu] != had) {
+        had = s_scale[tu];
+        s = scales[had];
+      }
+      float f[8];
+      C::values(w[u][0], f);
+      C::values(w[u][1], f + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = at[u] >= 0 ? f[e] * s : 0.0f;
+      __builtin_nontemporal_store(
+          R::of(f), reinterpret_cast<typename R::V*>(out + tu * a.so[kv][1]));
+    }
+  }
 }
 
 constexpr int64_t kMaxThreads8 = 1ll << 32;  // a grid's dimension holds fewer
 
 template <typename T, bool E4M3, bool PACKED>
 static int launch_append(AppendArgs& a, hipStream_t s) {
-  const int64_t wgs = (PACKED ? a.items : a.items * a.B) * 2 * a.H;
   const int64_t runs = static_cast<int64_t>(a.block) * a.runs;
+  const bool both = runs <= 256;
+  const int64_t wgs = (PACKED ? a.items : a.items * a.B) * (both ? 1 : 2) * a.H;
   const int threads = runs <= 512 ? 64 : runs <= 2048 ? 256 : 1024;
   if (wgs >= (1ll << 31) || wgs * threads >= kMaxThreads8) return RCSA_ERR_SHAPE;
-  const dim3 grid(static_cast<unsigned>(wgs));
-  if (threads == 64) append_kernel<T, E4M3, PACKED, 64><<<grid, dim3(64), 0, s>>>(a);
-  else if (threads == 256) append_kernel<T, E4M3, PACKED, 256><<<grid, dim3(256), 0, s>>>(a);
-  else append_kernel<T, E4M3, PACKED, 1024><<<grid, dim3(1024), 0, s>>>(a);
+  const dim3 grid(static_cast<unsigned>(wgs)), block(static_cast<unsigned>(threads));
+  if (both) append_kernel<T, E4M3, PACKED, 64, true><<<grid, block, 0, s>>>(a);
+  else if (threads == 64) append_kernel<T, E4M3, PACKED, 64, false><<<grid, block, 0, s>>>(a);
+  else if (threads == 256) append_kernel<T, E4M3, PACKED, 256, false><<<grid, block, 0, s>>>(a);
+  else append_kernel<T, E4M3, PACKED, 1024, false><<<grid, block, 0, s>>>(a);
   return launch_status();
 }
 
@@ -224,11 +306,30 @@ static int append_type(AppendArgs& a, bool e4m3, hipStream_t s) {
 
 template <typename T>
 static int read_type(ReadArgs& a, bool e4m3, hipStream_t s) {
-  const int64_t wgs = (a.total + 255) / 256;
-  if (wgs * 256 >= kMaxThreads8) return RCSA_ERR_SHAPE;
-  const dim3 grid(static_cast<unsigned>(wgs), 2);
-  if (e4m3) read_kernel<T, true><<<grid, dim3(256), 0, s>>>(a);
-  else read_kernel<T, false><<<grid, dim3(256), 0, s>>>(a);
+  // a token's runs on whole wavefronts, tokens side by side where they are few
+  const int64_t per = static_cast<int64_t>(a.runs) * a.H;
+  const int64_t passes = (per + kReadThreads - 1) / kReadThreads;
+  const int64_t columns = (per + passes - 1) / passes;
+  const int64_t side = columns >= 256 ? 1 : (256 / columns < kReadTokens ? 256 / columns
+                                                                         : kReadTokens);
+  const int64_t threads = (columns * side + kWave - 1) / kWave * kWave;
+  // eight tokens a thread, fewer where that leaves compute units without a workgroup
+  int64_t nt = side * 8 < kReadTokens ? side * 8 : kReadTokens;
+  while (nt > side && static_cast<int64_t>(a.B) * ((a.L + nt - 1) / nt) * passes * 2 < 1024)
+    nt = (nt / 2 + side - 1) / side * side;
+  nt = nt < threads ? nt : threads;
+  a.columns = static_cast<int>(columns);
+  a.side = static_cast<int>(side);
+  a.tokens = static_cast<int>(nt);
+  a.groups = static_cast<int>((a.L + nt - 1) / nt);
+  a.by_groups = divisor(static_cast<uint32_t>(a.groups));
+  a.by_columns = divisor(static_cast<uint32_t>(columns));
+  const int64_t wgs = static_cast<int64_t>(a.groups) * a.B;
+  if (wgs * threads >= kMaxThreads8) return RCSA_ERR_SHAPE;
+  const dim3 grid(static_cast<unsigned>(wgs), 2, static_cast<unsigned>(passes));
+  const dim3 block(static_cast<unsigned>(threads));
+  if (e4m3) read_kernel<T, true><<<grid, block, 0, s>>>(a);
+  else read_kernel<T, false><<<grid, block, 0, s>>>(a);
   return launch_status();
 }
 
@@ -364,10 +465,8 @@ extern "C" int rcsa_read_cache(const void* k_codes, const void* v_codes, int cod
   a.page = static_cast<int>(page_size);
   a.block = static_cast<int>(block_size);
   a.by_runs = divisor(static_cast<uint32_t>(a.runs));
-  a.by_L = divisor(static_cast<uint32_t>(a.L));
   a.by_page = divisor(static_cast<uint32_t>(a.page));
   a.by_block = divisor(static_cast<uint32_t>(a.block));
-  a.total = dims[0] * dims[1] * dims[2] * a.runs;
   const bool e4m3 = code == RCSA_CODE_E4M3;
   if (dtype == RCSA_BF16) return read_type<__bf16>(a, e4m3, stream);
   if (dtype == RCSA_F16) return read_type<_Float16>(a, e4m3, stream);
