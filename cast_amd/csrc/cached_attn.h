@@ -145,32 +145,42 @@ __device__ __forceinline__ int row_shift(float most) {
 
 // A share's tiles one after the other: where the codes of the present one are, and which scales
 // are its.  All of it is scalar work, which takes its turn with the vector work of a wavefront:
-// WHOLE (pages and blocks of whole tiles) steps along a page by additions and looks into
-// the table where a page ends, a page ahead; otherwise the two halves of 16 keys are looked up
-// each on their own.  Past the share's last tile, and on pages that are not there, the codes
+// pages of whole tiles (WHOLE) are stepped along by additions, the table is looked into where one
+// ends, a page ahead; otherwise the two halves of 16 keys are looked up each on their own.
+// FORM kWhole: blocks of whole tiles, one scale a tile; kHalves: blocks of 16 keys, two; kAny:
+// pages or blocks of neither, the entries of a tile asked for a tile ahead.  Arguments that only
+// some steps need are read again there: scalar registers are short.  Past the share's last tile, and on pages that are not there, the codes
 // stand where some page's are: they are read, and not seen.
-template <bool WHOLE>
+enum CodeForm { kWhole, kHalves, kAny };
+inline CodeForm code_form(const WindowArgs& a) {
+  if (!a.whole_tiles) return kAny;
+  return a.mark % kTileKeys == 0 ? kWhole : a.mark == kTileKeys / 2 ? kHalves : kAny;
+}
+template <CodeForm FORM>
 struct Scales {
-  static constexpr int N = WHOLE ? 1 : 2;
+  static constexpr int N = FORM == kWhole ? 1 : 2;
   float k[N], v[N];
 };
-template <bool WHOLE>
+template <CodeForm FORM>
 struct TileRef {
-  static constexpr int N = WHOLE ? 1 : 2;
+  static constexpr int N = FORM == kWhole ? 1 : 2;
   int key, there;  // the first key, -1: no tile; which halves are there (bits)
   int k[N], v[N];  // where their scales are
 };
-template <bool WHOLE, typename A>
+template <CodeForm FORM, typename A>
 struct CodeStream {
+  static constexpr bool WHOLE = FORM != kAny;
   A& a;
   const int32_t* table;
   int hk, page, mark;
   uint32_t krb, vrb;
   int left, sinks, window;  // tiles left, those of the first keys, the window's first key
-  int col, slot, in_mark, ahead;
+  int slot, in_mark;
+  int col, ahead;            // WHOLE: the column of the page, the entry behind it
+  int key1, ahead1;          // kAny: the next tile's first key, its pages `ahead` and `ahead1`
   const char *kp, *vp;
   int page1, slot1;
-  TileRef<WHOLE> ref;
+  TileRef<FORM> ref;
 
   __device__ __forceinline__ CodeStream(A& args, const Place& p)
       : a(args),
@@ -183,9 +193,37 @@ struct CodeStream {
     left = p.steps;
     sinks = p.tiles.sink_n - p.begin;
     window = p.tiles.win_t0 * kTileKeys;
-    slot1 = page1 = ahead = 0;
-    const int first = sinks > 0 ? p.begin * kTileKeys : window - sinks * kTileKeys;
-    jump(args, left > 0 ? first : -1);
+    slot1 = page1 = in_mark = col = key1 = ahead1 = 0;
+    const int first = left <= 0 ? -1 : sinks > 0 ? p.begin * kTileKeys
+                                                 : window - sinks * kTileKeys;
+    if constexpr (WHOLE) {
+      jump(args, first);
+    } else {
+      look(args, first);
+      pass(args);
+      look(args, after(first));
+    }
+  }
+  // kAny: the first key of the tile behind the present one.
+  __device__ __forceinline__ int after(int key) const {
+    return left <= 1 ? -1 : sinks == 1 ? window : key + kTileKeys;
+  }
+  template <typename X>
+  __device__ __forceinline__ void look(X& x, int key) {
+    key1 = key;
+    const int half = (key < 0 ? 0 : key) >> 4;
+    ahead = entry(x, divide(half, x.by_half_page));
+    ahead1 = entry(x, divide(half + 1, x.by_half_page));
+  }
+  template <typename X>
+  __device__ __forceinline__ void pass(X& x) {
+    ref.key = key1;
+    const int k = key1 < 0 ? 0 : key1;
+    slot = k - divide(k >> 4, x.by_half_page) * page;
+    slot1 = slot + 16 < page ? slot + 16 : 0;
+    page1 = ahead1;
+    on_page(x, 0, ahead, slot);
+    on_page(x, 1, page1, slot1);
   }
   template <typename X>
   __device__ __forceinline__ int entry(X& x, int c) const {
@@ -221,6 +259,10 @@ struct CodeStream {
     if constexpr (WHOLE) {
       ref.there = there ? 3 : 0;
       in_mark = at_slot - nth * mark;
+      if constexpr (FORM == kHalves) {
+        ref.k[1] = ref.k[0] + x.sks[1];
+        ref.v[1] = ref.v[0] + x.svs[1];
+      }
     } else {
       ref.there = h == 0 ? (there ? 1 : 0) : ref.there + (there ? 2 : 0);
     }
@@ -231,22 +273,13 @@ struct CodeStream {
     const int k = key < 0 ? 0 : key;
     col = divide(k >> 4, x.by_half_page);
     slot = k - col * page;
-    const int page0 = entry(x, col);
-    on_page(x, 0, page0, slot);
-    if constexpr (WHOLE) {
-      ahead = entry(x, col + 1);
-    } else {
-      const bool same = slot + 16 < page;
-      slot1 = same ? slot + 16 : 0;
-      page1 = same ? page0 : entry(x, col + 1);
-      on_page(x, 1, page1, slot1);
-    }
+    on_page(x, 0, entry(x, col), slot);
+    ahead = entry(x, col + 1);
   }
   __device__ __forceinline__ void next() {
     --left;
     --sinks;
     if constexpr (WHOLE) {
-      // (arguments that only a new page needs are read again there: scalar registers are short)
       if (left <= 0) {
         ref.key = -1;
         return;
@@ -267,6 +300,15 @@ struct CodeStream {
       }
       kp += kTileKeys * krb;
       vp += kTileKeys * vrb;
+      if constexpr (FORM == kHalves) {
+        const int dk = 2 * (ref.k[1] - ref.k[0]), dv = 2 * (ref.v[1] - ref.v[0]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          ref.k[h] += dk;
+          ref.v[h] += dv;
+        }
+        return;
+      }
       in_mark += kTileKeys;
       if (in_mark >= mark) {
         LateArgs& x = late_args();
@@ -275,7 +317,9 @@ struct CodeStream {
         ref.v[0] += x.svs[1];
       }
     } else {
-      jump(a, left <= 0 ? -1 : sinks == 0 ? window : ref.key + kTileKeys);
+      LateArgs& x = late_args();
+      pass(x);
+      look(x, after(ref.key));
     }
   }
   // The first rows of a half.
@@ -283,7 +327,7 @@ struct CodeStream {
     if constexpr (WHOLE) {
       return {kp + h * 16 * krb, vp + h * 16 * vrb};
     } else {
-      return h == 0 ? At{kp, vp} : row_at(a, ref.there & 2, page1, slot1);
+      return h == 0 ? At{kp, vp} : row_at(late_args(), ref.there & 2, page1, slot1);
     }
   }
 };
@@ -293,12 +337,12 @@ __device__ __forceinline__ float scale_or_0(float s) {
   return u - 1u < 0x7e800000u - 1u ? s : 0.0f;
 }
 // The scales of a tile (ks, vs: of the key head), 0 for a half that is not there.
-template <bool WHOLE>
-__device__ __forceinline__ Scales<WHOLE> scales_of(const TileRef<WHOLE>& t, const float* ks,
+template <CodeForm FORM>
+__device__ __forceinline__ Scales<FORM> scales_of(const TileRef<FORM>& t, const float* ks,
                                                    const float* vs) {
-  Scales<WHOLE> r;
+  Scales<FORM> r;
 #pragma unroll
-  for (int h = 0; h < TileRef<WHOLE>::N; ++h) {
+  for (int h = 0; h < TileRef<FORM>::N; ++h) {
     r.k[h] = scale_or_0(ld_const(ks + t.k[h]));
     r.v[h] = (t.there >> h) & 1 ? scale_or_0(ld_const(vs + t.v[h])) : 0.0f;
   }

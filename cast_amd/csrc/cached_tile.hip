@@ -19,9 +19,9 @@ struct CodeTile : RowTile<_Float16, D> {
   float c, more, inv_f;
 
   // (a branch of its own: scales change where a block ends)
-  template <bool WHOLE>
-  __device__ __forceinline__ void take(const Scales<WHOLE>& sc, int hf) {
-    constexpr int N = Scales<WHOLE>::N;
+  template <CodeForm FORM>
+  __device__ __forceinline__ void take(const Scales<FORM>& sc, int hf) {
+    constexpr int N = Scales<FORM>::N;
 #pragma unroll
     for (int h = 0; h < N; ++h)
       if (__float_as_uint(sc.v[h]) >= unit.bits) {
@@ -39,8 +39,8 @@ struct CodeTile : RowTile<_Float16, D> {
     inv_f = __builtin_amdgcn_rcpf(f);
   }
 
-  template <bool WHOLE, typename Bits, typename Pre>
-  __device__ __forceinline__ void step8(const char* tile, const Scales<WHOLE>& sc, bool changed,
+  template <CodeForm FORM, typename Bits, typename Pre>
+  __device__ __forceinline__ void step8(const char* tile, const Scales<FORM>& sc, bool changed,
                                         int hf, bool inside,
                                         Bits&& bits, Pre&& prefetch) {
     // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
@@ -62,7 +62,7 @@ struct CodeTile : RowTile<_Float16, D> {
     __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
     __builtin_amdgcn_sched_barrier(0);
     prefetch();
-    if (!WHOLE || changed) take<WHOLE>(sc, hf);
+    if (FORM != kWhole || changed) take<FORM>(sc, hf);
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
@@ -129,7 +129,7 @@ struct CodeTile : RowTile<_Float16, D> {
   }
 };
 
-template <typename T, bool E4M3, int D, bool WHOLE>
+template <typename T, bool E4M3, int D, CodeForm FORM>
 __global__ void __launch_bounds__(256)
 __attribute__((amdgpu_waves_per_eu(D == 64 ? 4 : 3, D == 64 ? 4 : 3)))
 cached_tile_kernel(WindowArgs a) {
@@ -196,7 +196,7 @@ cached_tile_kernel(WindowArgs a) {
     t.c_less = E4M3 ? 0.0f : -Widen<E4M3>::kMore * unit * pair_sum(sum_of<R::QSTEPS>(t.q_op));
   }
 
-  CodeStream<WHOLE, WindowArgs> codes(a, p);
+  CodeStream<FORM, WindowArgs> codes(a, p);
   const uint32_t krb = codes.krb, vrb = codes.vrb;
 
   // Copies: a wavefront moves rows 8 w .. 8 w + 7 of a tile, which lie in its half w / 2, as they
@@ -238,7 +238,7 @@ cached_tile_kernel(WindowArgs a) {
   // j - 2 by then); its codes landed in raw slot j % 2, asked for during step j - 3.
   const float* const ks = a.ks + p.hk * a.sks[2];
   const float* const vs = a.vs + p.hk * a.svs[2];
-  typedef TileRef<WHOLE> Ref;
+  typedef TileRef<FORM> Ref;
   Ref e0 = codes.ref, e1, e2;
   stage(r_0);
   __builtin_amdgcn_sched_barrier(0);
@@ -248,7 +248,7 @@ cached_tile_kernel(WindowArgs a) {
   __builtin_amdgcn_sched_barrier(0);
   codes.next();
   e2 = codes.ref;
-  Scales<WHOLE> sc = scales_of(e0, ks, vs);
+  Scales<FORM> sc = scales_of(e0, ks, vs);
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));
   widen(r_0, s_0);
   __builtin_amdgcn_sched_barrier(0);  // (its codes are in registers)
@@ -262,7 +262,7 @@ cached_tile_kernel(WindowArgs a) {
     char* const raw_slot = J == 0 ? r_1 : r_0;
     asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int key = e0.key, there = e0.there;
-    const Scales<WHOLE> ns = sc;
+    const Scales<FORM> ns = sc;
     const bool changed = __float_as_uint(ns.k[0]) != had_k || __float_as_uint(ns.v[0]) != had_v;
     had_k = __float_as_uint(ns.k[0]);
     had_v = __float_as_uint(ns.v[0]);
@@ -271,7 +271,7 @@ cached_tile_kernel(WindowArgs a) {
     e2 = codes.ref;
     const bool inside = key >= 0 && there == 3 && key + kTileKeys <= w_first.hi &&
                         (key >= w_last.lo || key + kTileKeys <= a.sinks);
-    t.template step8<WHOLE>(
+    t.template step8<FORM>(
         tile, ns, changed, hf, inside,
         [&]() __attribute__((always_inline)) {
           return key < 0 ? 0u : seen_bits(late_args(), p, p.row0 + lr, hf, key, there);
@@ -334,10 +334,11 @@ cached_tile_kernel(WindowArgs a) {
 template <typename T, bool E4M3, int D>
 static void launch(WindowArgs& a, dim3 grid, hipStream_t s) {
   const dim3 block(256);
-  if (a.whole_tiles && a.mark % kTileKeys == 0)
-    cached_tile_kernel<T, E4M3, D, true><<<grid, block, 0, s>>>(a);
-  else
-    cached_tile_kernel<T, E4M3, D, false><<<grid, block, 0, s>>>(a);
+  switch (code_form(a)) {
+    case kWhole: cached_tile_kernel<T, E4M3, D, kWhole><<<grid, block, 0, s>>>(a); break;
+    case kHalves: cached_tile_kernel<T, E4M3, D, kHalves><<<grid, block, 0, s>>>(a); break;
+    case kAny: cached_tile_kernel<T, E4M3, D, kAny><<<grid, block, 0, s>>>(a); break;
+  }
 }
 template <typename T>
 static void launch_type(WindowArgs& a, bool e4m3, int64_t D, dim3 grid, hipStream_t s) {

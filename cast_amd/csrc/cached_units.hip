@@ -2,22 +2,27 @@
 // most 32 rows of a key head, dealt as in window_units.hip to workgroups of eight wavefronts
 // or to units of one.
 //
-// Codes go from memory to the matrix operands through registers alone: a lane of S = K Q^T
-// holds a key's channels, which are contiguous; a lane of O^T = V^T P^T holds D / 32
-// neighbouring channels of the 16 keys whose weights it has, one load a key (a load
-// instruction covers two whole rows), turned byte by byte into operands.
+// The codes of values go from memory to the matrix operands through registers alone: a lane of
+// O^T = V^T P^T holds D / 32 neighbouring channels of the 16 keys whose weights it has, one
+// load a key (a load instruction covers two whole rows), turned byte by byte into operands.
+// A lane of S = K Q^T holds a key's channels: loaded as they stand, every load would touch 32
+// lines for a fourth of each (48 ragged requests, 248 us with two tiles in flight so, in more
+// lines than the first cache has), so keys are loaded by whole rows and go through LDS.
 #include "cached_attn.h"
 
 namespace rcsa {
 
-template <typename T, bool E4M3, int D, bool WHOLE, bool GROUP>
+template <typename T, bool E4M3, int D, CodeForm FORM, bool GROUP>
 __global__ void __launch_bounds__(GROUP ? 64 * kGroupWaves : 64)
-__attribute__((amdgpu_waves_per_eu(2, 2)))
+__attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 cached_unit_kernel(WindowArgs a) {
+  constexpr bool WHOLE = FORM != kAny;
   constexpr int NW = GROUP ? kGroupWaves : 1;
   constexpr int KL = D / 32, NDT = D / 32;  // loads of a key's half row; channels of a lane
   typedef typename Half<T>::op8 op8;
-  __shared__ __attribute__((aligned(16))) float s_o[GROUP ? NW : 1][GROUP ? kFewRows * D : 4];
+  // a wavefront's keys; of a workgroup, its partial rows
+  constexpr int TILE = kTileKeys * D, SLOT = GROUP ? kFewRows * D * 4 : TILE;
+  __shared__ __attribute__((aligned(1024))) char s_k[NW][SLOT];
   __shared__ float2 s_ml[NW][kFewRows];
   const int lane = threadIdx.x & 63, hf = lane >> 5, lr = lane & 31;
   const int wave = GROUP ? uniform_int(static_cast<int>(threadIdx.x) >> 6) : 0;
@@ -69,25 +74,38 @@ cached_unit_kernel(WindowArgs a) {
     less = E4M3 ? 0.0f : -Widen<E4M3>::kMore / Widen<E4M3>::kUnit * pair_sum(sum_of<2 * KL>(q_op));
   }
 
-  // A step's codes: the lane's key of the tile is lr (16 bytes at hf * 16 of every 32), its
-  // channels of key 8 (r / 4) + 4 hf + r % 4 are NDT lr and the next ones.
-  struct Tile {
-    v4i k[KL];
-    uint32_t v[16];
+  // A tile's keys: load i takes rows i RPC + lane / CPR, chunks of 16 bytes, which lie in LDS swizzled
+  // by row so that the reads of a chunk of 16 keys meet no bank twice.  The lane's key is lr, its channels
+  // those of chunks 2 i + hf; its channels of the values of key 8 (r / 4) + 4 hf + r % 4 are
+  // NDT lr and the next ones.
+  constexpr int CPR = D / 16, RPC = 64 / CPR, LOADS = kTileKeys / RPC;
+  auto swizzle = [](int row) __attribute__((always_inline)) -> int {
+    return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
   };
-  CodeStream<WHOLE, WindowArgs> codes(a, p);
+  CodeStream<FORM, WindowArgs> codes(a, p);
   const uint32_t krb = codes.krb, vrb = codes.vrb;
-  auto load_k = [&](v4i (&k)[KL]) __attribute__((always_inline)) {
-    const char* at;
-    if constexpr (WHOLE) {
-      at = codes.kp + (lr * krb + hf * 16);
-    } else {
-      const auto h0 = codes.half(0), h1 = codes.half(1);
-      at = (lr < 16 ? h0.k : h1.k) + ((lr & 15) * krb + hf * 16);
-    }
+  const int crow = lane / CPR;
+  const int k_lo = crow * static_cast<int>(krb) + lane % CPR * 16;
+  v4i kr[LOADS];
+  auto load_k = [&]() __attribute__((always_inline)) {
+    const char* from = codes.half(0).k;
 #pragma unroll
-    for (int i = 0; i < KL; ++i) k[i] = *reinterpret_cast<const v4i*>(at + 32 * i);
+    for (int i = 0; i < LOADS; ++i) {
+      if (!WHOLE && i * RPC == 16) from = codes.half(1).k;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(from), 0, (WHOLE ? 32 : 16) * static_cast<int>(krb), kRsrcWord3);
+      kr[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(
+          rs, k_lo, (WHOLE ? i * RPC : i * RPC & 15) * static_cast<int>(krb), 0));
+    }
   };
+  char* const slot = s_k[wave];
+  int k_to[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i)
+    k_to[i] = i * 1024 + crow * D + ((lane % CPR) ^ swizzle(i * RPC + crow)) * 16;
+  int k_at[KL];
+#pragma unroll
+  for (int i = 0; i < KL; ++i) k_at[i] = lr * D + (((2 * i + hf) ^ swizzle(lr)) * 16);
   int v_lo[4];  // rows 4 hf + 0 .. 3; the others are 8, 16 and 24 further
 #pragma unroll
   for (int j = 0; j < 4; ++j) v_lo[j] = static_cast<int>((4 * hf + j) * vrb + NDT * lr);
@@ -113,12 +131,12 @@ cached_unit_kernel(WindowArgs a) {
 
   const float* const ks = a.ks + p.hk * a.sks[2];
   const float* const vs = a.vs + p.hk * a.svs[2];
-  Tile t;
-  load_k(t.k);
-  load_v(t.v);
-  TileRef<WHOLE> cur = codes.ref;
-  Scales<WHOLE> sc = scales_of(cur, ks, vs);
+  uint32_t v[16];
+  TileRef<FORM> cur = codes.ref;
+  load_k();
+  load_v(v);
   codes.next();
+  Scales<FORM> sc = scales_of(cur, ks, vs);
   v16f o_acc[NDT];
 #pragma unroll
   for (int x = 0; x < NDT; ++x)
@@ -128,29 +146,33 @@ cached_unit_kernel(WindowArgs a) {
   Unit2 unit = least_unit();  // of the accumulators
   constexpr int kShift = Half<_Float16>::kShift;
 
+  // `codes` stands at the tile behind the present one: its keys are asked for as soon as the
+  // present ones are in LDS, its values as soon as the present ones are in operands.
   for (int s = 0; s < p.steps; ++s) {
     const int key = cur.key, there = cur.there;
-    const Scales<WHOLE> ns = sc;
+    const Scales<FORM> ns = sc;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) *reinterpret_cast<v4i*>(slot + k_to[i]) = kr[i];
+    const bool more = s + 1 < p.steps;
+    cur = codes.ref;
+    if (more) load_k();
+    v4i kc[KL];
+#pragma unroll
+    for (int i = 0; i < KL; ++i) kc[i] = *reinterpret_cast<const v4i*>(slot + k_at[i]);
     v16f s_acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KL; ++i) {
+    for (int i = 0; i < KL; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         s_acc = Half<_Float16>::mfma(
-            widen8<E4M3, false>(static_cast<uint32_t>(t.k[i][2 * j]),
-                         static_cast<uint32_t>(t.k[i][2 * j + 1])),
+            widen8<E4M3, false>(static_cast<uint32_t>(kc[i][2 * j]),
+                                static_cast<uint32_t>(kc[i][2 * j + 1])),
             q_op[2 * i + j], s_acc);
-    }
-    const bool more = s + 1 < p.steps;
-    if (more) {
-      load_k(t.k);
-      cur = codes.ref;
-      sc = scales_of(cur, ks, vs);
-    }
+    sc = scales_of(cur, ks, vs);
     // logits in log2 units: r < 8 of the first half's keys, the others of the second's
-    constexpr int N = Scales<WHOLE>::N;
+    constexpr int N = Scales<FORM>::N;
     const float c0 = c_row * ns.k[0], c1 = c_row * ns.k[N - 1];
     float rv[16];
 #pragma unroll
@@ -208,9 +230,9 @@ cached_unit_kernel(WindowArgs a) {
     l_run += part;
     uint32_t tamed[16];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) tamed[r] = Widen<E4M3>::tame(Widen<E4M3>::finite(t.v[r]));
+    for (int r = 0; r < 16; ++r) tamed[r] = Widen<E4M3>::tame(Widen<E4M3>::finite(v[r]));
     if (more) {
-      load_v(t.v);
+      load_v(v);
       codes.next();
     }
 #pragma unroll
@@ -232,7 +254,8 @@ cached_unit_kernel(WindowArgs a) {
   const bool live = lr < p.n_rows;
   if (GROUP || p.shares > 1) {
     const int64_t ws_row = GROUP ? 0 : static_cast<int64_t>(blockIdx.x) * e.Lq * e.G;
-    float* const part_o = GROUP ? s_o[wave] : e.ws_o + ws_row * D;
+    float* const part_o =
+        GROUP ? reinterpret_cast<float*>(slot) : e.ws_o + ws_row * D;
     float2* const part_ml = GROUP ? s_ml[wave] : e.ws_ml + ws_row;
     if (live) {
 #pragma unroll
@@ -274,7 +297,7 @@ cached_unit_kernel(WindowArgs a) {
         if (ml.x == -INFINITY) continue;
         const float f = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
         sum += f;
-        const v4f o = *reinterpret_cast<const v4f*>(s_o[s] + row * D + c);
+        const v4f o = *reinterpret_cast<const v4f*>(s_k[s] + (row * D + c) * 4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = join(f, o[i], acc[i]);
       }
@@ -292,22 +315,25 @@ cached_unit_kernel(WindowArgs a) {
   }
 }
 
-template <typename T, bool E4M3, int D, bool WHOLE>
+template <typename T, bool E4M3, int D, CodeForm FORM>
 static int launch(WindowArgs& a, int64_t units, hipStream_t s) {
   if (a.units == 0) {
     const dim3 grid(static_cast<unsigned>(a.B * a.Hk)), block(64 * kGroupWaves);
-    cached_unit_kernel<T, E4M3, D, WHOLE, true><<<grid, block, 0, s>>>(a);
+    cached_unit_kernel<T, E4M3, D, FORM, true><<<grid, block, 0, s>>>(a);
     return launch_status();
   }
-  cached_unit_kernel<T, E4M3, D, WHOLE, false>
+  cached_unit_kernel<T, E4M3, D, FORM, false>
       <<<dim3(static_cast<unsigned>(units)), dim3(64), 0, s>>>(a);
   return launch_unit_merge(a, std::is_same<T, __bf16>::value ? 0 : 1, D, s);
 }
 
 template <typename T, bool E4M3, int D>
 static int launch_form(WindowArgs& a, int64_t units, hipStream_t s) {
-  return a.whole_tiles && a.mark % kTileKeys == 0 ? launch<T, E4M3, D, true>(a, units, s)
-                                                  : launch<T, E4M3, D, false>(a, units, s);
+  switch (code_form(a)) {
+    case kWhole: return launch<T, E4M3, D, kWhole>(a, units, s);
+    case kHalves: return launch<T, E4M3, D, kHalves>(a, units, s);
+    default: return launch<T, E4M3, D, kAny>(a, units, s);
+  }
 }
 template <typename T>
 static int launch_type(WindowArgs& a, bool e4m3, int64_t D, int64_t units, hipStream_t s) {
