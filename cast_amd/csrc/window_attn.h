@@ -60,6 +60,7 @@ struct WindowArgs {
   int n_ranks;
   int units;       // few rows in units: wavefronts of one round
   float per_unit;  // 1 / units
+  int unit_tiles;  // kUnitTiles, of codes kCodeUnitTiles
 };
 
 constexpr int kFewRows = 32;        // rows of a key head that one wavefront takes
@@ -148,17 +149,19 @@ __device__ __forceinline__ int units_of(int tiles, int chunk) {
 // One round of the wavefronts that fit (a.units) where that leaves units of up to
 // kUnitTiles tiles; beyond, units of that size, or more of them than four rounds.  A unit
 // costs about 5 us before its first tile has landed (a tile streams in 0.4 to 1), and the
-// units of a last, short round leave compute units idle.
+// units of a last, short round leave compute units idle.  Tiles of 8-bit codes are half the
+// bytes: units of twice as many (48 ragged requests of up to 32768 keys: of 16 tiles 222 us, 32
+// 213, 64 259).
 // (Sums and products in fp32, at most 14 roundings of 2^-24, that the factor rounds up: a plan,
 // the same for every wavefront.  The tiles of all requests pass 32 bits where tables share
 // pages; a request has at most 2^25, so that a chunk of kMostTiles leaves it whole.)
-constexpr int kLeastTiles = 2, kUnitTiles = 16, kMostTiles = 1 << 26;
+constexpr int kLeastTiles = 2, kUnitTiles = 16, kCodeUnitTiles = 32, kMostTiles = 1 << 26;
 __device__ __forceinline__ int chunk_of(const WindowArgs& a, float total) {
   const float t = total * static_cast<float>(a.Hk) * 1.000001f;
   auto chunk = [](float x) { return static_cast<int>(fminf(x, kMostTiles)) + 1; };
   const int one = chunk(t * a.per_unit);
   int c = chunk(t * (0.25f * a.per_unit));
-  c = c < kUnitTiles ? kUnitTiles : c;
+  c = c < a.unit_tiles ? a.unit_tiles : c;
   c = c < one ? c : one;
   return c < kLeastTiles ? kLeastTiles : c;
 }
@@ -732,10 +735,23 @@ __device__ __forceinline__ void finish_rows(const Place& p, RowTile<T, D>& t, fl
 // is searched by counting the blocks at or above one, a lane a request.
 constexpr int kMaxRanked = 512;
 
+// Over the lanes, of values that are not negative, in registers: a shuffle through LDS takes
+// ten times as long.
+template <typename F>
+__device__ __forceinline__ int lanes_fold(int x, F&& f) {
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true));  // row_shr:1
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true));  // row_shr:2
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true));  // row_shr:4
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true));  // row_shr:8
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, true));  // row_bcast:15
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, true));  // row_bcast:31
+  return __builtin_amdgcn_readlane(x, kWave - 1);
+}
 __device__ __forceinline__ int lanes_sum(int x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, kWave);
-  return uniform_int(x);
+  return lanes_fold(x, [](int a, int b) __attribute__((always_inline)) { return a + b; });
+}
+__device__ __forceinline__ int lanes_max(int x) {
+  return lanes_fold(x, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; });
 }
 struct Packed {
   int b, rblock;  // b -1: no such block
@@ -771,19 +787,15 @@ __device__ __forceinline__ Packed packed_at(const WindowArgs& a, int rank, int l
     int c = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
+      if (i * kWave >= a.B) break;
       const int x = at[i] + n[i] - level;
       c += x < 0 ? 0 : (x < n[i] ? x : n[i]);
     }
     return lanes_sum(c);
   };
   int lo = 0, hi = top;  // from(lo) > rank >= from(hi)
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const int other = __shfl_xor(hi, o, kWave);
-    hi = other > hi ? other : hi;
-  }
-  hi = uniform_int(hi);
   if (from(0) <= rank) return {-1, 0};
+  hi = lanes_max(hi);
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (from(mid) > rank) lo = mid;

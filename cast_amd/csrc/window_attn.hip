@@ -272,6 +272,7 @@ static int run(const void* q, const void* k, const void* v, void* out, float* ls
   a.by_rblocks = divisor(static_cast<uint32_t>(a.n_rblocks));
   a.by_heads = divisor(static_cast<uint32_t>(a.B * a.Hk));
   a.units = n_split == 0 ? static_cast<int>(units_of_round(dims)) : 0;
+  a.unit_tiles = codes ? kCodeUnitTiles : kUnitTiles;
   a.per_unit = a.units ? 1.0f / static_cast<float>(a.units) : 0.0f;
   const int64_t xcd_items = xcd_items_of(dims);
   if (xcd_items >= (1ll << 30)) return RCSA_ERR_SHAPE;
