@@ -753,6 +753,23 @@ __device__ __forceinline__ int lanes_sum(int x) {
 __device__ __forceinline__ int lanes_max(int x) {
   return lanes_fold(x, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; });
 }
+// Which block of ranks and key head workgroup `id` of a share takes (rank -1: none).  Longest
+// first: the key heads of a rank side by side.  In their order: XCD x (workgroups go
+// round-robin) a contiguous run of a key head's ranks, so that neighbours share most of their
+// window in its L2 (clips of up to 20 frames, window 12 and the first, 24 heads 2572 us; key heads
+// side by side 2710).
+struct RankAt {
+  int rank, hk;
+};
+__device__ __forceinline__ RankAt rank_at(const WindowArgs& a, int id) {
+  if (a.descending) {
+    const int rank = divide(id, a.by_Hk);
+    return {rank, id - rank * a.Hk};
+  }
+  const int item = id % kNumXcd * a.xcd_items + id / kNumXcd;
+  const int hk = divide(item, a.by_rblocks);
+  return {hk < a.Hk ? item - hk * a.n_ranks : -1, hk};
+}
 struct Packed {
   int b, rblock;  // b -1: no such block
 };

@@ -9,8 +9,10 @@ namespace rcsa {
 template <typename T, int D>
 __global__ void __launch_bounds__(256) packed_merge_kernel(WindowArgs a) {
   constexpr int CPR = D / 8, BM = 128, WGS = BM * CPR / 256;  // workgroups of a row block
-  const int item = static_cast<int>(blockIdx.x) / WGS, rank = divide(item, a.by_Hk);
-  const Packed it = packed_at(a, rank, threadIdx.x & 63);
+  const int id = static_cast<int>(blockIdx.x) / WGS;
+  const RankAt at = rank_at(a, id);
+  if (at.rank < 0) return;
+  const Packed it = packed_at(a, at.rank, threadIdx.x & 63);
   if (it.b < 0) return;
   Place p;
   p.b = it.b;
@@ -18,10 +20,9 @@ __global__ void __launch_bounds__(256) packed_merge_kernel(WindowArgs a) {
   const int v = static_cast<int>(blockIdx.x) % WGS * 256 + threadIdx.x;
   const int in_block = v / CPR, c = v % CPR, row = it.rblock * BM + in_block;
   if (row >= n_rows) return;
-  const int hk = item - rank * a.Hk;
-  const int qi = divide(row, a.by_G), head = hk * a.G + row - qi * a.G;
-  const int64_t all_rows = static_cast<int64_t>(a.n_ranks) * a.Hk * BM;
-  const int64_t wrow = static_cast<int64_t>(item) * BM + in_block;
+  const int qi = divide(row, a.by_G), head = at.hk * a.G + row - qi * a.G;
+  const int64_t all_rows = static_cast<int64_t>(a.xcd_items) * kNumXcd * BM;
+  const int64_t wrow = static_cast<int64_t>(id) * BM + in_block;
   float mx = -INFINITY;
   for (int s = 0; s < a.n_split; ++s) mx = fmaxf(mx, a.ws_ml[s * all_rows + wrow].x);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -53,7 +54,7 @@ __global__ void __launch_bounds__(256) packed_merge_kernel(WindowArgs a) {
 
 template <typename T, int D>
 static int launch(WindowArgs& a, hipStream_t s) {
-  const int64_t items = static_cast<int64_t>(a.n_ranks) * a.Hk;
+  const int64_t items = static_cast<int64_t>(a.xcd_items) * kNumXcd;
   constexpr int64_t merges = 128 * (D / 8) / 256;
   if (items * a.n_split * 256 >= kMaxThreads || items * merges * 256 >= kMaxThreads)
     return RCSA_ERR_SHAPE;
@@ -69,8 +70,11 @@ int launch_window_packed(WindowArgs& a, int type, int64_t D, hipStream_t s) {
   return D == 128 ? launch<_Float16, 128>(a, s) : launch<_Float16, 64>(a, s);
 }
 
-// Row blocks of a key head of packed requests, at most.
+// Row blocks of a key head of packed requests, at most; of an XCD.
 static int64_t ranks_of(const int64_t* d) { return (d[1] * (d[3] / d[4])) / 128 + d[0]; }
+static int64_t xcd_ranks_of(const int64_t* d) {
+  return (ranks_of(d) * d[4] + kNumXcd - 1) / kNumXcd;
+}
 
 static bool packed_dims(const int64_t* d) {
   for (int i = 0; i < 6; ++i)
@@ -100,7 +104,7 @@ extern "C" int rcsa_packed_attn_plan(const int64_t* dims, int64_t max_keys, int6
 
 extern "C" int64_t rcsa_packed_attn_workspace_bytes(const int64_t* dims, int64_t n_split) {
   if (!dims || !packed_dims(dims) || n_split < 1 || n_split > 64) return -1;
-  return n_split == 1 ? 0 : n_split * ranks_of(dims) * dims[4] * 128 * (dims[5] * 4 + 8);
+  return n_split == 1 ? 0 : n_split * xcd_ranks_of(dims) * kNumXcd * 128 * (dims[5] * 4 + 8);
 }
 
 extern "C" int rcsa_packed_attn(const void* q, const void* k, const void* v, void* out, float* lse,
@@ -149,6 +153,8 @@ extern "C" int rcsa_packed_attn(const void* q, const void* k, const void* v, voi
   a.q_off = q_offsets;
   a.k_off = k_offsets;
   a.n_ranks = static_cast<int>(ranks_of(dims));
+  a.xcd_items = static_cast<int>(xcd_ranks_of(dims));
+  a.by_rblocks = divisor(static_cast<uint32_t>(a.n_ranks));
   a.window = static_cast<int>(window < most ? window : 0);
   a.sinks = static_cast<int>(sinks < most ? sinks : most);
   a.block = static_cast<int>(block < most ? block : most);

@@ -48,15 +48,16 @@ window_kernel(WindowArgs a) {
   int share, q_len, item_row0;
   int64_t ws_row;
   if constexpr (FORM == kPacked) {
-    // the key heads of a row block side by side, its shares a grid apart
-    const int each = a.n_ranks * a.Hk, id = static_cast<int>(blockIdx.x);
+    // (the shares of a row block a grid apart)
+    const int each = a.xcd_items * kNumXcd, id = static_cast<int>(blockIdx.x);
     share = id / each;
-    const int item = id - share * each, rank = divide(item, a.by_Hk);
-    const Packed it = packed_at(a, rank, lane);
+    const RankAt at = rank_at(a, id - share * each);
+    if (at.rank < 0) return;
+    const Packed it = packed_at(a, at.rank, lane);
     if (it.b < 0) return;
     p.shares = a.n_split;
     p.b = it.b;
-    p.hk = item - rank * a.Hk;
+    p.hk = at.hk;
     q_len = packed_place(a, p);
     item_row0 = it.rblock * BM;
     ws_row = static_cast<int64_t>(id) * BM + wave * 32;
