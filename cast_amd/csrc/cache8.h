@@ -22,9 +22,9 @@ template <>
 struct Code8<false> {
   // The scale of a block whose largest value is `most`: most / 127, rounded to fp32.
   static __device__ __forceinline__ float scale_for(float most) { return most / 127.0f; }
-  // The codes nearest x / s, ties to even.  t = x * inv is off by 2^-22 of it, below 2^-15, so
+  // The codes nearest x / s, ties to even.  t = x * inv is off by 2^-23 of it, below 1.6e-5, so
   // that the whole number next to t is the quotient's unless t is that near the border of two
-  // codes.  Where a lane has such a t (one value in 2000), the remainder x - q s decides: it
+  // codes.  Where a lane has such a t (one value in 25000), the remainder x - q s decides: it
   // is exact (fp32 values on a grid no finer than half of s's last place, below 2^24 steps of
   // it).  t + 1.5 2^23 is t rounded, its code in the lowest byte.  Infinities saturate, NaN
   // becomes 0.
@@ -42,32 +42,45 @@ struct Code8<false> {
       return x == x ? d : 0;
     }
     // `plain`: no infinity or NaN among the values of the wavefront
-    __device__ __forceinline__ uint2 eight(const float* x, bool plain) const {
+    template <typename R>
+    __device__ __forceinline__ uint2 eight(const typename R::V& v, bool plain) const {
       constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
-      float u[8], off = 0.0f;
+      uint2 w = make_uint2(0u, 0u);
+      if (!plain) {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          w.x |= static_cast<uint32_t>(exactly(static_cast<float>(v[i])) & 255) << (8 * i);
+          w.y |= static_cast<uint32_t>(exactly(static_cast<float>(v[4 + i])) & 255) << (8 * i);
+        }
+        return w;
+      }
+      // (finite values only: |x / s| is 127 at most, but for roundings)
+      uint32_t pair[4];
+      auto pack = [](float u0, float u1) __attribute__((always_inline)) -> uint32_t {
+        return __builtin_amdgcn_perm(__float_as_uint(u1), __float_as_uint(u0), 0x0c0c0400u);
+      };
+      float off = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float t = x[i] * inv;
-        u[i] = t + kMagic;
-        off = fmaxf(off, fabsf(t - (u[i] - kMagic)));
+      for (int i = 0; i < 4; ++i) {
+        const float t0 = static_cast<float>(v[2 * i]) * inv;
+        const float t1 = static_cast<float>(v[2 * i + 1]) * inv;
+        const float u0 = t0 + kMagic, u1 = t1 + kMagic;
+        off = fmaxf(fmaxf(off, fabsf(t0 - (u0 - kMagic))), fabsf(t1 - (u1 - kMagic)));
+        pair[i] = pack(u0, u1);
       }
-      uint2 w;
-      if (!plain || __ballot(off > 0.4999f) != 0) {
-        auto four = [&](const float* y) __attribute__((always_inline)) -> uint32_t {
-          return (exactly(y[0]) & 255) | (exactly(y[1]) & 255) << 8 | (exactly(y[2]) & 255) << 16 |
-                 static_cast<uint32_t>(exactly(y[3])) << 24;
+      if (__ballot(off > 0.49998f) != 0) {
+        auto near = [&](float x) __attribute__((always_inline)) -> float {
+          const float u = fmaf(x, inv, kMagic);
+          const float r = fmaf(kMagic - u, s, x), far = fabsf(r), half = 0.5f * s;
+          const bool move = far > half || (far == half && (__float_as_uint(u) & 1u));
+          return move ? u + (r < 0.0f ? -1.0f : 1.0f) : u;
         };
-        w = make_uint2(four(x), four(x + 4));
-      } else {
-        auto four = [&](const float* y) __attribute__((always_inline)) -> uint32_t {
-          const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(y[1]), __float_as_uint(y[0]),
-                                                    0x0c0c0400u);
-          const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(y[3]), __float_as_uint(y[2]),
-                                                    0x0c0c0400u);
-          return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
-        };
-        w = make_uint2(four(u), four(u + 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          pair[i] = pack(near(static_cast<float>(v[2 * i])), near(static_cast<float>(v[2 * i + 1])));
       }
+      w = make_uint2(__builtin_amdgcn_perm(pair[1], pair[0], 0x05040100u),
+                     __builtin_amdgcn_perm(pair[3], pair[2], 0x05040100u));
       return w;
     }
   };
@@ -110,7 +123,10 @@ struct Code8<true> {
       const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
       return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true));
     }
-    __device__ __forceinline__ uint2 eight(const float* x, bool plain) const {
+    template <typename R>
+    __device__ __forceinline__ uint2 eight(const typename R::V& v, bool plain) const {
+      float x[8];
+      R::floats(v, x);
       float y[8];
       if (plain && power) {
 #pragma unroll

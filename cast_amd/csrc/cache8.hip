@@ -47,7 +47,8 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t m) {
 // blocks that a wavefront holds twice): one pass over them, the largest first, HELD runs of 8
 // channels a thread in registers, more of them read again.
 template <typename T, bool E4M3, bool PACKED, int THREADS, bool BOTH>
-__global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(THREADS)
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && THREADS < 1024 ? 8 : 4, 8))) append_kernel(AppendArgs a) {
   using C = Code8<E4M3>;
   using R = Run8<T>;
   typedef typename R::V V;
@@ -165,10 +166,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(AppendArgs a) {
     const typename C::To to_code(s);
     auto store = [&](int i, const V& v) __attribute__((always_inline)) {
       const int row = divide(i, a.by_runs);
-      float f[8];
-      R::floats(v, f);
       *reinterpret_cast<uint2*>(codes + (from + row) * a.sc[kv][1] + (i - row * a.runs) * 8) =
-          to_code.eight(f, plain);
+          to_code.template eight<R>(v, plain);
     };
 #pragma unroll
     for (int k = 0; k < HELD; ++k)
