@@ -858,8 +858,8 @@ int rcsa_read_cache(const void* k_codes, const void* v_codes, int code, const fl
  * rcsa_cached_attn: rcsa_window_attn over such pages; q and out bf16 or fp16, D 64 or 128,
  *   out = softmax(sm_scale q . (c_k s_k)) (c_v s_v).
  * Arguments as there, with the type of the codes, their scales (scale_strides: host array of 6,
- * page, block, head of the scales of keys and of values) and block_size; block_table and
- * k_lengths are wanted.  A scale that is no positive number below 2^126 counts as 0; a value
+ * page, block, head of the scales of keys and of values) and block_size; block_table is
+ * wanted.  A scale that is no positive number below 2^126 counts as 0; a value
  * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.
  * Token (slot) strides and pointers of the codes are multiples of 16.  The plan and the workspace
  * are rcsa_window_attn's.
