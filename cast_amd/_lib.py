@@ -90,6 +90,7 @@ SIGNATURES: dict[str, list] = {
     "rcsa_packed_attn_plan": [_P, _I, ctypes.POINTER(c_int64)],
     "rcsa_packed_attn_workspace_bytes": [_P, _I],
     "rcsa_packed_attn": [_P] * 5 + [c_int, _P, _P, _P, _P, _I, _I, _I, c_float, _I, _P, _I, _P],
+    "rcsa_cached_attn_plan": [_P, _I, ctypes.POINTER(c_int64)],
     "rcsa_cached_attn": [_P, _P, _P, c_int, _P, _P, _P, _P, c_int] + [_P] * 6 + [_I] * 8
                         + [c_float, _I, _P, _I, _P],
     "rcsa_append_cache": [_P, _P, c_int, _P, _P, _P, _P, _P, _P, _P, c_int, _P, _P, _P] + [_I] * 5

@@ -55,6 +55,7 @@ struct Api {
   decltype(&rcsa_window_attn_plan) window_attn_plan = nullptr;
   decltype(&rcsa_window_attn_workspace_bytes_for) window_attn_workspace_bytes = nullptr;
   decltype(&rcsa_window_attn) window_attn = nullptr;
+  decltype(&rcsa_cached_attn_plan) cached_attn_plan = nullptr;
   decltype(&rcsa_cached_attn) cached_attn = nullptr;
   decltype(&rcsa_packed_attn_plan) packed_attn_plan = nullptr;
   decltype(&rcsa_packed_attn_workspace_bytes) packed_attn_workspace_bytes = nullptr;
@@ -98,6 +99,7 @@ void bind_library(const std::string& path) {
   bind_one(h, "rcsa_window_attn_plan", api.window_attn_plan);
   bind_one(h, "rcsa_window_attn_workspace_bytes_for", api.window_attn_workspace_bytes);
   bind_one(h, "rcsa_window_attn", api.window_attn);
+  bind_one(h, "rcsa_cached_attn_plan", api.cached_attn_plan);
   bind_one(h, "rcsa_cached_attn", api.cached_attn);
   bind_one(h, "rcsa_packed_attn_plan", api.packed_attn_plan);
   bind_one(h, "rcsa_packed_attn_workspace_bytes", api.packed_attn_workspace_bytes);
@@ -1364,7 +1366,8 @@ std::vector<at::Tensor> window_attention(
   if (ns < -1) {
     int64_t most = max_keys >= 0 ? std::min(max_keys, Lk) : Lk;
     if (window > 0 && window < Lk && sinks < Lk) most = std::min(most, window + sinks + Lq);
-    check_status(a, op, a.window_attn_plan(dims, most, &ns));
+    check_status(a, op, codes ? a.cached_attn_plan(dims, most, &ns)
+                              : a.window_attn_plan(dims, most, &ns));
   }
   at::Tensor ws;
   const int64_t ws_bytes = a.window_attn_workspace_bytes(dims, ns, Lk, window, sinks);

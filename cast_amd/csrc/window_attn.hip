@@ -143,15 +143,19 @@ using namespace rcsa;
 // as one (measured over 1210 tiles, 168 blocks: n 1 725 us, 2 526, 3 424, 4 440, 5 482, 6 448,
 // 8 512); kFixed tiles for the start, as many and one a share for the join (128 blocks of 250
 // tiles: n 2 95, 4 81, 6 83, 8 89; 168 of 83: n 1 57, 3 51, 5 62; 128 of 16: n 1 19, 2 26).
+// The form for few rows, where one fits.
+static bool plan_few(const int64_t* dims, int64_t tiles, int64_t* n_split) {
+  const bool units = units_fit(dims);
+  if (!group_fits(dims) && !units) return false;
+  *n_split = group_fits(dims) && (!units || one_group(dims, tiles)) ? -1 : 0;
+  return true;
+}
+
 extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
   const int64_t tiles = (max_keys + kTileKeys - 1) / kTileKeys;
-  const bool units = units_fit(dims);
-  if (group_fits(dims) || units) {
-    *n_split = group_fits(dims) && (!units || one_group(dims, tiles)) ? -1 : 0;
-    return RCSA_OK;
-  }
+  if (plan_few(dims, tiles, n_split)) return RCSA_OK;
   *n_split = 1;
   const int64_t cux = xcd_cus(), items = xcd_items_of(dims);
   const int64_t tail = items % cux;
@@ -161,6 +165,34 @@ extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int6
   for (int64_t n = 2; n <= 16 && n * 4 <= tiles; ++n) {
     const int64_t c = (tail * n + cux - 1) / cux, each = (tiles + n - 1) / n;
     const int64_t cost = (c == 1 ? each : (9 * c - 2) * each / 9) + 2 * kFixed + n;
+    if (cost < best - best / 16) {
+      best = cost;
+      *n_split = n;
+    }
+  }
+  return RCSA_OK;
+}
+
+// Over codes, in a lone workgroup's times for a tile (1.25 us: widening the codes leaves less to
+// overlap than tiles of 16 bits do, and more to gain from workgroups beside it): a share's tiles,
+// 1.3 and 1.5 times as long with one and two workgroups beside it; the joining launch, and a
+// share's rows written and read again.  17 queries of 32 heads on 8 of D 128, 16 requests of 3082
+// keys, in 1, 2, 4, 6, 8 shares 126, 79, 62, 60, 70 us; 318 of 24 heads, 862 keys, in 1, 2, 3, 6:
+// 41, 34, 33, 35; 100 of 8 heads, 2 of 20000 keys, in 1, 4, 8, 16: 707, 201, 115, 79.
+extern "C" int rcsa_cached_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
+  if (!dims || !n_split) return RCSA_ERR_NULL;
+  if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
+  const int64_t tiles = (max_keys + kTileKeys - 1) / kTileKeys;
+  if (plan_few(dims, tiles, n_split)) return RCSA_OK;
+  *n_split = 1;
+  const int64_t cux = xcd_cus(), items = xcd_items_of(dims);
+  const int64_t tail = items % cux;
+  constexpr int64_t kBeside[4] = {0, 16, 21, 24};  // sixteenths, of up to three on a compute unit
+  int64_t best = 16 * tiles + 32;
+  for (int64_t n = 2; tail != 0 && n <= 32 && n * 4 <= tiles; ++n) {
+    const int64_t c = (tail * n + cux - 1) / cux, each = (tiles + n - 1) / n;
+    const int64_t cost =
+        each * (c / 3 * kBeside[3] + kBeside[c % 3]) + 152 + tail * n * dims[5] / 64;
     if (cost < best - best / 16) {
       best = cost;
       *n_split = n;

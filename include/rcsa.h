@@ -861,9 +861,10 @@ int rcsa_read_cache(const void* k_codes, const void* v_codes, int code, const fl
  * page, block, head of the scales of keys and of values) and block_size; block_table is
  * wanted.  A scale that is no positive number below 2^126 counts as 0; a value
  * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.
- * Token (slot) strides and pointers of the codes are multiples of 16.  The plan and the workspace
- * are rcsa_window_attn's.
+ * Token (slot) strides and pointers of the codes are multiples of 16.  The workspace is
+ * rcsa_window_attn's; rcsa_cached_attn_plan picks n_split as rcsa_window_attn_plan does there.
  */
+int rcsa_cached_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split);
 int rcsa_cached_attn(const void* q, const void* k_codes, const void* v_codes, int code,
                      const float* k_scales, const float* v_scales, void* out, float* lse,
                      int dtype, const int64_t* dims, const int64_t* strides,

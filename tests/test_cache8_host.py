@@ -189,3 +189,21 @@ def test_wrappers_refuse_host_tensors():
                  lambda: ops.packed_attention(x[0], x[0], x[0], ints, n_split=0)):
         with pytest.raises(ValueError, match="packed_attention"):
             call()
+
+
+def test_cached_plan(lib):
+    n = ctypes.c_int64(-1)
+    plan = lambda dims, most: lib.rcsa_cached_attn_plan(_arr(*dims), most, ctypes.byref(n))
+    few = ctypes.c_int64(-1)
+    for dims, most in (((1, 1, 4096, 8, 8, 128), 4096), ((1, 1, 4096, 8, 8, 128), 512)):
+        assert plan(dims, most) == 0  # few rows: as over 16 bits
+        assert lib.rcsa_window_attn_plan(_arr(*dims), most, ctypes.byref(few)) == 0
+        assert n.value == few.value <= 0
+    assert plan((1, 64, 4096, 8, 8, 128), 64) == 0 and n.value == 1
+    assert plan((1, 100, 20000, 8, 8, 128), 20000) == 0 and 8 <= n.value <= 32
+    assert lib.rcsa_window_attn_workspace_bytes(_arr(1, 100, 20000, 8, 8, 128), n.value) > 0
+    assert plan((256, 100, 20000, 8, 8, 128), 20000) == 0 and n.value == 1  # whole rounds
+    assert plan((1, 64, 4096, 8, 3, 128), 4096) == SHAPE
+    assert plan((1, 64, 4096, 8, 8, 128), -1) == SHAPE
+    assert lib.rcsa_cached_attn_plan(None, 1, ctypes.byref(n)) == NULL
+    assert lib.rcsa_cached_attn_plan(_arr(1, 64, 64, 8, 8, 128), 1, None) == NULL

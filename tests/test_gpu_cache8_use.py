@@ -361,3 +361,17 @@ def test_packed_refusals(dev):
     out = torch.full_like(q, 3.0)
     ops.packed_attention(q, k, v, offs[:1], out=out)  # no requests: rows of nobody
     assert (out == 3.0).all()
+
+
+@pytest.mark.parametrize("n_split", [None, 17, 64])
+def test_many_shares(dev, n_split):
+    """A chunk over a long cache: more shares than some rows have tiles."""
+    from cast_amd import ops
+    B, Lq, Hq, Hk, D = 2, 70, 4, 2, 128
+    lens = [4000, 75]
+    cache = _cache(dev, I8, B, 130, 64, 64, Hk, D, 63, seed=9)
+    held = Held(cache)
+    q = torch.randn(B, Lq, Hq, D, generator=torch.Generator().manual_seed(4)).to(BF)
+    out = ops.paged_attention(q.to(dev), cache, _i32(lens, dev), n_split=n_split)
+    for b, n in enumerate(lens):
+        _check(out[b], q[b], held, b, n, 0, 0, dev)
