@@ -12,9 +12,14 @@
 
 namespace rcsa {
 
+// Wavefronts to a SIMD: those of D 64 leave registers for two workgroups of eight on a compute
+// unit (48 requests of 1599 keys, 7 queries of 12 heads 57.7 us, so 51.4; 12 heads of 64 x 2000
+// keys 66.5 and 60.7), or for three units.
+constexpr int cached_waves(int D, bool group) { return D == 64 ? (group ? 4 : 3) : 2; }
+
 template <typename T, bool E4M3, int D, CodeForm FORM, bool GROUP>
 __global__ void __launch_bounds__(GROUP ? 64 * kGroupWaves : 64)
-__attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
+__attribute__((amdgpu_waves_per_eu(cached_waves(D, GROUP), cached_waves(D, GROUP))))
 cached_unit_kernel(WindowArgs a) {
   constexpr bool WHOLE = FORM != kAny;
   constexpr int NW = GROUP ? kGroupWaves : 1;
@@ -106,9 +111,11 @@ cached_unit_kernel(WindowArgs a) {
   int k_at[KL];
 #pragma unroll
   for (int i = 0; i < KL; ++i) k_at[i] = lr * D + (((2 * i + hf) ^ swizzle(lr)) * 16);
-  int v_lo[4];  // rows 4 hf + 0 .. 3; the others are 8, 16 and 24 further
+  // rows 4 hf + 0 .. 3; the others are 8, 16 and 24 further (registers that are short hold one)
+  constexpr int VL = GROUP && D == 64 ? 1 : 4;
+  int v_lo[VL];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v_lo[j] = static_cast<int>((4 * hf + j) * vrb + NDT * lr);
+  for (int j = 0; j < VL; ++j) v_lo[j] = static_cast<int>((4 * hf + j) * vrb + NDT * lr);
   auto load_v = [&](uint32_t (&v)[16]) __attribute__((always_inline)) {
     const char* from = codes.half(0).v;
 #pragma unroll
@@ -118,13 +125,14 @@ cached_unit_kernel(WindowArgs a) {
           const_cast<char*>(from), 0, (WHOLE ? 32 : 16) * static_cast<int>(vrb), kRsrcWord3);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int off = (8 * (j >> 2) + (WHOLE ? 16 * h : 0)) * static_cast<int>(vrb);
+        const int off = (8 * (j >> 2) + (VL == 1 ? j & 3 : 0) + (WHOLE ? 16 * h : 0)) *
+                        static_cast<int>(vrb);
         if constexpr (NDT == 4)
           v[8 * h + j] = static_cast<uint32_t>(
-              __builtin_amdgcn_raw_buffer_load_b32(rs, v_lo[j & 3], off, 0));
+              __builtin_amdgcn_raw_buffer_load_b32(rs, v_lo[j & (VL - 1)], off, 0));
         else
           v[8 * h + j] = static_cast<uint16_t>(
-              __builtin_amdgcn_raw_buffer_load_b16(rs, v_lo[j & 3], off, 0));
+              __builtin_amdgcn_raw_buffer_load_b16(rs, v_lo[j & (VL - 1)], off, 0));
       }
     }
   };
@@ -244,14 +252,18 @@ cached_unit_kernel(WindowArgs a) {
 
   // The end of the rows: lane (row, hf) holds channels 32 g' + ... : register r of product x is
   // channel NDT (8 (r / 4) + 4 hf + r % 4) + x.
+  // (the thread's place is found anew: the loop leaves no registers to hold it)
   LateArgs& e = late_args();
-  const Row my = row_of(e, p, lr);
+  const int at_end = static_cast<int>(
+      __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)));
+  const int row_end = at_end & 31, hf_end = at_end >> 5;
+  const Row my = row_of(e, p, row_end);
   const float l = pair_sum(l_run);
   const float inv = l > 0.0f ? __uint_as_float(unit.bits) / l : l;  // (a NaN sum stays one)
   auto value = [&](int r, int x) __attribute__((always_inline)) -> float {
     return l == 0.0f ? 0.0f : o_acc[x][r] * (1 << Widen<E4M3>::kShift) * inv;
   };
-  const bool live = lr < p.n_rows;
+  const bool live = row_end < p.n_rows;
   if (GROUP || p.shares > 1) {
     const int64_t ws_row = GROUP ? 0 : static_cast<int64_t>(blockIdx.x) * e.Lq * e.G;
     float* const part_o =
@@ -260,12 +272,12 @@ cached_unit_kernel(WindowArgs a) {
     if (live) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float* const at = part_o + lr * D + NDT * (8 * (r >> 2) + 4 * hf + (r & 3));
+        float* const at = part_o + row_end * D + NDT * (8 * (r >> 2) + 4 * hf_end + (r & 3));
 #pragma unroll
         for (int x = 0; x < NDT; ++x) at[x] = value(r, x);
       }
-      if (hf == 0)
-        part_ml[lr] = make_float2(l > 0.0f ? m_run : (l == 0.0f ? -INFINITY : l), l);
+      if (hf_end == 0)
+        part_ml[row_end] = make_float2(l > 0.0f ? m_run : (l == 0.0f ? -INFINITY : l), l);
     }
   } else if (live) {
     T* const op = static_cast<T*>(e.out) + p.b * e.so[0] + static_cast<int64_t>(my.qi) * e.so[1] +
@@ -276,15 +288,15 @@ cached_unit_kernel(WindowArgs a) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) w4[x] = static_cast<T>(value(r + x / NDT, x % NDT));
       *reinterpret_cast<typename Half<T>::op4*>(
-          op + NDT * (8 * (r >> 2) + 4 * hf + (r & 3))) = w4;
+          op + NDT * (8 * (r >> 2) + 4 * hf_end + (r & 3))) = w4;
     }
-    if (hf == 0 && e.lse)
+    if (hf_end == 0 && e.lse)
       e.lse[(static_cast<int64_t>(p.b) * e.Hq + my.head) * e.Lq + my.qi] =
           l == 0.0f ? -INFINITY : (m_run + __log2f(l)) * 0.69314718055994531f;
   }
   if constexpr (GROUP) {
     __syncthreads();
-    for (int i = threadIdx.x; i < p.n_rows * (D / 4); i += 64 * NW) {
+    for (int i = 64 * wave + at_end; i < p.n_rows * (D / 4); i += 64 * NW) {
       const int row = i / (D / 4), c = i % (D / 4) * 4;
       float mx = -INFINITY;
 #pragma unroll

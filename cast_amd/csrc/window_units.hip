@@ -175,14 +175,24 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
     return (first + static_cast<int64_t>(s) * a.Hk) * R + row;
   };
   const int c = tid % CPR, g = tid / CPR;
-  // (the thread's first share is asked for ahead of the maximum: with scalar loads of a single
-  // request's lengths one token over 1024 keys of 8 heads 11.0 us, so 10.6; over 4096 15.2, 14.8)
-  float2 ml = make_float2(-INFINITY, 0.0f);
-  float ov[8];
-  if (g < shares) {
-    ml = a.ws_ml[at(g)];
-    Vec8<float>::load(a.ws_o + at(g) * D + c * 8, ov);
-  }
+  // A thread's shares come U at a time (96 rows of D 128 in 391 units each: one by one 18.7 us,
+  // so 11.9; four at a time would leave six wavefronts to a SIMD), the first ones ahead of the
+  // maximum.  They are added one after the other, so U changes no result.
+  constexpr int U = 3;
+  float2 ml[U];
+  float ov[U][8];
+  auto ask = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * GROUPS;
+      ml[u] = make_float2(-INFINITY, 0.0f);
+      if (s < shares) {
+        ml[u] = a.ws_ml[at(s)];
+        Vec8<float>::load(a.ws_o + at(s) * D + c * 8, ov[u]);
+      }
+    }
+  };
+  ask(g);
   float mx = -INFINITY;
   for (int s = tid; s < shares; s += 256) mx = fmaxf(mx, a.ws_ml[at(s)].x);
   mx = wave_max(mx);
@@ -191,16 +201,16 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
   mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   float sum = 0.0f;
-  for (int s = g; s < shares; s += GROUPS) {
-    if (s != g) {
-      ml = a.ws_ml[at(s)];
-      Vec8<float>::load(a.ws_o + at(s) * D + c * 8, ov);
-    }
-    if (ml.x == -INFINITY) continue;
-    const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - mx);
-    sum += w;
+  for (int s = g; s < shares; s += U * GROUPS) {
+    if (s != g) ask(s);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = join(w, ov[j], acc[j]);
+    for (int u = 0; u < U; ++u) {
+      if (ml[u].x == -INFINITY) continue;
+      const float w = ml[u].y * __builtin_amdgcn_exp2f(ml[u].x - mx);
+      sum += w;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = join(w, ov[u][j], acc[j]);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) s_acc[g][c * 8 + j] = acc[j];
