@@ -8,6 +8,11 @@
 // A lane of S = K Q^T holds a key's channels: loaded as they stand, every load would touch 32
 // lines for a fourth of each (48 ragged requests, 248 us with two tiles in flight so, in more
 // lines than the first cache has), so keys are loaded by whole rows and go through LDS.
+//
+// Bound by HBM where the cache is long: 48 requests of up to 32768 keys, 32 heads on 8 of D 128,
+// 205 us for 1.02 GB (5.0 TB/s) and 7 for the join; there keys by their lanes' rows took 228 us, by
+// copies to LDS 222, units of 16 tiles 219.  Short calls are latency: 1 request, 1024 keys of 8
+// heads 8.8 us and 3.4 for the join.
 #include "cached_attn.h"
 
 namespace rcsa {
