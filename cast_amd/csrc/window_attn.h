@@ -777,7 +777,8 @@ __device__ __forceinline__ Packed packed_at(const WindowArgs& a, int rank, int l
   auto blocks_of = [&](int b, int* level) __attribute__((always_inline)) -> int {
     const RowsOf q = rows_of(a.q_off, b, a.Lq), k = rows_of(a.k_off, b, a.Lk);
     const int before = k.count - q.count;
-    *level = static_cast<int>((before > 0 ? static_cast<int64_t>(before) * a.G : 0) >> 7);
+    const int64_t full = (before > 0 ? static_cast<int64_t>(before) * a.G : 0) >> 7;
+    *level = static_cast<int>(full < (1 << 29) ? full : 1 << 29);  // (an order alone)
     return (q.count * a.G + 127) >> 7;
   };
   if (!a.descending) {

@@ -833,8 +833,8 @@ int rcsa_packed_attn(const void* q, const void* k, const void* v, void* out, flo
  *
  * rcsa_read_cache: rows t of k_out, v_out [B][L][H][D] (bf16, fp16 or fp32) become keys
  * starts[b] + t (NULL: t) of request b, c * s in fp32 rounded once, as far as they are below
- * lengths[b] (int32 [B]); hidden keys give 0, the rows of keys from lengths[b] on, or past the
- * table, are left as they were.
+ * lengths[b] (int32 [B]); hidden keys give 0, the rows of keys from lengths[b] on, past the
+ * table, or below 0 are left as they were.
  *
  * strides: host array of 18, in elements: batch, token, head of k, v (append) or page, slot, head
  * of the codes of keys, values (read) first; then page, slot, head of the codes (append) or page, block,
@@ -860,7 +860,8 @@ int rcsa_read_cache(const void* k_codes, const void* v_codes, int code, const fl
  * Arguments as there, with the type of the codes, their scales (scale_strides: host array of 6,
  * page, block, head of the scales of keys and of values) and block_size; block_table is
  * wanted.  A scale that is no positive number below 2^126 counts as 0; a value
- * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.
+ * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.  Logits
+ * of rows of q with values past 2^100 may overflow.
  * Token (slot) strides and pointers of the codes are multiples of 16.  The workspace is
  * rcsa_window_attn's; rcsa_cached_attn_plan picks n_split as rcsa_window_attn_plan does there.
  */

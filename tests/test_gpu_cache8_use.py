@@ -375,3 +375,46 @@ def test_many_shares(dev, n_split):
     out = ops.paged_attention(q.to(dev), cache, _i32(lens, dev), n_split=n_split)
     for b, n in enumerate(lens):
         _check(out[b], q[b], held, b, n, 0, 0, dev)
+
+
+@pytest.mark.parametrize("beside", ["pages", "slots"])
+def test_keys_and_values_in_one_allocation(dev, beside):
+    """Keys and values of a page (or a slot) side by side: views of one tensor."""
+    from cast_amd import ops
+    B, H, D, page, block, n = 2, 2, 64, 32, 16, 75
+    shape = (10, 2, page, H, D) if beside == "pages" else (10, page, 2, H, D)
+    store = torch.zeros(shape, dtype=I8, device=dev)
+    scales = torch.zeros(10, page // block, 2, H, device=dev)
+    kc, vc = store.unbind(1 if beside == "pages" else 2)
+    ks, vs = scales.unbind(2)
+    table = torch.arange(10, device=dev, dtype=torch.int32).view(B, 5)
+    cache = ops.QuantizedCache(kc, vc, ks, vs, table)
+    held = Held(cache)
+    g = torch.Generator().manual_seed(8)
+    k, v = (torch.randn(B, n, H, D, generator=g).to(BF).to(dev) for _ in range(2))
+    ops.append_cache(k, v, cache)
+    for b in range(B):
+        held.append(b, k[b], v[b], 0)
+    held.check(cache, [n] * B)
+    got = ops.read_cache(cache, _i32([n] * B, dev), size=n)
+    for rows in (1, 80):
+        q = torch.randn(B, rows, 4, D, generator=g).to(BF)
+        out = ops.paged_attention(q.to(dev), cache, _i32([n] * B, dev))
+        for b in range(B):
+            _check(out[b], q[b], held, b, n, 0, 0, dev)
+            for kv in range(2):
+                assert torch.equal(got[kv][b].cpu(), held.keys(kv, b, n).to(BF))
+
+
+def test_packed_many_heads_over_many_keys(dev):
+    """65535 heads over so many keys that rows times keys pass 2^38: every row is taken.  The
+    values are 1, so the outputs are, to the roundings of the weights (2^-8 each, which their
+    sum has too) and of the result."""
+    from cast_amd import ops
+    G, Tk, D = 65535, 4_195_000, 64
+    k = torch.zeros(Tk, 1, D, dtype=BF, device=dev)
+    q = torch.zeros(1, G, D, dtype=BF, device=dev)
+    out = torch.full((1, G, D), 9.0, dtype=BF, device=dev)
+    ops.packed_attention(q, k, torch.ones_like(k), _i32([0, 1], dev), k_offsets=_i32([0, Tk], dev),
+                         out=out)
+    assert ((out.float() - 1.0).abs() <= 2 * 2.0 ** -8).all()
