@@ -307,3 +307,32 @@ def test_append_graph_and_stream(dev):
             c.append(1, b, v[b].cpu(), at[b])
         c.check()
         _check_read(out[1], c, 1, [0] * B, [n + 1 for n in at], BF)
+
+
+@pytest.mark.parametrize("code", [I8, F8])
+def test_far_pages(dev, code):
+    """Codes, tokens and dense rows whose offsets pass 32 bits."""
+    from cast_amd import ops
+    B, L, H, D, pages, page, block = 2, 70, 2, 64, 12, 32, 16
+    c = Cache(dev, 21, code, pages, page, block, H, D, (B, 3))
+    near = c.cache()
+    store = torch.empty(pages, 1 << 29, dtype=torch.int8, device=dev)  # 6.4 GB
+    size = page * H * D
+    far = [store[:, i * size:(i + 1) * size].view(code).unflatten(1, (page, H, D))
+           for i in range(2)]
+    far[0].view(torch.uint8).copy_(near.k.view(torch.uint8))
+    far[1].view(torch.uint8).copy_(near.v.view(torch.uint8))
+    far = ops.QuantizedCache(*far, near.k_scale.clone(), near.v_scale.clone(), near.table)
+    rows = torch.empty(B * L, 1 << 23, dtype=BF, device=dev)[:, :4 * H * D]  # 2.3 GB
+    k, v, ko, vo = rows.unflatten(1, (4, H, D)).unflatten(0, (B, L)).unbind(2)
+    for seed, t in enumerate((k, v)):
+        t.copy_(_tokens(seed, t.shape, BF))
+    starts, ends = _i32([0, 9], dev), _i32([L, 9 + L], dev)
+    ops.append_cache(k.contiguous(), v.contiguous(), near, starts)
+    ops.append_cache(k, v, far, starts)
+    for a, b in ((near.k, far.k), (near.v, far.v)):
+        assert torch.equal(a.view(torch.uint8), b.contiguous().view(torch.uint8))
+    assert torch.equal(near.k_scale, far.k_scale) and torch.equal(near.v_scale, far.v_scale)
+    want = ops.read_cache(near, ends, size=L, starts=starts)
+    ops.read_cache(far, ends, size=L, starts=starts, out=(ko, vo))
+    assert torch.equal(ko, want[0]) and torch.equal(vo, want[1])

@@ -194,3 +194,22 @@ def test_graph_and_stream(dev):
         torch.cuda.synchronize()
         for out in outs:
             _check(out, None, q, k, v, offs, offs, 0, 0, 1, True, 128 ** -0.5, fill=9.0)
+
+
+def test_far_rows(dev):
+    """Keys, values, queries and outputs whose offsets pass 32 bits."""
+    from cast_amd import ops
+    T, Tk, Hq, D, wide = 310, 10000, 2, 128, 1 << 18
+    q, k, v = _inputs(6, T, Tk, Hq, 1, D, BF)
+    store = torch.empty(Tk, wide, dtype=BF, device=dev)  # 5.2 GB
+    far_k, far_v = store[:, :D].unsqueeze(1), store[:, D:2 * D].unsqueeze(1)
+    far_k.copy_(k)
+    far_v.copy_(v)
+    far_q = store[-T:, 2 * D:4 * D].unflatten(1, (Hq, D))
+    far_o = store[-T:, 4 * D:6 * D].unflatten(1, (Hq, D))
+    far_q.copy_(q)
+    offs, k_offs = _i32([0, 300, 310], dev), _i32([0, 9000, 10000], dev)
+    for kw in (dict(), dict(window=400), dict(n_split=3)):
+        want = ops.packed_attention(q.to(dev), k.to(dev), v.to(dev), offs, k_offsets=k_offs, **kw)
+        ops.packed_attention(far_q, far_k, far_v, offs, k_offsets=k_offs, out=far_o, **kw)
+        assert torch.equal(far_o, want), kw
