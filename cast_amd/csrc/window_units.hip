@@ -155,12 +155,12 @@ window_unit_kernel(WindowArgs a) {
 }
 
 // The units of every row joined: w_s = l_s 2^(m_s - M), out = sum w_s O_s / sum w_s.  A
-// workgroup takes one row, its threads (share, 8 channels); the shares are added in a
-// fixed order.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
-  constexpr int CPR = D / 8, GROUPS = 256 / CPR;
-  __shared__ float s_acc[GROUPS][D], s_sum[GROUPS], s_max[4];
+// workgroup takes one row, its threads (share, C channels); the shares are added in a
+// fixed order, the same for any C.
+template <typename T, int D, int C>
+__global__ void __launch_bounds__(2048 / C) window_unit_merge_kernel(WindowArgs a) {
+  constexpr int THREADS = 2048 / C, CPR = D / C, GROUPS = THREADS / CPR;
+  __shared__ float s_acc[GROUPS][D], s_sum[GROUPS], s_max[THREADS / kWave];
   const int tid = threadIdx.x, lane = tid & 63;
   const int R = a.Lq * a.G;
   const int row = static_cast<int>(blockIdx.x) % R;
@@ -175,12 +175,12 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
     return (first + static_cast<int64_t>(s) * a.Hk) * R + row;
   };
   const int c = tid % CPR, g = tid / CPR;
-  // A thread's shares come U at a time (96 rows of D 128 in 391 units each: one by one 18.7 us,
-  // so 11.9; four at a time would leave six wavefronts to a SIMD), the first ones ahead of the
-  // maximum.  They are added one after the other, so U changes no result.
-  constexpr int U = 3;
+  // A thread's shares come U at a time, the first ones ahead of the maximum, and are added one
+  // after the other, so U changes no result either (96 rows of D 128 in 391 units each: one
+  // by one 18.7 us, three at a time 11.9; more would leave fewer wavefronts to a SIMD).
+  constexpr int U = 24 / C;
   float2 ml[U];
-  float ov[U][8];
+  float ov[U][C];
   auto ask = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -188,18 +188,24 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
       ml[u] = make_float2(-INFINITY, 0.0f);
       if (s < shares) {
         ml[u] = a.ws_ml[at(s)];
-        Vec8<float>::load(a.ws_o + at(s) * D + c * 8, ov[u]);
+#pragma unroll
+        for (int j = 0; j < C; j += 4)
+          *reinterpret_cast<v4f*>(ov[u] + j) =
+              *reinterpret_cast<const v4f*>(a.ws_o + at(s) * D + c * C + j);
       }
     }
   };
   ask(g);
   float mx = -INFINITY;
-  for (int s = tid; s < shares; s += 256) mx = fmaxf(mx, a.ws_ml[at(s)].x);
+  for (int s = tid; s < shares; s += THREADS) mx = fmaxf(mx, a.ws_ml[at(s)].x);
   mx = wave_max(mx);
   if (lane == 0) s_max[tid >> 6] = mx;
   __syncthreads();
-  mx = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < THREADS / kWave; ++i) mx = fmaxf(mx, s_max[i]);
+  float acc[C];
+#pragma unroll
+  for (int j = 0; j < C; ++j) acc[j] = 0.0f;
   float sum = 0.0f;
   for (int s = g; s < shares; s += U * GROUPS) {
     if (s != g) ask(s);
@@ -209,11 +215,11 @@ __global__ void __launch_bounds__(256) window_unit_merge_kernel(WindowArgs a) {
       const float w = ml[u].y * __builtin_amdgcn_exp2f(ml[u].x - mx);
       sum += w;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = join(w, ov[u][j], acc[j]);
+      for (int j = 0; j < C; ++j) acc[j] = join(w, ov[u][j], acc[j]);
     }
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s_acc[g][c * 8 + j] = acc[j];
+  for (int j = 0; j < C; ++j) s_acc[g][c * C + j] = acc[j];
   if (c == 0) s_sum[g] = sum;
   __syncthreads();
   if (tid >= D) return;
@@ -235,7 +241,12 @@ template <typename T, int D>
 static int merge(WindowArgs& a, hipStream_t s) {
   // (at most 2^24 rows, of 256 threads: units_fit)
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hk * a.Lq * a.G;
-  window_unit_merge_kernel<T, D><<<dim3(static_cast<unsigned>(rows)), dim3(256), 0, s>>>(a);
+  // Where the rows fill the card once or twice, more threads a row have more loads in flight
+  // (whole calls, with C 8 and 4: 96 rows in 391 units 33.1 us, 30.8; 32 in 64 13.2, 12.7; 1920
+  // rows in 25 28.6, 32.6).
+  const dim3 grid(static_cast<unsigned>(rows));
+  if (rows <= 512) window_unit_merge_kernel<T, D, 4><<<grid, dim3(512), 0, s>>>(a);
+  else window_unit_merge_kernel<T, D, 8><<<grid, dim3(256), 0, s>>>(a);
   return launch_status();
 }
 
