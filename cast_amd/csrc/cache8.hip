@@ -8,11 +8,11 @@
 // rcsa_read_cache: c * s in fp32, rounded once.
 //
 // Both are bound by HBM, or by a launch's start and end.  An append holds a block's values in
-// registers between the maximum and the codes, so that they are read once: 3520 tokens x 24 heads of
-// D 128, bf16 to int8, 17.2 us for 65 MB (3.8 TB/s; with the read of the new rows 31.5, and 51 with
-// every value near a border divided exactly); 11 packed prompts of up to 8192 tokens x 4 heads
-// of 64 in blocks of 16, fp16 to e4m3, 11.9.  64 requests' tokens 4.6 to 5.  A read of 38720 tokens x
-// 24 heads of 128 takes 131 us (714 MB, 5.4 TB/s; with a place found for each run 249, and 192).
+// registers between the maximum and the codes, so that they are read once: 3520 tokens x 24 heads
+// of D 128, bf16 to int8, 17.2 us for 65 MB (3.8 TB/s; with the read of the new rows 31.5, and 51
+// with every value near a border divided exactly); 11 packed prompts of up to 8192 tokens x 4 heads
+// of 64 in blocks of 16, fp16 to e4m3, 11.9.  64 requests' tokens 4.6 to 5.  A read of 38720 tokens
+// x 24 heads of 128 takes 131 us (714 MB, 5.4 TB/s; with a place found for each run 249).
 #include "cache8.h"
 #include "packed.h"
 
@@ -55,7 +55,8 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t m) {
 // channels a thread in registers, more of them read again.
 template <typename T, bool E4M3, bool PACKED, int THREADS, bool BOTH>
 __global__ void __launch_bounds__(THREADS)
-__attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && THREADS < 1024 ? 8 : 4, 8))) append_kernel(AppendArgs a) {
+__attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 && THREADS < 1024 ? 8 : 4, 8)))
+append_kernel(AppendArgs a) {
   using C = Code8<E4M3>;
   using R = Run8<T>;
   typedef typename R::V V;

@@ -149,8 +149,9 @@ __device__ __forceinline__ int row_shift(float most) {
 // ends, a page ahead; otherwise the two halves of 16 keys are looked up each on their own.
 // FORM kWhole: blocks of whole tiles, one scale a tile; kHalves: blocks of 16 keys, two; kAny:
 // pages or blocks of neither, the entries of a tile asked for a tile ahead.  Arguments that only
-// some steps need are read again there: scalar registers are short.  Past the share's last tile, and on pages that are not there, the codes
-// stand where some page's are: they are read, and not seen.
+// some steps need are read again there: scalar registers are short.  Past the share's last tile,
+// and on pages that are not there, the codes stand where some page's are: they are read, and not
+// seen.
 enum CodeForm { kWhole, kHalves, kAny };
 inline CodeForm code_form(const WindowArgs& a) {
   if (!a.whole_tiles) return kAny;

@@ -84,9 +84,9 @@ cached_unit_kernel(WindowArgs a) {
     less = E4M3 ? 0.0f : -Widen<E4M3>::kMore / Widen<E4M3>::kUnit * pair_sum(sum_of<2 * KL>(q_op));
   }
 
-  // A tile's keys: load i takes rows i RPC + lane / CPR, chunks of 16 bytes, which lie in LDS swizzled
-  // by row so that the reads of a chunk of 16 keys meet no bank twice.  The lane's key is lr, its channels
-  // those of chunks 2 i + hf; its channels of the values of key 8 (r / 4) + 4 hf + r % 4 are
+  // A tile's keys: load i takes rows i RPC + lane / CPR, chunks of 16 bytes, which lie in LDS
+  // swizzled by row so that the reads of a chunk of 16 keys meet no bank twice.  The lane's key is
+  // lr, its channels those of chunks 2 i + hf; its channels of the values of key 8 (r / 4) + 4 hf + r % 4 are
   // NDT lr and the next ones.
   constexpr int CPR = D / 16, RPC = 64 / CPR, LOADS = kTileKeys / RPC;
   auto swizzle = [](int row) __attribute__((always_inline)) -> int {

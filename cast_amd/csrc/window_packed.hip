@@ -3,8 +3,9 @@
 // many keys go first where there is no window (see packed_at).
 //
 // Bound by the matrix pipe under the power limit: 9 prompts of up to 8192 tokens behind up to
-// 1500 held ones, 32 heads on 8 of D 128, 1475 us, 1150 TFLOP/s (pipe 69% busy at 1.66 GHz); clips of
-// up to 20 frames of 880 under a window of 12 and the first, 24 heads, 2540 us, 1140 TFLOP/s (72%).
+// 1500 held ones, 32 heads on 8 of D 128, 1475 us, 1150 TFLOP/s (pipe 69% busy at 1.66 GHz); clips
+// of up to 20 frames of 880 under a window of 12 and the first, 24 heads, 2540 us, 1140 TFLOP/s
+// (72%).
 // 40 prompts of up to 301 tokens take 11.8 us: a launch, the search and one short row block.
 #include "window_tile.h"
 

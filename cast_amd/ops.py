@@ -21,7 +21,8 @@ __all__ = [
     "pool_query", "pool_key", "block_scores", "select_topk", "quantize_key",
     "sparse_attn_bf16", "sparse_attn_int8", "pack_tokens", "unpack_tokens", "row_budgets",
     "quantize_key_select", "order_lists", "rope", "norm_rope", "PagedCache",
-    "window_attention", "paged_attention", "packed_attention", "QuantizedCache", "append_cache", "read_cache",
+    "window_attention", "paged_attention", "packed_attention", "QuantizedCache", "append_cache",
+    "read_cache",
 ]
 
 
