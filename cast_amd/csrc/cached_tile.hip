@@ -8,8 +8,7 @@
 // There: codes through registers ahead of LDS 1359 us; through LDS, three workgroups on a compute
 // unit 1038; places carried from tile to tile instead of found for each 931; keys as subnormal
 // fp16 numbers (a byte permutation alone) 913.  Without the scales' loads, whose scalar returns
-// every wait for LDS waits for, 862 (a wrong result); as vector loads 935, pages of 16 keys 1015
-// instead of 1050.
+// every wait for LDS waits for, 862 (a wrong result).
 #include "cached_attn.h"
 
 namespace rcsa {
@@ -27,34 +26,27 @@ struct CodeTile : RowTile<_Float16, D> {
   // scale and log2 of the weights' factor f), 1 / f
   float c, more, inv_f;
 
-  // (a branch of its own: scales change where a block ends)
-  template <CodeForm FORM>
-  __device__ __forceinline__ void take(const Scales<FORM>& sc, int hf) {
-    constexpr int N = Scales<FORM>::N;
+  // A key's and a value's scale of the lane's half; `top`: the larger value scale's bits.
+  __device__ __forceinline__ void take(float ks, float vs, uint32_t top) {
+    if (top >= unit.bits) {
+      const float f = raise_unit(unit, __uint_as_float(top));
 #pragma unroll
-    for (int h = 0; h < N; ++h)
-      if (__float_as_uint(sc.v[h]) >= unit.bits) {
-        const float f = raise_unit(unit, sc.v[h]);
+      for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < R::NDT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
-      }
-    const float ks = N == 1 ? sc.k[0] : hf ? sc.k[N - 1] : sc.k[0];
-    const float vs = N == 1 ? sc.v[0] : hf ? sc.v[N - 1] : sc.v[0];
+        for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
+    }
     c = fmaxf(c_row * ks, 0x1p-126f);  // (0 * -inf is NaN)
     const float f = fmaxf(vs * unit.inv, 0x1p-60f);
     more = fmaf(c_less, ks, __builtin_amdgcn_logf(f));
     inv_f = __builtin_amdgcn_rcpf(f);
   }
 
-  template <CodeForm FORM, typename Bits, typename Pre>
-  __device__ __forceinline__ void step8(const char* tile, const Scales<FORM>& sc, bool changed,
-                                        int hf, bool inside,
-                                        Bits&& bits, Pre&& prefetch) {
+  template <CodeForm FORM, typename Take, typename Bits, typename Pre>
+  __device__ __forceinline__ void step8(const char* tile, bool inside, Take&& scales, Bits&& bits,
+                                        Pre&& prefetch) {
     // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
     v4i kraw[R::QSTEPS];
-    constexpr int HELD = 8;
+    constexpr int HELD = FORM == kWhole ? 8 : 4;
     int far = 64;
     asm volatile("" : "+s"(far));
 #pragma unroll
@@ -70,8 +62,9 @@ struct CodeTile : RowTile<_Float16, D> {
     __builtin_amdgcn_sched_group_barrier(0x100, R::QSTEPS, 0);
     __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
     __builtin_amdgcn_sched_barrier(0);
+    if (FORM != kWhole) scales();
     prefetch();
-    if (FORM != kWhole || changed) take<FORM>(sc, hf);
+    if (FORM == kWhole) scales();
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
@@ -245,6 +238,11 @@ cached_tile_kernel(WindowArgs a) {
 
   // Tile j is in slot j % 2 as fp16, written during step j - 1 (every wavefront has left step
   // j - 2 by then); its codes landed in raw slot j % 2, asked for during step j - 3.
+  // One scale a tile is asked for by a scalar load, used where it differs from the last one's.
+  // Scales of halves come by vector loads, ahead of a later tile's copies: scalar ones return out
+  // of order, so that waits for LDS would wait for them too (2926 queries on 4737 keys in pages of
+  // 48, 24 heads 285 us, so 271; 318 on 862 in pages of 16 30.4 and 29.3; with one scale a tile the
+  // case above 912, and 935 that way).
   const float* const ks = a.ks + p.hk * a.sks[2];
   const float* const vs = a.vs + p.hk * a.svs[2];
   typedef TileRef<FORM> Ref;
@@ -257,8 +255,20 @@ cached_tile_kernel(WindowArgs a) {
   __builtin_amdgcn_sched_barrier(0);
   codes.next();
   e2 = codes.ref;
-  Scales<FORM> sc = scales_of(e0, ks, vs);
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));
+  float k_scale, v_scale;
+  auto load_scales = [&](const Ref& e) __attribute__((always_inline)) {
+    if constexpr (FORM == kWhole) {
+      const Scales<FORM> sc = scales_of(e, ks, vs);
+      k_scale = sc.k[0];
+      v_scale = sc.v[0];
+    } else {
+      int ki = hf ? e.k[1] : e.k[0], vi = hf ? e.v[1] : e.v[0];
+      k_scale = ks[ki];
+      v_scale = vs[vi];
+    }
+  };
+  load_scales(e0);
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));  // (the first tile's copies have landed)
   widen(r_0, s_0);
   __builtin_amdgcn_sched_barrier(0);  // (its codes are in registers)
   stage(r_0);
@@ -269,27 +279,47 @@ cached_tile_kernel(WindowArgs a) {
     char* const tile = J == 0 ? s_0 : s_1;
     char* const fill = J == 0 ? s_1 : s_0;
     char* const raw_slot = J == 0 ? r_1 : r_0;
-    asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    // (behind the copies that have to have landed: a tile's, and its scales)
+    if constexpr (FORM == kWhole)
+      asm volatile("s_waitcnt vmcnt(2) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int key = e0.key, there = e0.there;
-    const Scales<FORM> ns = sc;
-    const bool changed = __float_as_uint(ns.k[0]) != had_k || __float_as_uint(ns.v[0]) != had_v;
-    had_k = __float_as_uint(ns.k[0]);
-    had_v = __float_as_uint(ns.v[0]);
+    const float kn = k_scale, vn = v_scale;
+    const bool changed = __float_as_uint(kn) != had_k || __float_as_uint(vn) != had_v;
+    if constexpr (FORM == kWhole) {
+      had_k = __float_as_uint(kn);
+      had_v = __float_as_uint(vn);
+    }
     e0 = e1;
     e1 = e2;
     e2 = codes.ref;
     const bool inside = key >= 0 && there == 3 && key + kTileKeys <= w_first.hi &&
                         (key >= w_last.lo || key + kTileKeys <= a.sinks);
     t.template step8<FORM>(
-        tile, ns, changed, hf, inside,
+        tile, inside,
+        [&]() __attribute__((always_inline)) {
+          if constexpr (FORM == kWhole) {
+            if (changed) t.take(kn, vn, __float_as_uint(vn));
+          } else {
+            const float v = (there >> hf) & 1 ? scale_or_0(vn) : 0.0f;
+            auto of_lane = [&](int l) __attribute__((always_inline)) -> uint32_t {
+              return static_cast<uint32_t>(
+                  __builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), l));
+            };
+            const uint32_t first = of_lane(0), second = of_lane(32);
+            t.take(scale_or_0(kn), v, first > second ? first : second);
+          }
+        },
         [&]() __attribute__((always_inline)) {
           return key < 0 ? 0u : seen_bits(late_args(), p, p.row0 + lr, hf, key, there);
         },
         [&]() __attribute__((always_inline)) {
           widen(raw_slot, fill);
+          if constexpr (FORM != kWhole) load_scales(e0);
           __builtin_amdgcn_sched_barrier(0);
           stage(raw_slot);
-          sc = scales_of(e0, ks, vs);
+          if constexpr (FORM == kWhole) load_scales(e0);
           codes.next();
         });
   };
