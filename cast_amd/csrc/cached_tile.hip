@@ -268,7 +268,9 @@ cached_tile_kernel(WindowArgs a) {
     }
   };
   load_scales(e0);
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(2));  // (the first tile's copies have landed)
+  // (the first tile's copies have landed; of scales by vector loads, all: what the barriers
+  // below count begins with the next copies)
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(FORM == kWhole ? 2 : 0));
   widen(r_0, s_0);
   __builtin_amdgcn_sched_barrier(0);  // (its codes are in registers)
   stage(r_0);
