@@ -182,12 +182,24 @@ append_kernel(AppendArgs a) {
       if (tid + k * THREADS < runs) store(tid + k * THREADS, held[j][k]);
     for (int i = tid + HELD * THREADS; i < runs; i += THREADS) store(i, load(kv, x, i));
     if (s != s0) {  // (a block's first scale, or a larger one)
-      for (int i = tid; i < from * a.runs; i += THREADS) {
-        const int row = divide(i, a.by_runs);
-        uint2* const p =
-            reinterpret_cast<uint2*>(codes + row * a.sc[kv][1] + (i - row * a.runs) * 8);
-        const uint2 w = *p;
-        *p = make_uint2(C::again(w.x, s0, s), C::again(w.y, s0, s));
+      constexpr int U = BOTH ? 1 : 4;  // loads in flight (BOTH: values are still held)
+      const int kept = from * a.runs;
+      for (int i0 = tid; i0 < kept; i0 += U * THREADS) {
+        uint2* p[U];
+        uint2 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * THREADS;
+          if (i >= kept) break;
+          const int row = divide(i, a.by_runs);
+          p[u] = reinterpret_cast<uint2*>(codes + row * a.sc[kv][1] + (i - row * a.runs) * 8);
+          w[u] = *p[u];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i0 + u * THREADS >= kept) break;
+          *p[u] = make_uint2(C::again(w[u].x, s0, s), C::again(w[u].y, s0, s));
+        }
       }
       // (every thread has read the block's old scale before the barrier, or, of one
       // wavefront, before this store)
@@ -294,7 +306,11 @@ static int launch_append(AppendArgs& a, hipStream_t s) {
   const int64_t runs = static_cast<int64_t>(a.block) * a.runs;
   const bool both = runs <= 256;
   const int64_t wgs = (PACKED ? a.items : a.items * a.B) * (both ? 1 : 2) * a.H;
-  const int threads = runs <= 512 ? 64 : runs <= 2048 ? 256 : 1024;
+  // A wavefront for small blocks; 1024 threads where large ones may get many tokens at once (5
+  // tokens of 64 requests, 4 heads of D 256 in blocks of 256: 16.5 us by 1024 threads, 8.0 by 256;
+  // 54 and 51 where every block's scale grows).
+  const int64_t fresh = static_cast<int64_t>(a.L < a.block ? a.L : a.block) * a.runs;
+  const int threads = runs <= 512 ? 64 : fresh <= 2048 ? 256 : 1024;
   if (wgs >= (1ll << 31) || wgs * threads >= kMaxThreads8) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs)), block(static_cast<unsigned>(threads));
   if (both) append_kernel<T, E4M3, PACKED, 64, true><<<grid, block, 0, s>>>(a);
