@@ -6,9 +6,10 @@
 //   (q . c_k) * s_k sm_scale,   out = sum_j w_j s_vj c_vj / sum_j w_j.
 // Queries become fp16 with a power of two a row that brings its largest value to [2^14,
 // 2^15): bf16 rows lose nothing down to 2^-29 of it, and 2^-39 of it at most below.
-// A weight takes the scale of its value's block, relative to a power of two 2^e no smaller than
-// any scale of the row's keys so far, before it is rounded to fp16; e grows with the tiles (the
-// accumulators move by the difference), and the sums of weights know nothing of it.  A weight
+// A weight takes the scale of its value's block, relative to a power of two 2^e above any scale of
+// the keys that the wavefront's rows have seen so far, before it is rounded to fp16; e grows with
+// the tiles (the accumulators move by the difference), and the sums of weights know nothing of it.
+// A block that no row sees may have any scale: it counts as 0.  A weight
 // below 2^-32 of the largest, in a block whose scale is as large, is lost: values that
 // differ by more than that between blocks give the smaller ones no more than fp32 sums would
 // have left of them.

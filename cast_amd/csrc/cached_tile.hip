@@ -62,17 +62,21 @@ struct CodeTile : RowTile<_Float16, D> {
     __builtin_amdgcn_sched_group_barrier(0x100, R::QSTEPS, 0);
     __builtin_amdgcn_sched_group_barrier(0x008, R::QSTEPS, 0);
     __builtin_amdgcn_sched_barrier(0);
-    if (FORM != kWhole) scales();
-    prefetch();
-    if (FORM == kWhole) scales();
+    if (FORM == kWhole) prefetch();
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
+    // the wavefront's lanes that see a key: a block that none sees may have any scale, which must
+    // not raise the unit
+    uint64_t seeing = ~0ull;
     if (!inside) {
       const uint32_t seen = bits();
+      seeing = __ballot(seen != 0);
 #pragma unroll
       for (int r = 0; r < 16; ++r) rv[r] = ((seen >> r) & 1u) ? rv[r] : -INFINITY;
     }
+    scales(seeing);
+    if (FORM != kWhole) prefetch();
     v8hf p_op[2];
     auto exps = [&]() __attribute__((always_inline)) -> float {
       const float bias = more + (this->m_run == -INFINITY ? 0.0f : -this->m_run);
@@ -288,11 +292,6 @@ cached_tile_kernel(WindowArgs a) {
       asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     const int key = e0.key, there = e0.there;
     const float kn = k_scale, vn = v_scale;
-    const bool changed = __float_as_uint(kn) != had_k || __float_as_uint(vn) != had_v;
-    if constexpr (FORM == kWhole) {
-      had_k = __float_as_uint(kn);
-      had_v = __float_as_uint(vn);
-    }
     e0 = e1;
     e1 = e2;
     e2 = codes.ref;
@@ -300,11 +299,16 @@ cached_tile_kernel(WindowArgs a) {
                         (key >= w_last.lo || key + kTileKeys <= a.sinks);
     t.template step8<FORM>(
         tile, inside,
-        [&]() __attribute__((always_inline)) {
+        [&](uint64_t seeing) __attribute__((always_inline)) {
           if constexpr (FORM == kWhole) {
-            if (changed) t.take(kn, vn, __float_as_uint(vn));
+            const float v = seeing != 0 ? vn : 0.0f;
+            if (__float_as_uint(kn) != had_k || __float_as_uint(v) != had_v)
+              t.take(kn, v, __float_as_uint(v));
+            had_k = __float_as_uint(kn);
+            had_v = __float_as_uint(v);
           } else {
-            const float v = (there >> hf) & 1 ? scale_or_0(vn) : 0.0f;
+            const bool sees = (hf ? seeing >> 32 : seeing & 0xffffffffu) != 0;
+            const float v = ((there >> hf) & 1) && sees ? scale_or_0(vn) : 0.0f;
             auto of_lane = [&](int l) __attribute__((always_inline)) -> uint32_t {
               return static_cast<uint32_t>(
                   __builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), l));

@@ -163,7 +163,7 @@ cached_unit_kernel(WindowArgs a) {
   // present ones are in LDS, its values as soon as the present ones are in operands.
   for (int s = 0; s < p.steps; ++s) {
     const int key = cur.key, there = cur.there;
-    const Scales<FORM> ns = sc;
+    Scales<FORM> ns = sc;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) *reinterpret_cast<v4i*>(slot + k_to[i]) = kr[i];
     const bool more = s + 1 < p.steps;
@@ -193,10 +193,14 @@ cached_unit_kernel(WindowArgs a) {
     const bool inside = there == 3 && key + kTileKeys <= first.hi &&
                         (key >= last.lo || key + kTileKeys <= a.sinks);
     if (!inside) {
-      const uint32_t seen = seen_keys(late_args(), p, lr, key, there) >> (4 * hf);
+      const uint32_t all = seen_keys(late_args(), p, lr, key, there), seen = all >> (4 * hf);
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         rv[r] = (seen >> (8 * (r >> 2) + (r & 3))) & 1u ? rv[r] : -INFINITY;
+      // (a block that no row sees may have any scale, which must not raise the unit)
+#pragma unroll
+      for (int h = 0; h < N; ++h)
+        if (__ballot((all & (N == 1 ? ~0u : 0xffffu << (16 * h))) != 0) == 0) ns.v[h] = 0.0f;
     }
     // the scales of the values, relative to the largest so far
 #pragma unroll
