@@ -67,7 +67,7 @@ struct CodeTile : RowTile<_Float16, D> {
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
     // the wavefront's lanes that see a key: a block that none sees may have any scale, which must
-    // not raise the unit
+    // neither raise the unit nor, of keys, add c_less times it to masked logits
     uint64_t seeing = ~0ull;
     if (!inside) {
       const uint32_t seen = bits();
@@ -301,20 +301,20 @@ cached_tile_kernel(WindowArgs a) {
         tile, inside,
         [&](uint64_t seeing) __attribute__((always_inline)) {
           if constexpr (FORM == kWhole) {
-            const float v = seeing != 0 ? vn : 0.0f;
-            if (__float_as_uint(kn) != had_k || __float_as_uint(v) != had_v)
-              t.take(kn, v, __float_as_uint(v));
-            had_k = __float_as_uint(kn);
+            const float k = seeing != 0 ? kn : 0.0f, v = seeing != 0 ? vn : 0.0f;
+            if (__float_as_uint(k) != had_k || __float_as_uint(v) != had_v)
+              t.take(k, v, __float_as_uint(v));
+            had_k = __float_as_uint(k);
             had_v = __float_as_uint(v);
           } else {
             const bool sees = (hf ? seeing >> 32 : seeing & 0xffffffffu) != 0;
-            const float v = ((there >> hf) & 1) && sees ? scale_or_0(vn) : 0.0f;
+            const float k = sees ? scale_or_0(kn) : 0.0f, v = sees ? scale_or_0(vn) : 0.0f;
             auto of_lane = [&](int l) __attribute__((always_inline)) -> uint32_t {
               return static_cast<uint32_t>(
                   __builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), l));
             };
             const uint32_t first = of_lane(0), second = of_lane(32);
-            t.take(scale_or_0(kn), v, first > second ? first : second);
+            t.take(k, v, first > second ? first : second);
           }
         },
         [&]() __attribute__((always_inline)) {

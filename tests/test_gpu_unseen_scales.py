@@ -133,3 +133,43 @@ def test_value_scales_that_other_rows_see(dev, code, page, mark, window):
             got = _call(p.cache(1, free, far), q, [Lk], window, 0, 1, dev)
             assert torch.equal(got[0][:, own], want[0][:, own]), (own, far)
             assert torch.equal(got[1][:, :, own], want[1][:, :, own]), (own, far)
+
+
+@pytest.mark.parametrize("code,dtype", [(I8, BF), (F8, HF)])
+@pytest.mark.parametrize("Lq,Hq,D,page,mark,window,sinks", CASES)
+def test_key_scales_of_unseen_blocks(dev, code, dtype, Lq, Hq, D, page, mark, window, sinks):
+    """Queries of either sign's sum: what a code's offset takes off a logit has it too."""
+    Hk, k_len = 2, [Lq + 9, 170 + Lq % 2, 332]
+    p = Pages(dev, Lq + page, code, k_len, page, mark, Hk, D, -(-400 // page))
+    q = _queries(Lq, (3, Lq, Hq, D), dtype) - 0.2
+    q[:, :, 0] = -q[:, :, 0]
+    seen = _seen_of(Lq, k_len, window, sinks)
+    free = p.unseen(seen)
+    for n_split in _forms(Lq, Hq, Hk):
+        print("unseen keys", code, Lq, page, mark, window, n_split, flush=True)
+        want = _call(p.cache(0, free, 0.0), q, k_len, window, sinks, n_split, dev)
+        p.check(*want, q, seen, D ** -0.5)
+        for far in (1e6, 1e20, 2.0 ** 125):
+            got = _call(p.cache(0, free, far), q, k_len, window, sinks, n_split, dev)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (n_split, far)
+
+
+@pytest.mark.parametrize("page,mark", [(32, 16), (48, 16), (64, 32), (48, 48)])
+@pytest.mark.parametrize("window", [0, 64])
+def test_key_scales_that_other_rows_see(dev, page, mark, window):
+    """As for the values: scales so large that a logit's offset overflows."""
+    Lq, Lk, Hk, D = 128, 192, 1, 128
+    p = Pages(dev, page + mark, I8, [Lk], page, mark, Hk, D, Lk // page)
+    seen = so.visible(Lq, Lk, window, 0, 1)
+    for sign in (-1.0, 1.0):
+        q = sign * (_queries(9, (1, Lq, 1, D), BF) + 0.3)
+        for own, free in ((slice(0, 96), p.unseen([seen[:96]])),
+                          (slice(32, 128), p.unseen([seen[32:]]))):
+            if not free.any():
+                continue
+            print("other rows' keys", page, mark, window, own, sign, flush=True)
+            want = _call(p.cache(0, free, 1e-3), q, [Lk], window, 0, 1, dev)
+            for far in (1e20, 2.0 ** 125):
+                got = _call(p.cache(0, free, far), q, [Lk], window, 0, 1, dev)
+                assert torch.equal(got[0][:, own], want[0][:, own]), (own, far)
+                assert torch.equal(got[1][:, :, own], want[1][:, :, own]), (own, far)
