@@ -7,9 +7,9 @@
 // Queries become fp16 with a power of two a row that brings its largest value to [2^14,
 // 2^15): bf16 rows lose nothing down to 2^-29 of it, and 2^-39 of it at most below.
 // A weight takes the scale of its value's block, relative to a power of two 2^e above any scale of
-// the keys that the wavefront's rows have seen so far, before it is rounded to fp16; e grows with
-// the tiles (the accumulators move by the difference), and the sums of weights know nothing of it.
-// A block that no row sees may have any scale: it counts as 0.  A weight
+// the keys that the row has seen so far, before it is rounded to fp16; e grows with the tiles (the
+// accumulators move by the difference), and the sums of weights know nothing of it.  A block may
+// have any scale for the rows that do not see it: it counts as 0 there.  A weight
 // below 2^-32 of the largest, in a block whose scale is as large, is lost: values that
 // differ by more than that between blocks give the smaller ones no more than fp32 sums would
 // have left of them.
@@ -350,17 +350,22 @@ __device__ __forceinline__ Scales<FORM> scales_of(const TileRef<FORM>& t, const 
   }
   return r;
 }
-// The unit 2^e of the accumulators: above the scales of all values so far.
-struct Unit2 {
-  uint32_t bits;  // of 2^e
-  float inv;      // 2^-e
-};
-__device__ __forceinline__ Unit2 least_unit() { return {1u << 23, 0x1p126f}; }
-// The least power of two above scale s, and the factor from unit u to it.
-__device__ __forceinline__ float raise_unit(Unit2& u, float s) {
+// `s` in the lanes of a mask, 0 in the others.
+__device__ __forceinline__ float in_lanes(uint64_t mask, float s) {
+  return __builtin_amdgcn_inverse_ballot_w64(mask) ? s : 0.0f;
+}
+// The unit 2^e of a row's accumulators, as its bits: above the scales of all values that it has
+// seen so far.
+constexpr uint32_t kLeastUnit = 1u << 23;
+__device__ __forceinline__ float per_unit(uint32_t unit) {  // 2^-e
+  return __uint_as_float((254u << 23) - unit);
+}
+// The unit raised above a scale s, where it is not, and the factor to it.
+__device__ __forceinline__ float raise_unit(uint32_t& unit, float s) {
   const uint32_t e = (__float_as_uint(s) >> 23) + 1u;  // (at most 253)
-  const uint32_t down = e - (u.bits >> 23);
-  u = {e << 23, __uint_as_float((254u - e) << 23)};
+  if (__float_as_uint(s) < unit) return 1.0f;
+  const uint32_t down = e - (unit >> 23);
+  unit = e << 23;
   return down >= 127u ? 0.0f : __uint_as_float((127u - down) << 23);
 }
 

@@ -21,22 +21,23 @@ struct CodeTile : RowTile<_Float16, D> {
   // The products are q . (c + 128) 2^-24 for int8 codes: a logit in log2 units is the product
   // times c_row times the key's scale, and c_less times it.
   float c_row, c_less;
-  Unit2 unit;   // of the accumulators
+  uint32_t unit;  // of the row's accumulators
   // what a tile's scales give: a product's factor, what is added to it (c_less times the key's
   // scale and log2 of the weights' factor f), 1 / f
   float c, more, inv_f;
 
-  // A key's and a value's scale of the lane's half; `top`: the larger value scale's bits.
-  __device__ __forceinline__ void take(float ks, float vs, uint32_t top) {
-    if (top >= unit.bits) {
-      const float f = raise_unit(unit, __uint_as_float(top));
+  // A key's and a value's scale of the lane's half, 0 where the row sees none of it; `top`: the
+  // larger value scale of the row's halves.
+  __device__ __forceinline__ void take(float ks, float vs, float top) {
+    if (__ballot(__float_as_uint(top) >= unit) != 0) {
+      const float f = raise_unit(unit, top);
 #pragma unroll
       for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) this->o_acc[dt][r] *= f;
     }
     c = fmaxf(c_row * ks, 0x1p-126f);  // (0 * -inf is NaN)
-    const float f = fmaxf(vs * unit.inv, 0x1p-60f);
+    const float f = fmaxf(vs * per_unit(unit), 0x1p-60f);
     more = fmaf(c_less, ks, __builtin_amdgcn_logf(f));
     inv_f = __builtin_amdgcn_rcpf(f);
   }
@@ -46,13 +47,13 @@ struct CodeTile : RowTile<_Float16, D> {
                                         Pre&& prefetch) {
     // (the chunks' places are sums modulo 2 of the first one's and theirs: registers are short)
     v4i kraw[R::QSTEPS];
-    constexpr int HELD = FORM == kWhole ? 8 : 4;
+    constexpr int HELD = FORM == kWhole ? 7 : 4;
     int far = 64;
     asm volatile("" : "+s"(far));
 #pragma unroll
     for (int st = 0; st < R::QSTEPS; ++st)
       kraw[st] = *reinterpret_cast<const v4i*>(
-          tile + (st < HELD ? this->k_off[st] : this->k_off[st - HELD] ^ far));
+          tile + (st < HELD ? this->k_off[st] : this->k_off[st - 4] ^ far));
     v16f s_acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
@@ -66,16 +67,18 @@ struct CodeTile : RowTile<_Float16, D> {
     float rv[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) rv[r] = s_acc[r];
-    // the wavefront's lanes that see a key: a block that none sees may have any scale, which must
-    // neither raise the unit nor, of keys, add c_less times it to masked logits
-    uint64_t seeing = ~0ull;
+    // the lanes that see a key: a block that a row does not see may have any scale, which must
+    // neither raise its unit nor, of keys, add c_less times it to masked logits
+    uint64_t seeing = ~0ull, sees0 = ~0ull, sees1 = ~0ull;  // of the lane's half; of each half
     if (!inside) {
       const uint32_t seen = bits();
       seeing = __ballot(seen != 0);
+      sees0 = (seeing & 0xffffffffull) | seeing << 32;
+      sees1 = (seeing >> 32) | (seeing & ~0xffffffffull);
 #pragma unroll
       for (int r = 0; r < 16; ++r) rv[r] = ((seen >> r) & 1u) ? rv[r] : -INFINITY;
     }
-    scales(seeing);
+    scales(seeing, sees0, sees1);
     if (FORM != kWhole) prefetch();
     v8hf p_op[2];
     auto exps = [&]() __attribute__((always_inline)) -> float {
@@ -180,7 +183,7 @@ cached_tile_kernel(WindowArgs a) {
 
   C t;
   t.init(lane);
-  t.unit = least_unit();
+  t.unit = kLeastUnit;
   {
     const Row r = row_of(a, p, p.row0 + lr);
     const T* const row = static_cast<const T*>(a.q) + p.b * a.sq[0] +
@@ -299,22 +302,22 @@ cached_tile_kernel(WindowArgs a) {
                         (key >= w_last.lo || key + kTileKeys <= a.sinks);
     t.template step8<FORM>(
         tile, inside,
-        [&](uint64_t seeing) __attribute__((always_inline)) {
+        [&](uint64_t seeing, uint64_t sees0, uint64_t sees1) __attribute__((always_inline)) {
           if constexpr (FORM == kWhole) {
-            const float k = seeing != 0 ? kn : 0.0f, v = seeing != 0 ? vn : 0.0f;
-            if (__float_as_uint(k) != had_k || __float_as_uint(v) != had_v)
-              t.take(k, v, __float_as_uint(v));
-            had_k = __float_as_uint(k);
-            had_v = __float_as_uint(v);
+            if (!inside || __float_as_uint(kn) != had_k || __float_as_uint(vn) != had_v) {
+              const float v = in_lanes(sees0 | sees1, vn);
+              t.take(in_lanes(sees0 | sees1, kn), v, v);
+            }
+            had_k = inside ? __float_as_uint(kn) : ~0u;
+            had_v = __float_as_uint(vn);
           } else {
-            const bool sees = (hf ? seeing >> 32 : seeing & 0xffffffffu) != 0;
-            const float k = sees ? scale_or_0(kn) : 0.0f, v = sees ? scale_or_0(vn) : 0.0f;
-            auto of_lane = [&](int l) __attribute__((always_inline)) -> uint32_t {
-              return static_cast<uint32_t>(
-                  __builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(v)), l));
+            const float of_half = scale_or_0(vn);
+            auto of_lane = [&](int l) __attribute__((always_inline)) -> float {
+              return __uint_as_float(static_cast<uint32_t>(
+                  __builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(of_half)), l)));
             };
-            const uint32_t first = of_lane(0), second = of_lane(32);
-            t.take(k, v, first > second ? first : second);
+            t.take(in_lanes(seeing, scale_or_0(kn)), in_lanes(seeing, of_half),
+                   fmaxf(in_lanes(sees0, of_lane(0)), in_lanes(sees1, of_lane(32))));
           }
         },
         [&]() __attribute__((always_inline)) {
@@ -339,7 +342,7 @@ cached_tile_kernel(WindowArgs a) {
   // the end of the wavefront's rows
   LateArgs& e = late_args();
   const float l = pair_sum(t.l_run), m = t.m_run;
-  const float inv = l > 0.0f ? __uint_as_float(t.unit.bits) / l : l;  // (a NaN sum stays one)
+  const float inv = l > 0.0f ? __uint_as_float(t.unit) / l : l;  // (a NaN sum stays one)
 #pragma unroll
   for (int dt = 0; dt < R::NDT; ++dt)
 #pragma unroll

@@ -113,9 +113,10 @@ cached_unit_kernel(WindowArgs a) {
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
     k_to[i] = i * 1024 + crow * D + ((lane % CPR) ^ swizzle(i * RPC + crow)) * 16;
-  int k_at[KL];
+  constexpr int AT = GROUP && D == 64 ? 1 : KL;  // (registers that are short hold one of two)
+  int k_at[AT];
 #pragma unroll
-  for (int i = 0; i < KL; ++i) k_at[i] = lr * D + (((2 * i + hf) ^ swizzle(lr)) * 16);
+  for (int i = 0; i < AT; ++i) k_at[i] = lr * D + (((2 * i + hf) ^ swizzle(lr)) * 16);
   // rows 4 hf + 0 .. 3; the others are 8, 16 and 24 further (registers that are short hold one)
   constexpr int VL = GROUP && D == 64 ? 1 : 4;
   int v_lo[VL];
@@ -156,22 +157,25 @@ cached_unit_kernel(WindowArgs a) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) o_acc[x][r] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;
-  Unit2 unit = least_unit();  // of the accumulators
+  uint32_t unit = kLeastUnit;  // of the row's accumulators
   constexpr int kShift = Half<_Float16>::kShift;
 
   // `codes` stands at the tile behind the present one: its keys are asked for as soon as the
   // present ones are in LDS, its values as soon as the present ones are in operands.
   for (int s = 0; s < p.steps; ++s) {
     const int key = cur.key, there = cur.there;
-    Scales<FORM> ns = sc;
+    const Scales<FORM> ns = sc;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) *reinterpret_cast<v4i*>(slot + k_to[i]) = kr[i];
     const bool more = s + 1 < p.steps;
     cur = codes.ref;
     if (more) load_k();
     v4i kc[KL];
+    int second = 32;
+    asm volatile("" : "+s"(second));
 #pragma unroll
-    for (int i = 0; i < KL; ++i) kc[i] = *reinterpret_cast<const v4i*>(slot + k_at[i]);
+    for (int i = 0; i < KL; ++i)
+      kc[i] = *reinterpret_cast<const v4i*>(slot + (i < AT ? k_at[i] : k_at[0] ^ second));
     v16f s_acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_acc[r] = 0.0f;
@@ -192,27 +196,28 @@ cached_unit_kernel(WindowArgs a) {
     for (int r = 0; r < 16; ++r) rv[r] = (s_acc[r] + less) * (r < 8 ? c0 : c1);
     const bool inside = there == 3 && key + kTileKeys <= first.hi &&
                         (key >= last.lo || key + kTileKeys <= a.sinks);
+    uint64_t sees0 = ~0ull, sees1 = ~0ull;  // lanes of rows that see a key of the halves
     if (!inside) {
-      const uint32_t all = seen_keys(late_args(), p, lr, key, there), seen = all >> (4 * hf);
+      const int at = lane_again();
+      const uint32_t all = seen_keys(late_args(), p, at & 31, key, there);
+      const uint32_t seen = all >> (at >> 5) * 4;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         rv[r] = (seen >> (8 * (r >> 2) + (r & 3))) & 1u ? rv[r] : -INFINITY;
-      // (a block that no row sees may have any scale, which must not raise the unit)
-#pragma unroll
-      for (int h = 0; h < N; ++h)
-        if (__ballot((all & (N == 1 ? ~0u : 0xffffu << (16 * h))) != 0) == 0) ns.v[h] = 0.0f;
+      sees0 = __ballot((all & (N == 1 ? ~0u : 0xffffu)) != 0);
+      sees1 = N == 1 ? sees0 : __ballot((all & 0xffff0000u) != 0);
     }
-    // the scales of the values, relative to the largest so far
+    // the scales of the values that the row sees, relative to the largest so far
+    const float top = fmaxf(in_lanes(sees0, ns.v[0]), in_lanes(sees1, ns.v[N - 1]));
+    if (__ballot(__float_as_uint(top) >= unit) != 0) {
+      const float f = raise_unit(unit, top);
 #pragma unroll
-    for (int h = 0; h < N; ++h)
-      if (__float_as_uint(ns.v[h]) >= unit.bits) {
-        const float f = raise_unit(unit, ns.v[h]);
+      for (int x = 0; x < NDT; ++x)
 #pragma unroll
-        for (int x = 0; x < NDT; ++x)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o_acc[x][r] *= f;
-      }
-    const float f0 = ns.v[0] * unit.inv, f1 = ns.v[N - 1] * unit.inv;
+        for (int r = 0; r < 16; ++r) o_acc[x][r] *= f;
+    }
+    const float f0 = in_lanes(sees0, ns.v[0] * per_unit(unit));
+    const float f1 = in_lanes(sees1, ns.v[N - 1] * per_unit(unit));
     v8hf p_op[2];
     auto exps = [&]() __attribute__((always_inline)) -> float {
       const float bias = m_run == -INFINITY ? 0.0f : -m_run;
@@ -268,7 +273,7 @@ cached_unit_kernel(WindowArgs a) {
   const int row_end = at_end & 31, hf_end = at_end >> 5;
   const Row my = row_of(e, p, row_end);
   const float l = pair_sum(l_run);
-  const float inv = l > 0.0f ? __uint_as_float(unit.bits) / l : l;  // (a NaN sum stays one)
+  const float inv = l > 0.0f ? __uint_as_float(unit) / l : l;  // (a NaN sum stays one)
   auto value = [&](int r, int x) __attribute__((always_inline)) -> float {
     return l == 0.0f ? 0.0f : o_acc[x][r] * (1 << Widen<E4M3>::kShift) * inv;
   };

@@ -173,3 +173,27 @@ def test_key_scales_that_other_rows_see(dev, page, mark, window):
                 got = _call(p.cache(0, free, far), q, [Lk], window, 0, 1, dev)
                 assert torch.equal(got[0][:, own], want[0][:, own]), (own, far)
                 assert torch.equal(got[1][:, :, own], want[1][:, :, own]), (own, far)
+
+
+@pytest.mark.parametrize("kv", [0, 1])
+@pytest.mark.parametrize("code,dtype", [(I8, BF), (F8, HF)])
+@pytest.mark.parametrize("page,mark", [(32, 16), (48, 16), (64, 32), (48, 48)])
+@pytest.mark.parametrize("Lq,window", [(30, 0), (30, 40), (100, 0), (100, 50)])
+def test_scales_that_later_rows_see(dev, kv, code, dtype, page, mark, Lq, window):
+    """Rows beside each other (few, or blocks of them): any scale of a block that starts behind
+    a row's position, or ends ahead of its window, leaves the row within the bound of the scales
+    that it sees."""
+    Lk, Hk, D = 300, 1, 128
+    p = Pages(dev, page + mark, code, [Lk], page, mark, Hk, D, -(-Lk // page))
+    q = _queries(9, (1, Lq, 1, D), dtype) - 0.2
+    seen = so.visible(Lq, Lk, window, 0, 1)
+    cut = 288 - (Lk - Lq)  # the rows ahead of key 288, a block's first whatever the mark
+    for rows in (slice(0, cut), slice(Lq - 8, Lq)):
+        free = p.unseen([seen[rows]])
+        if not free.any():
+            continue
+        for n_split in _forms(Lq, 1, Hk):
+            for far in (1e6, 1e20, 2.0 ** 125):
+                print("later rows", kv, code, page, mark, Lq, window, rows, n_split, far, flush=True)
+                out, lse = _call(p.cache(kv, free, far), q, [Lk], window, 0, n_split, dev)
+                p.check(out[:, rows], lse[:, :, rows], q[:, rows], [seen[rows]], D ** -0.5)
