@@ -908,6 +908,13 @@ void want_apart(const char* op, const at::Tensor& out, const char* name, const a
                     other);
 }
 
+// Nor the lengths, starts, offsets and tables that the kernel reads beside it.
+void want_apart_of(const char* op, const at::Tensor& out, const char* name,
+                   std::initializer_list<const c10::optional<at::Tensor>*> read) {
+  for (const auto* t : read)
+    if (t->has_value()) want_apart(op, out, name, **t, "what says where its rows are");
+}
+
 // (the stride of a dimension of one element says nothing)
 void put_strides(const at::Tensor& t, int64_t* s) {
   for (int64_t i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 0;
@@ -1200,6 +1207,7 @@ void append_cache(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_
     want_apart(op, *outs[i].first, outs[i].second, k, "k");
     want_apart(op, *outs[i].first, outs[i].second, v, "v");
     want_apart(op, *outs[i].first, outs[i].second, table, "the block table");
+    want_apart_of(op, *outs[i].first, outs[i].second, {&starts, &lengths, &offsets});
     for (int j = 0; j < i; ++j)
       want_apart(op, *outs[i].first, outs[i].second, *outs[j].first, outs[j].second);
   }
@@ -1263,6 +1271,8 @@ std::vector<at::Tensor> read_cache(
     if (!k_out_.has_value()) continue;
     for (const auto* t : {&k_codes, &v_codes, &k_scale, &v_scale, &table})
       want_apart(op, *o.first, o.second, *t, "the cache");
+    want_apart(op, *o.first, o.second, lengths, "the lengths");
+    want_apart_of(op, *o.first, o.second, {&starts});
   }
   if (k_out_.has_value()) want_apart(op, k_out, "k_out", v_out, "v_out");
   if (k_out.numel() == 0) return {k_out, v_out};
@@ -1352,6 +1362,7 @@ std::vector<at::Tensor> window_attention(
       want_apart(op, out, "out", *k_scale, "the key scales");
       want_apart(op, out, "out", *v_scale, "the value scales");
     }
+    want_apart_of(op, out, "out", {&table, &q_lengths, &k_lengths});
   }
   std::vector<at::Tensor> res{out};
   if (return_lse) res.push_back(at::empty({B, Hq, Lq}, q.options().dtype(at::kFloat)));
@@ -1451,6 +1462,8 @@ std::vector<at::Tensor> packed_attention(
     want_apart(op, out, "out", q, "q");
     want_apart(op, out, "out", k, "k");
     want_apart(op, out, "out", v, "v");
+    want_apart(op, out, "out", offsets, "the offsets");
+    want_apart_of(op, out, "out", {&k_offsets_});
   }
   std::vector<at::Tensor> res{out};
   if (return_lse) res.push_back(at::empty({Hq, T}, q.options().dtype(at::kFloat)));
