@@ -163,7 +163,7 @@ struct Code8<true> {
 // its own).
 template <typename T>
 struct Run8 {
-  typedef T V __attribute__((ext_vector_type(8)));
+  typedef T V __attribute__((ext_vector_type(8), aligned(16)));
   static constexpr uint32_t kInfinity =
       std::is_same<T, __bf16>::value ? 0x7f80u : std::is_same<T, _Float16>::value ? 0x7c00u
                                                                                   : 0x7f800000u;

@@ -368,7 +368,7 @@ static bool cache_dims(const int64_t* dims, int64_t max_pages, int64_t n_pages, 
          page % block == 0 && block % 16 == 0 && block <= (1 << 16) && max_pages < kMostSlots / page;
 }
 
-// Strides of rows of 8-channel runs (elements), and their pointers.
+// Strides of rows (elements), a multiple of `unit`, and pointers of rows of codes.
 static bool strides_ok(const int64_t* s, int n, int64_t unit) {
   for (int i = 0; i < n; ++i)
     if (s[i] < 0 || s[i] % unit) return false;
@@ -383,6 +383,8 @@ using namespace rcsa;
 static bool float_type(int dtype) {
   return dtype == RCSA_BF16 || dtype == RCSA_F16 || dtype == RCSA_F32;
 }
+// Elements of 16 bytes.
+static int64_t row_unit(int dtype) { return dtype == RCSA_F32 ? 4 : 8; }
 static bool code_type(int code) { return code == RCSA_CODE_INT8 || code == RCSA_CODE_E4M3; }
 
 extern "C" int rcsa_append_cache(const void* k, const void* v, int dtype, const int64_t* dims,
@@ -401,7 +403,9 @@ extern "C" int rcsa_append_cache(const void* k, const void* v, int dtype, const 
   if (dims[0] <= 0 || dims[0] >= (1 << 20) ||
       !cache_dims(each, max_pages, n_pages, page_size, block_size))
     return RCSA_ERR_SHAPE;
-  if (!strides_ok(strides, 12, 8) || !strides_ok(strides + 12, 6, 1)) return RCSA_ERR_STRIDE;
+  if (!strides_ok(strides, 6, row_unit(dtype)) || !strides_ok(strides + 6, 6, 8) ||
+      !strides_ok(strides + 12, 6, 1))
+    return RCSA_ERR_STRIDE;
   if (!aligned16(k) || !aligned16(v) || !aligned8(k_codes) || !aligned8(v_codes))
     return RCSA_ERR_ALIGN;
   AppendArgs a{};
@@ -458,7 +462,7 @@ extern "C" int rcsa_read_cache(const void* k_codes, const void* v_codes, int cod
   if (!float_type(dtype) || !code_type(code)) return RCSA_ERR_DTYPE;
   if (!cache_dims(dims, max_pages, n_pages, page_size, block_size)) return RCSA_ERR_SHAPE;
   if (!strides_ok(strides, 6, 8) || !strides_ok(strides + 6, 6, 1) ||
-      !strides_ok(strides + 12, 6, 8))
+      !strides_ok(strides + 12, 6, row_unit(dtype)))
     return RCSA_ERR_STRIDE;
   if (!aligned16(k_out) || !aligned16(v_out) || !aligned8(k_codes) || !aligned8(v_codes))
     return RCSA_ERR_ALIGN;
