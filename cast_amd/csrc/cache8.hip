@@ -308,8 +308,12 @@ static int launch_append(AppendArgs& a, hipStream_t s) {
   const int64_t wgs = (PACKED ? a.items : a.items * a.B) * (both ? 1 : 2) * a.H;
   // A wavefront for small blocks; 1024 threads where large ones may get many tokens at once (5
   // tokens of 64 requests, 4 heads of D 256 in blocks of 256: 16.5 us by 1024 threads, 8.0 by 256;
-  // 54 and 51 where every block's scale grows).
-  const int64_t fresh = static_cast<int64_t>(a.L < a.block ? a.L : a.block) * a.runs;
+  // 54 and 51 where every block's scale grows).  Packed requests: what one of them has on average
+  // (the same tokens packed 15.0 by 1024 threads, 5.9 by 256; 1 of 300 requests' 65.5, 12.7; 64 of 40
+  // tokens 16.0, 9.4); a longer one's blocks are gone through in rounds (one of 3000 beside 63 of
+  // 5: 19.1, 28.7).
+  const int64_t each = PACKED ? (a.L + a.B - 1) / a.B : a.L;
+  const int64_t fresh = (each < a.block ? each : a.block) * a.runs;
   const int threads = runs <= 512 ? 64 : fresh <= 2048 ? 256 : 1024;
   if (wgs >= (1ll << 31) || wgs * threads >= kMaxThreads8) return RCSA_ERR_SHAPE;
   const dim3 grid(static_cast<unsigned>(wgs)), block(static_cast<unsigned>(threads));
