@@ -9,10 +9,12 @@
 // A weight takes the scale of its value's block, relative to a power of two 2^e above any scale of
 // the keys that the row has seen so far, before it is rounded to fp16; e grows with the tiles (the
 // accumulators move by the difference), and the sums of weights know nothing of it.  A block may
-// have any scale for the rows that do not see it: it counts as 0 there.  A weight
-// below 2^-32 of the largest, in a block whose scale is as large, is lost: values that
-// differ by more than that between blocks give the smaller ones no more than fp32 sums would
-// have left of them.
+// have any scale for the rows that do not see it: it counts as 0 there.  A weight below 2^-31 of
+// the row's largest, in a block whose scale is the largest that the row has met, is lost (it may
+// be 2^6 where the largest is 2^7, and fp16 drops what is below 2^-25); in a block of a scale
+// 2^-n of that, one below 2^(n - 31).  That is relative to the largest scale met, not to the
+// result: a seen block of a far larger scale takes bits from the others' weights even where its
+// own are next to nothing.
 #pragma once
 #include "window_attn.h"
 

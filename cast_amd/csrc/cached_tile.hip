@@ -3,12 +3,12 @@
 // wavefront that copied them (once a workgroup, not once a wavefront) one tile ahead.
 //
 // Bound by the matrix and the vector pipe, whose times add within a wavefront: four frames of 880
-// rows on the last twenty of 44 and the first, 24 heads of D 128 in int8 pages of 128 keys, 888 us,
-// 900 TFLOP/s, the matrix pipe 47% and the vector pipe 50% busy at 2.0 GHz, no bank conflicts.
-// There: codes through registers ahead of LDS 1359 us; through LDS, three workgroups on a compute
-// unit 1038; places carried from tile to tile instead of found for each 931; keys as subnormal
-// fp16 numbers (a byte permutation alone) 913.  Without the scales' loads, whose scalar returns
-// every wait for LDS waits for, 862 (a wrong result).
+// rows on the last twenty of 44 and the first, 24 heads of D 128 in int8 pages of 128 keys, 890 to
+// 940 us by card, 850 to 900 TFLOP/s, the matrix pipe 46% and the vector pipe 50% busy at 2.0 GHz,
+// no bank conflicts.  There, on a card that takes 888: codes through registers ahead of LDS 1359 us;
+// through LDS, three workgroups on a compute unit 1038; places carried from tile to tile instead of
+// found for each 931; keys as subnormal fp16 numbers (a byte permutation alone) 913.  Without the
+// scales' loads, whose scalar returns every wait for LDS waits for, 862 (a wrong result).
 #include "cached_attn.h"
 
 namespace rcsa {

@@ -10,16 +10,17 @@
 // lines than the first cache has), so keys are loaded by whole rows and go through LDS.
 //
 // Bound by HBM where the cache is long: 48 requests of up to 32768 keys, 32 heads on 8 of D 128,
-// 205 us for 1.02 GB (5.0 TB/s) and 7 for the join; there keys by their lanes' rows took 228 us, by
-// copies to LDS 222, units of 16 tiles 219.  Short calls are latency: 1 request, 1024 keys of 8
-// heads 8.8 us and 3.4 for the join.
+// 191 us for 1.02 GB (5.3 TB/s) and 7 for the join; in all 198, and while that was 213 keys by
+// their lanes' rows took 228 us, by copies to LDS 222.  Short calls are latency: 1 request, 1024
+// keys of 8 heads 8.2 us and 3 to 4 for the join.
 #include "cached_attn.h"
 
 namespace rcsa {
 
 // Wavefronts to a SIMD: those of D 64 leave registers for two workgroups of eight on a compute
 // unit (48 requests of 1599 keys, 7 queries of 12 heads 57.7 us, so 51.4; 12 heads of 64 x 2000
-// keys 66.5 and 60.7), or for three units.
+// keys 66.5 and 60.7), or for three units.  (Those workgroups have 128 registers, which int8 codes
+// with two scales a tile fill.)
 constexpr int cached_waves(int D, bool group) { return D == 64 ? (group ? 4 : 3) : 2; }
 
 template <typename T, bool E4M3, int D, CodeForm FORM, bool GROUP>

@@ -150,8 +150,8 @@ __device__ __forceinline__ int units_of(int tiles, int chunk) {
 // kUnitTiles tiles; beyond, units of that size, or more of them than four rounds.  A unit
 // costs about 5 us before its first tile has landed (a tile streams in 0.4 to 1), and the
 // units of a last, short round leave compute units idle.  Tiles of 8-bit codes are half the
-// bytes: units of twice as many (48 ragged requests of up to 32768 keys: of 16 tiles 222 us, 32
-// 213, 64 259).
+// bytes: units of twice as many (48 ragged requests of up to 32768 keys: of 16 tiles 211 us, 32
+// 198, 64 257).
 // (Sums and products in fp32, at most 14 roundings of 2^-24, that the factor rounds up: a plan,
 // the same for every wavefront.  The tiles of all requests pass 32 bits where tables share
 // pages; a request has at most 2^25, so that a chunk of kMostTiles leaves it whole.)

@@ -136,13 +136,6 @@ static int64_t xcd_whole_of(int64_t items, int64_t n_split) {
 
 using namespace rcsa;
 
-// Few rows of a key head go to one workgroup (n_split -1) or to units of one wavefront (0),
-// more to blocks of 128 rows.  Of these the ones past an XCD's whole rounds (one block to a
-// compute unit) leave compute units idle: their keys go to n_split workgroups.  c =
-// ceil(tail n / U) of them on a compute unit overlap a little and take c - 2/9 times as long
-// as one (measured over 1210 tiles, 168 blocks: n 1 725 us, 2 526, 3 424, 4 440, 5 482, 6 448,
-// 8 512); kFixed tiles for the start, as many and one a share for the join (128 blocks of 250
-// tiles: n 2 95, 4 81, 6 83, 8 89; 168 of 83: n 1 57, 3 51, 5 62; 128 of 16: n 1 19, 2 26).
 // The form for few rows, where one fits.
 static bool plan_few(const int64_t* dims, int64_t tiles, int64_t* n_split) {
   const bool units = units_fit(dims);
@@ -151,6 +144,13 @@ static bool plan_few(const int64_t* dims, int64_t tiles, int64_t* n_split) {
   return true;
 }
 
+// Few rows of a key head go to one workgroup (n_split -1) or to units of one wavefront (0),
+// more to blocks of 128 rows.  Of these the ones past an XCD's whole rounds (one block to a
+// compute unit) leave compute units idle: their keys go to n_split workgroups.  c =
+// ceil(tail n / U) of them on a compute unit overlap a little and take c - 2/9 times as long
+// as one (measured over 1210 tiles, 168 blocks: n 1 725 us, 2 526, 3 424, 4 440, 5 482, 6 448,
+// 8 512); kFixed tiles for the start, as many and one a share for the join (128 blocks of 250
+// tiles: n 2 95, 4 81, 6 83, 8 89; 168 of 83: n 1 57, 3 51, 5 62; 128 of 16: n 1 19, 2 26).
 extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;
@@ -173,12 +173,13 @@ extern "C" int rcsa_window_attn_plan(const int64_t* dims, int64_t max_keys, int6
   return RCSA_OK;
 }
 
-// Over codes, in a lone workgroup's times for a tile (1.25 us: widening the codes leaves less to
-// overlap than tiles of 16 bits do, and more to gain from workgroups beside it): a share's tiles,
-// 1.3 and 1.5 times as long with one and two workgroups beside it; the joining launch, and a
-// share's rows written and read again.  17 queries of 32 heads on 8 of D 128, 16 requests of 3082
-// keys, in 1, 2, 4, 6, 8 shares 126, 79, 62, 60, 70 us; 318 of 24 heads, 862 keys, in 1, 2, 3, 6:
-// 41, 34, 33, 35; 100 of 8 heads, 2 of 20000 keys, in 1, 4, 8, 16: 707, 201, 115, 79.
+// Over codes the same choice by another cost, in a lone workgroup's times for a tile (1.25 us:
+// widening the codes leaves less to overlap than tiles of 16 bits do, and more to gain from
+// workgroups beside it): a share's tiles, 1.3 and 1.5 times as long with one and two workgroups
+// beside it; the joining launch, and a share's rows written and read again.  17 queries of 32
+// heads on 8 of D 128, 16 requests of 3082 keys, in 1, 2, 4, 6, 8 shares 126, 79, 62, 60, 70 us;
+// 318 of 24 heads, 862 keys, in 1, 2, 3, 6: 41, 34, 33, 35; 100 of 8 heads, 2 of 20000 keys, in
+// 1, 4, 8, 16: 707, 201, 115, 79.
 extern "C" int rcsa_cached_attn_plan(const int64_t* dims, int64_t max_keys, int64_t* n_split) {
   if (!dims || !n_split) return RCSA_ERR_NULL;
   if (!window_dims(dims) || max_keys < 0) return RCSA_ERR_SHAPE;

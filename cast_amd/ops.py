@@ -1374,8 +1374,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache | QuantizedCache, lengths
     Over a :class:`QuantizedCache` (``rcsa_cached_attn``) keys and values are the c * s that its
     codes stand for; q and the products are of 16 bits, the weights of fp16 with their value's scale.
     A scale that is no positive number below 2^126 counts as 0, and so does a value's e4m3 code
-    that holds no number (:func:`append_cache` writes none).  Rows of q with values past 2^100
-    may overflow.
+    that holds no number (:func:`append_cache` writes none).  Blocks that a row does not see may
+    hold any scales and codes; beside a seen block whose value scale is 2^n larger, a weight below
+    2^(n - 31) of the row's largest counts as 0.  Rows of q with values past 2^100 may overflow.
 
     Pages that no row sees are not read, so their table entries may be anything; an entry
     outside the pages hides its keys; tables may share pages.  ``max_length`` bounds the lengths (what the table

@@ -860,8 +860,10 @@ int rcsa_read_cache(const void* k_codes, const void* v_codes, int code, const fl
  * Arguments as there, with the type of the codes, their scales (scale_strides: host array of 6,
  * page, block, head of the scales of keys and of values) and block_size; block_table is
  * wanted.  A scale that is no positive number below 2^126 counts as 0; a value
- * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.  Logits
- * of rows of q with values past 2^100 may overflow.
+ * code of e4m3 that holds no number counts as 0, a key's makes the rows that see it NaN.  Blocks
+ * that a row does not see may hold any scales and codes; beside a seen block whose value scale is
+ * 2^n larger, a weight below 2^(n - 31) of the row's largest counts as 0.  Logits of rows of q
+ * with values past 2^100 may overflow.
  * Token (slot) strides and pointers of the codes are multiples of 16.  The workspace is
  * rcsa_window_attn's; rcsa_cached_attn_plan picks n_split as rcsa_window_attn_plan does there.
  */
